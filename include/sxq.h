@@ -56,6 +56,7 @@ typedef enum {
     SXQ_Q8_0 = 8,
     SXQ_Q4K = 12,
     SXQ_Q8K = 15,
+    SXQ_BF16 = 30,
 } sxq_dtype;
 
 /* sxq_qmm_forward flags */
@@ -192,6 +193,82 @@ sxq_status sxq_embed_quantize(int device, int scheme, const float *table, int64_
  * gives a zero row), enqueued on `stream`. */
 sxq_status sxq_embed_gather(int device, int scheme, const uint8_t *q, const float *scale, int64_t rows, int64_t h,
                             const int32_t *ids, int n, float *out, void *stream);
+
+/* ---- Paged key/value cache ----------------------------------------------------------
+ * The cache of many requests as a pool of pages, so that a request holds the pages of its
+ * own length rather than max_seq positions (the reference's KvCache grows one tensor per
+ * stream, crates/syrinx-fish/src/s2/nn.rs:221-254; no paged counterpart there).  Page
+ * `table[r][p / page_size]` holds position p of request r; a slot is page * page_size + p %
+ * page_size.  All pointers are device pointers, every call enqueues on `stream`, allocates
+ * nothing and may be captured into a graph.  Lengths, page ids, slots and rows are read on
+ * the device and checked there: an id outside the pool counts as an absent page, a slot or
+ * row outside its range as no token, a length outside 0 .. max_blocks * page_size as the
+ * nearest of the two. */
+typedef struct {
+    int32_t dtype;     /* SXQ_F32, SXQ_F16 or SXQ_BF16 */
+    int32_t n_kv_heads;
+    int32_t head_dim;  /* a multiple of 8, 8..256 */
+    int32_t page_size; /* positions per page: a power of two, 16..1024 */
+    int32_t n_pages;   /* n_pages * page_size < 2^31 */
+    void *k, *v;       /* the pools, 16-byte aligned, laid out alike: */
+    int64_t page_stride, head_stride, pos_stride; /* elements, multiples of 16 bytes; a head's row at one
+                                                     position is contiguous */
+} sxq_kv_pages;
+
+/* Block tables and slot maps from the requests' lengths.  Request r of n_rows holds lens[r]
+ * positions in the pages table[r][0 .. ceil(lens[r] / page_size)) (table row stride
+ * table_stride, max_blocks entries each); free_list[0 .. *free_count) is the stack of free
+ * pages (its array holds n_pages).  add[r] >= 0 grows request r by so many tokens, add[r] < 0
+ * shrinks it by -add[r] (to no less than 0):
+ *   - first the pages that shrinking leaves unused are pushed, in reverse, so that the first
+ *     of them (requests ascending, then blocks) is on top, and their table entries become -1;
+ *   - then growing requests pop the pages they need, requests ascending.  A request is refused
+ *     -- its length and table row stay, it has no tokens -- with status 2 if its table row is
+ *     too short, 1 if it needs pages and the pages asked for up to and with it (refused
+ *     requests' included) exceed the free ones, 3 if the tokens asked for up to and with it
+ *     exceed `capacity`; otherwise status 0.
+ * An accepted step is undone exactly -- table, stack and lengths -- by the call with add
+ * negated.  cu int32 [n_rows + 1]: the first token of each accepted request, then their
+ * number T; token t < T of the map: slots[t], pos[t] (its position) and rows[t] (its
+ * request), requests ascending; entries T .. capacity - 1 are -1.  capacity may be 0 (the
+ * three maps are then not touched).  n_rows * max_blocks and max_blocks * page_size < 2^31. */
+sxq_status sxq_kv_reserve(int device, int page_size, int n_pages, int n_rows, int max_blocks, const int32_t *add,
+                          int32_t *lens, int32_t *table, int64_t table_stride, int32_t *free_list,
+                          int32_t *free_count, int capacity, int32_t *cu, int32_t *slots, int32_t *pos,
+                          int32_t *rows, int32_t *status, void *stream);
+
+/* New tokens into the pages: the glue between the fused QKV projection and attention
+ * (crates/syrinx-fish/src/s2/nn.rs:325-339, crates/syrinx-lm/src/cv2/attention.rs:50-66).
+ * Token t's row of qkv (row_stride elements apart, in_dtype SXQ_F32, SXQ_F16 or SXQ_BF16)
+ * holds n_heads query heads, then the key heads, then the value heads.  Queries and keys get
+ * an RMSNorm over the head (q_norm / k_norm f32 [head_dim], either may be NULL) and RoPE by the
+ * f32 tables cos / sin [max_pos][head_dim / 2] at pos[t] (clamped to the tables; both NULL: no
+ * rotation), pairs (2i, 2i+1) if interleaved, else (i, i + head_dim / 2).  Keys and values go to
+ * slots[t] of the pages, queries to q_out [n_tokens][n_heads * head_dim] in in_dtype (NULL:
+ * not computed).  Arithmetic in f32, one rounding at each store.  A token whose slot lies
+ * outside the pool writes nothing.  Tokens with one slot write it in no particular order. */
+sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, const void *qkv, int64_t row_stride,
+                         int n_tokens, int n_heads, const float *q_norm, const float *k_norm, float eps,
+                         const float *cos, const float *sin, int max_pos, int interleaved, const int32_t *pos,
+                         const int32_t *slots, void *q_out, void *stream);
+
+/* Attention of one new token per query row over its request's pages (decode: nn.rs:340-352,
+ * attention.rs:67-76):
+ *   out[b][h] = sum_j p_j v_j,  p = softmax_j(scale * q[b][h] . k_j),  j < lens[rows[b]],
+ * over KV head h / (n_heads / n_kv_heads) (n_heads a multiple of n_kv_heads).  q and out:
+ * rows of n_heads * head_dim, q_stride / out_stride elements apart (multiples of 16 bytes,
+ * 16-byte aligned), q_dtype the pages' type, or SXQ_F32 over SXQ_BF16 pages; out has q's type.
+ * Scores, softmax and sums are f32.  rows int32 [n_q]: the table row of each query (NULL: b);
+ * a query whose row lies outside 0 .. n_rows - 1 leaves its out row as it was.  A request
+ * without positions (or whose pages are all absent) gives zeros.
+ * workspace (sxq_kv_attention_workspace bytes, 256-byte aligned) is zeroed by the caller
+ * before its first use; every call leaves it ready for the next of the same or smaller
+ * n_q * n_heads.  Calls that share one must not overlap. */
+sxq_status sxq_kv_attention_workspace(const sxq_kv_pages *pages, int n_q, int n_heads, size_t *bytes);
+sxq_status sxq_kv_attention(int device, const sxq_kv_pages *pages, int q_dtype, const void *q, int64_t q_stride,
+                            int n_q, int n_heads, const int32_t *rows, const int32_t *lens, int n_rows,
+                            const int32_t *table, int64_t table_stride, int max_blocks, float scale, void *out,
+                            int64_t out_stride, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- Decoder step: the callers of QMatMul in one autoregressive LM token ------------
  *

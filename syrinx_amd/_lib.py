@@ -72,6 +72,10 @@ _SIGS = {
     "sxq_embed_scheme": (_I, [_I, _I64, _P]),
     "sxq_embed_quantize": (_I, [_I, _I, _P, _I64, _I64, _P, _P, _P]),
     "sxq_embed_gather": (_I, [_I, _I, _P, _P, _I64, _I64, _P, _I, _P, _P]),
+    "sxq_kv_reserve": (_I, [_I, _I, _I, _I, _I, _P, _P, _P, _I64, _P, _P, _I, _P, _P, _P, _P, _P, _P]),
+    "sxq_kv_append": (_I, [_I, _P, _I, _P, _I64, _I, _I, _P, _P, _F, _P, _P, _I, _I, _P, _P, _P, _P]),
+    "sxq_kv_attention_workspace": (_I, [_P, _I, _I, _P]),
+    "sxq_kv_attention": (_I, [_I, _P, _I, _P, _I64, _I, _I, _P, _P, _I, _P, _I64, _I, _F, _P, _I64, _P, _SZ, _P]),
     "sxq_lm_step": (_I, [_P, _I, _P, _P, _P, _P, _P, _U, _P]),
     "sxq_lm_read_kv": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _P]),
     "sxq_lm_prefill": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _U, _P, _SZ, _P]),

@@ -1,0 +1,361 @@
+// sxq_paged.hip -- the paged key/value cache: page allocation with block tables and slot maps
+// (sxq_kv_reserve), and new tokens into the pages (sxq_kv_append).  include/sxq.h states both.
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+
+#include "../../include/sxq.h"
+#include "sxq_abi.h"
+#include "sxq_paged.h"
+#include "sxq_paged_launch.h"
+
+using namespace sxq;
+using namespace sxq::abi;
+
+namespace {
+
+// ---------------------------------------------------------------------------- reserve
+// Sums of pages fit 31 bits (n_rows * max_blocks < 2^31); sums of tokens saturate at
+// 2^31 - 1 (the capacity they are compared with is at most that).
+SXQ_DEV int sat_add(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, 0x7FFFFFFFu); }
+
+struct Pair {
+    int pages, tokens;
+};
+SXQ_DEV Pair operator+(Pair a, Pair b) { return {a.pages + b.pages, sat_add(a.tokens, b.tokens)}; }
+
+// Inclusive scan over the workgroup's NT threads; `total` gets the sum.  red: NT / 64 pairs.
+template <int NT>
+SXQ_DEV Pair block_scan(Pair v, Pair* red, Pair& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const Pair u = {__shfl_up(v.pages, o, 64), __shfl_up(v.tokens, o, 64)};
+        if (lane >= o) v = u + v;
+    }
+    if (NT == 64) {
+        total = {__shfl(v.pages, 63, 64), __shfl(v.tokens, 63, 64)};
+        return v;
+    }
+    __syncthreads();  // the last scan's readers are done with red
+    if (lane == 63) red[wave] = v;
+    __syncthreads();
+    Pair before = {0, 0}, sum = {0, 0};
+    for (int w = 0; w < NT / 64; ++w) {
+        if (w == wave) before = sum;
+        sum = sum + red[w];
+    }
+    total = sum;
+    return before + v;
+}
+
+// The last i with first[i] <= j, over n ascending firsts (first[0] <= j).
+SXQ_DEV int owner(const int* first, int n, int j) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (first[mid] <= j) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// One workgroup, NT requests at a time: the sums that order the requests are prefix sums, and
+// the pages and tokens of a chunk are dealt over the threads, each finding its request in the
+// chunk's offsets.
+template <int NT>
+__global__ __launch_bounds__(NT) void k_kv_reserve(const KvReserve A) {
+    __shared__ Pair red[NT / 64 + 1];
+    __shared__ int s_first[NT], s_block[NT], s_tok[NT], s_old[NT];
+    const int tid = threadIdx.x, n = A.n_rows, P = 1 << A.shift;
+    const int64_t top = (int64_t)A.max_blocks << A.shift;
+    const int count = min(max(A.free_count[0], 0), A.n_pages);
+
+    auto load = [&](int r, int& a, int& old) {
+        a = r < n ? A.add[r] : 0;
+        old = r < n ? kv_clamp_len(A.lens[r], A.max_blocks, A.shift) : 0;
+    };
+    auto shrunk = [&](int a, int old) { return (int)max((int64_t)old + a, (int64_t)0); };
+
+    // 1. pages given back
+    int freed = 0;
+    for (int r0 = 0; r0 < n; r0 += NT) {
+        int a, old;
+        load(r0 + tid, a, old);
+        Pair total;
+        block_scan<NT>({a < 0 ? kv_blocks(old, A.shift) - kv_blocks(shrunk(a, old), A.shift) : 0, 0}, red, total);
+        freed += total.pages;
+    }
+    int done = 0;
+    for (int r0 = 0; r0 < n && freed; r0 += NT) {
+        int a, old;
+        load(r0 + tid, a, old);
+        const int b0 = kv_blocks(shrunk(a, old), A.shift), m = a < 0 ? kv_blocks(old, A.shift) - b0 : 0;
+        Pair total;
+        const int first = block_scan<NT>({m, 0}, red, total).pages - m;
+        s_first[tid] = first;
+        s_block[tid] = b0;
+        __syncthreads();
+        for (int j = tid; j < total.pages; j += NT) {
+            const int i = owner(s_first, min(NT, n - r0), j);
+            int32_t* e = A.table + (int64_t)(r0 + i) * A.table_stride + s_block[i] + (j - s_first[i]);
+            const int at = count + freed - 1 - (done + j);
+            if (at < A.n_pages) A.free_list[at] = *e;
+            *e = -1;
+        }
+        done += total.pages;
+        __syncthreads();
+    }
+    __syncthreads();  // the pushed pages are visible to the pops below
+
+    // 2. pages and tokens handed out
+    const int avail = min(count + freed, A.n_pages);
+    Pair asked = {0, 0}, given = {0, 0};
+    if (tid == 0) A.cu[0] = 0;
+    for (int r0 = 0; r0 < n; r0 += NT) {
+        const int r = r0 + tid;
+        int a, old;
+        load(r, a, old);
+        const int64_t grown = (int64_t)old + a;
+        const bool wide = a >= 0 && grown > top;
+        const bool grow = a >= 0 && !wide;
+        const int b0 = kv_blocks(old, A.shift);
+        Pair want = {0, 0}, total;
+        if (grow) want = {kv_blocks((int)grown, A.shift) - b0, a};
+        const Pair upto = asked + block_scan<NT>(want, red, total);
+        asked = asked + total;
+        const int status = wide ? 2 : want.pages > 0 && upto.pages > avail ? 1
+                                  : want.tokens > 0 && upto.tokens > A.capacity ? 3 : 0;
+        const bool ok = grow && status == 0;
+        if (!ok) want = {0, 0};
+        const Pair mine = block_scan<NT>(want, red, total);
+        s_first[tid] = mine.pages - want.pages;
+        s_tok[tid] = mine.tokens - want.tokens;
+        s_block[tid] = b0;
+        s_old[tid] = old;
+        if (r < n) {
+            A.cu[r + 1] = given.tokens + mine.tokens;
+            A.status[r] = status;
+            A.lens[r] = a < 0 ? shrunk(a, old) : ok ? (int)grown : old;
+        }
+        __syncthreads();
+        const int rows = min(NT, n - r0);
+        for (int j = tid; j < total.pages; j += NT) {
+            const int i = owner(s_first, rows, j);
+            A.table[(int64_t)(r0 + i) * A.table_stride + s_block[i] + (j - s_first[i])] =
+                A.free_list[avail - 1 - (given.pages + j)];
+        }
+        __syncthreads();  // the new table entries are read by the tokens' threads
+        for (int j = tid; j < total.tokens; j += NT) {
+            const int i = owner(s_tok, rows, j);
+            const int pos = s_old[i] + (j - s_tok[i]), t = given.tokens + j;
+            A.slots[t] = kv_slot(A.table[(int64_t)(r0 + i) * A.table_stride + (pos >> A.shift)], pos, A.shift, A.n_pages);
+            A.pos[t] = pos;
+            A.rows[t] = r0 + i;
+        }
+        given = given + total;
+        __syncthreads();
+    }
+    for (int t = given.tokens + tid; t < A.capacity; t += NT) A.slots[t] = A.pos[t] = A.rows[t] = -1;
+    if (tid == 0) A.free_count[0] = avail - given.pages;
+}
+
+// ---------------------------------------------------------------------------- append
+// One wave per (token, head) of the fused row: lane i holds pairs i and i + 64 of the head.
+template <typename TI, typename TC>
+__global__ __launch_bounds__(64) void k_kv_append(const KvAppend A, const KvPool P) {
+    const int t = blockIdx.x, hid = blockIdx.y, lane = threadIdx.x, hd = P.hd, half = hd / 2;
+    const int slot = A.slots[t];
+    if (slot < 0 || slot >= P.n_pages << P.shift) return;
+    const bool is_q = hid < A.nh, is_k = !is_q && hid < A.nh + P.nkv;
+    if (is_q && !A.q_out) return;
+    const TI* src = (const TI*)A.qkv + (int64_t)t * A.row_stride + (int64_t)hid * hd;
+    const float* w = is_q ? A.q_norm : is_k ? A.k_norm : nullptr;
+    const bool rot = A.cos && (is_q || is_k);
+    const int p = min(max(A.pos[t], 0), A.max_pos - 1);
+    float a[2], b[2], ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int i = lane + 64 * j;
+        a[j] = b[j] = 0.0f;
+        if (i < half) {
+            a[j] = to_f32(src[A.interleaved ? 2 * i : i]);
+            b[j] = to_f32(src[A.interleaved ? 2 * i + 1 : i + half]);
+        }
+        ss += a[j] * a[j] + b[j] * b[j];
+    }
+    if (w) {
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    }
+    const float den = w ? sqrtf(ss / (float)hd + A.eps) : 1.0f;
+    const int kh = hid - A.nh - (is_k ? 0 : P.nkv);
+    TC* cd = (TC*)(is_k ? P.k : P.v) + (is_q ? 0 : kv_slot_base(P, slot, kh));
+    TI* qd = (TI*)A.q_out + ((int64_t)t * A.nh + hid) * hd;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int i = lane + 64 * j;
+        if (i >= half) break;
+        const int ia = A.interleaved ? 2 * i : i, ib = A.interleaved ? 2 * i + 1 : i + half;
+        float x = a[j], y = b[j];
+        if (w) {
+            x = x / den * w[ia];
+            y = y / den * w[ib];
+        }
+        if (rot) {
+            const float c = A.cos[(int64_t)p * half + i], s = A.sin[(int64_t)p * half + i];
+            const float u = x * c - y * s;
+            y = y * c + x * s;
+            x = u;
+        }
+        if (is_q) {
+            qd[ia] = from_f32<TI>(x);
+            qd[ib] = from_f32<TI>(y);
+        } else {
+            cd[ia] = from_f32<TC>(x);
+            cd[ib] = from_f32<TC>(y);
+        }
+    }
+}
+
+template <typename TI>
+void append_by_cache(const KvAppend& a, const KvPool& p, dim3 grid, hipStream_t s) {
+    if (p.dtype == kF32) hipLaunchKernelGGL((k_kv_append<TI, float>), grid, dim3(64), 0, s, a, p);
+    else if (p.dtype == kF16) hipLaunchKernelGGL((k_kv_append<TI, _Float16>), grid, dim3(64), 0, s, a, p);
+    else hipLaunchKernelGGL((k_kv_append<TI, __bf16>), grid, dim3(64), 0, s, a, p);
+}
+
+bool kv_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
+bool pow2_page(int p) { return p >= 16 && p <= 1024 && (p & (p - 1)) == 0; }
+
+}  // namespace
+
+namespace sxq {
+
+hipError_t launch_kv_reserve(const KvReserve& a, hipStream_t s) {
+    if (a.n_rows <= 64) hipLaunchKernelGGL(k_kv_reserve<64>, dim3(1), dim3(64), 0, s, a);
+    else hipLaunchKernelGGL(k_kv_reserve<1024>, dim3(1), dim3(1024), 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_append(const KvAppend& a, const KvPool& p, hipStream_t s) {
+    const dim3 grid(a.n_tokens, a.nh + 2 * p.nkv);
+    if (a.dtype == kF32) append_by_cache<float>(a, p, grid, s);
+    else if (a.dtype == kF16) append_by_cache<_Float16>(a, p, grid, s);
+    else append_by_cache<__bf16>(a, p, grid, s);
+    return hipGetLastError();
+}
+
+namespace abi {
+
+sxq_status kv_pool(const char* who, const sxq_kv_pages* g, bool pointers, KvPool* out) {
+    if (!g) return fail(SXQ_ERR_INVALID, "%s: null pages", who);
+    if (!kv_dtype(g->dtype)) return fail(SXQ_ERR_DTYPE, "%s: page dtype %d (f32, f16 or bf16)", who, g->dtype);
+    if (!pow2_page(g->page_size))
+        return fail(SXQ_ERR_INVALID, "%s: page_size %d is not a power of two in 16..1024", who, g->page_size);
+    if (g->n_pages < 1 || (int64_t)g->n_pages * g->page_size > 0x7FFFFFFF)
+        return fail(SXQ_ERR_INVALID, "%s: n_pages %d (1 or more, n_pages * page_size below 2^31)", who, g->n_pages);
+    if (g->n_kv_heads < 1 || g->n_kv_heads > 1024)
+        return fail(SXQ_ERR_INVALID, "%s: n_kv_heads %d", who, g->n_kv_heads);
+    if (g->head_dim < 8 || g->head_dim > 256 || g->head_dim % 8)
+        return fail(SXQ_ERR_SHAPE, "%s: head_dim %d is not a multiple of 8 in 8..256", who, g->head_dim);
+    const int64_t unit = 16 / type_size(g->dtype), most = (int64_t)1 << 50;
+    for (int64_t st : {g->page_stride, g->head_stride, g->pos_stride})
+        if (st < g->head_dim || st % unit || st > most)
+            return fail(SXQ_ERR_SHAPE, "%s: page strides (%lld, %lld, %lld) must be multiples of %lld elements, at least head_dim",
+                        who, (long long)g->page_stride, (long long)g->head_stride, (long long)g->pos_stride, (long long)unit);
+    if (pointers && (!g->k || !g->v)) return fail(SXQ_ERR_INVALID, "%s: null page pool", who);
+    if (((uintptr_t)g->k | (uintptr_t)g->v) & 15) return fail(SXQ_ERR_INVALID, "%s: the page pools must be 16-byte aligned", who);
+    out->k = g->k;
+    out->v = g->v;
+    out->page_stride = g->page_stride;
+    out->head_stride = g->head_stride;
+    out->pos_stride = g->pos_stride;
+    out->dtype = g->dtype;
+    out->nkv = g->n_kv_heads;
+    out->hd = g->head_dim;
+    out->page = g->page_size;
+    out->shift = __builtin_ctz((unsigned)g->page_size);
+    out->n_pages = g->n_pages;
+    return SXQ_OK;
+}
+
+}  // namespace abi
+}  // namespace sxq
+
+extern "C" {
+
+sxq_status sxq_kv_reserve(int device, int page_size, int n_pages, int n_rows, int max_blocks, const int32_t* add,
+                          int32_t* lens, int32_t* table, int64_t table_stride, int32_t* free_list,
+                          int32_t* free_count, int capacity, int32_t* cu, int32_t* slots, int32_t* pos,
+                          int32_t* rows, int32_t* status, void* stream) {
+    if (!pow2_page(page_size))
+        return fail(SXQ_ERR_INVALID, "kv_reserve: page_size %d is not a power of two in 16..1024", page_size);
+    if (n_pages < 1 || (int64_t)n_pages * page_size > 0x7FFFFFFF)
+        return fail(SXQ_ERR_INVALID, "kv_reserve: n_pages %d (1 or more, n_pages * page_size below 2^31)", n_pages);
+    if (n_rows < 1 || max_blocks < 1 || (int64_t)n_rows * max_blocks > 0x7FFFFFFF ||
+        (int64_t)max_blocks * page_size > 0x7FFFFFFF)
+        return fail(SXQ_ERR_INVALID, "kv_reserve: a table of %d rows of %d blocks", n_rows, max_blocks);
+    if (table_stride < max_blocks) return fail(SXQ_ERR_SHAPE, "kv_reserve: table_stride %lld below max_blocks %d", (long long)table_stride, max_blocks);
+    if (capacity < 0) return fail(SXQ_ERR_INVALID, "kv_reserve: capacity %d", capacity);
+    if (!add || !lens || !table || !free_list || !free_count || !cu || !status || (capacity > 0 && (!slots || !pos || !rows)))
+        return fail(SXQ_ERR_INVALID, "kv_reserve: null pointer");
+    DeviceGuard g(device);
+    HIP_TRY(g.err, "hipSetDevice");
+    KvReserve a;
+    a.shift = __builtin_ctz((unsigned)page_size);
+    a.n_pages = n_pages;
+    a.n_rows = n_rows;
+    a.max_blocks = max_blocks;
+    a.capacity = capacity;
+    a.table_stride = table_stride;
+    a.add = add;
+    a.lens = lens;
+    a.table = table;
+    a.free_list = free_list;
+    a.free_count = free_count;
+    a.cu = cu;
+    a.slots = slots;
+    a.pos = pos;
+    a.rows = rows;
+    a.status = status;
+    HIP_TRY(launch_kv_reserve(a, (hipStream_t)stream), "kv_reserve");
+    return SXQ_OK;
+}
+
+sxq_status sxq_kv_append(int device, const sxq_kv_pages* pages, int in_dtype, const void* qkv, int64_t row_stride,
+                         int n_tokens, int n_heads, const float* q_norm, const float* k_norm, float eps,
+                         const float* cos, const float* sin, int max_pos, int interleaved, const int32_t* pos,
+                         const int32_t* slots, void* q_out, void* stream) {
+    KvPool p;
+    if (sxq_status st = kv_pool("kv_append", pages, n_tokens > 0, &p)) return st;
+    if (!kv_dtype(in_dtype)) return fail(SXQ_ERR_DTYPE, "kv_append: qkv dtype %d (f32, f16 or bf16)", in_dtype);
+    if (n_tokens < 0 || n_heads < 1 || n_heads > 16384) return fail(SXQ_ERR_INVALID, "kv_append: %d tokens of %d heads", n_tokens, n_heads);
+    const int64_t width = ((int64_t)n_heads + 2 * p.nkv) * p.hd;
+    if (row_stride < width) return fail(SXQ_ERR_SHAPE, "kv_append: row_stride %lld below the row's %lld elements", (long long)row_stride, (long long)width);
+    if ((cos == nullptr) != (sin == nullptr) || (cos && max_pos < 1))
+        return fail(SXQ_ERR_INVALID, "kv_append: RoPE takes both tables and max_pos >= 1");
+    if (n_tokens == 0) return SXQ_OK;
+    if (!qkv || !slots || (cos && !pos)) return fail(SXQ_ERR_INVALID, "kv_append: null pointer");
+    DeviceGuard g(device);
+    HIP_TRY(g.err, "hipSetDevice");
+    KvAppend a;
+    a.qkv = qkv;
+    a.row_stride = row_stride;
+    a.dtype = in_dtype;
+    a.n_tokens = n_tokens;
+    a.nh = n_heads;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.eps = eps;
+    a.cos = cos;
+    a.sin = sin;
+    a.max_pos = max_pos;
+    a.interleaved = interleaved != 0;
+    a.pos = pos;
+    a.slots = slots;
+    a.q_out = q_out;
+    HIP_TRY(launch_kv_append(a, p, (hipStream_t)stream), "kv_append");
+    return SXQ_OK;
+}
+
+}  // extern "C"
