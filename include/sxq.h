@@ -211,8 +211,9 @@ typedef struct {
     int32_t page_size; /* positions per page: a power of two, 16..1024 */
     int32_t n_pages;   /* n_pages * page_size < 2^31 */
     void *k, *v;       /* the pools, 16-byte aligned, laid out alike: */
-    int64_t page_stride, head_stride, pos_stride; /* elements, multiples of 16 bytes; a head's row at one
-                                                     position is contiguous */
+    int64_t page_stride, head_stride, pos_stride; /* elements, multiples of 16 bytes, at least head_dim; a
+                                                     head's row at one position is contiguous; pos_stride
+                                                     at most 2^24 */
 } sxq_kv_pages;
 
 /* Block tables and slot maps from the requests' lengths.  Request r of n_rows holds lens[r]
@@ -260,7 +261,10 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
  * 16-byte aligned), q_dtype the pages' type, or SXQ_F32 over SXQ_BF16 pages; out has q's type.
  * Scores, softmax and sums are f32.  rows int32 [n_q]: the table row of each query (NULL: b);
  * a query whose row lies outside 0 .. n_rows - 1 leaves its out row as it was.  A request
- * without positions (or whose pages are all absent) gives zeros.
+ * without positions (or whose pages are all absent) gives zeros.  max_blocks * page_size at
+ * most 2^30.  What lies past a request's length, in its last page or elsewhere, may hold
+ * anything; a key or value of its own that is not finite makes the outputs that read it not
+ * finite.  Two calls on the same inputs give the same bits.
  * workspace (sxq_kv_attention_workspace bytes, 256-byte aligned) is zeroed by the caller
  * before its first use; every call leaves it ready for the next of the same or smaller
  * n_q * n_heads.  Calls that share one must not overlap. */

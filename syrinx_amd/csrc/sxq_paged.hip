@@ -263,6 +263,7 @@ sxq_status kv_pool(const char* who, const sxq_kv_pages* g, bool pointers, KvPool
         if (st < g->head_dim || st % unit || st > most)
             return fail(SXQ_ERR_SHAPE, "%s: page strides (%lld, %lld, %lld) must be multiples of %lld elements, at least head_dim",
                         who, (long long)g->page_stride, (long long)g->head_stride, (long long)g->pos_stride, (long long)unit);
+    if (g->pos_stride > 1 << 24) return fail(SXQ_ERR_SHAPE, "%s: pos_stride %lld above 2^24 elements", who, (long long)g->pos_stride);
     if (pointers && (!g->k || !g->v)) return fail(SXQ_ERR_INVALID, "%s: null page pool", who);
     if (((uintptr_t)g->k | (uintptr_t)g->v) & 15) return fail(SXQ_ERR_INVALID, "%s: the page pools must be 16-byte aligned", who);
     out->k = g->k;

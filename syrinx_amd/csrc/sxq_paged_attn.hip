@@ -6,75 +6,530 @@
 #include "sxq_abi.h"
 #include "sxq_paged.h"
 #include "sxq_paged_launch.h"
+#include "sxq_sync_dev.h"
 
 using namespace sxq;
 using namespace sxq::abi;
 
 namespace {
 
-// One workgroup per (query, head): 256 positions at a time, a thread per position for the
-// scores, then per element of the value for the weighted sum; running maximum and sum.
-template <typename TQ, typename TC>
-__global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPool P) {
-    __shared__ float sq[256], sp[256], red[8];
-    __shared__ int sid[256];
-    const int b = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, hd = P.hd;
-    const int r = A.rows ? A.rows[b] : b;
-    if (r < 0 || r >= A.n_rows) return;
-    const int len = kv_clamp_len(A.lens[r], A.max_blocks, P.shift), kh = h / (A.nh / P.nkv);
-    if (tid < hd) sq[tid] = to_f32(((const TQ*)A.q)[b * A.q_stride + (int64_t)h * hd + tid]);
-    const TC *kp = (const TC*)P.k, *vp = (const TC*)P.v;
-    float m = -INFINITY, l = 0.0f, acc = 0.0f;
-    __syncthreads();
-    for (int p0 = 0; p0 < len; p0 += 256) {
-        const int p = p0 + tid;
-        const int id = p < len ? A.table[r * A.table_stride + (p >> P.shift)] : -1;
-        const bool ok = kv_page_ok(id, P.n_pages);
-        float s = -INFINITY;
-        if (ok) {
-            const TC* k = kp + kv_page_base(P, id, kh) + (int64_t)(p & (P.page - 1)) * P.pos_stride;
-            s = 0.0f;
-            for (int d = 0; d < hd; ++d) s += sq[d] * to_f32(k[d]);
-            s *= A.scale;
-        }
-        float mx = s;
-        for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
-        if ((tid & 63) == 0) red[tid >> 6] = mx;
-        __syncthreads();
-        const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-        const float base = mn > -INFINITY ? mn : 0.0f;  // every score -inf or NaN so far
-        const float e = ok ? expf(s - base) : 0.0f;
-        float sum = e;
-        for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        sp[tid] = e;
-        sid[tid] = ok ? id : -1;
-        if ((tid & 63) == 0) red[4 + (tid >> 6)] = sum;
-        __syncthreads();
-        const float al = m > -INFINITY ? expf(m - base) : 1.0f;
-        l = l * al + (red[4] + red[5] + red[6] + red[7]);
-        acc *= al;
-        m = mn;
-        if (tid < hd)
-            for (int j = 0; j < 256; ++j)
-                if (sid[j] >= 0)
-                    acc += sp[j] * to_f32(vp[kv_page_base(P, sid[j], kh) + (int64_t)((p0 + j) & (P.page - 1)) * P.pos_stride + tid]);
-        __syncthreads();
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// ---- how the work is split ---------------------------------------------------------------
+// In units of 32 positions.  All queries' tiles together are cut into pieces of one length
+// for every query: the total over kvTarget(), at least kMinTiles, so that the grid's size
+// needs no length: a query gets ceil(tiles / piece) items, at most target + n_q in all.  Of
+// the queries with more than one item there are fewer than target, of their items fewer
+// than 2 * target: their partials and counters have places for so many.
+constexpr int kTile = 32;
+constexpr int kWaves = 4;
+constexpr int kMinTiles = 4;       // one tile a wave
+constexpr int kTargetGroups = 1024;
+constexpr int kCountBytes = 1 << 18;
+
+SXQ_HD int attend_head_tiles(int nh, int nkv) { return (nh / nkv + 15) / 16; }
+// A power of two (the pieces' length is then a shift).
+SXQ_HD int attend_target(int nh, int nkv) {
+    const int groups = nkv * attend_head_tiles(nh, nkv);
+    int t = 256;
+    while (t > 1 && t * groups > kTargetGroups) t >>= 1;
+    return t;
+}
+// A partial: {m, l} and the weighted sum of one head over one item.
+SXQ_HD size_t attend_part_floats(int hd) { return (size_t)hd + 4; }
+
+SXQ_DEV int tiles_of(int len) { return (len + kTile - 1) / kTile; }  // (of -1, no query: 0)
+
+struct Item {
+    int b, row, len;      // query, its table row, its positions
+    int first, tiles;     // this item's tiles of 32 positions
+    int index, count;     // which item of the query, of how many
+    int part0, slot;      // a split query's first partial and its counter
+};
+
+// Item x of the launch, found by every wave from the lengths: false if there is none.
+SXQ_DEV bool find_item(const KvAttend& A, const KvPool& P, int log_target, int x, Item& it) {
+    const int lane = threadIdx.x & 63;
+    auto load = [&](int b, int& row, int& len) {
+        row = b < A.n_q ? (A.rows ? A.rows[b] : b) : -1;
+        const bool live = (uint32_t)row < (uint32_t)A.n_rows;
+        len = live ? kv_clamp_len(A.lens[row], A.max_blocks, P.shift) : -1;
+    };
+    int row, len;
+    load(lane, row, len);
+    uint64_t total = (uint64_t)tiles_of(len);
+    for (int b0 = 64; b0 < A.n_q; b0 += 64) {
+        int r, n;
+        load(b0 + lane, r, n);
+        total += (uint64_t)tiles_of(n);
     }
-    if (tid < hd) ((TQ*)A.out)[b * A.out_stride + (int64_t)h * hd + tid] = from_f32<TQ>(l == 0.0f ? 0.0f : acc / l);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) total += (uint64_t)__shfl_xor((unsigned long long)total, o, 64);
+    int piece = (int)((total + (1u << log_target) - 1) >> log_target);
+    piece = max(kMinTiles, (piece + kWaves - 1) / kWaves * kWaves);
+    int items0 = 0, single0 = 0, split0 = 0;  // over the queries before this block of 64
+    for (int b0 = 0; b0 < A.n_q; b0 += 64) {
+        if (b0) load(b0 + lane, row, len);
+        const int tiles = tiles_of(len);
+        const int n = len < 0 ? 0 : max(1, (tiles + piece - 1) / piece);
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += u;
+        }
+        const uint64_t single = __ballot(n == 1), split = __ballot(n > 1);
+        const uint64_t mine = __ballot(x >= items0 + incl - n && x < items0 + incl);
+        if (mine) {
+            const int src = __builtin_ctzll(mine);
+            const uint64_t below = ((uint64_t)1 << src) - 1;
+            it.b = b0 + src;
+            it.row = __builtin_amdgcn_readlane(row, src);
+            it.len = __builtin_amdgcn_readlane(len, src);
+            it.count = __builtin_amdgcn_readlane(n, src);
+            const int start = items0 + __builtin_amdgcn_readlane(incl, src) - it.count;
+            it.index = x - start;
+            it.first = it.index * piece;
+            it.tiles = min(piece, tiles_of(it.len) - it.first);
+            it.part0 = start - single0 - __builtin_popcountll(single & below);
+            it.slot = split0 + __builtin_popcountll(split & below);
+            return true;
+        }
+        items0 += __builtin_amdgcn_readlane(incl, 63);
+        single0 += __builtin_popcountll(single);
+        split0 += __builtin_popcountll(split);
+    }
+    return false;
+}
+
+// ---- the matrix operands of each page type -----------------------------------------------
+// Scores: A = 16 keys x k head elements, B = the queries' k elements x 16 heads; the sum over
+// k may take the elements in any order, so lane (r = lane % 16, g = lane / 16) simply loads 16
+// bytes of key r.  A lane of the result holds head r of positions 4 g + i.  Weighted values:
+// A = 16 value columns x positions, B = the weights, positions x 16 heads, where again any
+// order of the positions does: the weights are used in the registers the scores came in, and
+// lane (r, g) loads VW columns of the rows 4 g + i.  16-bit values then want two positions in
+// a register where the load gave two columns: one byte permute per result register.
+// Result: head r, columns of r' = 4 g + i.
+template <typename T>
+struct PageOps;
+
+template <>
+struct PageOps<float> {
+    static constexpr int kHalves = 1;  // 16-position halves of a wave's tile
+    static constexpr int kWeightShift = 0;
+};
+template <>
+struct PageOps<__bf16> {
+    static constexpr int kHalves = 2;
+    static constexpr int kWeightShift = 0;
+    typedef v8bf V8;
+    static SXQ_DEV v4f mfma(V8 a, V8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct PageOps<_Float16> {
+    static constexpr int kHalves = 2;
+    // The weights times 2^13, numerator and denominator alike: the second f16 part of a weight
+    // is then exact down to 2^-38 of the largest (f16's smallest step, 2^-24, would lose the
+    // small weights of a long flat row).
+    static constexpr int kWeightShift = 13;
+    typedef v8h V8;
+    static SXQ_DEV v4f mfma(V8 a, V8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// Exchanges lanes 32..63 of a with lanes 0..31 of b; odd 16-lane rows of a with even ones of b.
+SXQ_DEV void swap32(float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+}
+SXQ_DEV void swap16(float& a, float& b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    a = __uint_as_float(r[0]);
+    b = __uint_as_float(r[1]);
+}
+// Over the four lanes of one head (lane % 16).
+SXQ_DEV float head_max(float v) {
+    float a = v, b = v;
+    swap32(a, b);
+    v = a = b = fmaxf(a, b);
+    swap16(a, b);
+    return fmaxf(a, b);
+}
+SXQ_DEV float head_sum(float v) {
+    float a = v, b = v;
+    swap32(a, b);
+    v = a + b;
+    a = b = v;
+    swap16(a, b);
+    return a + b;
+}
+SXQ_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename T, int HDP>
+struct Shape {
+    static constexpr int kVW = sizeof(T) == 4 ? 4 : HDP / 16 < 8 ? HDP / 16 : 8;  // value columns a load
+    static constexpr int kBlk = HDP / (16 * kVW);
+    static constexpr int kD = HDP / 16;       // result registers (x 4) of a lane
+    static constexpr int kKS = sizeof(T) == 4 ? HDP / 16 : HDP / 32;  // 16-byte key loads a lane and half
+    static constexpr int kH = PageOps<T>::kHalves;
+};
+
+// One head of one item, {m, l} and the sum: m is the maximum of scale * log2(e) * score (or
+// 0 where none is above -inf), l and the sum carry the weights 2^(x - m + kWeightShift).
+template <typename TQ, typename T, int HDP, bool FULL>
+__global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPool P, int log_target) {
+    typedef Shape<T, HDP> S;
+    typedef PageOps<T> O;
+    constexpr int H = S::kH, KS = S::kKS, VW = S::kVW, BLK = S::kBlk, D = S::kD;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int QP = F32 || sizeof(TQ) == 2 ? 1 : 3;  // 16-bit parts of a query element, exact together
+    constexpr int WP = F32 ? 1 : sizeof(TQ) == 2 ? 2 : 3;  // of a weight (rounded at 2^-18, or 2^-22, of itself)
+    __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+    __shared__ __attribute__((aligned(16))) float s_acc[kWaves][16][HDP + 4];
+    __shared__ bool s_last;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    Item it;
+    if (!find_item(A, P, log_target, blockIdx.x, it)) return;
+    const int hd = FULL ? HDP : P.hd, G = A.nh / P.nkv;
+    const int ht = attend_head_tiles(A.nh, P.nkv);
+    const int kh = blockIdx.y / ht, h0 = kh * G + (blockIdx.y - kh * ht) * 16;
+    const int heads = min(16, (kh + 1) * G - h0);
+
+    // the queries: B operands, in the element order of the key loads
+    const TQ* qrow = (const TQ*)A.q + (int64_t)it.b * A.q_stride + (int64_t)(h0 + min(r, heads - 1)) * hd;
+    uint32_t qreg[QP][KS][4];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const int col = (F32 ? 16 : 32) * s + (F32 ? 4 : 8) * g;
+        const bool in = FULL || col < hd;
+        const TQ* src = qrow + (in ? col : 0);
+        if constexpr (QP == 1) {
+            const v4u v = *(const v4u*)src;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qreg[0][s][e] = in ? v[e] : 0;
+        } else {
+            float f[8];
+            *(v4f*)f = *(const v4f*)src;
+            *(v4f*)(f + 4) = *(const v4f*)(src + 4);
+#pragma unroll
+            for (int q = 0; q < QP; ++q) {
+                v8bf part;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    part[e] = (__bf16)(in ? f[e] : 0.0f);
+                    f[e] -= (float)part[e];
+                }
+                const v4u u = __builtin_bit_cast(v4u, part);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) qreg[q][s][e] = u[e];
+            }
+        }
+    }
+
+    // where this lane reads within a half tile's 16 positions (bytes)
+    const int ps = (int)P.pos_stride * (int)sizeof(T);
+    const uint32_t kcol = (F32 ? 4 : 8) * g * (int)sizeof(T), vcol = VW * r * (int)sizeof(T);
+    const uint32_t koff = (uint32_t)(r * ps), voff = (uint32_t)(4 * g * ps);
+    const int32_t* table = A.table + (int64_t)it.row * A.table_stride;
+    const int last_block = kv_blocks(it.len, P.shift) - 1;
+    const int t_end = (it.first + it.tiles) * (kTile / 16);  // in halves
+    // the page of half tile t (16 positions), or -1; only halves with a position are asked for
+    auto page_of = [&](int t) { return __builtin_amdgcn_readfirstlane(table[min(t >> (P.shift - 4), last_block)]); };
+
+    v4f acc[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) acc[d] = (v4f){0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.0f;
+    const float scale2 = A.scale * 1.44269504088896340736f;
+
+    uint32_t kreg[H][KS][4], vreg[H][4][BLK][VW * sizeof(T) / 4];
+    int id[H];
+    auto half_base = [&](const void* pool, int t, int page) {
+        const int safe = kv_page_ok(page, P.n_pages) ? page : 0;
+        return (const char*)pool + (kv_page_base(P, safe, kh) + (int64_t)((t * 16) & (P.page - 1)) * P.pos_stride) * (int64_t)sizeof(T);
+    };
+    auto load_k = [&](int t) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const char* base = half_base(P.k, t + h, id[h]);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const uint32_t col = (uint32_t)(64 * s) + kcol;  // 16 f32 or 32 16-bit elements a step
+                const bool in = FULL || col < (uint32_t)hd * sizeof(T);
+                const v4u v = *(const v4u*)(base + (koff + (in ? col : 0)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kreg[h][s][e] = v[e];
+            }
+        }
+    };
+    auto load_v = [&](int t) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const char* base = half_base(P.v, t + h, id[h]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int b = 0; b < BLK; ++b) {
+                    const uint32_t col = (uint32_t)(b * 16 * VW * (int)sizeof(T)) + vcol;
+                    const bool in = FULL || col < (uint32_t)hd * sizeof(T);
+                    const char* src = base + (int64_t)i * ps + (voff + (in ? col : 0));
+                    if constexpr (VW * sizeof(T) == 16) {
+                        const v4u v = *(const v4u*)src;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) vreg[h][i][b][e] = v[e];
+                    } else {
+                        const v2u v = *(const v2u*)src;
+                        vreg[h][i][b][0] = v[0];
+                        vreg[h][i][b][1] = v[1];
+                    }
+                }
+        }
+    };
+
+    // wave w takes the item's tiles w, w + 4, ...
+    int t = it.first * (kTile / 16) + wave * H;
+    const int t_last = (it.len + 15) / 16 - 1;  // the last half with a position
+    auto ids = [&](int t) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) id[h] = t + h <= t_last ? page_of(t + h) : -1;
+    };
+    if (t < t_end && t <= t_last) {
+        ids(t);
+        load_k(t);
+        load_v(t);
+    }
+    while (t < t_end && t <= t_last) {
+        const int next = t + kWaves * H;
+        const bool more = next < t_end && next <= t_last;
+        // scores
+        float x[H][4];
+        int okh[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            okh[h] = kv_page_ok(id[h], P.n_pages);
+            v4f c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if constexpr (!FULL) {
+                    const bool in = (uint32_t)(64 * s) + kcol < (uint32_t)hd * sizeof(T);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) kreg[h][s][e] = in ? kreg[h][s][e] : 0;
+                }
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kreg[h][s][e]),
+                                                                 __uint_as_float(qreg[0][s][e]), c, 0, 0, 0);
+                } else {
+                    const v4u kk = {kreg[h][s][0], kreg[h][s][1], kreg[h][s][2], kreg[h][s][3]};
+#pragma unroll
+                    for (int q = QP - 1; q >= 0; --q) {  // the small parts first
+                        const v4u qq = {qreg[q][s][0], qreg[q][s][1], qreg[q][s][2], qreg[q][s][3]};
+                        c = O::mfma(__builtin_bit_cast(typename O::V8, kk), __builtin_bit_cast(typename O::V8, qq), c);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[h][i] = c[i] * scale2;
+        }
+        const bool cut = (t + H) * 16 > it.len;  // some position lies past the end
+        bool absent = false;
+#pragma unroll
+        for (int h = 0; h < H; ++h) absent |= !okh[h];
+        const bool partial = cut || absent;
+        if (partial)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!okh[h] || (t + h) * 16 + 4 * g + i >= it.len) x[h][i] = -INFINITY;
+        if (more) {
+            ids(next);
+            load_k(next);
+        }
+        // the running maximum moves only where a score passes it
+        float mx = x[0][0];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[h][i]);
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, head_max(mx));
+            const float al = m > -INFINITY ? exp2_fast(m - mn) : 1.0f;  // nothing but zeros before
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < D; ++d) acc[d] *= al;
+            m = mn;
+        }
+        const float base = (m > -INFINITY ? m : 0.0f) - (float)O::kWeightShift;
+        float w[H][4];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[h][i] = exp2_fast(x[h][i] - base);
+                l += w[h][i];
+            }
+        // values that no weight belongs to may hold anything: zeros in their place
+        if (partial)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = okh[h] && (t + h) * 16 + 4 * g + i < it.len;
+#pragma unroll
+                    for (int b = 0; b < BLK; ++b)
+#pragma unroll
+                        for (int e = 0; e < (int)(VW * sizeof(T) / 4); ++e) vreg[h][i][b][e] = in ? vreg[h][i][b][e] : 0;
+                }
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int b = 0; b < BLK; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[4 * b + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vreg[0][i][b][e]), w[0][i],
+                                                                              acc[4 * b + e], 0, 0, 0);
+        } else {
+            typename O::V8 part[WP];
+#pragma unroll
+            for (int p = 0; p < WP; ++p)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    part[p][j] = (T)w[j >> 2][j & 3];
+                    w[j >> 2][j & 3] -= (float)part[p][j];
+                }
+#pragma unroll
+            for (int b = 0; b < BLK; ++b)
+#pragma unroll
+                for (int e = 0; e < VW; ++e) {
+                    v4u a;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)  // positions 2 j and 2 j + 1 of the lane's eight
+                        a[j] = __builtin_amdgcn_perm(vreg[j >> 1][2 * (j & 1) + 1][b][e / 2], vreg[j >> 1][2 * (j & 1)][b][e / 2],
+                                                     e & 1 ? 0x07060302 : 0x05040100);
+#pragma unroll
+                    for (int p = WP - 1; p >= 0; --p)
+                        acc[b * VW + e] = O::mfma(__builtin_bit_cast(typename O::V8, a), part[p], acc[b * VW + e]);
+                }
+        }
+        if (more) load_v(next);
+        t = next;
+    }
+    l = head_sum(l);
+
+    // the four waves' sums
+    if (g == 0) {
+        s_m[wave][r] = m;
+        s_l[wave][r] = l;
+    }
+    __syncthreads();
+    float M = s_m[0][r];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, s_m[w][r]);
+    {
+        const float f = m > -INFINITY ? exp2_fast(m - M) : 1.0f;  // (no weights, or NaN: as they are)
+#pragma unroll
+        for (int b = 0; b < BLK; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < VW; ++e)
+                    s_acc[wave][r][b * 16 * VW + (4 * g + i) * VW + e] = acc[b * VW + e][i] * f;
+    }
+    __syncthreads();
+    const int n_out = heads * (hd / 4);
+    float* parts = (float*)((char*)A.ws + kCountBytes);
+    const size_t pf = attend_part_floats(hd);
+    const bool split = it.count > 1;
+    for (int o = tid; o < n_out; o += 256) {
+        const int h = o / (hd / 4), c = 4 * (o - h * (hd / 4));
+        float Mh = s_m[0][h], L = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) Mh = fmaxf(Mh, s_m[w][h]);
+        v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float mw = s_m[w][h];
+            L += s_l[w][h] * (mw > -INFINITY ? exp2_fast(mw - Mh) : 1.0f);
+            v += *(const v4f*)&s_acc[w][h][c];
+        }
+        if (!split) {
+            TQ* dst = (TQ*)A.out + (int64_t)it.b * A.out_stride + (int64_t)(h0 + h) * hd + c;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dst[e] = from_f32<TQ>(L == 0.0f ? 0.0f : v[e] / L);
+        } else {
+            float* dst = parts + ((size_t)(it.part0 + it.index) * A.nh + h0 + h) * pf;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store_agent(dst + 4 + c + e, v[e]);
+            if (c == 0) {
+                store_agent(dst, Mh);
+                store_agent(dst + 1, L);
+            }
+        }
+    }
+    if (!split) return;
+    // the last of the query's items to arrive joins them, in their order
+    unsigned* counter = (unsigned*)A.ws + ((size_t)it.slot * gridDim.y + blockIdx.y) * 16;
+    if (!publish_and_count(counter, it.count, &s_last)) return;
+    if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int o = tid; o < n_out; o += 256) {
+        const int h = o / (hd / 4), c = 4 * (o - h * (hd / 4));
+        const float* src = parts + ((size_t)it.part0 * A.nh + h0 + h) * pf;
+        const size_t step = (size_t)A.nh * pf;
+        float Mh = -INFINITY;
+        for (int i = 0; i < it.count; ++i) Mh = fmaxf(Mh, load_agent(src + i * step));
+        float L = 0.0f;
+        v4f v = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < it.count; ++i) {
+            const float* s = src + i * step;
+            const float mi = load_agent(s), f = mi > -INFINITY ? exp2_fast(mi - Mh) : 1.0f;
+            L += load_agent(s + 1) * f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += load_agent(s + 4 + c + e) * f;
+        }
+        TQ* dst = (TQ*)A.out + (int64_t)it.b * A.out_stride + (int64_t)(h0 + h) * hd + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dst[e] = from_f32<TQ>(L == 0.0f ? 0.0f : v[e] / L);
+    }
+}
+
+template <typename TQ, typename T>
+void attend_by_width(const KvAttend& a, const KvPool& p, dim3 grid, int log_target, hipStream_t s) {
+#define SXQ_AT(HDP, FULL) hipLaunchKernelGGL((k_kv_attend<TQ, T, HDP, FULL>), grid, dim3(256), 0, s, a, p, log_target)
+    if (p.hd == 64) SXQ_AT(64, true);
+    else if (p.hd == 128) SXQ_AT(128, true);
+    else if (p.hd == 256) SXQ_AT(256, true);
+    else if (p.hd < 64) SXQ_AT(64, false);
+    else if (p.hd < 128) SXQ_AT(128, false);
+    else SXQ_AT(256, false);
+#undef SXQ_AT
 }
 
 }  // namespace
 
 namespace sxq {
 
-size_t kv_attend_workspace(const KvPool& p, int n_q, int nh) { return 256; }
+size_t kv_attend_workspace(const KvPool& p, int n_q, int nh) {
+    return kCountBytes + 2 * (size_t)attend_target(nh, p.nkv) * nh * attend_part_floats(p.hd) * sizeof(float);
+}
 
 hipError_t launch_kv_attend(const KvAttend& a, const KvPool& p, hipStream_t s) {
-    const dim3 grid(a.n_q, a.nh);
-    if (p.dtype == kF32) hipLaunchKernelGGL((k_kv_attend<float, float>), grid, dim3(256), 0, s, a, p);
-    else if (p.dtype == kF16) hipLaunchKernelGGL((k_kv_attend<_Float16, _Float16>), grid, dim3(256), 0, s, a, p);
-    else if (a.q_dtype == kF32) hipLaunchKernelGGL((k_kv_attend<float, __bf16>), grid, dim3(256), 0, s, a, p);
-    else hipLaunchKernelGGL((k_kv_attend<__bf16, __bf16>), grid, dim3(256), 0, s, a, p);
+    const int target = attend_target(a.nh, p.nkv);
+    const dim3 grid(target + a.n_q, p.nkv * attend_head_tiles(a.nh, p.nkv));
+    const int lt = __builtin_ctz((unsigned)target);
+    if (p.dtype == kF32) attend_by_width<float, float>(a, p, grid, lt, s);
+    else if (p.dtype == kF16) attend_by_width<_Float16, _Float16>(a, p, grid, lt, s);
+    else if (a.q_dtype == kF32) attend_by_width<float, __bf16>(a, p, grid, lt, s);
+    else attend_by_width<__bf16, __bf16>(a, p, grid, lt, s);
     return hipGetLastError();
 }
 
@@ -106,7 +561,7 @@ sxq_status sxq_kv_attention(int device, const sxq_kv_pages* pages, int q_dtype, 
     if (q_stride < width || out_stride < width || q_stride % unit || out_stride % unit)
         return fail(SXQ_ERR_SHAPE, "kv_attention: q_stride %lld, out_stride %lld (multiples of %lld elements, rows of %lld)",
                     (long long)q_stride, (long long)out_stride, (long long)unit, (long long)width);
-    if (n_rows < 1 || max_blocks < 1 || table_stride < max_blocks || (int64_t)max_blocks * p.page > 0x7FFFFFFF)
+    if (n_rows < 1 || max_blocks < 1 || table_stride < max_blocks || (int64_t)max_blocks * p.page > 1 << 30)
         return fail(SXQ_ERR_INVALID, "kv_attention: a table of %d rows of %d blocks, stride %lld", n_rows, max_blocks, (long long)table_stride);
     if (!rows && n_q > n_rows) return fail(SXQ_ERR_SHAPE, "kv_attention: %d queries over %d table rows", n_q, n_rows);
     if (!(scale - scale == 0.0f)) return fail(SXQ_ERR_INVALID, "kv_attention: scale is not finite");

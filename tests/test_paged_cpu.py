@@ -39,6 +39,7 @@ BAD_PAGES = [
     (dict(strides=(4096, 1028, 64)), _lib.ERR_SHAPE, "strides"),
     (dict(strides=(-4096, 1024, 64)), _lib.ERR_SHAPE, "strides"),
     (dict(strides=(0, 1024, 64)), _lib.ERR_SHAPE, "strides"),
+    (dict(strides=(1 << 32, 1 << 30, 1 << 25)), _lib.ERR_SHAPE, "pos_stride"),
     (dict(k=None), _lib.ERR_INVALID, "null page pool"),
     (dict(v=264), _lib.ERR_INVALID, "16-byte"),
 ]
