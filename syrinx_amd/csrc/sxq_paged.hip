@@ -63,7 +63,7 @@ SXQ_DEV int owner(const int* first, int n, int j) {
 // the pages and tokens of a chunk are dealt over the threads, each finding its request in the
 // chunk's offsets.
 template <int NT>
-__global__ __launch_bounds__(NT) void k_kv_reserve(const KvReserve A) {
+__global__ __launch_bounds__(NT) void k_kv_reserve(const KvReserve A, bool inline_map) {
     __shared__ Pair red[NT / 64 + 1];
     __shared__ int s_first[NT], s_block[NT], s_tok[NT], s_old[NT];
     const int tid = threadIdx.x, n = A.n_rows, P = 1 << A.shift;
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const KvReserve A) {
                 A.free_list[avail - 1 - (given.pages + j)];
         }
         __syncthreads();  // the new table entries are read by the tokens' threads
-        for (int j = tid; j < total.tokens; j += NT) {
+        for (int j = tid; inline_map && j < total.tokens; j += NT) {
             const int i = owner(s_tok, rows, j);
             const int pos = s_old[i] + (j - s_tok[i]), t = given.tokens + j;
             A.slots[t] = kv_slot(A.table[(int64_t)(r0 + i) * A.table_stride + (pos >> A.shift)], pos, A.shift, A.n_pages);
@@ -155,73 +155,123 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const KvReserve A) {
         given = given + total;
         __syncthreads();
     }
-    for (int t = given.tokens + tid; t < A.capacity; t += NT) A.slots[t] = A.pos[t] = A.rows[t] = -1;
+    for (int t = given.tokens + tid; inline_map && t < A.capacity; t += NT) A.slots[t] = A.pos[t] = A.rows[t] = -1;
     if (tid == 0) A.free_count[0] = avail - given.pages;
 }
 
+// The map of many tokens, from the offsets, lengths and tables that k_kv_reserve left: a
+// workgroup finds the requests of its first and last token among all, each thread its own
+// between those two (prompts of hundreds of tokens: one step or two).
+constexpr int kMapTokens = 1024;
+__global__ __launch_bounds__(256) void k_kv_map(const KvReserve A) {
+    const int t0 = blockIdx.x * kMapTokens, total = A.cu[A.n_rows];
+    const int t_end = min(t0 + kMapTokens, total);
+    int lo = 0, n = 0;
+    if (t0 < total) {
+        lo = owner(A.cu, A.n_rows, t0);
+        n = owner(A.cu, A.n_rows, t_end - 1) + 1 - lo;
+    }
+    for (int t = t0 + threadIdx.x; t < min(t0 + kMapTokens, A.capacity); t += 256) {
+        int slot = -1, pos = -1, row = -1;
+        if (t < t_end) {
+            row = lo + owner(A.cu + lo, n, t);
+            pos = A.lens[row] - (A.cu[row + 1] - t);
+            slot = kv_slot(A.table[(int64_t)row * A.table_stride + (pos >> A.shift)], pos, A.shift, A.n_pages);
+        }
+        A.slots[t] = slot;
+        A.pos[t] = pos;
+        A.rows[t] = row;
+    }
+}
+
 // ---------------------------------------------------------------------------- append
-// One wave per (token, head) of the fused row: lane i holds pairs i and i + 64 of the head.
+// Four consecutive elements as f32, at any element's alignment, and back.
+template <typename T>
+SXQ_DEV void load4(const T* p, float* f) {
+    typedef T v4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    const v4 v = *(const v4*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = to_f32(v[e]);
+}
+template <typename T>
+SXQ_DEV void store4(T* p, const float* f) {
+    typedef T v4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    v4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(f[e]);
+    *(v4*)p = v;
+}
+
+// Eight elements of a head a lane -- four RoPE pairs, as two vectors of four: (8 j, 8 j + 4)
+// interleaved, (4 j, hd / 2 + 4 j) in halves -- so that a head takes hd / 8 lanes (rounded up
+// to a power of two, LH), a wave 64 / LH heads of one token, the norm's sum stays among
+// neighbouring lanes and no element changes lanes.
 template <typename TI, typename TC>
-__global__ __launch_bounds__(64) void k_kv_append(const KvAppend A, const KvPool P) {
-    const int t = blockIdx.x, hid = blockIdx.y, lane = threadIdx.x, hd = P.hd, half = hd / 2;
+__global__ __launch_bounds__(256) void k_kv_append(const KvAppend A, const KvPool P, int log_lh) {
+    const int t = blockIdx.x, hd = P.hd, half = hd / 2, lh = 1 << log_lh;
+    const int hid = blockIdx.y * (256 >> log_lh) + (threadIdx.x >> log_lh), j = threadIdx.x & (lh - 1);
+    const int heads = A.nh + 2 * P.nkv;
+    const bool live = hid < heads && 8 * j < hd;
     const int slot = A.slots[t];
     if (slot < 0 || slot >= P.n_pages << P.shift) return;
     const bool is_q = hid < A.nh, is_k = !is_q && hid < A.nh + P.nkv;
-    if (is_q && !A.q_out) return;
-    const TI* src = (const TI*)A.qkv + (int64_t)t * A.row_stride + (int64_t)hid * hd;
     const float* w = is_q ? A.q_norm : is_k ? A.k_norm : nullptr;
+    const int o1 = A.interleaved ? 8 * j : 4 * j, o2 = A.interleaved ? 8 * j + 4 : half + 4 * j;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (live) {
+        const TI* src = (const TI*)A.qkv + (int64_t)t * A.row_stride + (int64_t)hid * hd;
+        load4(src + o1, x);
+        load4(src + o2, x + 4);
+    }
+    float c[4], s[4];
     const bool rot = A.cos && (is_q || is_k);
-    const int p = min(max(A.pos[t], 0), A.max_pos - 1);
-    float a[2], b[2], ss = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int i = lane + 64 * j;
-        a[j] = b[j] = 0.0f;
-        if (i < half) {
-            a[j] = to_f32(src[A.interleaved ? 2 * i : i]);
-            b[j] = to_f32(src[A.interleaved ? 2 * i + 1 : i + half]);
-        }
-        ss += a[j] * a[j] + b[j] * b[j];
+    if (live && rot) {
+        const int p = min(max(A.pos[t], 0), A.max_pos - 1);
+        load4(A.cos + (int64_t)p * half + 4 * j, c);
+        load4(A.sin + (int64_t)p * half + 4 * j, s);
     }
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+    for (int o = lh >> 1; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+    if (!live || (is_q && !A.q_out)) return;
     if (w) {
+        const float inv = 1.0f / sqrtf(ss / (float)hd + A.eps);
+        float g[8];
+        load4(w + o1, g);
+        load4(w + o2, g + 4);
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * g[e];
     }
-    const float den = w ? sqrtf(ss / (float)hd + A.eps) : 1.0f;
-    const int kh = hid - A.nh - (is_k ? 0 : P.nkv);
-    TC* cd = (TC*)(is_k ? P.k : P.v) + (is_q ? 0 : kv_slot_base(P, slot, kh));
-    TI* qd = (TI*)A.q_out + ((int64_t)t * A.nh + hid) * hd;
+    if (rot) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int i = lane + 64 * j;
-        if (i >= half) break;
-        const int ia = A.interleaved ? 2 * i : i, ib = A.interleaved ? 2 * i + 1 : i + half;
-        float x = a[j], y = b[j];
-        if (w) {
-            x = x / den * w[ia];
-            y = y / den * w[ib];
+        for (int e = 0; e < 4; ++e) {  // pair e of the lane
+            float &a = A.interleaved ? x[2 * e] : x[e], &b = A.interleaved ? x[2 * e + 1] : x[4 + e];
+            const float u = a * c[e] - b * s[e];
+            b = b * c[e] + a * s[e];
+            a = u;
         }
-        if (rot) {
-            const float c = A.cos[(int64_t)p * half + i], s = A.sin[(int64_t)p * half + i];
-            const float u = x * c - y * s;
-            y = y * c + x * s;
-            x = u;
-        }
-        if (is_q) {
-            qd[ia] = from_f32<TI>(x);
-            qd[ib] = from_f32<TI>(y);
-        } else {
-            cd[ia] = from_f32<TC>(x);
-            cd[ib] = from_f32<TC>(y);
-        }
+    }
+    if (is_q) {
+        TI* dst = (TI*)A.q_out + ((int64_t)t * A.nh + hid) * hd;
+        store4(dst + o1, x);
+        store4(dst + o2, x + 4);
+    } else {
+        TC* dst = (TC*)(is_k ? P.k : P.v) + kv_slot_base(P, slot, hid - A.nh - (is_k ? 0 : P.nkv));
+        store4(dst + o1, x);
+        store4(dst + o2, x + 4);
     }
 }
 
 template <typename TI>
-void append_by_cache(const KvAppend& a, const KvPool& p, dim3 grid, hipStream_t s) {
-    if (p.dtype == kF32) hipLaunchKernelGGL((k_kv_append<TI, float>), grid, dim3(64), 0, s, a, p);
-    else if (p.dtype == kF16) hipLaunchKernelGGL((k_kv_append<TI, _Float16>), grid, dim3(64), 0, s, a, p);
-    else hipLaunchKernelGGL((k_kv_append<TI, __bf16>), grid, dim3(64), 0, s, a, p);
+void append_by_cache(const KvAppend& a, const KvPool& p, hipStream_t s) {
+    int log_lh = 0;
+    while (8 << log_lh < p.hd) ++log_lh;
+    const int per = 256 >> log_lh;  // heads a workgroup
+    const dim3 grid(a.n_tokens, (a.nh + 2 * p.nkv + per - 1) / per);
+    if (p.dtype == kF32) hipLaunchKernelGGL((k_kv_append<TI, float>), grid, dim3(256), 0, s, a, p, log_lh);
+    else if (p.dtype == kF16) hipLaunchKernelGGL((k_kv_append<TI, _Float16>), grid, dim3(256), 0, s, a, p, log_lh);
+    else hipLaunchKernelGGL((k_kv_append<TI, __bf16>), grid, dim3(256), 0, s, a, p, log_lh);
 }
 
 bool kv_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
@@ -232,16 +282,18 @@ bool pow2_page(int p) { return p >= 16 && p <= 1024 && (p & (p - 1)) == 0; }
 namespace sxq {
 
 hipError_t launch_kv_reserve(const KvReserve& a, hipStream_t s) {
-    if (a.n_rows <= 64) hipLaunchKernelGGL(k_kv_reserve<64>, dim3(1), dim3(64), 0, s, a);
-    else hipLaunchKernelGGL(k_kv_reserve<1024>, dim3(1), dim3(1024), 0, s, a);
+    const bool wave = a.n_rows <= 64, inline_map = a.capacity <= (wave ? 256 : 2048);
+    if (wave) hipLaunchKernelGGL(k_kv_reserve<64>, dim3(1), dim3(64), 0, s, a, inline_map);
+    else hipLaunchKernelGGL(k_kv_reserve<1024>, dim3(1), dim3(1024), 0, s, a, inline_map);
+    if (!inline_map)
+        hipLaunchKernelGGL(k_kv_map, dim3((a.capacity + kMapTokens - 1) / kMapTokens), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
 hipError_t launch_kv_append(const KvAppend& a, const KvPool& p, hipStream_t s) {
-    const dim3 grid(a.n_tokens, a.nh + 2 * p.nkv);
-    if (a.dtype == kF32) append_by_cache<float>(a, p, grid, s);
-    else if (a.dtype == kF16) append_by_cache<_Float16>(a, p, grid, s);
-    else append_by_cache<__bf16>(a, p, grid, s);
+    if (a.dtype == kF32) append_by_cache<float>(a, p, s);
+    else if (a.dtype == kF16) append_by_cache<_Float16>(a, p, s);
+    else append_by_cache<__bf16>(a, p, s);
     return hipGetLastError();
 }
 

@@ -70,7 +70,7 @@ class PagedKvCache:
         device = torch.device(device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
-        self.device, self.dtype = device, dtype
+        self.device, self.dtype, self._index = device, dtype, device.index
         self.n_layers, self.n_kv_heads, self.head_dim = int(n_layers), int(n_kv_heads), int(head_dim)
         self.n_pages, self.page_size = int(n_pages), int(page_size)
         self.max_rows, self.max_len = int(max_rows), int(max_len)
@@ -106,7 +106,8 @@ class PagedKvCache:
         return self._layer_refs[layer]
 
     def _want(self, what, t, dtype, numel=None):
-        if t.device != self.device or t.dtype != dtype or not t.is_contiguous() or (numel and t.numel() != numel):
+        if (t.dtype is not dtype or t.device != self.device or not t.is_contiguous()
+                or (numel is not None and t.numel() != numel)):
             size = f" of {numel} elements" if numel else ""
             raise ValueError(f"PagedKvCache: {what} must be a contiguous {dtype} tensor{size} on {self.device}, got "
                              f"{t.dtype} {tuple(t.shape)} on {t.device}")
@@ -145,10 +146,11 @@ class PagedKvCache:
                 if t is None or t.numel() != size:
                     raise ValueError(f"PagedKvCache.reserve: out.{name} must hold {size} elements")
                 self._want(f"out.{name}", t, torch.int32)
-        check(lib().sxq_kv_reserve(self.device.index, self.page_size, self.n_pages, self.max_rows, self.max_blocks,
-                                   _ptr(add), _ptr(self.lens), _ptr(self.table), self.table.stride(0), _ptr(self.free),
-                                   _ptr(self.free_count), cap, _ptr(out.cu), _ptr(out.slots), _ptr(out.pos),
-                                   _ptr(out.rows), _ptr(out.status), self._stream()))
+        check(lib().sxq_kv_reserve(self._index, self.page_size, self.n_pages, self.max_rows, self.max_blocks,
+                                   add.data_ptr(), self.lens.data_ptr(), self.table.data_ptr(), self.max_blocks,
+                                   self.free.data_ptr(), self.free_count.data_ptr(), cap, out.cu.data_ptr(),
+                                   out.slots.data_ptr(), out.pos.data_ptr(), out.rows.data_ptr(), out.status.data_ptr(),
+                                   self._stream()))
         return out
 
     # -- new tokens -----------------------------------------------------------------------
@@ -188,7 +190,7 @@ class PagedKvCache:
             out = torch.empty((tokens, n_heads * hd), dtype=qkv.dtype, device=self.device)
         else:
             self._want("out", out, qkv.dtype, tokens * n_heads * hd)
-        check(lib().sxq_kv_append(self.device.index, self._layer(layer), _DTYPES[qkv.dtype], _ptr(qkv), stride, tokens,
+        check(lib().sxq_kv_append(self._index, self._layer(layer), _DTYPES[qkv.dtype], _ptr(qkv), stride, tokens,
                                   n_heads, _ptr(q_norm), _ptr(k_norm), eps, _ptr(cos), _ptr(sin),
                                   cos.shape[0] if cos is not None else 0, int(bool(interleaved)), _ptr(slot_map.pos),
                                   _ptr(slot_map.slots), _ptr(out), self._stream()))
@@ -261,8 +263,8 @@ class PagedKvCache:
             workspace = self._kept_workspace(n, n_heads)
         else:
             self._want("workspace", workspace, torch.uint8)
-        check(lib().sxq_kv_attention(self.device.index, self._layer(layer), _DTYPES[q.dtype], _ptr(q), q_stride, n,
+        check(lib().sxq_kv_attention(self._index, self._layer(layer), _DTYPES[q.dtype], _ptr(q), q_stride, n,
                                      n_heads, _ptr(rows), _ptr(self.lens), self.max_rows, _ptr(self.table),
-                                     self.table.stride(0), self.max_blocks, scale, _ptr(out), out_stride,
+                                     self.max_blocks, self.max_blocks, scale, _ptr(out), out_stride,
                                      _ptr(workspace), workspace.numel(), self._stream()))
         return out
