@@ -2,6 +2,8 @@
 // (sxq_kv_attention; include/sxq.h states it).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/sxq.h"
 #include "sxq_abi.h"
 #include "sxq_paged.h"
@@ -20,68 +22,92 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
 // ---- how the work is split ---------------------------------------------------------------
-// In units of 32 positions.  All queries' tiles together are cut into pieces of one length
-// for every query: the total over kvTarget(), at least kMinTiles, so that the grid's size
-// needs no length: a query gets ceil(tiles / piece) items, at most target + n_q in all.  Of
-// the queries with more than one item there are fewer than target, of their items fewer
-// than 2 * target: their partials and counters have places for so many.
+// Per KV head and 16 of its query heads, a query's tiles of 32 positions are cut evenly into
+// items of at most `piece` tiles, one a workgroup, where piece is the total of all queries'
+// tiles over attend_target(): the grid, target + n_q, needs no length, and ragged queries
+// weigh on the card by their lengths.  Fewer than target queries have more than one item, and
+// fewer than 2 * target items belong to those: so many partials and counters have a place.
+// The last of a query's items to finish joins them.
+// (One equal share of the line of all tiles a workgroup, whole queries and the ends of two,
+// measured: 64 queries of 1000..16384 positions 259 us against 264; 16 of 256..2040, where a
+// workgroup's second query waits for the end of its first, 32 against 20.)
 constexpr int kTile = 32;
 constexpr int kWaves = 4;
-constexpr int kMinTiles = 4;       // one tile a wave
-constexpr int kTargetGroups = 1024;
-constexpr int kCountBytes = 1 << 18;
+constexpr int kMinTiles = 4;    // of an item: one a wave
+constexpr int kMaxItems = 256;  // of one query
+constexpr int kCountBytes = 1 << 18;  // 64 bytes a split query, KV head and 16 heads
 
 SXQ_HD int attend_head_tiles(int nh, int nkv) { return (nh / nkv + 15) / 16; }
-// A power of two (the pieces' length is then a shift).
-SXQ_HD int attend_target(int nh, int nkv) {
-    const int groups = nkv * attend_head_tiles(nh, nkv);
-    int t = 256;
-    while (t > 1 && t * groups > kTargetGroups) t >>= 1;
-    return t;
+// Workgroups per KV head and 16 query heads that the card holds at once (four a CU at head
+// widths up to 64, two up to 128, one above, by their registers).
+inline int attend_slots(int nh, int nkv, int hd) {
+    const int all = hd <= 64 ? 1024 : hd <= 128 ? 512 : 256;
+    return std::max(1, all / (nkv * attend_head_tiles(nh, nkv)));
 }
-// A partial: {m, l} and the weighted sum of one head over one item.
+// Few queries: all items (fewer than target + n_q) resident at once, no second round for a few.
+// Many: smaller items, dealt as workgroups finish.  Measured at 32 / 8 heads of 128, 64 slots
+// (us): 16 queries of 256..2040 positions by 48 / 64 / 256 pieces 19.5 / 21.0 / 27.9; one of
+// 131071 by 64 / 128 / 256 104 / 114 / 122; 64 of 1000..16384 by 64 / 128 / 256 306 / 271 / 267.
+inline int attend_target(int n_q, int nh, int nkv, int hd) {
+    const int slots = attend_slots(nh, nkv, hd);
+    return std::min(kMaxItems, std::max(1, n_q <= slots / 2 ? slots - n_q + 1 : 4 * slots));
+}
+// The most of any number of queries.
+inline int attend_target_max(int nh, int nkv, int hd) { return std::min(kMaxItems, 4 * attend_slots(nh, nkv, hd)); }
+// A partial: {m, l} and the weighted sum of one head.
 SXQ_HD size_t attend_part_floats(int hd) { return (size_t)hd + 4; }
 
 SXQ_DEV int tiles_of(int len) { return (len + kTile - 1) / kTile; }  // (of -1, no query: 0)
 
+// Inclusive sum over the wave (row shifts, then the rows' last lanes broadcast onwards).
+SXQ_DEV int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+
+// Lane l's query of the block of 64 from b0: its table row and length (-1: none).
+SXQ_DEV void load_query(const KvAttend& A, const KvPool& P, int b0, int& row, int& len) {
+    const int b = b0 + (threadIdx.x & 63);
+    len = A.lens[min(b, A.n_rows - 1)];  // a guess in flight with the row, which most often is b
+    row = b < A.n_q ? (A.rows ? A.rows[b] : b) : -1;
+    const bool live = (uint32_t)row < (uint32_t)A.n_rows;
+    if (live && row != b) len = A.lens[row];
+    len = live ? kv_clamp_len(len, A.max_blocks, P.shift) : -1;
+}
+
 struct Item {
-    int b, row, len;      // query, its table row, its positions
-    int first, tiles;     // this item's tiles of 32 positions
-    int index, count;     // which item of the query, of how many
-    int part0, slot;      // a split query's first partial and its counter
+    int b, row, len;   // query, its table row, its positions
+    int first, tiles;  // this item's tiles of 32 positions
+    int index, count;  // which item of the query, of how many
+    int part0, slot;   // a split query's first partial and its counter
 };
 
 // Item x of the launch, found by every wave from the lengths: false if there is none.
-SXQ_DEV bool find_item(const KvAttend& A, const KvPool& P, int log_target, int x, Item& it) {
-    const int lane = threadIdx.x & 63;
-    auto load = [&](int b, int& row, int& len) {
-        row = b < A.n_q ? (A.rows ? A.rows[b] : b) : -1;
-        const bool live = (uint32_t)row < (uint32_t)A.n_rows;
-        len = live ? kv_clamp_len(A.lens[row], A.max_blocks, P.shift) : -1;
-    };
+SXQ_DEV bool find_item(const KvAttend& A, const KvPool& P, int target, int x, Item& it) {
     int row, len;
-    load(lane, row, len);
-    uint64_t total = (uint64_t)tiles_of(len);
+    load_query(A, P, 0, row, len);
+    int total = __builtin_amdgcn_readlane(wave_scan(tiles_of(len)), 63);
     for (int b0 = 64; b0 < A.n_q; b0 += 64) {
         int r, n;
-        load(b0 + lane, r, n);
-        total += (uint64_t)tiles_of(n);
+        load_query(A, P, b0, r, n);
+        total += __builtin_amdgcn_readlane(wave_scan(tiles_of(n)), 63);
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) total += (uint64_t)__shfl_xor((unsigned long long)total, o, 64);
-    int piece = (int)((total + (1u << log_target) - 1) >> log_target);
-    piece = max(kMinTiles, (piece + kWaves - 1) / kWaves * kWaves);
+    const int piece = max(kMinTiles, (total + target - 1) / target);
     int items0 = 0, single0 = 0, split0 = 0;  // over the queries before this block of 64
     for (int b0 = 0; b0 < A.n_q; b0 += 64) {
-        if (b0) load(b0 + lane, row, len);
+        if (b0) load_query(A, P, b0, row, len);
         const int tiles = tiles_of(len);
-        const int n = len < 0 ? 0 : max(1, (tiles + piece - 1) / piece);
-        int incl = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(incl, o, 64);
-            if (lane >= o) incl += u;
-        }
+        // an even cut: the fewest items of at most piece tiles (short ones: as many for each wave)
+        int n = max(1, (tiles + piece - 1) / piece);
+        int per = (tiles + n - 1) / n;
+        if (per <= 4 * kWaves) per = (per + kWaves - 1) / kWaves * kWaves;
+        n = len < 0 ? 0 : max(1, per ? (tiles + per - 1) / per : 1);
+        const int incl = wave_scan(n);
         const uint64_t single = __ballot(n == 1), split = __ballot(n > 1);
         const uint64_t mine = __ballot(x >= items0 + incl - n && x < items0 + incl);
         if (mine) {
@@ -92,9 +118,10 @@ SXQ_DEV bool find_item(const KvAttend& A, const KvPool& P, int log_target, int x
             it.len = __builtin_amdgcn_readlane(len, src);
             it.count = __builtin_amdgcn_readlane(n, src);
             const int start = items0 + __builtin_amdgcn_readlane(incl, src) - it.count;
+            const int mine_per = __builtin_amdgcn_readlane(per, src);
             it.index = x - start;
-            it.first = it.index * piece;
-            it.tiles = min(piece, tiles_of(it.len) - it.first);
+            it.first = it.index * mine_per;
+            it.tiles = min(mine_per, tiles_of(it.len) - it.first);
             it.part0 = start - single0 - __builtin_popcountll(single & below);
             it.slot = split0 + __builtin_popcountll(split & below);
             return true;
@@ -170,6 +197,16 @@ SXQ_DEV float head_sum(float v) {
 }
 SXQ_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// Four columns of an output row: the weighted sum over the weights' sum, zeros without any.
+template <typename TQ>
+SXQ_DEV void store_out(const KvAttend& A, int b, int64_t at, v4f v, float l, TQ*) {
+    typedef TQ v4 __attribute__((ext_vector_type(4)));
+    v4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = from_f32<TQ>(l == 0.0f ? 0.0f : v[e] / l);
+    *(v4*)((TQ*)A.out + (int64_t)b * A.out_stride + at) = o;
+}
+
 template <typename T, int HDP>
 struct Shape {
     static constexpr int kVW = sizeof(T) == 4 ? 4 : HDP / 16 < 8 ? HDP / 16 : 8;  // value columns a load
@@ -182,7 +219,7 @@ struct Shape {
 // One head of one item, {m, l} and the sum: m is the maximum of scale * log2(e) * score (or
 // 0 where none is above -inf), l and the sum carry the weights 2^(x - m + kWeightShift).
 template <typename TQ, typename T, int HDP, bool FULL>
-__global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPool P, int log_target) {
+__global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPool P, int target) {
     typedef Shape<T, HDP> S;
     typedef PageOps<T> O;
     constexpr int H = S::kH, KS = S::kKS, VW = S::kVW, BLK = S::kBlk, D = S::kD;
@@ -191,16 +228,23 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
     constexpr int WP = F32 ? 1 : sizeof(TQ) == 2 ? 2 : 3;  // of a weight (rounded at 2^-18, or 2^-22, of itself)
     __shared__ float s_m[kWaves][16], s_l[kWaves][16];
     __shared__ __attribute__((aligned(16))) float s_acc[kWaves][16][HDP + 4];
+    __shared__ v4f s_red[256];
     __shared__ bool s_last;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 15, g = lane >> 4;
-    Item it;
-    if (!find_item(A, P, log_target, blockIdx.x, it)) return;
     const int hd = FULL ? HDP : P.hd, G = A.nh / P.nkv;
     const int ht = attend_head_tiles(A.nh, P.nkv);
     const int kh = blockIdx.y / ht, h0 = kh * G + (blockIdx.y - kh * ht) * 16;
     const int heads = min(16, (kh + 1) * G - h0);
+    const float scale2 = A.scale * 1.44269504088896340736f;
+    // where this lane reads within a half tile's 16 positions (bytes)
+    const int ps = (int)P.pos_stride * (int)sizeof(T);
+    const uint32_t kcol = (F32 ? 4 : 8) * g * (int)sizeof(T), vcol = VW * r * (int)sizeof(T);
+    const uint32_t koff = (uint32_t)(r * ps), voff = (uint32_t)(4 * g * ps);
+
+    Item it;
+    if (!find_item(A, P, target, blockIdx.x, it)) return;
 
     // the queries: B operands, in the element order of the key loads
     const TQ* qrow = (const TQ*)A.q + (int64_t)it.b * A.q_stride + (int64_t)(h0 + min(r, heads - 1)) * hd;
@@ -233,27 +277,30 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
         }
     }
 
-    // where this lane reads within a half tile's 16 positions (bytes)
-    const int ps = (int)P.pos_stride * (int)sizeof(T);
-    const uint32_t kcol = (F32 ? 4 : 8) * g * (int)sizeof(T), vcol = VW * r * (int)sizeof(T);
-    const uint32_t koff = (uint32_t)(r * ps), voff = (uint32_t)(4 * g * ps);
     const int32_t* table = A.table + (int64_t)it.row * A.table_stride;
-    const int last_block = kv_blocks(it.len, P.shift) - 1;
-    const int t_end = (it.first + it.tiles) * (kTile / 16);  // in halves
-    // the page of half tile t (16 positions), or -1; only halves with a position are asked for
-    auto page_of = [&](int t) { return __builtin_amdgcn_readfirstlane(table[min(t >> (P.shift - 4), last_block)]); };
+    const int t_last = (it.len + 15) / 16 - 1;  // the last half tile (16 positions) with a position
+    const int t_end = min((it.first + it.tiles) * (kTile / 16), t_last + 1);
+    // Wave w takes the tiles w, w + 4, ... of the segment.  Lane j holds the page of the wave's
+    // half tile j of a batch of 64 (-1: absent), so that a tile's addresses wait for no load;
+    // the next batch is loaded when one begins.
+    const int t0 = it.first * (kTile / 16) + wave * H, log_p = P.shift - 4;
+    auto page_batch = [&](int batch) {
+        const int t = t0 + (batch * 64 + lane) / H * (kWaves * H) + (lane & (H - 1));
+        int id = -1;
+        if (t < t_end) id = table[t >> log_p];
+        return kv_page_ok(id, P.n_pages) ? id : -1;
+    };
+    int pages = page_batch(0), pages_next = -1;
 
     v4f acc[D];
 #pragma unroll
     for (int d = 0; d < D; ++d) acc[d] = (v4f){0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
-    const float scale2 = A.scale * 1.44269504088896340736f;
 
     uint32_t kreg[H][KS][4], vreg[H][4][BLK][VW * sizeof(T) / 4];
     int id[H];
     auto half_base = [&](const void* pool, int t, int page) {
-        const int safe = kv_page_ok(page, P.n_pages) ? page : 0;
-        return (const char*)pool + (kv_page_base(P, safe, kh) + (int64_t)((t * 16) & (P.page - 1)) * P.pos_stride) * (int64_t)sizeof(T);
+        return (const char*)pool + (kv_page_base(P, max(page, 0), kh) + (int64_t)((t * 16) & (P.page - 1)) * P.pos_stride) * (int64_t)sizeof(T);
     };
     auto load_k = [&](int t) {
 #pragma unroll
@@ -293,27 +340,27 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
         }
     };
 
-    // wave w takes the item's tiles w, w + 4, ...
-    int t = it.first * (kTile / 16) + wave * H;
-    const int t_last = (it.len + 15) / 16 - 1;  // the last half with a position
-    auto ids = [&](int t) {
+    int t = t0, k = 0;  // the tile's first half, its number in the batch
+    auto ids = [&]() {
 #pragma unroll
-        for (int h = 0; h < H; ++h) id[h] = t + h <= t_last ? page_of(t + h) : -1;
+        for (int h = 0; h < H; ++h) id[h] = __builtin_amdgcn_readlane(pages, k * H + h);
     };
-    if (t < t_end && t <= t_last) {
-        ids(t);
+    if (t < t_end) {
+        ids();
         load_k(t);
         load_v(t);
+        if (t + 64 / H * (kWaves * H) < t_end) pages_next = page_batch(1);
     }
-    while (t < t_end && t <= t_last) {
+    int batch = 1;
+    while (t < t_end) {
         const int next = t + kWaves * H;
-        const bool more = next < t_end && next <= t_last;
+        const bool more = next < t_end;
         // scores
         float x[H][4];
         int okh[H];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-            okh[h] = kv_page_ok(id[h], P.n_pages);
+            okh[h] = id[h] >= 0;
             v4f c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -351,7 +398,12 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
                 for (int i = 0; i < 4; ++i)
                     if (!okh[h] || (t + h) * 16 + 4 * g + i >= it.len) x[h][i] = -INFINITY;
         if (more) {
-            ids(next);
+            if (++k == 64 / H) {
+                k = 0;
+                pages = pages_next;
+                pages_next = page_batch(++batch);
+            }
+            ids();
             load_k(next);
         }
         // the running maximum moves only where a score passes it
@@ -446,12 +498,14 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
                     s_acc[wave][r][b * 16 * VW + (4 * g + i) * VW + e] = acc[b * VW + e][i] * f;
     }
     __syncthreads();
-    const int n_out = heads * (hd / 4);
-    float* parts = (float*)((char*)A.ws + kCountBytes);
-    const size_t pf = attend_part_floats(hd);
+    const int per = hd / 4, n_out = heads * per;  // four columns a thread
+    const size_t pf = attend_part_floats(hd), step = (size_t)A.nh * pf;  // a partial's floats; from slot to slot
+    float* parts = (float*)((char*)A.ws + kCountBytes) + (size_t)h0 * pf;
     const bool split = it.count > 1;
+    const __amdgpu_buffer_rsrc_t mine =
+        coherent_rsrc(parts + (it.part0 + it.index) * step, (uint32_t)(heads * pf * sizeof(float)));
     for (int o = tid; o < n_out; o += 256) {
-        const int h = o / (hd / 4), c = 4 * (o - h * (hd / 4));
+        const int h = o / per, c = 4 * (o - h * per);
         float Mh = s_m[0][h], L = 0.0f;
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) Mh = fmaxf(Mh, s_m[w][h]);
@@ -463,48 +517,94 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
             v += *(const v4f*)&s_acc[w][h][c];
         }
         if (!split) {
-            TQ* dst = (TQ*)A.out + (int64_t)it.b * A.out_stride + (int64_t)(h0 + h) * hd + c;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) dst[e] = from_f32<TQ>(L == 0.0f ? 0.0f : v[e] / L);
+            store_out(A, it.b, (h0 + h) * hd + c, v, L, (TQ*)nullptr);
         } else {
-            float* dst = parts + ((size_t)(it.part0 + it.index) * A.nh + h0 + h) * pf;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) store_agent(dst + 4 + c + e, v[e]);
-            if (c == 0) {
-                store_agent(dst, Mh);
-                store_agent(dst + 1, L);
-            }
+            store16_coherent(mine, (uint32_t)((h * pf + 4 + c) * sizeof(float)), make_float4(v[0], v[1], v[2], v[3]));
+            if (c == 0) store16_coherent(mine, (uint32_t)(h * pf * sizeof(float)), make_float4(Mh, L, 0.f, 0.f));
         }
     }
     if (!split) return;
-    // the last of the query's items to arrive joins them, in their order
+    // The last of the query's items to arrive joins them, in their order: a wave takes every
+    // fourth head, reads its {m, l} of all items at once and leaves the items' factors in LDS;
+    // then the sums, the items dealt over the threads that share four columns.  A thread's
+    // first eight are in flight while the factors are made.
     unsigned* counter = (unsigned*)A.ws + ((size_t)it.slot * gridDim.y + blockIdx.y) * 16;
     if (!publish_and_count(counter, it.count, &s_last)) return;
-    if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int o = tid; o < n_out; o += 256) {
-        const int h = o / (hd / 4), c = 4 * (o - h * (hd / 4));
-        const float* src = parts + ((size_t)it.part0 * A.nh + h0 + h) * pf;
-        const size_t step = (size_t)A.nh * pf;
-        float Mh = -INFINITY;
-        for (int i = 0; i < it.count; ++i) Mh = fmaxf(Mh, load_agent(src + i * step));
-        float L = 0.0f;
-        v4f v = {0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < it.count; ++i) {
-            const float* s = src + i * step;
-            const float mi = load_agent(s), f = mi > -INFINITY ? exp2_fast(mi - Mh) : 1.0f;
-            L += load_agent(s + 1) * f;
+    {
+        if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const __amdgpu_buffer_rsrc_t all = coherent_rsrc(parts + it.part0 * step, 0xFFFFFFFFu);
+        auto slot = [&](int i) { return (uint32_t)(i * step * sizeof(float)); };
+        const int sub = n_out < 256 ? 256 / n_out : 1;  // threads that share four columns
+        const int k0 = n_out < 256 ? tid / n_out : 0;
+        auto column = [&](int o) {
+            const int h = o / per;
+            return (uint32_t)((h * pf + 4 + 4 * (o - h * per)) * sizeof(float));
+        };
+        const int first_o = n_out < 256 ? tid - k0 * n_out : tid;
+        // eight of a thread's partials from the i-th on (repeating the last; its factor is then 0)
+        auto fetch = [&](float4 (&p)[8], int o, int i) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] += load_agent(s + 4 + c + e) * f;
+            for (int u = 0; u < 8; ++u) p[u] = load16_coherent(all, column(o) + slot(min(i + u * sub, it.count - 1)));
+        };
+        float4 p[8];
+        fetch(p, min(first_o, n_out - 1), k0);
+        float* factor = &s_acc[0][0][0];  // [heads][kMaxItems]
+        static_assert(sizeof s_acc >= 16 * kMaxItems * sizeof(float), "the factors fit the waves' sums");
+        for (int h = wave; h < heads; h += kWaves) {
+            float4 ml[kMaxItems / 64];
+            float Mh = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kMaxItems / 64; ++j) {
+                const int i = lane + 64 * j;
+                ml[j] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+                if (i < it.count) ml[j] = load16_coherent(all, slot(i) + (uint32_t)(h * pf * sizeof(float)));
+                Mh = fmaxf(Mh, ml[j].x);
+            }
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) Mh = fmaxf(Mh, __shfl_xor(Mh, o, 64));
+#pragma unroll
+            for (int j = 0; j < kMaxItems / 64; ++j) {
+                const float f = ml[j].x > -INFINITY ? exp2_fast(ml[j].x - Mh) : 1.0f;
+                if (lane + 64 * j < it.count) factor[h * kMaxItems + lane + 64 * j] = f;
+                L += ml[j].y * f;
+            }
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o, 64);
+            if (lane == 0) s_l[0][h] = L;
         }
-        TQ* dst = (TQ*)A.out + (int64_t)it.b * A.out_stride + (int64_t)(h0 + h) * hd + c;
+        __syncthreads();
+        for (int o0 = 0; o0 < n_out; o0 += 256) {
+            const int o = first_o + o0;
+            const bool in = k0 < sub && o < n_out;
+            const int h = in ? o / per : 0;
+            v4f v = {0.f, 0.f, 0.f, 0.f};
+            if (in) {
+                if (o0) fetch(p, o, k0);
+                for (int i = k0; i < it.count;) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dst[e] = from_f32<TQ>(L == 0.0f ? 0.0f : v[e] / L);
+                    for (int u = 0; u < 8; ++u) {
+                        const int n = i + u * sub;
+                        const float f = n < it.count ? factor[h * kMaxItems + n] : 0.0f;
+                        if (n < it.count) v += (v4f){p[u].x * f, p[u].y * f, p[u].z * f, p[u].w * f};
+                    }
+                    i += 8 * sub;
+                    if (i < it.count) fetch(p, o, i);
+                }
+            }
+            if (sub > 1) {
+                s_red[tid] = v;
+                __syncthreads();
+                if (k0 == 0)
+                    for (int u = 1; u < sub; ++u) v += s_red[u * n_out + o];
+            }
+            if (in && k0 == 0) store_out(A, it.b, (h0 + h) * hd + 4 * (o - h * per), v, s_l[0][h], (TQ*)nullptr);
+        }
     }
 }
 
 template <typename TQ, typename T>
-void attend_by_width(const KvAttend& a, const KvPool& p, dim3 grid, int log_target, hipStream_t s) {
-#define SXQ_AT(HDP, FULL) hipLaunchKernelGGL((k_kv_attend<TQ, T, HDP, FULL>), grid, dim3(256), 0, s, a, p, log_target)
+void attend_by_width(const KvAttend& a, const KvPool& p, dim3 grid, int target, hipStream_t s) {
+#define SXQ_AT(HDP, FULL) hipLaunchKernelGGL((k_kv_attend<TQ, T, HDP, FULL>), grid, dim3(256), 0, s, a, p, target)
     if (p.hd == 64) SXQ_AT(64, true);
     else if (p.hd == 128) SXQ_AT(128, true);
     else if (p.hd == 256) SXQ_AT(256, true);
@@ -519,17 +619,19 @@ void attend_by_width(const KvAttend& a, const KvPool& p, dim3 grid, int log_targ
 namespace sxq {
 
 size_t kv_attend_workspace(const KvPool& p, int n_q, int nh) {
-    return kCountBytes + 2 * (size_t)attend_target(nh, p.nkv) * nh * attend_part_floats(p.hd) * sizeof(float);
+    return kCountBytes + 2 * (size_t)attend_target_max(nh, p.nkv, p.hd) * nh * attend_part_floats(p.hd) * sizeof(float);
 }
 
 hipError_t launch_kv_attend(const KvAttend& a, const KvPool& p, hipStream_t s) {
-    const int target = attend_target(a.nh, p.nkv);
-    const dim3 grid(target + a.n_q, p.nkv * attend_head_tiles(a.nh, p.nkv));
-    const int lt = __builtin_ctz((unsigned)target);
-    if (p.dtype == kF32) attend_by_width<float, float>(a, p, grid, lt, s);
-    else if (p.dtype == kF16) attend_by_width<_Float16, _Float16>(a, p, grid, lt, s);
-    else if (a.q_dtype == kF32) attend_by_width<float, __bf16>(a, p, grid, lt, s);
-    else attend_by_width<__bf16, __bf16>(a, p, grid, lt, s);
+    const int target = attend_target(a.n_q, a.nh, p.nkv, p.hd);
+    // (no more items than the table's width allows: workgroups that find none cost 1.4 us at
+    // one query of 500 positions)
+    const int64_t widest = (int64_t)a.n_q * (((int64_t)a.max_blocks * p.page + kTile * kMinTiles - 1) / (kTile * kMinTiles));
+    const dim3 grid((unsigned)std::min<int64_t>(target + a.n_q, widest), p.nkv * attend_head_tiles(a.nh, p.nkv));
+    if (p.dtype == kF32) attend_by_width<float, float>(a, p, grid, target, s);
+    else if (p.dtype == kF16) attend_by_width<_Float16, _Float16>(a, p, grid, target, s);
+    else if (a.q_dtype == kF32) attend_by_width<float, __bf16>(a, p, grid, target, s);
+    else attend_by_width<__bf16, __bf16>(a, p, grid, target, s);
     return hipGetLastError();
 }
 
@@ -563,6 +665,8 @@ sxq_status sxq_kv_attention(int device, const sxq_kv_pages* pages, int q_dtype, 
                     (long long)q_stride, (long long)out_stride, (long long)unit, (long long)width);
     if (n_rows < 1 || max_blocks < 1 || table_stride < max_blocks || (int64_t)max_blocks * p.page > 1 << 30)
         return fail(SXQ_ERR_INVALID, "kv_attention: a table of %d rows of %d blocks, stride %lld", n_rows, max_blocks, (long long)table_stride);
+    if ((int64_t)n_q * max_blocks * p.page > (int64_t)1 << 35)
+        return fail(SXQ_ERR_INVALID, "kv_attention: %d queries of up to %lld positions", n_q, (long long)max_blocks * p.page);
     if (!rows && n_q > n_rows) return fail(SXQ_ERR_SHAPE, "kv_attention: %d queries over %d table rows", n_q, n_rows);
     if (!(scale - scale == 0.0f)) return fail(SXQ_ERR_INVALID, "kv_attention: scale is not finite");
     if (n_q == 0) return SXQ_OK;

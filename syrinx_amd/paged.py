@@ -54,6 +54,10 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+# The current stream's handle without building a Stream object (2 us a call), where torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 class PagedKvCache:
     """Keys and values of up to max_rows requests of up to max_len positions in n_pages pages
     of page_size positions (a power of two, 16..1024).
@@ -98,7 +102,7 @@ class PagedKvCache:
                        _ptr(v), unit * self.n_kv_heads, unit, self.head_dim)
 
     def _stream(self):
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return _raw_stream(self._index) if _raw_stream else torch.cuda.current_stream(self.device).cuda_stream
 
     def _layer(self, layer):
         if not 0 <= layer < self.n_layers:
@@ -161,39 +165,44 @@ class PagedKvCache:
         [head_dim]) and RoPE by rope = (cos, sin) (f32 [positions, head_dim / 2]), keys and
         values into the layer's pages, the queries returned [T, n_heads * head_dim] in qkv's
         type.  A token without a slot leaves its row of out as it was."""
-        hd = self.head_dim
+        hd, dev, dtype, shape = self.head_dim, self.device, qkv.dtype, qkv.shape
         width = (n_heads + 2 * self.n_kv_heads) * hd
-        if qkv.device != self.device or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1 or \
-                qkv.dtype not in _DTYPES:
-            raise ValueError(f"PagedKvCache.append: qkv must be [T, {width}] f32, f16 or bf16 rows on {self.device}, got "
-                             f"{qkv.dtype} {tuple(qkv.shape)} on {qkv.device}")
-        tokens = qkv.shape[0]
+        code = _DTYPES.get(dtype)
+        if code is None or qkv.device != dev or len(shape) != 2 or shape[1] != width or qkv.stride(1) != 1:
+            raise ValueError(f"PagedKvCache.append: qkv must be [T, {width}] f32, f16 or bf16 rows on {dev}, got "
+                             f"{dtype} {tuple(shape)} on {qkv.device}")
+        tokens = shape[0]
         stride = qkv.stride(0) if tokens > 1 else width
         if stride < width:
             raise ValueError(f"PagedKvCache.append: qkv's rows overlap (stride {stride}, width {width})")
-        for name in ("slots", "pos"):
-            t = getattr(slot_map, name)
-            self._want(name, t, torch.int32)
-            if t.numel() < tokens:
-                raise ValueError(f"PagedKvCache.append: {tokens} tokens, a map of {t.numel()}")
-        for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if t is not None:
-                self._want(name, t, torch.float32, hd)
-        cos = sin = None
+        slots, pos = slot_map.slots, slot_map.pos
+        self._want("slots", slots, torch.int32)
+        self._want("pos", pos, torch.int32)
+        if slots.numel() < tokens or pos.numel() < tokens:
+            raise ValueError(f"PagedKvCache.append: {tokens} tokens, a map of {min(slots.numel(), pos.numel())}")
+        qn = kn = cos = sin = None
+        positions = 0
+        if q_norm is not None:
+            self._want("q_norm", q_norm, torch.float32, hd)
+            qn = q_norm.data_ptr()
+        if k_norm is not None:
+            self._want("k_norm", k_norm, torch.float32, hd)
+            kn = k_norm.data_ptr()
         if rope is not None:
-            cos, sin = rope
-            for name, t in (("cos", cos), ("sin", sin)):
-                self._want(name, t, torch.float32)
-                if t.dim() != 2 or t.shape[1] != hd // 2 or t.shape != cos.shape or t.shape[0] < 1:
+            c, s = rope
+            positions = c.shape[0]
+            for name, t in (("cos", c), ("sin", s)):
+                self._want(name, t, torch.float32, positions * (hd // 2))
+                if t.dim() != 2 or t.shape[1] != hd // 2 or positions < 1:
                     raise ValueError(f"PagedKvCache.append: {name} must be [positions, {hd // 2}], got {tuple(t.shape)}")
+            cos, sin = c.data_ptr(), s.data_ptr()
         if out is None:
-            out = torch.empty((tokens, n_heads * hd), dtype=qkv.dtype, device=self.device)
+            out = torch.empty((tokens, n_heads * hd), dtype=dtype, device=dev)
         else:
-            self._want("out", out, qkv.dtype, tokens * n_heads * hd)
-        check(lib().sxq_kv_append(self._index, self._layer(layer), _DTYPES[qkv.dtype], _ptr(qkv), stride, tokens,
-                                  n_heads, _ptr(q_norm), _ptr(k_norm), eps, _ptr(cos), _ptr(sin),
-                                  cos.shape[0] if cos is not None else 0, int(bool(interleaved)), _ptr(slot_map.pos),
-                                  _ptr(slot_map.slots), _ptr(out), self._stream()))
+            self._want("out", out, dtype, tokens * n_heads * hd)
+        check(lib().sxq_kv_append(self._index, self._layer(layer), code, qkv.data_ptr(), stride, tokens, n_heads, qn, kn,
+                                  eps, cos, sin, positions, 1 if interleaved else 0, pos.data_ptr(), slots.data_ptr(),
+                                  out.data_ptr(), self._stream()))
         return out
 
     # -- attention ------------------------------------------------------------------------
@@ -210,8 +219,11 @@ class PagedKvCache:
     def _kept_workspace(self, n_q, n_heads):
         """Eager calls: one workspace per stream, kept.  Under capture: a fresh one, owned by
         the graph, its zeroing recorded."""
-        with torch.cuda.device(self.device):
+        if torch.cuda.current_device() == self._index:
             capturing = torch.cuda.is_current_stream_capturing()
+        else:
+            with torch.cuda.device(self._index):
+                capturing = torch.cuda.is_current_stream_capturing()
         if capturing:
             return self.workspace(n_q, n_heads)
         stream = self._stream()
@@ -231,30 +243,28 @@ class PagedKvCache:
         default.  A row of no request (rows[n] < 0) leaves out[n] as it was (without `out`:
         unset); an empty request gives zeros.  workspace: `workspace(n, n_heads)`, to keep its
         zeroing out of a captured graph."""
-        hd = self.head_dim
-        if q.device != self.device or q.dim() not in (2, 3) or (q.dim() == 3 and q.shape[2] != hd) or \
-                q.dtype not in _DTYPES:
-            raise ValueError(f"PagedKvCache.attend: q must be [n, heads, {hd}] f32, f16 or bf16 on {self.device}, got "
-                             f"{q.dtype} {tuple(q.shape)} on {q.device}")
-        n = q.shape[0]
-        width = q.shape[1] * (hd if q.dim() == 3 else 1)
+        hd, dev, dtype, shape = self.head_dim, self.device, q.dtype, q.shape
+        code, dims = _DTYPES.get(dtype), len(shape)
+        if code is None or q.device != dev or dims not in (2, 3) or (dims == 3 and shape[2] != hd):
+            raise ValueError(f"PagedKvCache.attend: q must be [n, heads, {hd}] f32, f16 or bf16 on {dev}, got "
+                             f"{dtype} {tuple(shape)} on {q.device}")
+        n, width = shape[0], shape[1] * hd if dims == 3 else shape[1]
         if width == 0 or width % hd:
             raise ValueError(f"PagedKvCache.attend: q rows of {width} elements, heads of {hd}")
         n_heads = width // hd
-
-        def stride(what, t):
-            if t.stride(-1) != 1 or (t.dim() == 3 and t.shape[1] > 1 and t.stride(1) != hd):
-                raise ValueError(f"PagedKvCache.attend: each row of {what} must be contiguous, got strides {t.stride()}")
-            return t.stride(0) if n > 1 else width
-
-        q_stride = stride("q", q)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        elif out.device != self.device or out.dtype != q.dtype or out.shape != q.shape:
-            raise ValueError(f"PagedKvCache.attend: out must be {q.dtype} {tuple(q.shape)} on {self.device}")
-        out_stride = stride("out", out)
+            out = torch.empty(shape, dtype=dtype, device=dev)
+        elif out.device != dev or out.dtype is not dtype or out.shape != shape:
+            raise ValueError(f"PagedKvCache.attend: out must be {dtype} {tuple(shape)} on {dev}")
+        strides = []
+        for what, t in (("q", q), ("out", out)):
+            st = t.stride()
+            if st[-1] != 1 or (dims == 3 and shape[1] > 1 and st[1] != hd):
+                raise ValueError(f"PagedKvCache.attend: each row of {what} must be contiguous, got strides {st}")
+            strides.append(st[0] if n > 1 else width)
         if rows is not None:
             self._want("rows", rows, torch.int32, n)
+            rows = rows.data_ptr()
         if scale is None:
             scale = hd ** -0.5
         if n == 0:
@@ -263,8 +273,8 @@ class PagedKvCache:
             workspace = self._kept_workspace(n, n_heads)
         else:
             self._want("workspace", workspace, torch.uint8)
-        check(lib().sxq_kv_attention(self._index, self._layer(layer), _DTYPES[q.dtype], _ptr(q), q_stride, n,
-                                     n_heads, _ptr(rows), _ptr(self.lens), self.max_rows, _ptr(self.table),
-                                     self.max_blocks, self.max_blocks, scale, _ptr(out), out_stride,
-                                     _ptr(workspace), workspace.numel(), self._stream()))
+        check(lib().sxq_kv_attention(self._index, self._layer(layer), code, q.data_ptr(), strides[0], n, n_heads, rows,
+                                     self.lens.data_ptr(), self.max_rows, self.table.data_ptr(), self.max_blocks,
+                                     self.max_blocks, scale, out.data_ptr(), strides[1], workspace.data_ptr(),
+                                     workspace.numel(), self._stream()))
         return out
