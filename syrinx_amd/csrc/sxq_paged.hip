@@ -1,7 +1,8 @@
 // sxq_paged.hip -- the paged key/value cache: page allocation with block tables and slot maps
 // (sxq_kv_reserve), and new tokens into the pages (sxq_kv_append).  include/sxq.h states both.
 #include <hip/hip_runtime.h>
-#include <hip/hip_bf16.h>
+
+#include <algorithm>
 
 #include "../../include/sxq.h"
 #include "sxq_abi.h"
@@ -18,158 +19,299 @@ namespace {
 // 2^31 - 1 (the capacity they are compared with is at most that).
 SXQ_DEV int sat_add(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, 0x7FFFFFFFu); }
 
-struct Pair {
-    int pages, tokens;
+struct Sums {
+    int freed, pages, tokens;
 };
-SXQ_DEV Pair operator+(Pair a, Pair b) { return {a.pages + b.pages, sat_add(a.tokens, b.tokens)}; }
+SXQ_DEV Sums operator+(Sums a, Sums b) { return {a.freed + b.freed, a.pages + b.pages, sat_add(a.tokens, b.tokens)}; }
 
-// Inclusive scan over the workgroup's NT threads; `total` gets the sum.  red: NT / 64 pairs.
+// Sum over the workgroup's threads before this one; `total` gets the sum of all.  red: NT / 64.
 template <int NT>
-SXQ_DEV Pair block_scan(Pair v, Pair* red, Pair& total) {
+SXQ_DEV Sums block_scan(Sums mine, Sums* red, Sums& total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    Sums v = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const Pair u = {__shfl_up(v.pages, o, 64), __shfl_up(v.tokens, o, 64)};
+        const Sums u = {__shfl_up(v.freed, o, 64), __shfl_up(v.pages, o, 64), __shfl_up(v.tokens, o, 64)};
         if (lane >= o) v = u + v;
     }
+    Sums before = {__shfl_up(v.freed, 1, 64), __shfl_up(v.pages, 1, 64), __shfl_up(v.tokens, 1, 64)};
+    if (lane == 0) before = {0, 0, 0};
     if (NT == 64) {
-        total = {__shfl(v.pages, 63, 64), __shfl(v.tokens, 63, 64)};
-        return v;
+        total = {__shfl(v.freed, 63, 64), __shfl(v.pages, 63, 64), __shfl(v.tokens, 63, 64)};
+        return before;
     }
     __syncthreads();  // the last scan's readers are done with red
     if (lane == 63) red[wave] = v;
     __syncthreads();
-    Pair before = {0, 0}, sum = {0, 0};
+    Sums lower = {0, 0, 0}, sum = {0, 0, 0};
+#pragma unroll
     for (int w = 0; w < NT / 64; ++w) {
-        if (w == wave) before = sum;
+        if (w == wave) lower = sum;
         sum = sum + red[w];
     }
     total = sum;
-    return before + v;
+    return lower + before;
 }
 
-// The last i with first[i] <= j, over n ascending firsts (first[0] <= j).
+// The last i with first[i] <= j, over n ascending firsts (first[0] <= j); for U values of j at
+// once, so that the steps' LDS (or L2) reads overlap.
+template <int U>
+SXQ_DEV void owners(const int* first, int n, const int (&j)[U], int (&i)[U]) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) i[u] = 0;
+    for (int step = n > 1 ? 1 << (31 - __builtin_clz(n - 1)) : 0; step; step >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i[u] + step < n && first[i[u] + step] <= j[u]) i[u] += step;
+}
 SXQ_DEV int owner(const int* first, int n, int j) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= j) lo = mid;
-        else hi = mid;
+    const int jj[1] = {j};
+    int i[1];
+    owners(first, n, jj, i);
+    return i[0];
+}
+
+// The same by a whole wave for one j: 64 offsets a step.
+SXQ_DEV int wave_owner(const int* first, int n, int j) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0;
+    while (n > 1) {
+        const int step = (n + 63) / 64, at = lane * step;
+        const int k = __builtin_popcountll(__ballot(at < n && first[lo + min(at, n - 1)] <= j)) - 1;
+        lo += k * step;
+        n = min(step, n - k * step);
     }
     return lo;
 }
 
-// One workgroup, NT requests at a time: the sums that order the requests are prefix sums, and
-// the pages and tokens of a chunk are dealt over the threads, each finding its request in the
-// chunk's offsets.
-template <int NT>
-__global__ __launch_bounds__(NT) void k_kv_reserve(const KvReserve A, bool inline_map) {
-    __shared__ Pair red[NT / 64 + 1];
-    __shared__ int s_first[NT], s_block[NT], s_tok[NT], s_old[NT];
-    const int tid = threadIdx.x, n = A.n_rows, P = 1 << A.shift;
+// How much of a call one workgroup does by itself.
+enum ReserveMode {
+    kAllInline = 0,  // everything
+    kMapApart = 1,   // the token map by k_kv_map
+    kPagesApart = 2  // the pages by k_kv_pages too, from the offsets left in the (unwritten) map
+};
+
+// One workgroup, NT * R requests at a time, R a thread: the sums that order the requests are
+// prefix sums, and the pages and tokens of a chunk are dealt over the threads, each finding its
+// request in the chunk's offsets.
+template <int NT, int R>
+__global__ __launch_bounds__(NT) void k_kv_reserve(const KvReserve A, int mode) {
+    constexpr int CH = NT * R, U = 4;
+    __shared__ Sums red[NT / 64];
+    __shared__ int s_push[CH], s_keep[CH], s_pop[CH], s_have[CH], s_tok[CH], s_old[CH];
+    __shared__ int s_refused;
+    const int tid = threadIdx.x, n = A.n_rows;
     const int64_t top = (int64_t)A.max_blocks << A.shift;
     const int count = min(max(A.free_count[0], 0), A.n_pages);
 
-    auto load = [&](int r, int& a, int& old) {
-        a = r < n ? A.add[r] : 0;
-        old = r < n ? kv_clamp_len(A.lens[r], A.max_blocks, A.shift) : 0;
-    };
-    auto shrunk = [&](int a, int old) { return (int)max((int64_t)old + a, (int64_t)0); };
-
-    // 1. pages given back
-    int freed = 0;
-    for (int r0 = 0; r0 < n; r0 += NT) {
-        int a, old;
-        load(r0 + tid, a, old);
-        Pair total;
-        block_scan<NT>({a < 0 ? kv_blocks(old, A.shift) - kv_blocks(shrunk(a, old), A.shift) : 0, 0}, red, total);
-        freed += total.pages;
-    }
-    int done = 0;
-    for (int r0 = 0; r0 < n && freed; r0 += NT) {
-        int a, old;
-        load(r0 + tid, a, old);
-        const int b0 = kv_blocks(shrunk(a, old), A.shift), m = a < 0 ? kv_blocks(old, A.shift) - b0 : 0;
-        Pair total;
-        const int first = block_scan<NT>({m, 0}, red, total).pages - m;
-        s_first[tid] = first;
-        s_block[tid] = b0;
-        __syncthreads();
-        for (int j = tid; j < total.pages; j += NT) {
-            const int i = owner(s_first, min(NT, n - r0), j);
-            int32_t* e = A.table + (int64_t)(r0 + i) * A.table_stride + s_block[i] + (j - s_first[i]);
-            const int at = count + freed - 1 - (done + j);
-            if (at < A.n_pages) A.free_list[at] = *e;
-            *e = -1;
+    int a[R], old[R];
+    auto load = [&](int c0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = c0 + tid * R + i;
+            a[i] = r < n ? A.add[r] : 0;
+            old[i] = r < n ? kv_clamp_len(A.lens[r], A.max_blocks, A.shift) : 0;
         }
-        done += total.pages;
+    };
+    auto shrunk = [&](int i) { return (int)max((int64_t)old[i] + a[i], (int64_t)0); };
+    // what request i of the thread gives back and asks for
+    auto sums = [&](int i) -> Sums {
+        const int have = kv_blocks(old[i], A.shift);
+        if (a[i] < 0) return {have - kv_blocks(shrunk(i), A.shift), 0, 0};
+        const int64_t grown = (int64_t)old[i] + a[i];
+        if (grown > top) return {0, 0, 0};  // too long for its table row
+        return {0, kv_blocks((int)grown, A.shift) - have, a[i]};
+    };
+    auto thread_sum = [&]() {
+        Sums v = {0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < R; ++i) v = v + sums(i);
+        return v;
+    };
+    // the chunk's pages given back, `done` before them of `freed` in all
+    auto push = [&](int c0, Sums before, int total, int done, int freed) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            s_push[tid * R + i] = before.freed;
+            s_keep[tid * R + i] = kv_blocks(a[i] < 0 ? shrunk(i) : old[i], A.shift);
+            before.freed += sums(i).freed;
+        }
         __syncthreads();
+        const int rows = min(CH, n - c0);
+        for (int j0 = tid; j0 < total; j0 += U * NT) {
+            int j[U], i[U], id[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) j[u] = min(j0 + u * NT, total - 1);
+            owners(s_push, rows, j, i);
+            auto entry = [&](int u) { return A.table + (int64_t)(c0 + i[u]) * A.table_stride + s_keep[i[u]] + (j[u] - s_push[i[u]]); };
+#pragma unroll
+            for (int u = 0; u < U; ++u) id[u] = j0 + u * NT < total ? *entry(u) : 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int at = count + freed - 1 - (done + j[u]);
+                if (j0 + u * NT >= total) continue;
+                if (at < A.n_pages) A.free_list[at] = id[u];
+                *entry(u) = -1;
+            }
+        }
+        __syncthreads();  // before the pops read the stack, and the next chunk's offsets
+    };
+
+    // 1. requests beyond one chunk: every page given back is on the stack before one is taken
+    const bool chunks = n > CH;
+    int freed = 0;
+    if (chunks) {
+        Sums total;
+        for (int c0 = 0; c0 < n; c0 += CH) {
+            load(c0);
+            block_scan<NT>(thread_sum(), red, total);
+            freed += total.freed;
+        }
+        int done = 0;
+        for (int c0 = 0; c0 < n && freed && mode != kPagesApart; c0 += CH) {
+            load(c0);
+            const Sums before = block_scan<NT>(thread_sum(), red, total);
+            push(c0, before, total.freed, done, freed);
+            done += total.freed;
+        }
     }
-    __syncthreads();  // the pushed pages are visible to the pops below
 
     // 2. pages and tokens handed out
-    const int avail = min(count + freed, A.n_pages);
-    Pair asked = {0, 0}, given = {0, 0};
+    Sums asked = {0, 0, 0}, given = {0, 0, 0};
+    int avail = 0, pushed = 0;
     if (tid == 0) A.cu[0] = 0;
-    for (int r0 = 0; r0 < n; r0 += NT) {
-        const int r = r0 + tid;
-        int a, old;
-        load(r, a, old);
-        const int64_t grown = (int64_t)old + a;
-        const bool wide = a >= 0 && grown > top;
-        const bool grow = a >= 0 && !wide;
-        const int b0 = kv_blocks(old, A.shift);
-        Pair want = {0, 0}, total;
-        if (grow) want = {kv_blocks((int)grown, A.shift) - b0, a};
-        const Pair upto = asked + block_scan<NT>(want, red, total);
+    for (int c0 = 0; c0 < n; c0 += CH) {
+        load(c0);
+        Sums total;
+        Sums before = block_scan<NT>(thread_sum(), red, total);
+        if (!chunks) {
+            freed = total.freed;
+            if (freed && mode != kPagesApart) push(c0, before, freed, 0, freed);
+        }
+        Sums back = before;
+        avail = min(count + freed, A.n_pages);
+        if (tid == 0) s_refused = 0;
+        __syncthreads();
+        int status[R];
+        bool refused = false;
+        Sums upto = asked + before, want = {0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const Sums s = sums(i);
+            upto = upto + s;
+            status[i] = a[i] >= 0 && (int64_t)old[i] + a[i] > top ? 2 : s.pages > 0 && upto.pages > avail ? 1
+                        : s.tokens > 0 && upto.tokens > A.capacity ? 3 : 0;
+            if (status[i] == 0) want = want + s;
+            refused |= status[i] == 1 || status[i] == 3;
+        }
         asked = asked + total;
-        const int status = wide ? 2 : want.pages > 0 && upto.pages > avail ? 1
-                                  : want.tokens > 0 && upto.tokens > A.capacity ? 3 : 0;
-        const bool ok = grow && status == 0;
-        if (!ok) want = {0, 0};
-        const Pair mine = block_scan<NT>(want, red, total);
-        s_first[tid] = mine.pages - want.pages;
-        s_tok[tid] = mine.tokens - want.tokens;
-        s_block[tid] = b0;
-        s_old[tid] = old;
-        if (r < n) {
-            A.cu[r + 1] = given.tokens + mine.tokens;
-            A.status[r] = status;
-            A.lens[r] = a < 0 ? shrunk(a, old) : ok ? (int)grown : old;
+        const int chunk_freed = total.freed;
+        if (refused) s_refused = 1;
+        __syncthreads();
+        if (s_refused) before = block_scan<NT>(want, red, total);  // else all that was asked for is given
+        Sums at = before;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int r = c0 + tid * R + i, k = tid * R + i;
+            Sums s = sums(i);
+            if (status[i]) s = {0, 0, 0};
+            if (mode == kPagesApart && r < n) {
+                A.slots[r] = pushed + back.freed;
+                A.pos[r] = given.pages + at.pages;
+                A.rows[r] = kv_blocks(a[i] < 0 ? shrunk(i) : old[i], A.shift);
+                back.freed += sums(i).freed;
+            }
+            s_pop[k] = at.pages;
+            s_tok[k] = at.tokens;
+            s_have[k] = kv_blocks(old[i], A.shift);
+            s_old[k] = old[i];
+            at = at + s;
+            if (r < n) {
+                A.cu[r + 1] = given.tokens + at.tokens;
+                A.status[r] = status[i];
+                A.lens[r] = a[i] < 0 ? shrunk(i) : status[i] ? old[i] : old[i] + a[i];
+            }
         }
         __syncthreads();
-        const int rows = min(NT, n - r0);
-        for (int j = tid; j < total.pages; j += NT) {
-            const int i = owner(s_first, rows, j);
-            A.table[(int64_t)(r0 + i) * A.table_stride + s_block[i] + (j - s_first[i])] =
-                A.free_list[avail - 1 - (given.pages + j)];
+        const int rows = min(CH, n - c0);
+        pushed += chunk_freed;
+        for (int j0 = tid; j0 < total.pages && mode != kPagesApart; j0 += U * NT) {
+            int j[U], i[U], id[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                j[u] = min(j0 + u * NT, total.pages - 1);
+                id[u] = A.free_list[avail - 1 - (given.pages + j[u])];
+            }
+            owners(s_pop, rows, j, i);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j0 + u * NT < total.pages)
+                    A.table[(int64_t)(c0 + i[u]) * A.table_stride + s_have[i[u]] + (j[u] - s_pop[i[u]])] = id[u];
         }
         __syncthreads();  // the new table entries are read by the tokens' threads
-        for (int j = tid; inline_map && j < total.tokens; j += NT) {
+        for (int j = tid; mode == kAllInline && j < total.tokens; j += NT) {
             const int i = owner(s_tok, rows, j);
             const int pos = s_old[i] + (j - s_tok[i]), t = given.tokens + j;
-            A.slots[t] = kv_slot(A.table[(int64_t)(r0 + i) * A.table_stride + (pos >> A.shift)], pos, A.shift, A.n_pages);
+            A.slots[t] = kv_slot(A.table[(int64_t)(c0 + i) * A.table_stride + (pos >> A.shift)], pos, A.shift, A.n_pages);
             A.pos[t] = pos;
-            A.rows[t] = r0 + i;
+            A.rows[t] = c0 + i;
         }
         given = given + total;
         __syncthreads();
     }
-    for (int t = given.tokens + tid; inline_map && t < A.capacity; t += NT) A.slots[t] = A.pos[t] = A.rows[t] = -1;
-    if (tid == 0) A.free_count[0] = avail - given.pages;
+    for (int t = given.tokens + tid; mode == kAllInline && t < A.capacity; t += NT) A.slots[t] = A.pos[t] = A.rows[t] = -1;
+    if (tid == 0) {
+        A.free_count[0] = avail - given.pages;
+        if (mode == kPagesApart) {
+            A.slots[n] = pushed;
+            A.pos[n] = given.pages;
+            A.rows[n] = avail;
+        }
+    }
 }
 
-// The map of many tokens, from the offsets, lengths and tables that k_kv_reserve left: a
-// workgroup finds the requests of its first and last token among all, each thread its own
-// between those two (prompts of hundreds of tokens: one step or two).
+// The pages of many requests, from k_kv_reserve's offsets: the j-th page given back goes to
+// the stack's place for it and is the j-th page handed out, so one thread does both and no
+// other touches its table entries; beyond those the pages come off the old stack.  A workgroup
+// finds the requests of its first and last page, a thread its own between those.
+constexpr int kPagesPer = 256;
+__global__ __launch_bounds__(kPagesPer) void k_kv_pages(const KvReserve A) {
+    const int n = A.n_rows;
+    const int *push = A.slots, *pop = A.pos, *base = A.rows;
+    const int freed = push[n], given = pop[n], avail = base[n];
+    for (int j0 = blockIdx.x * kPagesPer; j0 < max(freed, given); j0 += gridDim.x * kPagesPer) {
+        const int j = j0 + threadIdx.x;
+        int id = -1;
+        if (j0 < freed) {
+            const int lo = wave_owner(push, n, j0), hi = wave_owner(push, n, min(j0 + kPagesPer, freed) - 1);
+            if (j < freed) {
+                const int i = lo + owner(push + lo, hi + 1 - lo, j), at = avail - 1 - j;
+                int32_t* e = A.table + (int64_t)i * A.table_stride + base[i] + (j - push[i]);
+                id = *e;
+                *e = -1;
+                if (at >= 0) A.free_list[at] = id;
+            }
+        }
+        if (j0 < given) {
+            const int lo = wave_owner(pop, n, j0), hi = wave_owner(pop, n, min(j0 + kPagesPer, given) - 1);
+            if (j < given) {
+                const int i = lo + owner(pop + lo, hi + 1 - lo, j);
+                if (j >= freed) id = A.free_list[avail - 1 - j];
+                A.table[(int64_t)i * A.table_stride + base[i] + (j - pop[i])] = id;
+            }
+        }
+    }
+}
+
+// The map of many tokens, from the offsets, lengths and tables: as above by tokens.
 constexpr int kMapTokens = 1024;
 __global__ __launch_bounds__(256) void k_kv_map(const KvReserve A) {
     const int t0 = blockIdx.x * kMapTokens, total = A.cu[A.n_rows];
     const int t_end = min(t0 + kMapTokens, total);
     int lo = 0, n = 0;
     if (t0 < total) {
-        lo = owner(A.cu, A.n_rows, t0);
-        n = owner(A.cu, A.n_rows, t_end - 1) + 1 - lo;
+        lo = wave_owner(A.cu, A.n_rows, t0);
+        n = wave_owner(A.cu, A.n_rows, t_end - 1) + 1 - lo;
     }
     for (int t = t0 + threadIdx.x; t < min(t0 + kMapTokens, A.capacity); t += 256) {
         int slot = -1, pos = -1, row = -1;
@@ -282,10 +424,14 @@ bool pow2_page(int p) { return p >= 16 && p <= 1024 && (p & (p - 1)) == 0; }
 namespace sxq {
 
 hipError_t launch_kv_reserve(const KvReserve& a, hipStream_t s) {
-    const bool wave = a.n_rows <= 64, inline_map = a.capacity <= (wave ? 256 : 2048);
-    if (wave) hipLaunchKernelGGL(k_kv_reserve<64>, dim3(1), dim3(64), 0, s, a, inline_map);
-    else hipLaunchKernelGGL(k_kv_reserve<1024>, dim3(1), dim3(1024), 0, s, a, inline_map);
-    if (!inline_map)
+    const bool wave = a.n_rows <= 64;
+    const int mode = a.capacity <= (wave ? 256 : 2048) ? kAllInline : wave || a.capacity <= a.n_rows ? kMapApart : kPagesApart;
+    if (wave) hipLaunchKernelGGL((k_kv_reserve<64, 1>), dim3(1), dim3(64), 0, s, a, mode);
+    else if (a.n_rows <= 1024) hipLaunchKernelGGL((k_kv_reserve<1024, 1>), dim3(1), dim3(1024), 0, s, a, mode);
+    else hipLaunchKernelGGL((k_kv_reserve<1024, 4>), dim3(1), dim3(1024), 0, s, a, mode);
+    if (mode == kPagesApart)
+        hipLaunchKernelGGL(k_kv_pages, dim3(std::min(256, (a.n_pages + kPagesPer - 1) / kPagesPer)), dim3(kPagesPer), 0, s, a);
+    if (mode != kAllInline)
         hipLaunchKernelGGL(k_kv_map, dim3((a.capacity + kMapTokens - 1) / kMapTokens), dim3(256), 0, s, a);
     return hipGetLastError();
 }
