@@ -354,6 +354,20 @@ enum {
 #define SXQ_LM_GRAPH 1u /* replay the step as a captured HIP graph (captured on first use per batch size) */
 
 sxq_status sxq_lm_create(int device, const sxq_lm_config *cfg, sxq_lm **out);
+/* The same engine over a paged cache (the operators above): every layer's keys and values in
+ * n_pages pages of page_size positions, of kv_dtype SXQ_F32 or SXQ_BF16, shared by all
+ * streams -- a stream holds the pages of its length, so max_seq (up to 2^20) reserves nothing
+ * but its RoPE row and table entries.  Steps and prefills take pages as streams grow, and are
+ * refused with SXQ_ERR_OOM before any GPU work when there are not enough; sxq_lm_reset and
+ * shorter sxq_lm_set_lengths give them back (longer ones take pages that hold what they
+ * held).  A prefill also lays one layer's keys and values out as f32 in its workspace.  Every
+ * other call is as for sxq_lm_create, except that sxq_fish_fast_expand refuses a paged engine
+ * (its cache is one frame's codes).  Keys and values are rounded once to kv_dtype; the
+ * attention's sums are in another order than the contiguous engine's. */
+sxq_status sxq_lm_create_paged(int device, const sxq_lm_config *cfg, int kv_dtype, int page_size, int n_pages,
+                               sxq_lm **out);
+/* Pages that no stream of a paged engine holds. */
+sxq_status sxq_lm_free_pages(const sxq_lm *lm, int *free_pages);
 /* Copy a QMatMul's weight into a projection slot (shape and dtype must match). */
 sxq_status sxq_lm_set_linear(sxq_lm *lm, int layer, int which, const sxq_qmm *w);
 /* Copy an f32 vector (norm weight, bias, embedding table) into a slot. */

@@ -61,6 +61,8 @@ _SIGS = {
     "sxq_qmm_destroy": (_I, [_P]),
     "sxq_fill_normal": (_I, [_I, _P, _I64, _U64, _F, _F, _P]),
     "sxq_lm_create": (_I, [_I, _P, _P]),
+    "sxq_lm_create_paged": (_I, [_I, _P, _I, _I, _I, _P]),
+    "sxq_lm_free_pages": (_I, [_P, _P]),
     "sxq_lm_set_linear": (_I, [_P, _I, _I, _P]),
     "sxq_lm_set_vector": (_I, [_P, _I, _I, _P, _I64, _I]),
     "sxq_lm_init_random": (_I, [_P, _U64, _F]),

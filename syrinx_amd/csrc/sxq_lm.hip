@@ -19,6 +19,7 @@
 
 #include "sxq_abi.h"
 #include "sxq_decoder.h"
+#include "sxq_paged_launch.h"
 
 using namespace sxq;
 using namespace sxq::abi;
@@ -101,6 +102,17 @@ struct sxq_lm {
     hipStream_t cap = nullptr;
     std::map<GraphKey, hipGraphExec_t> graphs;
     std::map<std::string, hipGraphExec_t> expand_graphs;  // keyed by the raw bytes of the arguments
+    // A paged engine (sxq_lm_create_paged): pages in place of kc / vc, one table and one stack of
+    // free pages for every layer (layer l's pool is pool's, l * pool_layer elements on).
+    bool paged = false;
+    KvPool pool{};
+    int64_t pool_layer = 0;
+    int max_blocks = 0;
+    int32_t *kv_table = nullptr, *kv_free = nullptr, *kv_free_count = nullptr;
+    int32_t *kv_add = nullptr, *kv_ones = nullptr;  // growths of a call; one token each
+    int32_t *kv_cu = nullptr, *kv_status = nullptr, *kv_slots = nullptr, *kv_pos = nullptr, *kv_rows = nullptr;
+    float* kv_ctx = nullptr;  // context rows of a step [max_batch][n_heads * head_dim]
+    void* kv_ws = nullptr;    // the attention's workspace
     void* pf = nullptr;  // prefill workspace, grown to the largest prompt batch so far
     size_t pf_size = 0;
     std::vector<void*> allocs;
@@ -197,6 +209,108 @@ size_t trace_floats(const sxq_lm* lm, int n) {
     return 2 * (size_t)n * lm->c.dim + (size_t)lm->c.n_layers * trace_layer_floats(lm, n);
 }
 
+// ---- paged engines ------------------------------------------------------------------
+// Grow streams 0..n-1 by add[] tokens (device), mapping up to `capacity` of them; moves d_len.
+hipError_t lm_reserve(sxq_lm* lm, const int32_t* add, int n, int capacity, int32_t* slots, int32_t* pos, int32_t* rows,
+                      hipStream_t s) {
+    KvReserve a{};
+    a.shift = lm->pool.shift;
+    a.n_pages = lm->pool.n_pages;
+    a.n_rows = n;
+    a.max_blocks = lm->max_blocks;
+    a.capacity = capacity;
+    a.limit = INT32_MAX;  // (the callers have counted the pages; a length may be set without a map)
+    a.table_stride = lm->max_blocks;
+    a.add = add;
+    a.lens = lm->d_len;
+    a.table = lm->kv_table;
+    a.free_list = lm->kv_free;
+    a.free_count = lm->kv_free_count;
+    a.cu = lm->kv_cu;
+    a.slots = slots;
+    a.pos = pos;
+    a.rows = rows;
+    a.status = lm->kv_status;
+    return launch_kv_reserve(a, s);
+}
+
+KvPool layer_pool(const sxq_lm* lm, int l) {
+    KvPool p = lm->pool;
+    const size_t off = (size_t)l * lm->pool_layer * type_size(p.dtype);
+    p.k = (uint8_t*)p.k + off;
+    p.v = (uint8_t*)p.v + off;
+    return p;
+}
+
+// Layer l's QK-norm + RoPE of T fused rows, keys and values into the pages, queries to q.
+hipError_t lm_append(sxq_lm* lm, int l, const float* qkv, int T, const int32_t* slots, const int32_t* pos, float* q,
+                     hipStream_t s) {
+    const sxq_lm_config& c = lm->c;
+    KvAppend a{};
+    a.qkv = qkv;
+    a.row_stride = lm->qkv_n;
+    a.dtype = kF32;
+    a.n_tokens = T;
+    a.nh = c.n_heads;
+    a.q_norm = c.qk_norm ? lm->layers[l].q_norm : nullptr;
+    a.k_norm = c.qk_norm ? lm->layers[l].k_norm : nullptr;
+    a.eps = c.norm_eps;
+    a.cos = lm->rope_cos;
+    a.sin = lm->rope_sin;
+    a.max_pos = c.max_seq;
+    a.interleaved = c.rope_interleaved;
+    a.pos = pos;
+    a.slots = slots;
+    a.q_out = q;
+    return launch_kv_append(a, layer_pool(lm, l), s);
+}
+
+hipError_t lm_attend(sxq_lm* lm, int l, const float* q, int n, float* ctx, hipStream_t s) {
+    KvAttend a{};
+    a.q = q;
+    a.q_stride = a.out_stride = lm->ctx;
+    a.q_dtype = kF32;
+    a.n_q = n;
+    a.nh = lm->c.n_heads;
+    a.lens = lm->d_len;
+    a.table = lm->kv_table;
+    a.n_rows = n;
+    a.max_blocks = lm->max_blocks;
+    a.table_stride = lm->max_blocks;
+    a.scale = (float)(1.0 / sqrt((double)lm->c.head_dim));
+    a.out = ctx;
+    a.ws = lm->kv_ws;
+    return launch_kv_attend(a, layer_pool(lm, l), s);
+}
+
+// N(0, 1) into n elements of a cache.
+hipError_t fill_cache(void* p, int64_t n, int dtype, uint64_t seed) {
+    if (dtype == kF32) return launch_fill_normal((float*)p, n, seed, 0.0f, 1.0f, nullptr);
+    const int64_t chunk = std::min<int64_t>(n, (int64_t)16 << 20);
+    float* tmp = nullptr;
+    hipError_t e = hipMalloc(&tmp, sizeof(float) * (size_t)chunk);
+    for (int64_t at = 0; at < n && e == hipSuccess; at += chunk) {
+        const int64_t m = std::min(chunk, n - at);
+        e = launch_fill_normal(tmp, m, seed * 1000003ull + (uint64_t)at, 0.0f, 1.0f, nullptr);
+        if (e == hipSuccess) e = launch_f32_to_bf16(tmp, m, (uint16_t*)p + at, nullptr);
+    }
+    if (tmp) {
+        (void)hipDeviceSynchronize();
+        (void)hipFree(tmp);
+    }
+    return e;
+}
+
+// Pages of all streams at these lengths; refuses what the pool does not hold.
+sxq_status check_pages(const sxq_lm* lm, const char* who, const std::vector<int>& lens) {
+    if (!lm->paged) return SXQ_OK;
+    int64_t need = 0;
+    for (int len : lens) need += kv_blocks(len, lm->pool.shift);
+    if (need > lm->pool.n_pages)
+        return fail(SXQ_ERR_OOM, "%s: the streams need %lld KV pages of %d", who, (long long)need, lm->pool.n_pages);
+    return SXQ_OK;
+}
+
 hipError_t enqueue_step(sxq_lm* lm, int n, bool from_embeds, hipStream_t s) {
     const sxq_lm_config& c = lm->c;
     hipError_t e = hipSuccess;
@@ -216,6 +330,7 @@ hipError_t enqueue_step(sxq_lm* lm, int n, bool from_embeds, hipStream_t s) {
         tr += floats;
         return p;
     };
+    if (lm->paged) STEP(lm_reserve(lm, lm->kv_ones, n, n, lm->kv_slots, lm->kv_pos, lm->kv_rows, s));
     // one stream through the fused attention: the embedding kernel also copies the step's
     // RoPE row, so that the attention splits issue their loads before the length returns
     const bool spec = lm->rope_row && n == 1 && lm->wo_fused && !from_embeds && !lm->embed_scheme;
@@ -271,7 +386,13 @@ hipError_t enqueue_step(sxq_lm* lm, int n, bool from_embeds, hipStream_t s) {
         if (tr) STEP(record(lm->qkv, (size_t)n * lm->qkv_n));
         const float* qn = c.qk_norm ? L.q_norm : nullptr;
         const float* kn = c.qk_norm ? L.k_norm : nullptr;
-        if (lm->attn_fused) {
+        if (lm->paged) {
+            STEP(lm_append(lm, l, lm->qkv, n, lm->kv_slots, lm->kv_pos, lm->qbuf, s));
+            if (tr) STEP(record(lm->qbuf, (size_t)n * lm->ctx));
+            STEP(lm_attend(lm, l, lm->qbuf, n, lm->kv_ctx, s));
+            if (tr) STEP(record(lm->kv_ctx, (size_t)n * lm->ctx));
+            STEP(launch_quantize_act(lm->vdt, false, lm->kv_ctx, lm->ctx, n, lm->ctx, lm->act_o, s));
+        } else if (lm->attn_fused) {
             float* q_slot = tr ? slot((size_t)n * lm->ctx) : nullptr;
             float* ctx_slot = tr ? slot((size_t)n * lm->ctx) : nullptr;
             if (wo_fused)
@@ -314,8 +435,8 @@ hipError_t enqueue_step(sxq_lm* lm, int n, bool from_embeds, hipStream_t s) {
     STEP(launch_gemv_rmsnorm(lm->head.w, norm_in(lm->h, lm->final_norm, lm->hn), n, lm->act_a, lm->logits, c.vocab,
                              c.head_bias ? lm->head_bias : nullptr, nullptr, 0, s, rec_a));
     if (tr) STEP(record(lm->hn, nd));
-    STEP(launch_argmax(lm->logits, n, c.vocab, lm->d_ids, lm->ids_per, lm->d_next, lm->d_len, lm->am_val, lm->am_idx,
-                       lm->am_count, s));
+    STEP(launch_argmax(lm->logits, n, c.vocab, lm->d_ids, lm->ids_per, lm->d_next, lm->paged ? nullptr : lm->d_len,
+                       lm->am_val, lm->am_idx, lm->am_count, s));
 #undef STEP
     lm->wo_dirty = false;
     return hipSuccess;
@@ -390,7 +511,7 @@ void destroy_lm(sxq_lm* lm) {
     delete lm;
 }
 
-sxq_status check_config(const sxq_lm_config* c) {
+sxq_status check_config(const sxq_lm_config* c, bool paged) {
     if (!c) return fail(SXQ_ERR_INVALID, "lm_create: null config");
     if (c->n_layers <= 0 || c->dim <= 0 || c->n_heads <= 0 || c->n_kv_heads <= 0 || c->head_dim <= 0 ||
         c->intermediate <= 0 || c->vocab <= 0 || c->max_seq <= 0)
@@ -399,7 +520,8 @@ sxq_status check_config(const sxq_lm_config* c) {
     if (c->n_heads % c->n_kv_heads) return fail(SXQ_ERR_SHAPE, "lm_create: n_heads %% n_kv_heads != 0");
     if (c->head_dim > 256 || c->head_dim < 32 || c->head_dim % 8)
         return fail(SXQ_ERR_SHAPE, "lm_create: head_dim must be a multiple of 8 in [32, 256]");
-    if (c->max_seq > kMaxSplits * kAttnSplit)
+    if (paged && c->max_seq > 1 << 20) return fail(SXQ_ERR_INVALID, "lm_create: max_seq %d exceeds 2^20 positions", c->max_seq);
+    if (!paged && c->max_seq > kMaxSplits * kAttnSplit)
         return fail(SXQ_ERR_INVALID, "lm_create: max_seq %d exceeds %d positions", c->max_seq, kMaxSplits * kAttnSplit);
     const int dt = c->weight_dtype;
     if (dt != kQ4K && dt != kQ8_0 && dt != kQ4_0) return fail(SXQ_ERR_DTYPE, "lm_create: weight dtype %d not supported", dt);
@@ -431,9 +553,19 @@ hipError_t pf_proj(const sxq_lm* lm, const QWeight& w, const float* x, const uin
 // Device buffers of one prefill of T tokens over n streams (offsets into lm->pf).
 struct PfLayout {
     size_t h, hn, qkv, q, cx, gu, af, act, gemm, tok, tiles, last, total;
+    size_t kv_map, kv_k, kv_v;  // paged: the slot map, one layer's keys and values as f32 [n][n_kv][span][hd]
+    int span;
 };
 
-PfLayout pf_layout(const sxq_lm* lm, int T, int n) {
+// The longest stream after a prefill.
+int pf_span(const PrefillMeta& pm) {
+    int m = 0;
+    for (int i = 0; i < pm.n; ++i) m = std::max(m, pm.lens[i] + pm.counts[i]);
+    return m;
+}
+
+PfLayout pf_layout(const sxq_lm* lm, int T, const PrefillMeta& pm) {
+    const int n = pm.n;
     const sxq_lm_config& c = lm->c;
     auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
     const size_t bs = block_size(lm->vdt), ab = act_block_bytes(lm->vdt);
@@ -468,6 +600,13 @@ PfLayout pf_layout(const sxq_lm* lm, int T, int n) {
     p.tok = take(sizeof(int) * 2 * (size_t)T);
     p.tiles = take(sizeof(int) * 4 * (size_t)(T + n));
     p.last = take(sizeof(int) * (size_t)n);
+    if (lm->paged) {
+        p.span = pf_span(pm);
+        const size_t kv = sizeof(float) * (size_t)n * c.n_kv_heads * p.span * c.head_dim;
+        p.kv_map = take(sizeof(int) * 3 * (size_t)T);
+        p.kv_k = take(kv);
+        p.kv_v = take(kv);
+    }
     p.total = o;
     return p;
 }
@@ -477,7 +616,7 @@ size_t pf_trace_floats(const sxq_lm* lm, int T) { return trace_floats(lm, T); }
 hipError_t enqueue_prefill(sxq_lm* lm, const PrefillMeta& pm, int T, const int* ids, const float* embeds,
                            float* logits_all, float* hidden_all, bool exact, float* tr, hipStream_t s) {
     const sxq_lm_config& c = lm->c;
-    const PfLayout P = pf_layout(lm, T, pm.n);
+    const PfLayout P = pf_layout(lm, T, pm);
     uint8_t* base = (uint8_t*)lm->pf;
     float* h = (float*)(base + P.h);
     float* hn = (float*)(base + P.hn);
@@ -508,6 +647,13 @@ hipError_t enqueue_prefill(sxq_lm* lm, const PrefillMeta& pm, int T, const int* 
     int n_tiles = 0;
     for (int i = 0; i < n; ++i) n_tiles += (pm.counts[i] + pm.tile_tokens - 1) / pm.tile_tokens;
     PF(launch_prefill_tables(pm, T, tok, tiles, last, s));
+    int32_t* kv_map = (int32_t*)(base + P.kv_map);
+    float *kv_k = (float*)(base + P.kv_k), *kv_v = (float*)(base + P.kv_v);
+    const int64_t kv_stride = (int64_t)c.n_kv_heads * P.span * c.head_dim;
+    if (lm->paged) {
+        PF(launch_kv_counts(pm, lm->kv_add, s));
+        PF(lm_reserve(lm, lm->kv_add, n, T, kv_map, kv_map + T, kv_map + 2 * (int64_t)T, s));
+    }
     if (embeds) {
         PF(hipMemcpyAsync(h, embeds, sizeof(float) * Td, hipMemcpyDeviceToDevice, s));
     } else if (c.n_codebooks > 0 || (c.tied_embedding && !lm->embed)) {
@@ -552,13 +698,22 @@ hipError_t enqueue_prefill(sxq_lm* lm, const PrefillMeta& pm, int T, const int* 
         PF(norm_proj(L.wqkv.w, L.attn_norm, qkv, L.bqkv, false));
         PF(record(hn, Td));
         PF(record(qkv, (size_t)T * lm->qkv_n));
-        PF(launch_prefill_rope_kv(qkv, T, lm->qkv_n, c.n_heads, c.n_kv_heads, c.head_dim,
-                                  c.qk_norm ? L.q_norm : nullptr, c.qk_norm ? L.k_norm : nullptr, c.norm_eps,
-                                  c.rope_interleaved, lm->rope_cos, lm->rope_sin, tok, q, kc, vc,
-                                  lm->kv_stream_stride, c.max_seq, s));
+        if (lm->paged) {
+            // the prompt's attention reads each stream's positions in one run: the pages, the
+            // new tokens' among them (so as later steps read them), laid out so for this layer
+            PF(lm_append(lm, l, qkv, T, kv_map, kv_map + T, q, s));
+            PF(launch_kv_gather(layer_pool(lm, l), lm->kv_table, lm->max_blocks, lm->max_blocks, lm->d_len, 0, n, 0,
+                                c.n_kv_heads, 0, P.span, kv_k, kv_v, s));
+        } else {
+            PF(launch_prefill_rope_kv(qkv, T, lm->qkv_n, c.n_heads, c.n_kv_heads, c.head_dim,
+                                      c.qk_norm ? L.q_norm : nullptr, c.qk_norm ? L.k_norm : nullptr, c.norm_eps,
+                                      c.rope_interleaved, lm->rope_cos, lm->rope_sin, tok, q, kc, vc,
+                                      lm->kv_stream_stride, c.max_seq, s));
+        }
         PF(record(q, (size_t)T * lm->ctx));
-        PF(launch_prefill_attn(q, kc, vc, tiles, n_tiles, c.n_heads, c.n_kv_heads, c.head_dim, c.max_seq,
-                               lm->kv_stream_stride, ctx_blocks && !tr ? nullptr : cx, ctx_blocks ? act : nullptr, s));
+        PF(launch_prefill_attn(q, lm->paged ? kv_k : kc, lm->paged ? kv_v : vc, tiles, n_tiles, c.n_heads, c.n_kv_heads,
+                               c.head_dim, lm->paged ? P.span : c.max_seq, lm->paged ? kv_stride : lm->kv_stream_stride,
+                               ctx_blocks && !tr ? nullptr : cx, ctx_blocks ? act : nullptr, s));
         PF(record(cx, (size_t)T * lm->ctx));
         if (!f16 && !ctx_blocks) PF(launch_quantize_act(lm->vdt, false, cx, lm->ctx, T, lm->ctx, act, s));
         PF(pf_proj(lm, L.wo.w, cx, act, T, h, L.bo, h, exact, gws, s));
@@ -595,20 +750,36 @@ hipError_t enqueue_prefill(sxq_lm* lm, const PrefillMeta& pm, int T, const int* 
     }
     PF(launch_argmax(lm->logits, n, c.vocab, lm->d_ids, lm->ids_per, lm->d_next, nullptr, lm->am_val, lm->am_idx,
                      lm->am_count, s));
-    PF(launch_prefill_advance(pm, lm->d_len, s));
+    if (!lm->paged) PF(launch_prefill_advance(pm, lm->d_len, s));
 #undef PF
     return hipSuccess;
 }
 
-}  // namespace
+// A paged engine's pages: `dtype` f32 or bf16.
+struct PageConfig {
+    int dtype, page_size, n_pages;
+};
 
-extern "C" {
-
-sxq_status sxq_lm_create(int device, const sxq_lm_config* cfg, sxq_lm** out) {
+sxq_status lm_create(int device, const sxq_lm_config* cfg, const PageConfig* pages, sxq_lm** out) {
     if (!out) return fail(SXQ_ERR_INVALID, "lm_create: null output handle");
     *out = nullptr;
-    sxq_status st = check_config(cfg);
+    sxq_status st = check_config(cfg, pages != nullptr);
     if (st != SXQ_OK) return st;
+    KvPool pool{};
+    if (pages) {
+        sxq_kv_pages k{};
+        k.dtype = pages->dtype;
+        k.n_kv_heads = cfg->n_kv_heads;
+        k.head_dim = cfg->head_dim;
+        k.page_size = pages->page_size;
+        k.n_pages = pages->n_pages;
+        k.pos_stride = cfg->head_dim;
+        k.head_stride = (int64_t)k.pos_stride * k.page_size;
+        k.page_stride = k.head_stride * k.n_kv_heads;
+        st = kv_pool("lm_create_paged", &k, false, &pool);
+        if (st != SXQ_OK) return st;
+        if (pool.dtype == kF16) return fail(SXQ_ERR_DTYPE, "lm_create_paged: pages of f32 or bf16 (the queries are f32)");
+    }
     DeviceGuard g(device);
     HIP_TRY(g.err, "hipSetDevice");
     sxq_lm* lm = new sxq_lm();
@@ -624,6 +795,12 @@ sxq_status sxq_lm_create(int device, const sxq_lm_config* cfg, sxq_lm** out) {
     lm->kv_stream_stride = (int64_t)c.n_kv_heads * c.max_seq * c.head_dim;
     lm->kv_layer_stride = lm->kv_stream_stride * c.max_batch;
     const int MB = c.max_batch, I = c.intermediate, hd = c.head_dim;
+    if (pages) {
+        lm->paged = true;
+        lm->pool = pool;
+        lm->pool_layer = pool.page_stride * pool.n_pages;
+        lm->max_blocks = kv_blocks(c.max_seq, pool.shift);
+    }
     hipError_t e = hipSuccess;
     auto A = [&](void** p, size_t bytes) {
         if (e == hipSuccess) e = dalloc(lm, p, bytes);
@@ -648,14 +825,28 @@ sxq_status sxq_lm_create(int device, const sxq_lm_config* cfg, sxq_lm** out) {
     if (c.n_codebooks > 0) A((void**)&lm->cb_embed, sizeof(float) * (size_t)c.n_codebooks * c.codebook_size * c.dim);
     A((void**)&lm->rope_cos, sizeof(float) * (size_t)c.max_seq * (hd / 2));
     A((void**)&lm->rope_sin, sizeof(float) * (size_t)c.max_seq * (hd / 2));
-    A((void**)&lm->kc, sizeof(float) * (size_t)lm->kv_layer_stride * c.n_layers);
-    A((void**)&lm->vc, sizeof(float) * (size_t)lm->kv_layer_stride * c.n_layers);
+    if (pages) {
+        const size_t bytes = (size_t)lm->pool_layer * c.n_layers * type_size(pool.dtype);
+        A(&lm->pool.k, bytes);
+        A(&lm->pool.v, bytes);
+        A((void**)&lm->kv_table, sizeof(int32_t) * (size_t)MB * lm->max_blocks);
+        A((void**)&lm->kv_free, sizeof(int32_t) * (size_t)pool.n_pages);
+        A((void**)&lm->kv_free_count, sizeof(int32_t));
+        for (int32_t** p : {&lm->kv_add, &lm->kv_ones, &lm->kv_status, &lm->kv_slots, &lm->kv_pos, &lm->kv_rows})
+            A((void**)p, sizeof(int32_t) * MB);
+        A((void**)&lm->kv_cu, sizeof(int32_t) * (MB + 1));
+        A((void**)&lm->kv_ctx, sizeof(float) * (size_t)MB * lm->ctx);
+        A(&lm->kv_ws, kv_attend_workspace(pool, MB, c.n_heads));
+    } else {
+        A((void**)&lm->kc, sizeof(float) * (size_t)lm->kv_layer_stride * c.n_layers);
+        A((void**)&lm->vc, sizeof(float) * (size_t)lm->kv_layer_stride * c.n_layers);
+        A((void**)&lm->part, sizeof(float) * (size_t)MB * c.n_heads * lm->max_splits * (hd + 4));
+    }
     A((void**)&lm->d_len, sizeof(int) * MB);
     A((void**)&lm->h, sizeof(float) * (size_t)MB * c.dim);
     A((void**)&lm->hn, sizeof(float) * (size_t)MB * c.dim);
     A((void**)&lm->qkv, sizeof(float) * (size_t)MB * lm->qkv_n);
     A((void**)&lm->qbuf, sizeof(float) * (size_t)MB * lm->ctx);
-    A((void**)&lm->part, sizeof(float) * (size_t)MB * c.n_heads * lm->max_splits * (hd + 4));
     A((void**)&lm->gu, sizeof(float) * (size_t)MB * 2 * I);
     A((void**)&lm->act_f32, sizeof(float) * (size_t)MB * I);
     A((void**)&lm->logits, sizeof(float) * (size_t)MB * c.vocab);
@@ -722,7 +913,16 @@ sxq_status sxq_lm_create(int device, const sxq_lm_config* cfg, sxq_lm** out) {
     if (e == hipSuccess && lm->rec_o) e = hipMemset(lm->rec_o, 0, sizeof(MmaRec) * (size_t)(lm->ctx / 256));
     if (e == hipSuccess && lm->rec_d) e = hipMemset(lm->rec_d, 0, sizeof(MmaRec) * (size_t)(I / 256));
     if (e == hipSuccess && lm->rec_ws.count) e = hipMemset(lm->rec_ws.count, 0, GemvRecWs::count_bytes());
-    lm->attn_fused = getenv("SXQ_ATTN_UNFUSED") == nullptr && attn_decode_fits(lm->vdt, c.n_heads, c.n_kv_heads, hd, lm->max_splits);
+    if (e == hipSuccess && pages) {
+        std::vector<int32_t> stack(pool.n_pages);
+        for (int i = 0; i < pool.n_pages; ++i) stack[i] = pool.n_pages - 1 - i;  // page 0 on top
+        e = hipMemcpy(lm->kv_free, stack.data(), sizeof(int32_t) * stack.size(), hipMemcpyHostToDevice);
+        if (e == hipSuccess) e = launch_fill_int(lm->kv_free_count, 1, pool.n_pages, nullptr);
+        if (e == hipSuccess) e = launch_fill_int(lm->kv_ones, MB, 1, nullptr);
+        if (e == hipSuccess) e = hipMemset(lm->kv_table, 0xFF, sizeof(int32_t) * (size_t)MB * lm->max_blocks);
+        if (e == hipSuccess) e = hipMemset(lm->kv_ws, 0, kv_attend_workspace(pool, MB, c.n_heads));
+    }
+    lm->attn_fused = !pages && getenv("SXQ_ATTN_UNFUSED") == nullptr && attn_decode_fits(lm->vdt, c.n_heads, c.n_kv_heads, hd, lm->max_splits);
     lm->swiglu = getenv("SXQ_SWIGLU_UNFUSED") == nullptr && swiglu_pair_fits(lm->layers[0].w13.w, lm->layers[0].w2.w);
     if (e == hipSuccess && lm->attn_fused &&
         attn_decode_prepare(lm->vdt, c.n_heads, c.n_kv_heads, hd, lm->max_splits) != hipSuccess) {
@@ -745,6 +945,27 @@ sxq_status sxq_lm_create(int device, const sxq_lm_config* cfg, sxq_lm** out) {
     }
     lm->h_len.assign(MB, 0);
     *out = lm;
+    return SXQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+sxq_status sxq_lm_create(int device, const sxq_lm_config* cfg, sxq_lm** out) { return lm_create(device, cfg, nullptr, out); }
+
+sxq_status sxq_lm_create_paged(int device, const sxq_lm_config* cfg, int kv_dtype, int page_size, int n_pages,
+                               sxq_lm** out) {
+    const PageConfig pages{kv_dtype, page_size, n_pages};
+    return lm_create(device, cfg, &pages, out);
+}
+
+sxq_status sxq_lm_free_pages(const sxq_lm* lm, int* free_pages) {
+    if (!lm || !free_pages) return fail(SXQ_ERR_INVALID, "lm_free_pages: null pointer");
+    if (!lm->paged) return fail(SXQ_ERR_INVALID, "lm_free_pages: not a paged engine");
+    int used = 0;
+    for (int len : lm->h_len) used += kv_blocks(len, lm->pool.shift);
+    *free_pages = lm->pool.n_pages - used;
     return SXQ_OK;
 }
 
@@ -938,6 +1159,21 @@ sxq_status sxq_lm_set_lengths(sxq_lm* lm, const int32_t* lengths, int n) {
     DeviceGuard g(lm->device);
     HIP_TRY(g.err, "hipSetDevice");
     HIP_TRY(hipDeviceSynchronize(), "lm_set_lengths");
+    if (lm->paged) {  // pages given back or taken (those of added positions hold what they held)
+        std::vector<int> lens = lm->h_len;
+        std::vector<int32_t> add(n);
+        for (int s = 0; s < n; ++s) {
+            add[s] = lengths[s] - lens[s];
+            lens[s] = lengths[s];
+        }
+        const sxq_status st = check_pages(lm, "lm_set_lengths", lens);
+        if (st != SXQ_OK) return st;
+        HIP_TRY(hipMemcpy(lm->kv_add, add.data(), sizeof(int32_t) * n, hipMemcpyHostToDevice), "lm_set_lengths");
+        HIP_TRY(lm_reserve(lm, lm->kv_add, n, 0, nullptr, nullptr, nullptr, nullptr), "lm_set_lengths");
+        HIP_TRY(hipDeviceSynchronize(), "lm_set_lengths");
+        lm->h_len = lens;
+        return SXQ_OK;
+    }
     for (int s = 0; s < n; ++s) lm->h_len[s] = lengths[s];
     HIP_TRY(hipMemcpy(lm->d_len, lm->h_len.data(), sizeof(int) * lm->c.max_batch, hipMemcpyHostToDevice), "lm_set_lengths");
     return SXQ_OK;
@@ -949,7 +1185,12 @@ sxq_status sxq_lm_reset(sxq_lm* lm, int n, void* stream) {
     std::lock_guard<std::mutex> lock(lm->mu);
     DeviceGuard g(lm->device);
     HIP_TRY(g.err, "hipSetDevice");
-    HIP_TRY(hipMemsetAsync(lm->d_len, 0, sizeof(int) * n, (hipStream_t)stream), "lm_reset");
+    if (lm->paged) {
+        HIP_TRY(launch_fill_int(lm->kv_add, n, INT32_MIN, (hipStream_t)stream), "lm_reset");
+        HIP_TRY(lm_reserve(lm, lm->kv_add, n, 0, nullptr, nullptr, nullptr, (hipStream_t)stream), "lm_reset");
+    } else {
+        HIP_TRY(hipMemsetAsync(lm->d_len, 0, sizeof(int) * n, (hipStream_t)stream), "lm_reset");
+    }
     for (int s = 0; s < n; ++s) lm->h_len[s] = 0;
     return SXQ_OK;
 }
@@ -967,9 +1208,10 @@ sxq_status sxq_lm_kv_fill_random(sxq_lm* lm, const int32_t* lengths, int n, uint
         std::lock_guard<std::mutex> lock(lm->mu);
         DeviceGuard g(lm->device);
         HIP_TRY(g.err, "hipSetDevice");
-        const int64_t total = lm->kv_layer_stride * lm->c.n_layers;
-        HIP_TRY(launch_fill_normal(lm->kc, total, seed * 2 + 11, 0.0f, 1.0f, nullptr), "lm_kv_fill_random");
-        HIP_TRY(launch_fill_normal(lm->vc, total, seed * 2 + 12, 0.0f, 1.0f, nullptr), "lm_kv_fill_random");
+        const int64_t total = (lm->paged ? lm->pool_layer : lm->kv_layer_stride) * lm->c.n_layers;
+        const int dt = lm->paged ? lm->pool.dtype : (int)kF32;
+        HIP_TRY(fill_cache(lm->paged ? lm->pool.k : lm->kc, total, dt, seed * 2 + 11), "lm_kv_fill_random");
+        HIP_TRY(fill_cache(lm->paged ? lm->pool.v : lm->vc, total, dt, seed * 2 + 12), "lm_kv_fill_random");
         HIP_TRY(hipDeviceSynchronize(), "lm_kv_fill_random");
     }
     return lengths ? sxq_lm_set_lengths(lm, lengths, n) : SXQ_OK;
@@ -984,13 +1226,19 @@ sxq_status sxq_lm_step(sxq_lm* lm, int n, const int32_t* ids, const float* embed
     for (int s = 0; s < n; ++s)
         if (lm->h_len[s] >= lm->c.max_seq)
             return fail(SXQ_ERR_INVALID, "lm_step: stream %d KV cache is full (%d positions)", s, lm->c.max_seq);
+    if (lm->paged) {
+        std::vector<int> lens = lm->h_len;
+        for (int s = 0; s < n; ++s) ++lens[s];
+        const sxq_status ok = check_pages(lm, "lm_step", lens);
+        if (ok != SXQ_OK) return ok;
+    }
     DeviceGuard g(lm->device);
     HIP_TRY(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;
     const bool emb = embeds != nullptr;
     if (ids) HIP_TRY(hipMemcpyAsync(lm->d_ids, ids, sizeof(int) * n * lm->ids_per, hipMemcpyDeviceToDevice, st), "lm_step: ids");
     if (emb) HIP_TRY(hipMemcpyAsync(lm->h, embeds, sizeof(float) * n * lm->c.dim, hipMemcpyDeviceToDevice, st), "lm_step: embeds");
-    lm->grid_splits = step_grid_splits(lm, n);
+    lm->grid_splits = lm->paged ? 0 : step_grid_splits(lm, n);
     if (flags & SXQ_LM_GRAPH) {
         const GraphKey key{n, emb, lm->trace, lm->grid_splits};
         auto it = lm->graphs.find(key);
@@ -1039,6 +1287,7 @@ sxq_status sxq_fish_fast_expand(sxq_lm* lm, int n, const float* hidden, const in
     if (!fish_sampling_fits(*params)) return fail(SXQ_ERR_INVALID, "fast_expand: top_k %d is negative", params->top_k);
     std::lock_guard<std::mutex> lock(lm->mu);
     if (lm->trace) return fail(SXQ_ERR_INVALID, "fast_expand: clear the step trace first");
+    if (lm->paged) return fail(SXQ_ERR_INVALID, "fast_expand: a paged engine (the frame's cache is n_codes positions)");
     DeviceGuard g(lm->device);
     HIP_TRY(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;
@@ -1115,7 +1364,13 @@ sxq_status sxq_lm_prefill(sxq_lm* lm, int n, const int32_t* counts, const int32_
     DeviceGuard g(lm->device);
     HIP_TRY(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;
-    const PfLayout P = pf_layout(lm, (int)T, n);
+    if (lm->paged) {
+        std::vector<int> lens = lm->h_len;
+        for (int s = 0; s < n; ++s) lens[s] += counts[s];
+        const sxq_status ok = check_pages(lm, "lm_prefill", lens);
+        if (ok != SXQ_OK) return ok;
+    }
+    const PfLayout P = pf_layout(lm, (int)T, pm);
     if (lm->pf_size < P.total) {
         HIP_TRY(hipDeviceSynchronize(), "lm_prefill: sync before regrowing the workspace");
         if (lm->pf) (void)hipFree(lm->pf);
@@ -1177,6 +1432,12 @@ sxq_status sxq_lm_read_kv(const sxq_lm* lm, int layer, int s, int g, int pos0, i
         return fail(SXQ_ERR_INVALID, "lm_read_kv: out of range");
     DeviceGuard gd(lm->device);
     HIP_TRY(gd.err, "hipSetDevice");
+    if (lm->paged) {
+        if (count == 0) return SXQ_OK;
+        HIP_TRY(launch_kv_gather(layer_pool(lm, layer), lm->kv_table, lm->max_blocks, lm->max_blocks, nullptr, s, 1, g, 1, pos0,
+                                 count, k_out, v_out, (hipStream_t)stream), "lm_read_kv");
+        return SXQ_OK;
+    }
     const int64_t off = (int64_t)layer * lm->kv_layer_stride + (int64_t)s * lm->kv_stream_stride +
                         ((int64_t)g * c.max_seq + pos0) * c.head_dim;
     const size_t bytes = sizeof(float) * (size_t)count * c.head_dim;

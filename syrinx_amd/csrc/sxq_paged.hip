@@ -6,6 +6,7 @@
 
 #include "../../include/sxq.h"
 #include "sxq_abi.h"
+#include "sxq_decoder.h"
 #include "sxq_paged.h"
 #include "sxq_paged_launch.h"
 
@@ -200,7 +201,7 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const KvReserve A, int mode) 
             const Sums s = sums(i);
             upto = upto + s;
             status[i] = a[i] >= 0 && (int64_t)old[i] + a[i] > top ? 2 : s.pages > 0 && upto.pages > avail ? 1
-                        : s.tokens > 0 && upto.tokens > A.capacity ? 3 : 0;
+                        : s.tokens > 0 && upto.tokens > A.limit ? 3 : 0;
             if (status[i] == 0) want = want + s;
             refused |= status[i] == 1 || status[i] == 3;
         }
@@ -249,7 +250,8 @@ __global__ __launch_bounds__(NT) void k_kv_reserve(const KvReserve A, int mode) 
                     A.table[(int64_t)(c0 + i[u]) * A.table_stride + s_have[i[u]] + (j[u] - s_pop[i[u]])] = id[u];
         }
         __syncthreads();  // the new table entries are read by the tokens' threads
-        for (int j = tid; mode == kAllInline && j < total.tokens; j += NT) {
+        const int mapped = min(total.tokens, A.capacity - min(given.tokens, A.capacity));
+        for (int j = tid; mode == kAllInline && j < mapped; j += NT) {
             const int i = owner(s_tok, rows, j);
             const int pos = s_old[i] + (j - s_tok[i]), t = given.tokens + j;
             A.slots[t] = kv_slot(A.table[(int64_t)(c0 + i) * A.table_stride + (pos >> A.shift)], pos, A.shift, A.n_pages);
@@ -416,6 +418,43 @@ void append_by_cache(const KvAppend& a, const KvPool& p, hipStream_t s) {
     else hipLaunchKernelGGL((k_kv_append<TI, __bf16>), grid, dim3(256), 0, s, a, p, log_lh);
 }
 
+// ---------------------------------------------------------------------------- gather
+// Eight elements of K and of V a thread.
+template <typename TC>
+__global__ __launch_bounds__(256) void k_kv_gather(const KvPool P, const int32_t* __restrict__ table, int64_t table_stride,
+                                                   int max_blocks, const int32_t* __restrict__ lens, int r0, int h0,
+                                                   int heads, int p0, int span, float* __restrict__ k,
+                                                   float* __restrict__ v) {
+    const int per = P.hd / 8, i = blockIdx.x * 256 + threadIdx.x, q = i / per, d = 8 * (i - q * per);
+    const int row = blockIdx.y / heads, h = blockIdx.y - row * heads, p = p0 + q;
+    if (q >= span || (lens && p >= kv_clamp_len(lens[r0 + row], max_blocks, P.shift))) return;
+    const int b = p >> P.shift;
+    const int slot = b < max_blocks ? kv_slot(table[(r0 + row) * table_stride + b], p, P.shift, P.n_pages) : -1;
+    const int64_t from = slot < 0 ? 0 : kv_slot_base(P, slot, h0 + h) + d;
+    const int64_t to = ((int64_t)blockIdx.y * span + q) * P.hd + d;
+#pragma unroll
+    for (int o = 0; o < 8; o += 4) {
+        float f[4] = {0.f, 0.f, 0.f, 0.f};
+        if (k) {
+            if (slot >= 0) load4((const TC*)P.k + from + o, f);
+            store4(k + to + o, f);
+        }
+        if (v) {
+            if (slot >= 0) load4((const TC*)P.v + from + o, f);
+            store4(v + to + o, f);
+        }
+    }
+}
+
+__global__ __launch_bounds__(64) void k_kv_counts(const PrefillMeta pm, int32_t* __restrict__ add) {
+    if ((int)threadIdx.x < pm.n) add[threadIdx.x] = pm.counts[threadIdx.x];
+}
+
+__global__ __launch_bounds__(256) void k_f32_to_bf16(const float* __restrict__ x, int64_t n, __bf16* __restrict__ y) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) y[i] = (__bf16)x[i];
+}
+
 bool kv_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
 bool pow2_page(int p) { return p >= 16 && p <= 1024 && (p & (p - 1)) == 0; }
 
@@ -440,6 +479,28 @@ hipError_t launch_kv_append(const KvAppend& a, const KvPool& p, hipStream_t s) {
     if (a.dtype == kF32) append_by_cache<float>(a, p, s);
     else if (a.dtype == kF16) append_by_cache<_Float16>(a, p, s);
     else append_by_cache<__bf16>(a, p, s);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table_stride, int max_blocks,
+                            const int32_t* lens, int r0, int rows, int h0, int heads, int p0, int span, float* k, float* v,
+                            hipStream_t s) {
+    const dim3 grid((unsigned)(((int64_t)span * (p.hd / 8) + 255) / 256), rows * heads);
+#define SXQ_GA(T) hipLaunchKernelGGL(k_kv_gather<T>, grid, dim3(256), 0, s, p, table, table_stride, max_blocks, lens, r0, h0, heads, p0, span, k, v)
+    if (p.dtype == kF32) SXQ_GA(float);
+    else if (p.dtype == kF16) SXQ_GA(_Float16);
+    else SXQ_GA(__bf16);
+#undef SXQ_GA
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_counts(const PrefillMeta& pm, int32_t* add, hipStream_t s) {
+    hipLaunchKernelGGL(k_kv_counts, dim3(1), dim3(64), 0, s, pm, add);
+    return hipGetLastError();
+}
+
+hipError_t launch_f32_to_bf16(const float* x, int64_t n, uint16_t* y, hipStream_t s) {
+    hipLaunchKernelGGL(k_f32_to_bf16, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, x, n, (__bf16*)y);
     return hipGetLastError();
 }
 
@@ -505,7 +566,7 @@ sxq_status sxq_kv_reserve(int device, int page_size, int n_pages, int n_rows, in
     a.n_pages = n_pages;
     a.n_rows = n_rows;
     a.max_blocks = max_blocks;
-    a.capacity = capacity;
+    a.capacity = a.limit = capacity;
     a.table_stride = table_stride;
     a.add = add;
     a.lens = lens;

@@ -7,7 +7,9 @@
 namespace sxq {
 
 struct KvReserve {
-    int shift, n_pages, n_rows, max_blocks, capacity;
+    int shift, n_pages, n_rows, max_blocks;
+    int capacity;  // entries of the map
+    int limit;     // tokens that may be handed out (the capacity, or more: the rest is not mapped)
     int64_t table_stride;
     const int32_t* add;
     int32_t *lens, *table, *free_list, *free_count, *cu, *slots, *pos, *rows, *status;
@@ -41,6 +43,18 @@ struct KvAttend {
 };
 size_t kv_attend_workspace(const KvPool& p, int n_q, int nh);
 hipError_t launch_kv_attend(const KvAttend& a, const KvPool& p, hipStream_t s);
+
+// One layer's positions p0 .. p0 + span - 1 of rows r0 .. r0 + rows - 1 and KV heads h0 .. as
+// f32 [row][head][span][hd] (either output may be null): with lens those below the row's length,
+// without it all.  An absent page reads as zeros.
+hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table_stride, int max_blocks,
+                            const int32_t* lens, int r0, int rows, int h0, int heads, int p0, int span, float* k, float* v,
+                            hipStream_t s);
+// add[i] = pm.counts[i], i < pm.n (a prompt's growths).
+struct PrefillMeta;
+hipError_t launch_kv_counts(const PrefillMeta& pm, int32_t* add, hipStream_t s);
+// bf16 (round to nearest even) of n f32 values.
+hipError_t launch_f32_to_bf16(const float* x, int64_t n, uint16_t* y, hipStream_t s);
 
 namespace abi {
 // The checks every entry point makes of its pages, and their kernel form.

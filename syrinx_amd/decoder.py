@@ -125,15 +125,31 @@ def fish_s2_fast_ar_config(n_layers=4, num_codebooks=10, residual_size=4096, max
 
 
 class DecoderLM:
-    """A decode-step engine (sxq_lm) on one GPU."""
+    """A decode-step engine (sxq_lm) on one GPU.
 
-    def __init__(self, cfg: DecoderConfig, device="cuda:0"):
+    With kv_pages, its cache is paged (sxq_lm_create_paged): that many pages of page_size
+    positions a layer, of kv_dtype (torch.float32 or torch.bfloat16), shared by all streams,
+    instead of max_seq f32 positions reserved for each."""
+
+    def __init__(self, cfg: DecoderConfig, device="cuda:0", kv_pages: int = None, page_size: int = 32,
+                 kv_dtype: torch.dtype = torch.float32):
         self.cfg = cfg
         self.device = torch.device(device)
         self._h = ctypes.c_void_p()
         self._c = cfg.to_c()
-        check(lib().sxq_lm_create(self._dev(), ctypes.byref(self._c), ctypes.byref(self._h)))
+        if kv_pages is None:
+            check(lib().sxq_lm_create(self._dev(), ctypes.byref(self._c), ctypes.byref(self._h)))
+        else:
+            code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(kv_dtype, -1)
+            check(lib().sxq_lm_create_paged(self._dev(), ctypes.byref(self._c), code, int(page_size), int(kv_pages),
+                                            ctypes.byref(self._h)))
         self.ids_per = 1 + cfg.n_codebooks
+
+    def free_pages(self) -> int:
+        """Pages that no stream of a paged engine holds."""
+        n = ctypes.c_int()
+        check(lib().sxq_lm_free_pages(self._h, ctypes.byref(n)))
+        return int(n.value)
 
     def _dev(self) -> int:
         return self.device.index if self.device.index is not None else torch.cuda.current_device()

@@ -136,11 +136,12 @@ def _layer_count(names, pattern: str) -> int:
     return max(idx) + 1 if idx else 0
 
 
-def cv2_engine(bag: Cv2Weights, max_seq: int = 1024, max_batch: int = 1, device="cuda:0") -> Qwen2Lm:
+def cv2_engine(bag: Cv2Weights, max_seq: int = 1024, max_batch: int = 1, device="cuda:0", **pages) -> Qwen2Lm:
     """A Qwen2Lm decode engine over a load_cv2_quantized bag: per layer q/k/v (fused on
     upload) with their biases, o, gate/up/down, the two RMSNorms; the final norm, the
     llm_decoder head with its bias, and speech_embedding as the (quantized) input table.
-    Geometry from the tensors; heads from head_dim 64 (cv2/mod.rs:36-56)."""
+    Geometry from the tensors; heads from head_dim 64 (cv2/mod.rs:36-56).  pages: DecoderLM's
+    kv_pages, page_size and kv_dtype, for a paged cache."""
     pre = "llm.model.model.layers"
     names = list(bag.qmm) + list(bag.w)
     L = _layer_count(names, re.escape(pre) + r"\.(\d+)\.")
@@ -155,7 +156,7 @@ def cv2_engine(bag: Cv2Weights, max_seq: int = 1024, max_batch: int = 1, device=
                                n_heads=q0[0] // hd, n_kv_heads=k0[0] // hd, head_dim=hd, intermediate=gate[0],
                                vocab=head[0], embed_rows=speech.rows_count if speech is not None else head[0] + 3,
                                head_bias=int("llm_decoder.bias" in bag.w))
-    lm = Qwen2Lm(cfg, device=device)
+    lm = Qwen2Lm(cfg, device=device, **pages)
     for l in range(L):
         p = f"{pre}.{l}"
         for slot, nm in ((WQ, "self_attn.q_proj"), (WK, "self_attn.k_proj"), (WV, "self_attn.v_proj"),
@@ -173,11 +174,11 @@ def cv2_engine(bag: Cv2Weights, max_seq: int = 1024, max_batch: int = 1, device=
     return lm
 
 
-def cosyvoice_lm(bag: Cv2Weights, max_seq: int = 1024, device="cuda:0"):
+def cosyvoice_lm(bag: Cv2Weights, max_seq: int = 1024, device="cuda:0", **pages):
     """Qwen2Lm (CosyVoice2) or Cv3Lm (CosyVoice3, told apart by the 6761-row bias-free head)
     ready to generate: cv2_engine over the bag plus its embedding tables (QEmbeds or dense)."""
     from .generate import COSYVOICE2, COSYVOICE3, CosyVoiceLm
-    lm = cv2_engine(bag, max_seq=max_seq, max_batch=1, device=device)
+    lm = cv2_engine(bag, max_seq=max_seq, max_batch=1, device=device, **pages)
     variant = COSYVOICE2 if lm.cfg.head_bias else COSYVOICE3
 
     def table(name):
@@ -397,14 +398,15 @@ def _wire_fish(lm, w: dict, base: str, L: int, dtype: GgmlDType, qk_norm: bool) 
 
 def fish_engines(w: dict, n_codebooks: int = 10, semantic_begin: int = 151678, semantic_end: int = 155773,
                  max_seq: int = 1280, max_batch: int = 1, dtype: GgmlDType = GgmlDType.Q4K, device="cuda:0",
-                 head_dim: int = 128):
+                 head_dim: int = 128, **pages):
     """SlowAr + FastAr over a load_fish_lm bag, projections quantized to `dtype`.  The slow
     head is tied to `embeddings` unless `output.weight` ships (slow_ar.rs:213-221), and the
     token embedding gathers the dense `embeddings.weight` either way (slow_ar.rs:117; a
     GGUF bag holds that table only quantized, and then the embedding dequantizes its
     rows).  qkv / o bias and QK-norm of each stack come from its tensors (slow_ar.rs:86-98,
     fast_ar.rs:53-65); a `fast_project_in` maps the slow hidden onto a narrower fast AR
-    (slow_ar.rs:230-243)."""
+    (slow_ar.rs:230-243).  pages: DecoderLM's kv_pages, page_size and kv_dtype, for a paged
+    cache of the slow AR."""
     Ls, Lf = _fish_layers(w, "layers"), _fish_layers(w, "fast_layers")
     emb = w["embeddings.weight"]
     vocab, dim = emb.shape
@@ -420,7 +422,7 @@ def fish_engines(w: dict, n_codebooks: int = 10, semantic_begin: int = 151678, s
                                  vocab=vocab, codebook_size=cb.shape[0] // n_codebooks, semantic_begin=semantic_begin,
                                  semantic_end=semantic_end, tied_embedding=int("output.weight" not in w),
                                  **_attn_flags(w, "layers"))
-    slow = SlowAr(cfg, device=device)
+    slow = SlowAr(cfg, device=device, **pages)
     _wire_fish(slow, w, "layers", Ls, dtype, bool(cfg.qk_norm))
     slow.set_linear(-1, HEAD, _q(w, "output.weight" if "output.weight" in w else "embeddings.weight", dtype))
     if not isinstance(emb, QTensor):
