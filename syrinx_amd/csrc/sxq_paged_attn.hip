@@ -8,6 +8,7 @@
 #include "sxq_abi.h"
 #include "sxq_paged.h"
 #include "sxq_paged_launch.h"
+#include "sxq_quant_dev.h"
 #include "sxq_sync_dev.h"
 
 using namespace sxq;
@@ -35,6 +36,12 @@ constexpr int kTile = 32;
 constexpr int kWaves = 4;
 constexpr int kMinTiles = 4;    // of an item: one a wave
 constexpr int kMaxItems = 256;  // of one query
+// With a card's worth of items this short (or shorter) latency counts: a join (publishing, an
+// atomic, two loads in turn) is 3 us, and a CU takes in a tile for each wave in 1.2 us (16-bit,
+// head width 128: 56 GB/s, whatever is in flight).  Queries up to kWholeTiles stay whole: one
+// of 256 positions 6.7 us against 8.5 split, of 384 8.4 / 8.7 (f32, width 64), of 500 9.0 / 8.6.
+constexpr int kFewTiles = 8;
+constexpr int kWholeTiles = 12;
 constexpr int kCountBytes = 1 << 18;  // 64 bytes a split query, KV head and 16 heads
 
 SXQ_HD int attend_head_tiles(int nh, int nkv) { return (nh / nkv + 15) / 16; }
@@ -48,12 +55,15 @@ inline int attend_slots(int nh, int nkv, int hd) {
 // Many: smaller items, dealt as workgroups finish.  Measured at 32 / 8 heads of 128, 64 slots
 // (us): 16 queries of 256..2040 positions by 48 / 64 / 256 pieces 19.5 / 21.0 / 27.9; one of
 // 131071 by 64 / 128 / 256 104 / 114 / 122; 64 of 1000..16384 by 64 / 128 / 256 306 / 271 / 267.
-inline int attend_target(int n_q, int nh, int nkv, int hd) {
-    const int slots = attend_slots(nh, nkv, hd);
-    return std::min(kMaxItems, std::max(1, n_q <= slots / 2 ? slots - n_q + 1 : 4 * slots));
+// (never more split queries than counters have a place: kCountBytes)
+inline int attend_target_max(int nh, int nkv, int hd) {
+    const int counters = kCountBytes / 64 / (nkv * attend_head_tiles(nh, nkv));
+    return std::max(1, std::min({kMaxItems, 4 * attend_slots(nh, nkv, hd), counters}));
 }
-// The most of any number of queries.
-inline int attend_target_max(int nh, int nkv, int hd) { return std::min(kMaxItems, 4 * attend_slots(nh, nkv, hd)); }
+inline int attend_target(int n_q, int nh, int nkv, int hd) {
+    const int slots = attend_slots(nh, nkv, hd), most = attend_target_max(nh, nkv, hd);
+    return n_q <= slots / 2 ? std::min(slots - n_q + 1, most) : most;
+}
 // A partial: {m, l} and the weighted sum of one head.
 SXQ_HD size_t attend_part_floats(int hd) { return (size_t)hd + 4; }
 
@@ -68,6 +78,17 @@ SXQ_DEV int wave_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
     v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
     return v;
+}
+
+// ceil(a / b), 0 <= a < 2^30, 0 < b < 2^30: below 2^22 the quotient from a reciprocal is off by
+// at most one either way.
+SXQ_DEV int ceil_div(int a, int b) {
+    if (a >= 1 << 22) return (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b);
+    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+    int r = a - q * b;
+    if (r < 0) r += b, --q;
+    if (r >= b) r -= b, ++q;
+    return q + (r > 0);
 }
 
 // Lane l's query of the block of 64 from b0: its table row and length (-1: none).
@@ -97,16 +118,19 @@ SXQ_DEV bool find_item(const KvAttend& A, const KvPool& P, int target, int x, It
         load_query(A, P, b0, r, n);
         total += __builtin_amdgcn_readlane(wave_scan(tiles_of(n)), 63);
     }
-    const int piece = max(kMinTiles, (total + target - 1) / target);
+    int piece = ceil_div(total, target);
+    const bool few = piece <= kFewTiles;
+    piece = max(kMinTiles, piece);
     int items0 = 0, single0 = 0, split0 = 0;  // over the queries before this block of 64
     for (int b0 = 0; b0 < A.n_q; b0 += 64) {
         if (b0) load_query(A, P, b0, row, len);
         const int tiles = tiles_of(len);
         // an even cut: the fewest items of at most piece tiles (short ones: as many for each wave)
-        int n = max(1, (tiles + piece - 1) / piece);
-        int per = (tiles + n - 1) / n;
+        int n = max(1, ceil_div(tiles, piece));
+        if (few && tiles <= kWholeTiles) n = 1;
+        int per = ceil_div(tiles, n);
         if (per <= 4 * kWaves) per = (per + kWaves - 1) / kWaves * kWaves;
-        n = len < 0 ? 0 : max(1, per ? (tiles + per - 1) / per : 1);
+        n = len < 0 ? 0 : max(1, ceil_div(tiles, max(per, 1)));
         const int incl = wave_scan(n);
         const uint64_t single = __ballot(n == 1), split = __ballot(n > 1);
         const uint64_t mine = __ballot(x >= items0 + incl - n && x < items0 + incl);
@@ -195,6 +219,12 @@ SXQ_DEV float head_sum(float v) {
     swap16(a, b);
     return a + b;
 }
+// 8 bytes coherent at agent scope, as load16_coherent.
+SXQ_DEV float2 load8_coherent(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 v = __builtin_bit_cast(f2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 16));
+    return make_float2(v.x, v.y);
+}
 SXQ_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Four columns of an output row: the weighted sum over the weights' sum, zeros without any.
@@ -202,8 +232,9 @@ template <typename TQ>
 SXQ_DEV void store_out(const KvAttend& A, int b, int64_t at, v4f v, float l, TQ*) {
     typedef TQ v4 __attribute__((ext_vector_type(4)));
     v4 o;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = from_f32<TQ>(l == 0.0f ? 0.0f : v[e] / l);
+    for (int e = 0; e < 4; ++e) o[e] = from_f32<TQ>(v[e] * inv);
     *(v4*)((TQ*)A.out + (int64_t)b * A.out_stride + at) = o;
 }
 
@@ -219,7 +250,8 @@ struct Shape {
 // One head of one item, {m, l} and the sum: m is the maximum of scale * log2(e) * score (or
 // 0 where none is above -inf), l and the sum carry the weights 2^(x - m + kWeightShift).
 template <typename TQ, typename T, int HDP, bool FULL>
-__global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPool P, int target) {
+__global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv_attend(const KvAttend A, const KvPool P,
+                                                                                        int target) {
     typedef Shape<T, HDP> S;
     typedef PageOps<T> O;
     constexpr int H = S::kH, KS = S::kKS, VW = S::kVW, BLK = S::kBlk, D = S::kD;
@@ -238,10 +270,16 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
     const int kh = blockIdx.y / ht, h0 = kh * G + (blockIdx.y - kh * ht) * 16;
     const int heads = min(16, (kh + 1) * G - h0);
     const float scale2 = A.scale * 1.44269504088896340736f;
-    // where this lane reads within a half tile's 16 positions (bytes)
-    const int ps = (int)P.pos_stride * (int)sizeof(T);
-    const uint32_t kcol = (F32 ? 4 : 8) * g * (int)sizeof(T), vcol = VW * r * (int)sizeof(T);
-    const uint32_t koff = (uint32_t)(r * ps), voff = (uint32_t)(4 * g * ps);
+    // where this lane reads within a half tile's 16 positions (bytes): 16 of key r at kcol + 64 s,
+    // and its columns of the values 4 g + i
+    const uint32_t ps = (uint32_t)P.pos_stride * (uint32_t)sizeof(T), row_bytes = (uint32_t)hd * sizeof(T);
+    const uint32_t kcol = 16 * g, koff = r * ps, vcol = VW * r * (uint32_t)sizeof(T);
+    uint32_t voff[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) voff[i] = (4 * g + i) * ps;
+    const char* kpool = (const char*)P.k + (int64_t)kh * P.head_stride * (int64_t)sizeof(T);
+    const char* vpool = (const char*)P.v + (int64_t)kh * P.head_stride * (int64_t)sizeof(T);
+    const int64_t page_bytes = P.page_stride * (int64_t)sizeof(T);
 
     Item it;
     if (!find_item(A, P, target, blockIdx.x, it)) return;
@@ -299,34 +337,36 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
 
     uint32_t kreg[H][KS][4], vreg[H][4][BLK][VW * sizeof(T) / 4];
     int id[H];
-    auto half_base = [&](const void* pool, int t, int page) {
-        return (const char*)pool + (kv_page_base(P, max(page, 0), kh) + (int64_t)((t * 16) & (P.page - 1)) * P.pos_stride) * (int64_t)sizeof(T);
-    };
-    auto load_k = [&](int t) {
+    // (scalar bases and 32-bit lane offsets: the loads take both as they are)
+    int64_t at[H];
+    auto place = [&](int t) {
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            const char* base = half_base(P.k, t + h, id[h]);
+        for (int h = 0; h < H; ++h)
+            at[h] = max(id[h], 0) * page_bytes + (int64_t)((uint32_t)(((t + h) * 16) & (P.page - 1)) * (uint64_t)ps);
+    };
+    auto load_k = [&]() {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const uint32_t col = (uint32_t)(64 * s) + kcol;  // 16 f32 or 32 16-bit elements a step
-                const bool in = FULL || col < (uint32_t)hd * sizeof(T);
-                const v4u v = *(const v4u*)(base + (koff + (in ? col : 0)));
+                v4u v;
+                if constexpr (FULL) v = *(const v4u*)(kpool + at[h] + 64 * s + (koff + kcol));
+                else v = *(const v4u*)(kpool + at[h] + (koff + (64 * s + kcol < row_bytes ? 64 * s + kcol : 0)));
 #pragma unroll
                 for (int e = 0; e < 4; ++e) kreg[h][s][e] = v[e];
             }
-        }
     };
-    auto load_v = [&](int t) {
+    auto load_v = [&]() {
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            const char* base = half_base(P.v, t + h, id[h]);
+        for (int h = 0; h < H; ++h)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int b = 0; b < BLK; ++b) {
-                    const uint32_t col = (uint32_t)(b * 16 * VW * (int)sizeof(T)) + vcol;
-                    const bool in = FULL || col < (uint32_t)hd * sizeof(T);
-                    const char* src = base + (int64_t)i * ps + (voff + (in ? col : 0));
+                    constexpr uint32_t kBlkBytes = 16 * VW * sizeof(T);
+                    const char* src;
+                    if constexpr (FULL) src = vpool + at[h] + b * kBlkBytes + (voff[i] + vcol);
+                    else src = vpool + at[h] + (voff[i] + (b * kBlkBytes + vcol < row_bytes ? b * kBlkBytes + vcol : 0));
                     if constexpr (VW * sizeof(T) == 16) {
                         const v4u v = *(const v4u*)src;
 #pragma unroll
@@ -337,7 +377,6 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
                         vreg[h][i][b][1] = v[1];
                     }
                 }
-        }
     };
 
     int t = t0, k = 0;  // the tile's first half, its number in the batch
@@ -346,9 +385,18 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
         for (int h = 0; h < H; ++h) id[h] = __builtin_amdgcn_readlane(pages, k * H + h);
     };
     if (t < t_end) {
-        ids();
-        load_k(t);
-        load_v(t);
+        // the first tile's pages by scalar loads, which do not queue behind the card's other
+        // vector loads
+        typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+        const scalar_ptr st = (scalar_ptr)(uintptr_t)table;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const int page = st[min(t + h, t_last) >> log_p];
+            id[h] = t + h <= t_last && kv_page_ok(page, P.n_pages) ? page : -1;
+        }
+        place(t);
+        load_k();
+        load_v();
         if (t + 64 / H * (kWaves * H) < t_end) pages_next = page_batch(1);
     }
     int batch = 1;
@@ -365,7 +413,7 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 if constexpr (!FULL) {
-                    const bool in = (uint32_t)(64 * s) + kcol < (uint32_t)hd * sizeof(T);
+                    const bool in = 64 * s + kcol < row_bytes;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) kreg[h][s][e] = in ? kreg[h][s][e] : 0;
                 }
@@ -404,7 +452,8 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
                 pages_next = page_batch(++batch);
             }
             ids();
-            load_k(next);
+            place(next);
+            load_k();
         }
         // the running maximum moves only where a score passes it
         float mx = x[0][0];
@@ -459,6 +508,7 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
                     part[p][j] = (T)w[j >> 2][j & 3];
                     w[j >> 2][j & 3] -= (float)part[p][j];
                 }
+            typename O::V8 cols[D];
 #pragma unroll
             for (int b = 0; b < BLK; ++b)
 #pragma unroll
@@ -468,12 +518,14 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
                     for (int j = 0; j < 4; ++j)  // positions 2 j and 2 j + 1 of the lane's eight
                         a[j] = __builtin_amdgcn_perm(vreg[j >> 1][2 * (j & 1) + 1][b][e / 2], vreg[j >> 1][2 * (j & 1)][b][e / 2],
                                                      e & 1 ? 0x07060302 : 0x05040100);
-#pragma unroll
-                    for (int p = WP - 1; p >= 0; --p)
-                        acc[b * VW + e] = O::mfma(__builtin_bit_cast(typename O::V8, a), part[p], acc[b * VW + e]);
+                    cols[b * VW + e] = __builtin_bit_cast(typename O::V8, a);
                 }
+#pragma unroll
+            for (int p = WP - 1; p >= 0; --p)  // the small parts first; D products between two of one register
+#pragma unroll
+                for (int d = 0; d < D; ++d) acc[d] = O::mfma(cols[d], part[p], acc[d]);
         }
-        if (more) load_v(next);
+        if (more) load_v();
         t = next;
     }
     l = head_sum(l);
@@ -499,11 +551,12 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
     }
     __syncthreads();
     const int per = hd / 4, n_out = heads * per;  // four columns a thread
-    const size_t pf = attend_part_floats(hd), step = (size_t)A.nh * pf;  // a partial's floats; from slot to slot
-    float* parts = (float*)((char*)A.ws + kCountBytes) + (size_t)h0 * pf;
+    // a partial's bytes; from item to item (all items of a query: below 2^27)
+    const uint32_t pf = (uint32_t)(attend_part_floats(hd) * sizeof(float)), step = (uint32_t)A.nh * pf;
+    char* parts = (char*)A.ws + kCountBytes + (size_t)h0 * pf;
     const bool split = it.count > 1;
     const __amdgpu_buffer_rsrc_t mine =
-        coherent_rsrc(parts + (it.part0 + it.index) * step, (uint32_t)(heads * pf * sizeof(float)));
+        coherent_rsrc(parts + (size_t)(it.part0 + it.index) * step, heads * pf);
     for (int o = tid; o < n_out; o += 256) {
         const int h = o / per, c = 4 * (o - h * per);
         float Mh = s_m[0][h], L = 0.0f;
@@ -519,86 +572,82 @@ __global__ __launch_bounds__(256) void k_kv_attend(const KvAttend A, const KvPoo
         if (!split) {
             store_out(A, it.b, (h0 + h) * hd + c, v, L, (TQ*)nullptr);
         } else {
-            store16_coherent(mine, (uint32_t)((h * pf + 4 + c) * sizeof(float)), make_float4(v[0], v[1], v[2], v[3]));
-            if (c == 0) store16_coherent(mine, (uint32_t)(h * pf * sizeof(float)), make_float4(Mh, L, 0.f, 0.f));
+            store16_coherent(mine, h * pf + 16 + 4 * c, make_float4(v[0], v[1], v[2], v[3]));
+            if (c == 0) store16_coherent(mine, h * pf, make_float4(Mh, L, 0.f, 0.f));
         }
     }
     if (!split) return;
-    // The last of the query's items to arrive joins them, in their order: a wave takes every
-    // fourth head, reads its {m, l} of all items at once and leaves the items' factors in LDS;
-    // then the sums, the items dealt over the threads that share four columns.  A thread's
-    // first eight are in flight while the factors are made.
+    // The last of the query's items to arrive joins them, in their order.  The loads go out
+    // first -- up to kFetch partials of four columns a thread (the items dealt over the threads
+    // that share them), then {m, l} of the wave's heads, every fourth, over all items -- and the
+    // latter give the items' factors, through LDS, while the partials are in flight.
     unsigned* counter = (unsigned*)A.ws + ((size_t)it.slot * gridDim.y + blockIdx.y) * 16;
+    const int sub = n_out < 256 ? 256 / n_out : 1;  // threads that share four columns
+    const int k0 = n_out < 256 ? tid / n_out : 0, o_first = tid - k0 * n_out;
+    const int h_first = min(o_first, n_out - 1) / per;
     if (!publish_and_count(counter, it.count, &s_last)) return;
-    {
-        if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const __amdgpu_buffer_rsrc_t all = coherent_rsrc(parts + it.part0 * step, 0xFFFFFFFFu);
-        auto slot = [&](int i) { return (uint32_t)(i * step * sizeof(float)); };
-        const int sub = n_out < 256 ? 256 / n_out : 1;  // threads that share four columns
-        const int k0 = n_out < 256 ? tid / n_out : 0;
-        auto column = [&](int o) {
-            const int h = o / per;
-            return (uint32_t)((h * pf + 4 + 4 * (o - h * per)) * sizeof(float));
-        };
-        const int first_o = n_out < 256 ? tid - k0 * n_out : tid;
-        // eight of a thread's partials from the i-th on (repeating the last; its factor is then 0)
-        auto fetch = [&](float4 (&p)[8], int o, int i) {
+    if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    constexpr int kFetch = 8;
+    const int count = it.count;
+    const __amdgpu_buffer_rsrc_t all = coherent_rsrc(parts + (size_t)it.part0 * step, 0xFFFFFFFFu);
+    float* factor = &s_acc[0][0][0];  // [heads][kMaxItems]
+    static_assert(sizeof s_acc >= 16 * kMaxItems * sizeof(float), "the factors fit the waves' sums");
+    bool first = true;
+    for (int o0 = 0; o0 < n_out; o0 += 256) {
+        const int o = o_first + o0, oc = min(o, n_out - 1), h = o0 ? oc / per : h_first;
+        const uint32_t from = h * pf + 16 + 16 * (oc - h * per);
+        v4f v = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < count; i0 += kFetch * sub) {
+            float4 p[kFetch];  // (past the last item it repeats, without effect)
 #pragma unroll
-            for (int u = 0; u < 8; ++u) p[u] = load16_coherent(all, column(o) + slot(min(i + u * sub, it.count - 1)));
-        };
-        float4 p[8];
-        fetch(p, min(first_o, n_out - 1), k0);
-        float* factor = &s_acc[0][0][0];  // [heads][kMaxItems]
-        static_assert(sizeof s_acc >= 16 * kMaxItems * sizeof(float), "the factors fit the waves' sums");
-        for (int h = wave; h < heads; h += kWaves) {
-            float4 ml[kMaxItems / 64];
-            float Mh = -INFINITY, L = 0.0f;
+            for (int u = 0; u < kFetch; ++u) p[u] = load16_coherent(all, from + min(i0 + k0 + u * sub, count - 1) * step);
+            if (first) {
+                first = false;
+                float mx[4], sum[4];
 #pragma unroll
-            for (int j = 0; j < kMaxItems / 64; ++j) {
-                const int i = lane + 64 * j;
-                ml[j] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-                if (i < it.count) ml[j] = load16_coherent(all, slot(i) + (uint32_t)(h * pf * sizeof(float)));
-                Mh = fmaxf(Mh, ml[j].x);
-            }
+                for (int q = 0; q < 4; ++q) mx[q] = -INFINITY, sum[q] = 0.0f;
+                for (int i = lane; i < count; i += 64) {
+                    float2 ml[4];
 #pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) Mh = fmaxf(Mh, __shfl_xor(Mh, o, 64));
+                    for (int q = 0; q < 4; ++q) ml[q] = load8_coherent(all, min(wave + kWaves * q, heads - 1) * pf + i * step);
 #pragma unroll
-            for (int j = 0; j < kMaxItems / 64; ++j) {
-                const float f = ml[j].x > -INFINITY ? exp2_fast(ml[j].x - Mh) : 1.0f;
-                if (lane + 64 * j < it.count) factor[h * kMaxItems + lane + 64 * j] = f;
-                L += ml[j].y * f;
-            }
-#pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o, 64);
-            if (lane == 0) s_l[0][h] = L;
-        }
-        __syncthreads();
-        for (int o0 = 0; o0 < n_out; o0 += 256) {
-            const int o = first_o + o0;
-            const bool in = k0 < sub && o < n_out;
-            const int h = in ? o / per : 0;
-            v4f v = {0.f, 0.f, 0.f, 0.f};
-            if (in) {
-                if (o0) fetch(p, o, k0);
-                for (int i = k0; i < it.count;) {
-#pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const int n = i + u * sub;
-                        const float f = n < it.count ? factor[h * kMaxItems + n] : 0.0f;
-                        if (n < it.count) v += (v4f){p[u].x * f, p[u].y * f, p[u].z * f, p[u].w * f};
+                    for (int q = 0; q < 4; ++q) {
+                        factor[(wave + kWaves * q) * kMaxItems + i] = ml[q].x;
+                        const float mn = fmaxf(mx[q], ml[q].x);
+                        const float up = mx[q] > -INFINITY ? exp2_fast(mx[q] - mn) : 1.0f;
+                        sum[q] = sum[q] * up + ml[q].y * (ml[q].x > -INFINITY ? exp2_fast(ml[q].x - mn) : 1.0f);
+                        mx[q] = mn;
                     }
-                    i += 8 * sub;
-                    if (i < it.count) fetch(p, o, i);
                 }
-            }
-            if (sub > 1) {
-                s_red[tid] = v;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float Mh = wave_max_rows(mx[q]);
+                    const float L = wave_sum_rows(sum[q] * (mx[q] > -INFINITY ? exp2_fast(mx[q] - Mh) : 1.0f));
+                    if (lane == 0) s_l[q][wave] = L;
+                    mx[q] = Mh;
+                }
+                for (int i = lane; i < count; i += 64)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float* f = factor + (wave + kWaves * q) * kMaxItems + i;
+                        *f = *f > -INFINITY ? exp2_fast(*f - mx[q]) : 1.0f;
+                    }
                 __syncthreads();
-                if (k0 == 0)
-                    for (int u = 1; u < sub; ++u) v += s_red[u * n_out + o];
             }
-            if (in && k0 == 0) store_out(A, it.b, (h0 + h) * hd + 4 * (o - h * per), v, s_l[0][h], (TQ*)nullptr);
+#pragma unroll
+            for (int u = 0; u < kFetch; ++u) {
+                const int n = i0 + k0 + u * sub;
+                const float f = factor[h * kMaxItems + min(n, count - 1)];
+                if (n < count) v += (v4f){p[u].x * f, p[u].y * f, p[u].z * f, p[u].w * f};
+            }
         }
+        if (sub > 1) {
+            s_red[tid] = v;
+            __syncthreads();
+            if (k0 == 0)
+                for (int u = 1; u < sub; ++u) v += s_red[u * n_out + o];
+        }
+        if (k0 == 0 && o < n_out) store_out(A, it.b, (h0 + h) * hd + 4 * (o - h * per), v, s_l[h >> 2][h & 3], (TQ*)nullptr);
     }
 }
 

@@ -448,6 +448,16 @@ def test_attend_long_caches(cuda, qt, ct, lens, nh, nkv, hd, page):
     _close(cache.attend(0, q), want, bound, DT[qt])
 
 
+def test_attend_more_heads_than_the_card_has_places(cuda):
+    """900 KV heads of 18 query heads (two tiles of 16 each): more workgroups a piece than split
+    queries have counters for."""
+    cache, g = _filled(cuda, 900, 8, 16, [1500, 400, 0, 33], "bf16", 12)
+    q = torch.randn((4, 900 * 18, 8), generator=g, device=cuda).bfloat16()
+    want, bound = _attend_reference(q, cache.k[0], cache.v[0], cache.table, cache.lens, range(4), 8 ** -0.5)
+    for _ in range(2):
+        _close(cache.attend(0, q), want, bound, torch.bfloat16)
+
+
 @pytest.mark.parametrize("n", [100, 300])
 def test_attend_many_requests(cuda, n):
     rng = np.random.default_rng(n)
