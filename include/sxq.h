@@ -265,9 +265,11 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
  * most 2^30.  What lies past a request's length, in its last page or elsewhere, may hold
  * anything; a key or value of its own that is not finite makes the outputs that read it not
  * finite.  Two calls on the same inputs give the same bits.
- * workspace (sxq_kv_attention_workspace bytes, 256-byte aligned) is zeroed by the caller
- * before its first use; every call leaves it ready for the next of the same or smaller
- * n_q * n_heads.  Calls that share one must not overlap. */
+ * workspace: sxq_kv_attention_workspace bytes, 256-byte aligned, of which the caller zeroes
+ * the first SXQ_KV_COUNTER_BYTES before its first use; every call leaves them zero, and the
+ * workspace good for any call that needs no more bytes.  Calls that share one must not
+ * overlap: a captured graph keeps one of its own. */
+#define SXQ_KV_COUNTER_BYTES 262144
 sxq_status sxq_kv_attention_workspace(const sxq_kv_pages *pages, int n_q, int n_heads, size_t *bytes);
 sxq_status sxq_kv_attention(int device, const sxq_kv_pages *pages, int q_dtype, const void *q, int64_t q_stride,
                             int n_q, int n_heads, const int32_t *rows, const int32_t *lens, int n_rows,

@@ -42,7 +42,7 @@ constexpr int kMaxItems = 256;  // of one query
 // of 256 positions 6.7 us against 8.5 split, of 384 8.4 / 8.7 (f32, width 64), of 500 9.0 / 8.6.
 constexpr int kFewTiles = 8;
 constexpr int kWholeTiles = 12;
-constexpr int kCountBytes = 1 << 18;  // 64 bytes a split query, KV head and 16 heads
+constexpr int kCountBytes = SXQ_KV_COUNTER_BYTES;  // 64 bytes a split query, KV head and 16 heads
 
 SXQ_HD int attend_head_tiles(int nh, int nkv) { return (nh / nkv + 15) / 16; }
 // Workgroups per KV head and 16 query heads that the card holds at once (four a CU at head
@@ -51,14 +51,16 @@ inline int attend_slots(int nh, int nkv, int hd) {
     const int all = hd <= 64 ? 1024 : hd <= 128 ? 512 : 256;
     return std::max(1, all / (nkv * attend_head_tiles(nh, nkv)));
 }
-// Few queries: all items (fewer than target + n_q) resident at once, no second round for a few.
-// Many: smaller items, dealt as workgroups finish.  Measured at 32 / 8 heads of 128, 64 slots
-// (us): 16 queries of 256..2040 positions by 48 / 64 / 256 pieces 19.5 / 21.0 / 27.9; one of
-// 131071 by 64 / 128 / 256 104 / 114 / 122; 64 of 1000..16384 by 64 / 128 / 256 306 / 271 / 267.
+// Few queries (up to half the slots): all items (fewer than target + n_q) resident at once, no
+// second round for a few.  Many: smaller items, dealt as workgroups finish.  Measured at 32 / 8
+// heads of 128, 64 slots (us): 16 queries of 256..2040 positions by 48 / 64 / 256 pieces 19.5 /
+// 21.0 / 27.9; 32 of 500..4000 by 33 / 128 / 256 51.1 / 58.2 / 55.7; one of 131071 by 64 / 128 /
+// 256 104 / 114 / 122; 64 of 1000..16384 by 64 / 128 / 256 293 / 269 / 270, 256 of 100..3000
+// 181 / 180 / 188.
 // (never more split queries than counters have a place: kCountBytes)
 inline int attend_target_max(int nh, int nkv, int hd) {
     const int counters = kCountBytes / 64 / (nkv * attend_head_tiles(nh, nkv));
-    return std::max(1, std::min({kMaxItems, 4 * attend_slots(nh, nkv, hd), counters}));
+    return std::max(1, std::min({kMaxItems, 2 * attend_slots(nh, nkv, hd), counters}));
 }
 inline int attend_target(int n_q, int nh, int nkv, int hd) {
     const int slots = attend_slots(nh, nkv, hd), most = attend_target_max(nh, nkv, hd);
@@ -247,7 +249,19 @@ struct Shape {
     static constexpr int kH = PageOps<T>::kHalves;
 };
 
-// One head of one item, {m, l} and the sum: m is the maximum of scale * log2(e) * score (or
+// One item of 16 query heads (or fewer) of one KV head: one pass over its keys and values, four
+// waves each with its own running maximum m, sum l and weighted values in registers, a tile of
+// 32 positions (16 of f32) at a time: scores and weighted values on the matrix cores, the next
+// tile's keys in flight once the scores are out, its values once they are used; nothing of a
+// tile goes through LDS.  The products cost 16 rows whatever the group size (6 % of the matrix
+// cores' time at 5.4 TB/s), so the bound is HBM, or latency for little work.  Measured
+// (32 / 8 heads of 128, bf16, us): 64 requests of 1000..16384 positions (1.44 GB) 268, 5.4 TB/s
+// where a plain read of 3 GB reaches 6.2; one of 131071 (537 MB) 104; 16 of 256..2040 with f32
+// queries (74 MB) 18.2; HBM traffic 1.01 of the bytes asked for.  Of the 18 about 3 are the
+// launch and the loads of lengths and table in turn, 4 the end: partials out, an atomic, the
+// join's loads.  Two tiles ahead rather than one (registers for two workgroups a CU either way)
+// changed nothing.
+// {m, l} and the sum: m is the maximum of scale * log2(e) * score (or
 // 0 where none is above -inf), l and the sum carry the weights 2^(x - m + kWeightShift).
 template <typename TQ, typename T, int HDP, bool FULL>
 __global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv_attend(const KvAttend A, const KvPool P,

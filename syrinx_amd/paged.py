@@ -27,6 +27,7 @@ import torch
 from ._lib import check, lib
 
 RELEASE = -(1 << 31)  # an `add` that empties any request
+_COUNTER_BYTES = 262144  # SXQ_KV_COUNTER_BYTES: the part of a workspace that starts as zeros
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _P = ctypes.c_void_p
@@ -207,14 +208,16 @@ class PagedKvCache:
 
     # -- attention ------------------------------------------------------------------------
     def workspace(self, n_q: int, n_heads: int) -> torch.Tensor:
-        """A zeroed workspace for attend over n_q queries (or fewer) of n_heads heads: one for
-        every captured graph, kept while the graph lives."""
+        """A workspace, ready for use, of attend over n_q queries of n_heads heads: one for every
+        captured graph, kept while the graph lives."""
         need = self._need.get((n_q, n_heads))
         if need is None:
             size = ctypes.c_size_t()
             check(lib().sxq_kv_attention_workspace(self._layer_refs[0], n_q, n_heads, ctypes.byref(size)))
             need = self._need[(n_q, n_heads)] = int(size.value)
-        return torch.zeros(need, dtype=torch.uint8, device=self.device)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        ws[:_COUNTER_BYTES].zero_()
+        return ws
 
     def _kept_workspace(self, n_q, n_heads):
         """Eager calls: one workspace per stream, kept.  Under capture: a fresh one, owned by
