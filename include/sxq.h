@@ -232,7 +232,8 @@ typedef struct {
  * negated.  cu int32 [n_rows + 1]: the first token of each accepted request, then their
  * number T; token t < T of the map: slots[t], pos[t] (its position) and rows[t] (its
  * request), requests ascending; entries T .. capacity - 1 are -1.  capacity may be 0 (the
- * three maps are then not touched).  n_rows * max_blocks and max_blocks * page_size < 2^31. */
+ * three maps are then not touched).  n_rows * max_blocks and max_blocks * page_size < 2^31,
+ * capacity at most 2^30. */
 sxq_status sxq_kv_reserve(int device, int page_size, int n_pages, int n_rows, int max_blocks, const int32_t *add,
                           int32_t *lens, int32_t *table, int64_t table_stride, int32_t *free_list,
                           int32_t *free_count, int capacity, int32_t *cu, int32_t *slots, int32_t *pos,
@@ -262,7 +263,7 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
  * Scores, softmax and sums are f32.  rows int32 [n_q]: the table row of each query (NULL: b);
  * a query whose row lies outside 0 .. n_rows - 1 leaves its out row as it was.  A request
  * without positions (or whose pages are all absent) gives zeros.  max_blocks * page_size at
- * most 2^30.  What lies past a request's length, in its last page or elsewhere, may hold
+ * most 2^30, n_q times that at most 2^35, n_q at most 2^20.  What lies past a request's length, in its last page or elsewhere, may hold
  * anything; a key or value of its own that is not finite makes the outputs that read it not
  * finite.  Two calls on the same inputs give the same bits.
  * workspace: sxq_kv_attention_workspace bytes, 256-byte aligned, of which the caller zeroes

@@ -914,9 +914,7 @@ sxq_status lm_create(int device, const sxq_lm_config* cfg, const PageConfig* pag
     if (e == hipSuccess && lm->rec_d) e = hipMemset(lm->rec_d, 0, sizeof(MmaRec) * (size_t)(I / 256));
     if (e == hipSuccess && lm->rec_ws.count) e = hipMemset(lm->rec_ws.count, 0, GemvRecWs::count_bytes());
     if (e == hipSuccess && pages) {
-        std::vector<int32_t> stack(pool.n_pages);
-        for (int i = 0; i < pool.n_pages; ++i) stack[i] = pool.n_pages - 1 - i;  // page 0 on top
-        e = hipMemcpy(lm->kv_free, stack.data(), sizeof(int32_t) * stack.size(), hipMemcpyHostToDevice);
+        e = launch_kv_stack(lm->kv_free, pool.n_pages, nullptr);
         if (e == hipSuccess) e = launch_fill_int(lm->kv_free_count, 1, pool.n_pages, nullptr);
         if (e == hipSuccess) e = launch_fill_int(lm->kv_ones, MB, 1, nullptr);
         if (e == hipSuccess) e = hipMemset(lm->kv_table, 0xFF, sizeof(int32_t) * (size_t)MB * lm->max_blocks);

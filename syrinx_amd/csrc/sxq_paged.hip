@@ -455,6 +455,12 @@ __global__ __launch_bounds__(256) void k_kv_gather(const KvPool P, const int32_t
     }
 }
 
+// Every page free, page 0 on top.
+__global__ __launch_bounds__(256) void k_kv_stack(int32_t* __restrict__ free_list, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) free_list[i] = n - 1 - i;
+}
+
 __global__ __launch_bounds__(64) void k_kv_counts(const PrefillMeta pm, int32_t* __restrict__ add) {
     if ((int)threadIdx.x < pm.n) add[threadIdx.x] = pm.counts[threadIdx.x];
 }
@@ -500,6 +506,11 @@ hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table
     else if (p.dtype == kF16) SXQ_GA(_Float16);
     else SXQ_GA(__bf16);
 #undef SXQ_GA
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_stack(int32_t* free_list, int n, hipStream_t s) {
+    hipLaunchKernelGGL(k_kv_stack, dim3((n + 255) / 256), dim3(256), 0, s, free_list, n);
     return hipGetLastError();
 }
 
@@ -565,7 +576,7 @@ sxq_status sxq_kv_reserve(int device, int page_size, int n_pages, int n_rows, in
         (int64_t)max_blocks * page_size > 0x7FFFFFFF)
         return fail(SXQ_ERR_INVALID, "kv_reserve: a table of %d rows of %d blocks", n_rows, max_blocks);
     if (table_stride < max_blocks) return fail(SXQ_ERR_SHAPE, "kv_reserve: table_stride %lld below max_blocks %d", (long long)table_stride, max_blocks);
-    if (capacity < 0) return fail(SXQ_ERR_INVALID, "kv_reserve: capacity %d", capacity);
+    if (capacity < 0 || capacity > 1 << 30) return fail(SXQ_ERR_INVALID, "kv_reserve: capacity %d (0..2^30)", capacity);
     if (!add || !lens || !table || !free_list || !free_count || !cu || !status || (capacity > 0 && (!slots || !pos || !rows)))
         return fail(SXQ_ERR_INVALID, "kv_reserve: null pointer");
     DeviceGuard g(device);

@@ -110,6 +110,27 @@ struct Item {
     int part0, slot;   // a split query's first partial and its counter
 };
 
+// The cut of every query, from all queries' tiles.
+struct Cut {
+    int piece;
+    bool few;
+    SXQ_DEV Cut(int total, int target) {
+        const int p = ceil_div(total, target);
+        few = p <= kFewTiles;
+        piece = max(kMinTiles, p);
+    }
+    // n items (0: no query) of per tiles: the fewest of at most piece tiles, evenly (short ones:
+    // as many for each wave)
+    SXQ_DEV void operator()(int len, int& n, int& per) const {
+        const int tiles = tiles_of(len);
+        n = max(1, ceil_div(tiles, piece));
+        if (few && tiles <= kWholeTiles) n = 1;
+        per = ceil_div(tiles, n);
+        if (per <= 4 * kWaves) per = (per + kWaves - 1) / kWaves * kWaves;
+        n = len < 0 ? 0 : max(1, ceil_div(tiles, max(per, 1)));
+    }
+};
+
 // Item x of the launch, found by every wave from the lengths: false if there is none.
 SXQ_DEV bool find_item(const KvAttend& A, const KvPool& P, int target, int x, Item& it) {
     int row, len;
@@ -120,19 +141,12 @@ SXQ_DEV bool find_item(const KvAttend& A, const KvPool& P, int target, int x, It
         load_query(A, P, b0, r, n);
         total += __builtin_amdgcn_readlane(wave_scan(tiles_of(n)), 63);
     }
-    int piece = ceil_div(total, target);
-    const bool few = piece <= kFewTiles;
-    piece = max(kMinTiles, piece);
+    const Cut cut(total, target);
     int items0 = 0, single0 = 0, split0 = 0;  // over the queries before this block of 64
     for (int b0 = 0; b0 < A.n_q; b0 += 64) {
         if (b0) load_query(A, P, b0, row, len);
-        const int tiles = tiles_of(len);
-        // an even cut: the fewest items of at most piece tiles (short ones: as many for each wave)
-        int n = max(1, ceil_div(tiles, piece));
-        if (few && tiles <= kWholeTiles) n = 1;
-        int per = ceil_div(tiles, n);
-        if (per <= 4 * kWaves) per = (per + kWaves - 1) / kWaves * kWaves;
-        n = len < 0 ? 0 : max(1, ceil_div(tiles, max(per, 1)));
+        int n, per;
+        cut(len, n, per);
         const int incl = wave_scan(n);
         const uint64_t single = __ballot(n == 1), split = __ballot(n > 1);
         const uint64_t mine = __ballot(x >= items0 + incl - n && x < items0 + incl);
@@ -157,6 +171,98 @@ SXQ_DEV bool find_item(const KvAttend& A, const KvPool& P, int target, int x, It
         split0 += __builtin_popcountll(split);
     }
     return false;
+}
+
+// Beyond kScanMax queries a launch of its own finds every query's items once (each workgroup's
+// walk over all lengths would be n_q^2): in the workspace, first item [n_q + 1] and, of each
+// query, {tiles an item, first partial, counter, -}.  us at 32 / 8 heads of 128: 300 queries of
+// 200..1000 positions 145 -> 123, 1024 of 100..600 370 -> 228, 4096 of 50..200 2798 -> 480; at 64
+// the launch and its hand-over (4) would cost more than the walk (0.2 a block of 64).
+constexpr int kScanMax = 256;
+SXQ_HD size_t attend_plan_bytes(int n_q) { return n_q <= kScanMax ? 0 : (((size_t)n_q + 1) * 4 + 255) / 256 * 256 + (size_t)n_q * 16; }
+struct Plan {
+    int* first;
+    int4* info;
+    SXQ_HD Plan(void* ws, int n_q)
+        : first((int*)((char*)ws + kCountBytes)), info((int4*)((char*)ws + kCountBytes + (((size_t)n_q + 1) * 4 + 255) / 256 * 256)) {}
+};
+
+__global__ __launch_bounds__(1024) void k_kv_attend_plan(const KvAttend A, const KvPool P, int target) {
+    __shared__ int red[3][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const Plan plan(A.ws, A.n_q);
+    // Sums of a, b, c over the workgroup's threads up to this one, and of all.
+    auto scan = [&](int (&v)[3], int (&all)[3]) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k) v[k] = wave_scan(v[k]);
+        __syncthreads();
+        if (lane == 63)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) red[k][wave] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            all[k] = 0;
+            int before = 0;
+            for (int w = 0; w < 16; ++w) {
+                if (w == wave) before = all[k];
+                all[k] += red[k][w];
+            }
+            v[k] += before;
+        }
+    };
+    int row, len, total = 0;
+    for (int b0 = 0; b0 < A.n_q; b0 += 1024) {
+        load_query(A, P, b0 + 64 * wave, row, len);
+        int v[3] = {tiles_of(len), 0, 0}, all[3];
+        scan(v, all);
+        total += all[0];
+    }
+    const Cut cut(total, target);
+    int done[3] = {0, 0, 0};  // items, items of split queries, split queries
+    for (int b0 = 0; b0 < A.n_q; b0 += 1024) {
+        load_query(A, P, b0 + 64 * wave, row, len);
+        int n, per;
+        cut(len, n, per);
+        int v[3] = {n, n > 1 ? n : 0, n > 1 ? 1 : 0}, all[3];
+        const int own[3] = {v[0], v[1], v[2]};
+        scan(v, all);
+        const int b = b0 + tid;
+        if (b < A.n_q) {
+            plan.first[b] = done[0] + v[0] - own[0];
+            plan.info[b] = make_int4(per, done[1] + v[1] - own[1], done[2] + v[2] - own[2], 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 3; ++k) done[k] += all[k];
+    }
+    if (tid == 0) plan.first[A.n_q] = done[0];
+}
+
+SXQ_DEV bool planned_item(const KvAttend& A, const KvPool& P, int x, Item& it) {
+    const Plan plan(A.ws, A.n_q);
+    if (x >= plan.first[A.n_q]) return false;
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = A.n_q;  // the last query whose first item is at most x, 64 a step
+    while (n > 1) {
+        const int step = (n + 63) / 64, at = lane * step;
+        const int k = __builtin_popcountll(__ballot(at < n && plan.first[lo + min(at, n - 1)] <= x)) - 1;
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int4 info = plan.info[lo];
+    const int start = __builtin_amdgcn_readfirstlane(plan.first[lo]);
+    it.b = lo;
+    it.row = __builtin_amdgcn_readfirstlane(A.rows ? A.rows[lo] : lo);
+    it.len = __builtin_amdgcn_readfirstlane(kv_clamp_len(A.lens[it.row], A.max_blocks, P.shift));
+    it.count = __builtin_amdgcn_readfirstlane(plan.first[lo + 1]) - start;
+    it.index = x - start;
+    const int per = __builtin_amdgcn_readfirstlane(info.x);
+    it.first = it.index * per;
+    it.tiles = min(per, tiles_of(it.len) - it.first);
+    it.part0 = __builtin_amdgcn_readfirstlane(info.y);
+    it.slot = __builtin_amdgcn_readfirstlane(info.z);
+    return true;
 }
 
 // ---- the matrix operands of each page type -----------------------------------------------
@@ -296,7 +402,7 @@ __global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv_
     const int64_t page_bytes = P.page_stride * (int64_t)sizeof(T);
 
     Item it;
-    if (!find_item(A, P, target, blockIdx.x, it)) return;
+    if (!(A.n_q > kScanMax ? planned_item(A, P, blockIdx.x, it) : find_item(A, P, target, blockIdx.x, it))) return;
 
     // the queries: B operands, in the element order of the key loads
     const TQ* qrow = (const TQ*)A.q + (int64_t)it.b * A.q_stride + (int64_t)(h0 + min(r, heads - 1)) * hd;
@@ -567,7 +673,7 @@ __global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv_
     const int per = hd / 4, n_out = heads * per;  // four columns a thread
     // a partial's bytes; from item to item (all items of a query: below 2^27)
     const uint32_t pf = (uint32_t)(attend_part_floats(hd) * sizeof(float)), step = (uint32_t)A.nh * pf;
-    char* parts = (char*)A.ws + kCountBytes + (size_t)h0 * pf;
+    char* parts = (char*)A.ws + kCountBytes + attend_plan_bytes(A.n_q) + (size_t)h0 * pf;
     const bool split = it.count > 1;
     const __amdgpu_buffer_rsrc_t mine =
         coherent_rsrc(parts + (size_t)(it.part0 + it.index) * step, heads * pf);
@@ -682,7 +788,7 @@ void attend_by_width(const KvAttend& a, const KvPool& p, dim3 grid, int target, 
 namespace sxq {
 
 size_t kv_attend_workspace(const KvPool& p, int n_q, int nh) {
-    return kCountBytes + 2 * (size_t)attend_target_max(nh, p.nkv, p.hd) * nh * attend_part_floats(p.hd) * sizeof(float);
+    return kCountBytes + attend_plan_bytes(n_q) + 2 * (size_t)attend_target_max(nh, p.nkv, p.hd) * nh * attend_part_floats(p.hd) * sizeof(float);
 }
 
 hipError_t launch_kv_attend(const KvAttend& a, const KvPool& p, hipStream_t s) {
@@ -691,6 +797,7 @@ hipError_t launch_kv_attend(const KvAttend& a, const KvPool& p, hipStream_t s) {
     // one query of 500 positions)
     const int64_t widest = (int64_t)a.n_q * (((int64_t)a.max_blocks * p.page + kTile * kMinTiles - 1) / (kTile * kMinTiles));
     const dim3 grid((unsigned)std::min<int64_t>(target + a.n_q, widest), p.nkv * attend_head_tiles(a.nh, p.nkv));
+    if (a.n_q > kScanMax) hipLaunchKernelGGL(k_kv_attend_plan, dim3(1), dim3(1024), 0, s, a, p, target);
     if (p.dtype == kF32) attend_by_width<float, float>(a, p, grid, target, s);
     else if (p.dtype == kF16) attend_by_width<_Float16, _Float16>(a, p, grid, target, s);
     else if (a.q_dtype == kF32) attend_by_width<float, __bf16>(a, p, grid, target, s);

@@ -50,6 +50,8 @@ hipError_t launch_kv_attend(const KvAttend& a, const KvPool& p, hipStream_t s);
 hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table_stride, int max_blocks,
                             const int32_t* lens, int r0, int rows, int h0, int heads, int p0, int span, float* k, float* v,
                             hipStream_t s);
+// A free stack of pages 0 .. n - 1, page 0 on top.
+hipError_t launch_kv_stack(int32_t* free_list, int n, hipStream_t s);
 // add[i] = pm.counts[i], i < pm.n (a prompt's growths).
 struct PrefillMeta;
 hipError_t launch_kv_counts(const PrefillMeta& pm, int32_t* add, hipStream_t s);

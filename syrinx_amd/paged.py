@@ -121,7 +121,7 @@ class PagedKvCache:
     def reserve(self, add, capacity=None, out: SlotMap = None) -> SlotMap:
         """Grow request r by add[r] tokens (add[r] < 0: shrink it; RELEASE empties it) and map
         the new tokens.  add: int32 [max_rows] on the GPU, or a sequence of ints (shorter: the
-        rest 0).  capacity: the map's length (with a sequence: by default its tokens).  out: a
+        rest 0; copied from the host, so not under capture).  capacity: the map's length (with a sequence: by default its tokens).  out: a
         map of an earlier call of this capacity, to write into.  Pages go to requests in order; a
         request that cannot get them stays as it was (status)."""
         if not torch.is_tensor(add):

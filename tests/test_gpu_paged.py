@@ -458,6 +458,32 @@ def test_attend_more_heads_than_the_card_has_places(cuda):
         _close(cache.attend(0, q), want, bound, torch.bfloat16)
 
 
+@pytest.mark.parametrize("n,long", [(129, 0), (1025, 40000), (2600, 9000)])
+def test_attend_thousands_of_queries(cuda, n, long):
+    """More queries than a workgroup walks over by itself, one of them far longer than the rest,
+    idle and repeated rows; twice, the second time on another order."""
+    rng = np.random.default_rng(n)
+    lens = [int(v) for v in np.exp(rng.uniform(0, math.log(90), n))]
+    lens[n // 3] = max(long, 1)
+    lens[n // 2] = 0
+    cache, g = _filled(cuda, 1, 16, 16, lens, "bf16", n)
+    for turn in range(2):
+        rows = torch.tensor(rng.integers(-1, n, 2 * n), dtype=torch.int32, device=cuda)
+        rows[7] = n // 3
+        rows[11] = n + 5
+        q = torch.randn((2 * n, 3, 16), generator=g, device=cuda).bfloat16()
+        out = torch.full_like(q, 9.0)
+        got = cache.attend(0, q, rows=rows, out=out)
+        live = (rows >= 0) & (rows < n)
+        assert bool((got[~live] == 9).all())
+        some = torch.cat([torch.tensor([7]), torch.from_numpy(rng.permutation(2 * n)[:400])])
+        some = some[live[some.to(cuda)].cpu()]
+        want, bound = _attend_reference(q[some], cache.k[0], cache.v[0], cache.table, cache.lens, rows[some].tolist(), 0.25)
+        _close(got[some], want, bound, torch.bfloat16)
+        few = some[:40]  # the same queries in a call of their own
+        _close(cache.attend(0, q[few].contiguous(), rows=rows[few].contiguous()), want[:40], bound[:40], torch.bfloat16)
+
+
 @pytest.mark.parametrize("n", [100, 300])
 def test_attend_many_requests(cuda, n):
     rng = np.random.default_rng(n)

@@ -92,7 +92,8 @@ def _attend(pages=None, dtype=BF16, q=256, q_stride=256, n_q=1, heads=4, lens=25
     (dict(n_q=(1 << 20) + 1), _lib.ERR_SHAPE), (dict(q_stride=248), _lib.ERR_SHAPE),
     (dict(q_stride=260), _lib.ERR_SHAPE), (dict(out_stride=260), _lib.ERR_SHAPE), (dict(n_q=5), _lib.ERR_SHAPE),
     (dict(n_rows=0), _lib.ERR_INVALID), (dict(blocks=0), _lib.ERR_INVALID), (dict(table_stride=7), _lib.ERR_INVALID),
-    (dict(blocks=1 << 27, table_stride=1 << 27), _lib.ERR_INVALID), (dict(scale=float("inf")), _lib.ERR_INVALID),
+    (dict(blocks=1 << 27, table_stride=1 << 27), _lib.ERR_INVALID),
+    (dict(blocks=1 << 26, table_stride=1 << 26, n_q=64, n_rows=64), _lib.ERR_INVALID), (dict(scale=float("inf")), _lib.ERR_INVALID),
     (dict(scale=float("nan")), _lib.ERR_INVALID), (dict(q=None), _lib.ERR_INVALID), (dict(lens=None), _lib.ERR_INVALID),
     (dict(table=None), _lib.ERR_INVALID), (dict(out=None), _lib.ERR_INVALID), (dict(ws=None), _lib.ERR_INVALID),
     (dict(q=264), _lib.ERR_INVALID), (dict(out=8), _lib.ERR_INVALID), (dict(ws=128), _lib.ERR_INVALID),
@@ -112,6 +113,7 @@ def _reserve(page=16, n_pages=4, n_rows=2, blocks=8, stride=8, capacity=4, null=
     (dict(page=24), _lib.ERR_INVALID), (dict(n_pages=0), _lib.ERR_INVALID), (dict(n_pages=1 << 28), _lib.ERR_INVALID),
     (dict(n_rows=0), _lib.ERR_INVALID), (dict(blocks=0), _lib.ERR_INVALID), (dict(stride=7), _lib.ERR_SHAPE),
     (dict(n_rows=1 << 20, blocks=1 << 12, stride=1 << 12), _lib.ERR_INVALID), (dict(capacity=-1), _lib.ERR_INVALID),
+    (dict(capacity=(1 << 30) + 1), _lib.ERR_INVALID),
 ] + [(dict(null=(k,)), _lib.ERR_INVALID) for k in ("add", "lens", "table", "free", "count", "cu", "slots", "pos", "rows",
                                                      "status")])
 def test_reserve_refusals(kw, code):
