@@ -82,15 +82,13 @@ SXQ_DEV int wave_scan(int v) {
     return v;
 }
 
-// ceil(a / b), 0 <= a < 2^30, 0 < b < 2^30: below 2^22 the quotient from a reciprocal is off by
-// at most one either way.
+// ceil(a / b), 0 <= a < 2^30, 0 < b < 2^30, without a branch: the first quotient from a
+// reciprocal is off by at most 2^8, the second, of what that leaves, by one either way.
 SXQ_DEV int ceil_div(int a, int b) {
-    if (a >= 1 << 22) return (int)(((uint32_t)a + (uint32_t)b - 1) / (uint32_t)b);
-    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
-    int r = a - q * b;
-    if (r < 0) r += b, --q;
-    if (r >= b) r -= b, ++q;
-    return q + (r > 0);
+    const float inv = __builtin_amdgcn_rcpf((float)b);
+    const int q0 = (int)((float)a * inv), r0 = a - q0 * b;
+    const int q1 = (int)((float)r0 * inv), r = r0 - q1 * b;
+    return q0 + q1 + (r > b ? 2 : r > 0 ? 1 : r <= -b ? -1 : 0);
 }
 
 // Lane l's query of the block of 64 from b0: its table row and length (-1: none).
