@@ -228,8 +228,8 @@ typedef struct {
  *     too short, 1 if it needs pages and the pages asked for up to and with it (refused
  *     requests' included) exceed the free ones, 3 if the tokens asked for up to and with it
  *     exceed `capacity`; otherwise status 0.
- * An accepted step is undone exactly -- table, stack and lengths -- by the call with add
- * negated.  cu int32 [n_rows + 1]: the first token of each accepted request, then their
+ * A call that refuses nothing is undone exactly -- table, stack and lengths -- by the call
+ * with add negated (and a capacity for what grows back), if no request shrank below 0.  cu int32 [n_rows + 1]: the first token of each accepted request, then their
  * number T; token t < T of the map: slots[t], pos[t] (its position) and rows[t] (its
  * request), requests ascending; entries T .. capacity - 1 are -1.  capacity may be 0 (the
  * three maps are then not touched).  n_rows * max_blocks and max_blocks * page_size < 2^31,
@@ -263,9 +263,10 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
  * Scores, softmax and sums are f32.  rows int32 [n_q]: the table row of each query (NULL: b);
  * a query whose row lies outside 0 .. n_rows - 1 leaves its out row as it was.  A request
  * without positions (or whose pages are all absent) gives zeros.  max_blocks * page_size at
- * most 2^30, n_q times that at most 2^35, n_q at most 2^20.  What lies past a request's length, in its last page or elsewhere, may hold
- * anything; a key or value of its own that is not finite makes the outputs that read it not
- * finite.  Two calls on the same inputs give the same bits.
+ * most 2^30, n_q times that at most 2^35, n_q at most 2^20.  What lies past a request's
+ * length, in its last page or elsewhere, may hold anything; a key or value of its own that is
+ * not finite makes the outputs that read it not finite.  Two calls on the same inputs give
+ * the same bits.
  * workspace: sxq_kv_attention_workspace bytes, 256-byte aligned, of which the caller zeroes
  * the first SXQ_KV_COUNTER_BYTES before its first use; every call leaves them zero, and the
  * workspace good for any call that needs no more bytes.  Calls that share one must not

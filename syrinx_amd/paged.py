@@ -64,7 +64,8 @@ class PagedKvCache:
     of page_size positions (a power of two, 16..1024).
 
     k, v: [n_layers, n_pages, n_kv_heads, page_size, head_dim]; table: int32 [max_rows, blocks];
-    lens: int32 [max_rows]; free: int32 [n_pages], of which the first free_count[0] are free."""
+    lens: int32 [max_rows]; free: int32 [n_pages], of which the first free_count[0] are free (to
+    be written in place, never replaced)."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, *, n_pages, page_size=32, max_rows, max_len,
                  dtype=torch.bfloat16, device="cuda:0"):
@@ -121,9 +122,10 @@ class PagedKvCache:
     def reserve(self, add, capacity=None, out: SlotMap = None) -> SlotMap:
         """Grow request r by add[r] tokens (add[r] < 0: shrink it; RELEASE empties it) and map
         the new tokens.  add: int32 [max_rows] on the GPU, or a sequence of ints (shorter: the
-        rest 0; copied from the host, so not under capture).  capacity: the map's length (with a sequence: by default its tokens).  out: a
-        map of an earlier call of this capacity, to write into.  Pages go to requests in order; a
-        request that cannot get them stays as it was (status)."""
+        rest 0; copied from the host, so not under capture).  capacity: the map's length (with
+        a sequence: by default its tokens).  out: a map of an earlier call of this capacity, to
+        write into.  Pages go to requests in order; a request that cannot get them stays as it
+        was (status)."""
         if not torch.is_tensor(add):
             add = [int(a) for a in add]
             if len(add) > self.max_rows:
