@@ -195,6 +195,39 @@ def test_reserve_reads_no_index_it_has_not_checked(cuda):
     assert slots[1] == -1 and slots[4] == -1  # the pages of lengths 15 and 63 are ids -7 and 12345
 
 
+@pytest.mark.parametrize("rows,cap", [(70, 100), (300, 5000), (1500, 9000)])
+def test_reserve_of_a_corrupted_state_stays_inside_its_arrays(cuda, rows, cap):
+    """Any lengths, page ids, free pages and free count, through every way the call is split into
+    launches: guard elements keep their values, slots lie in the pool or are -1."""
+    width, page, n_pages, guard = 7, 16, 400, 256
+    rng = np.random.default_rng(rows)
+    bad = np.array([-2**31, -7, -1, 0, 3, 90, 112, 113, 400, 5000, 2**31 - 1])
+
+    def guarded(n, values=None):
+        t = torch.full((n + 2 * guard,), 77, dtype=torch.int32, device=cuda)
+        if values is not None:
+            t[guard:guard + n] = torch.from_numpy(values.astype(np.int32)).to(cuda)
+        return t, t[guard:guard + n]
+
+    for count in (2**31 - 1, 350, -5):
+        arrays = {
+            "add": guarded(rows, rng.choice([1, 1, 5, 60, 112, -3, -2**31, 2**31 - 1], rows)),
+            "lens": guarded(rows, rng.choice(bad, rows)), "table": guarded(rows * width, rng.choice(bad, rows * width)),
+            "free": guarded(n_pages, rng.choice(bad, n_pages)), "count": guarded(1, np.array([count])),
+            "cu": guarded(rows + 1), "slots": guarded(cap), "pos": guarded(cap), "rows": guarded(cap), "status": guarded(rows)}
+        p = {k: ctypes.c_void_p(v[1].data_ptr()) for k, v in arrays.items()}
+        check(lib().sxq_kv_reserve(0, page, n_pages, rows, width, p["add"], p["lens"], p["table"], width, p["free"],
+                                   p["count"], cap, p["cu"], p["slots"], p["pos"], p["rows"], p["status"],
+                                   torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        for k, (whole, _) in arrays.items():
+            assert bool((whole[:guard] == 77).all()) and bool((whole[-guard:] == 77).all()), k
+        got = {k: v[1].cpu().numpy() for k, v in arrays.items()}
+        assert ((got["lens"] >= 0) & (got["lens"] <= width * page)).all() and 0 <= got["count"][0] <= n_pages
+        assert ((got["slots"] >= -1) & (got["slots"] < n_pages * page)).all() and got["cu"][-1] <= cap
+        assert (np.diff(got["cu"]) >= 0).all() and (got["rows"][got["cu"][-1]:] == -1).all()
+
+
 def test_reserve_python_refusals(cuda):
     cache = _small_cache(4, 64, 16, 8)
     with pytest.raises(ValueError):

@@ -64,7 +64,7 @@ def test_every_op_of_a_paged_step_matches_oracle(cuda, ora, kind):
 
 
 PROMPTS = {"fish_q4k_exact_1stream": (4, 16), "fish_q4k_gemm_after_cache": (2, 64), "fish_q8_0_ragged3": (9, 16),
-           "cv2_q8_0_embeds": (3, 32), "cv2_q4_0_gemm_rows": (9, 16)}
+           "cv2_q8_0_embeds": (3, 32), "cv2_q4_0_gemm_rows": (9, 16), "qwen3_4b_512_tokens": (17, 32)}
 
 
 @pytest.mark.parametrize("kind", list(PROMPTS))
