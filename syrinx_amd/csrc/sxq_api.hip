@@ -31,6 +31,7 @@ sxq_status fail(sxq_status code, const char* fmt, ...) {
 }
 
 sxq_status hip_fail(hipError_t e, const char* what) {
+    (void)hipGetLastError();  // reported here: not by the next launch of this thread as its own
     return fail(e == hipErrorOutOfMemory ? SXQ_ERR_OOM : SXQ_ERR_DEVICE, "%s: %s", what, hipGetErrorString(e));
 }
 

@@ -1,0 +1,196 @@
+// host_tests.hip -- the decode engine's host side on the simulated runtime: what a call does
+// to lengths, pages and workspaces when another call fails or runs beside it.
+//   host_tests NAME      runs one test, prints "ok"
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <cstdio>
+#include <cstdlib>
+#include <cstring>
+#include <map>
+
+#include "../../include/sxq.h"
+#include "sim_hip.h"
+#include "sxq_decoder.h"
+#include "sxq_paged.h"
+#include "sxq_paged_launch.h"
+
+using namespace sxq;
+
+#define EXPECT(c)                                                                                            \
+    do {                                                                                                     \
+        if (!(c)) {                                                                                          \
+            std::fprintf(stderr, "failed: %s (line %d; last error: %s)\n", #c, __LINE__, sxq_last_error()); \
+            std::exit(1);                                                                                    \
+        }                                                                                                    \
+    } while (0)
+
+namespace {
+
+// What the engine's last reserve worked on: its device lengths, table and free stack.
+KvReserve seen{};
+
+void reserve_rows(const KvReserve& a) {
+    seen = a;
+    auto blocks = [&](int64_t n) { return (int)((n + (1 << a.shift) - 1) >> a.shift); };
+    std::vector<int> back;
+    for (int r = 0; r < a.n_rows; ++r) {
+        if (a.add[r] >= 0) continue;
+        const int keep = (int)std::max<int64_t>(0, (int64_t)a.lens[r] + a.add[r]);
+        for (int b = blocks(keep); b < blocks(a.lens[r]); ++b) {
+            back.push_back(a.table[r * a.table_stride + b]);
+            a.table[r * a.table_stride + b] = -1;
+        }
+        a.lens[r] = keep;
+    }
+    for (auto it = back.rbegin(); it != back.rend(); ++it) a.free_list[a.free_count[0]++] = *it;
+    const int avail = a.free_count[0];
+    int64_t asked = 0, room = 0;
+    int t = 0;
+    a.cu[0] = 0;
+    for (int r = 0; r < a.n_rows; ++r) {
+        a.status[r] = 0;
+        if (a.add[r] >= 0) {
+            const int64_t grown = (int64_t)a.lens[r] + a.add[r];
+            const int have = blocks(a.lens[r]), need = blocks(grown) - have;
+            if (grown > (int64_t)a.max_blocks << a.shift) a.status[r] = 2;
+            else {
+                asked += need;
+                room += a.add[r];
+                if (need && asked > avail) a.status[r] = 1;
+                else if (a.add[r] && room > a.limit) a.status[r] = 3;
+                else {
+                    for (int b = have; b < have + need; ++b) a.table[r * a.table_stride + b] = a.free_list[--a.free_count[0]];
+                    for (int64_t p = a.lens[r]; p < grown; ++p, ++t)
+                        if (t < a.capacity) {
+                            a.slots[t] = kv_slot(a.table[r * a.table_stride + (p >> a.shift)], (int)p, a.shift, a.n_pages);
+                            a.pos[t] = (int)p;
+                            a.rows[t] = r;
+                        }
+                    a.lens[r] = (int)grown;
+                }
+            }
+        }
+        a.cu[r + 1] = t;
+    }
+    for (; t < a.capacity; ++t) a.slots[t] = a.pos[t] = a.rows[t] = -1;
+}
+
+// Bodies of the kernels that keep an engine's lengths and pages.
+void page_kernels() {
+    sim::kernel("k_kv_reserve", [](void** args) {
+        const KvReserve a = *(const KvReserve*)args[0];
+        return [a] { reserve_rows(a); };
+    });
+    sim::kernel("k_kv_stack", [](void** args) {
+        int32_t* list = *(int32_t**)args[0];
+        const int n = *(int*)args[1];
+        return [=] { for (int i = 0; i < n; ++i) list[i] = n - 1 - i; };
+    });
+    sim::kernel("k_fill_int", [](void** args) {
+        int* y = *(int**)args[0];
+        const int n = *(int*)args[1], v = *(int*)args[2];
+        return [=] { for (int i = 0; i < n; ++i) y[i] = v; };
+    });
+    sim::kernel("k_kv_counts", [](void** args) {
+        const PrefillMeta pm = *(const PrefillMeta*)args[0];
+        int32_t* add = *(int32_t**)args[1];
+        return [=] { for (int i = 0; i < pm.n; ++i) add[i] = pm.counts[i]; };
+    });
+}
+
+sxq_lm_config config(int max_seq, int max_batch) {
+    sxq_lm_config c{};
+    c.n_layers = 1;
+    c.dim = 256;
+    c.n_heads = 4;
+    c.n_kv_heads = 2;
+    c.head_dim = 64;
+    c.intermediate = 256;
+    c.vocab = 64;
+    c.max_seq = max_seq;
+    c.max_batch = max_batch;
+    c.weight_dtype = SXQ_Q8_0;
+    c.norm_eps = 1e-6f;
+    c.rope_theta = 1e6f;
+    return c;
+}
+
+struct Engine {
+    sxq_lm* lm = nullptr;
+    int n, pages;
+    std::vector<float> embeds, logits;
+    Engine(int pages_, int max_seq = 20000, int batch = 4, int page = 16) : n(batch), pages(pages_) {
+        const sxq_lm_config c = config(max_seq, batch);
+        EXPECT(sxq_lm_create_paged(0, &c, SXQ_F32, page, pages, &lm) == SXQ_OK);
+        embeds.resize((size_t)c.dim * 70000);
+        logits.resize((size_t)c.vocab * batch);
+    }
+    ~Engine() { sxq_lm_destroy(lm); }
+    sxq_status step(int streams, unsigned flags = 0) {
+        return sxq_lm_step(lm, streams, nullptr, embeds.data(), logits.data(), nullptr, nullptr, flags, nullptr);
+    }
+    sxq_status prefill(std::vector<int32_t> counts) {
+        return sxq_lm_prefill(lm, (int)counts.size(), counts.data(), nullptr, embeds.data(), logits.data(), nullptr, nullptr,
+                              0, nullptr, 0, nullptr);
+    }
+    std::vector<int32_t> lengths() {
+        std::vector<int32_t> v(n);
+        EXPECT(sxq_lm_get_lengths(lm, v.data(), n) == SXQ_OK);
+        return v;
+    }
+    int free_pages() {
+        int f = -1;
+        EXPECT(sxq_lm_free_pages(lm, &f) == SXQ_OK);
+        return f;
+    }
+    // The device's lengths are the host's, every page is held once or free once.
+    void consistent() {
+        EXPECT(seen.lens);
+        const std::vector<int32_t> host = lengths();
+        std::vector<int> times(pages, 0);
+        for (int s = 0; s < n; ++s) {
+            EXPECT(seen.lens[s] == host[s]);
+            for (int b = 0; b < kv_blocks(host[s], seen.shift); ++b) {
+                const int id = seen.table[s * seen.table_stride + b];
+                EXPECT(id >= 0 && id < pages);
+                ++times[id];
+            }
+        }
+        EXPECT(seen.free_count[0] == free_pages());
+        for (int i = 0; i < seen.free_count[0]; ++i) ++times[seen.free_list[i]];
+        for (int id = 0; id < pages; ++id) EXPECT(times[id] == 1);
+    }
+};
+
+// A call that fails leaves no error behind for the next one to report.
+void error_of_one_call() {
+    Engine e(100);
+    EXPECT(e.prefill({5, 20}) == SXQ_OK);
+    e.consistent();
+    sim::state().malloc_limit = 1 << 16;
+    EXPECT(e.prefill({900, 3}) == SXQ_ERR_OOM && std::strstr(sxq_last_error(), "workspace"));
+    sim::state().malloc_limit = (size_t)-1;
+    EXPECT(hipGetLastError() == hipSuccess);  // nor for the caller's own next launch
+    e.consistent();
+    EXPECT(e.step(2) == SXQ_OK);
+    e.consistent();
+    EXPECT((e.lengths() == std::vector<int32_t>{6, 21, 0, 0}));
+}
+
+const std::map<std::string, void (*)()> kTests = {
+    {"error_of_one_call", error_of_one_call},
+};
+
+}  // namespace
+
+int main(int argc, char** argv) {
+    const auto it = kTests.find(argc > 1 ? argv[1] : "");
+    if (it == kTests.end()) {
+        for (auto& t : kTests) std::puts(t.first.c_str());
+        return argc > 1;
+    }
+    page_kernels();
+    it->second();
+    std::puts("ok");
+}
