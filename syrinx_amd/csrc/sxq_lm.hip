@@ -113,6 +113,8 @@ struct sxq_lm {
     int32_t *kv_cu = nullptr, *kv_status = nullptr, *kv_slots = nullptr, *kv_pos = nullptr, *kv_rows = nullptr;
     float* kv_ctx = nullptr;  // context rows of a step [max_batch][n_heads * head_dim]
     void* kv_ws = nullptr;    // the attention's workspace
+    bool kv_moved = false;    // the call being enqueued has moved lengths and pages
+    bool kv_lost = false;     // a failed call's pages could not be put back: only a reset of all streams helps
     void* pf = nullptr;  // prefill workspace, grown to the largest prompt batch so far
     size_t pf_size = 0;
     std::vector<void*> allocs;
@@ -231,7 +233,26 @@ hipError_t lm_reserve(sxq_lm* lm, const int32_t* add, int n, int capacity, int32
     a.pos = pos;
     a.rows = rows;
     a.status = lm->kv_status;
-    return launch_kv_reserve(a, s);
+    return launch_kv_reserve(a, s, &lm->kv_moved);
+}
+
+// After a call whose enqueueing failed: if it had moved lengths and pages, they go back (a reserve
+// with the growths negated is its inverse), so that the device agrees with the host's lengths,
+// which move only when everything is enqueued.
+void lm_undo(sxq_lm* lm, const KvGrowths& g, hipStream_t s) {
+    if (!lm->paged || !lm->kv_moved) return;
+    (void)hipGetLastError();  // the failure's own, which the launches below would report
+    KvGrowths back{g.n, {}};
+    for (int i = 0; i < g.n; ++i) back.add[i] = -g.add[i];
+    hipError_t e = launch_kv_growths(back, lm->kv_add, s);
+    if (e == hipSuccess) e = lm_reserve(lm, lm->kv_add, g.n, 0, nullptr, nullptr, nullptr, s);
+    if (e != hipSuccess) lm->kv_lost = true;
+    (void)hipGetLastError();
+}
+
+sxq_status check_lost(const sxq_lm* lm, const char* who) {
+    if (!lm->kv_lost) return SXQ_OK;
+    return fail(SXQ_ERR_INVALID, "%s: an earlier call failed with its pages taken; reset all %d streams", who, lm->c.max_batch);
 }
 
 KvPool layer_pool(const sxq_lm* lm, int l) {
@@ -281,6 +302,15 @@ hipError_t lm_attend(sxq_lm* lm, int l, const float* q, int n, float* ctx, hipSt
     a.out = ctx;
     a.ws = lm->kv_ws;
     return launch_kv_attend(a, layer_pool(lm, l), s);
+}
+
+// Every stream empty, every page free.
+hipError_t empty_pages(sxq_lm* lm, hipStream_t s) {
+    hipError_t e = launch_fill_int(lm->d_len, lm->c.max_batch, 0, s);
+    if (e == hipSuccess) e = launch_fill_int(lm->kv_table, lm->c.max_batch * lm->max_blocks, -1, s);
+    if (e == hipSuccess) e = launch_kv_stack(lm->kv_free, lm->pool.n_pages, s);
+    if (e == hipSuccess) e = launch_fill_int(lm->kv_free_count, 1, lm->pool.n_pages, s);
+    return e;
 }
 
 // N(0, 1) into n elements of a cache.
@@ -651,7 +681,9 @@ hipError_t enqueue_prefill(sxq_lm* lm, const PrefillMeta& pm, int T, const int* 
     float *kv_k = (float*)(base + P.kv_k), *kv_v = (float*)(base + P.kv_v);
     const int64_t kv_stride = (int64_t)c.n_kv_heads * P.span * c.head_dim;
     if (lm->paged) {
-        PF(launch_kv_counts(pm, lm->kv_add, s));
+        KvGrowths g{n, {}};
+        for (int i = 0; i < n; ++i) g.add[i] = pm.counts[i];
+        PF(launch_kv_growths(g, lm->kv_add, s));
         PF(lm_reserve(lm, lm->kv_add, n, T, kv_map, kv_map + T, kv_map + 2 * (int64_t)T, s));
     }
     if (embeds) {
@@ -914,10 +946,8 @@ sxq_status lm_create(int device, const sxq_lm_config* cfg, const PageConfig* pag
     if (e == hipSuccess && lm->rec_d) e = hipMemset(lm->rec_d, 0, sizeof(MmaRec) * (size_t)(I / 256));
     if (e == hipSuccess && lm->rec_ws.count) e = hipMemset(lm->rec_ws.count, 0, GemvRecWs::count_bytes());
     if (e == hipSuccess && pages) {
-        e = launch_kv_stack(lm->kv_free, pool.n_pages, nullptr);
-        if (e == hipSuccess) e = launch_fill_int(lm->kv_free_count, 1, pool.n_pages, nullptr);
+        e = empty_pages(lm, nullptr);
         if (e == hipSuccess) e = launch_fill_int(lm->kv_ones, MB, 1, nullptr);
-        if (e == hipSuccess) e = hipMemset(lm->kv_table, 0xFF, sizeof(int32_t) * (size_t)MB * lm->max_blocks);
         if (e == hipSuccess) e = hipMemset(lm->kv_ws, 0, kv_attend_workspace(pool, MB, c.n_heads));
     }
     lm->attn_fused = !pages && getenv("SXQ_ATTN_UNFUSED") == nullptr && attn_decode_fits(lm->vdt, c.n_heads, c.n_kv_heads, hd, lm->max_splits);
@@ -1158,18 +1188,20 @@ sxq_status sxq_lm_set_lengths(sxq_lm* lm, const int32_t* lengths, int n) {
     HIP_TRY(g.err, "hipSetDevice");
     HIP_TRY(hipDeviceSynchronize(), "lm_set_lengths");
     if (lm->paged) {  // pages given back or taken (those of added positions hold what they held)
+        sxq_status st = check_lost(lm, "lm_set_lengths");
+        if (st != SXQ_OK) return st;
         std::vector<int> lens = lm->h_len;
-        std::vector<int32_t> add(n);
+        KvGrowths g{n, {}};
         for (int s = 0; s < n; ++s) {
-            add[s] = lengths[s] - lens[s];
+            g.add[s] = lengths[s] - lens[s];
             lens[s] = lengths[s];
         }
-        const sxq_status st = check_pages(lm, "lm_set_lengths", lens);
+        st = check_pages(lm, "lm_set_lengths", lens);
         if (st != SXQ_OK) return st;
-        HIP_TRY(hipMemcpy(lm->kv_add, add.data(), sizeof(int32_t) * n, hipMemcpyHostToDevice), "lm_set_lengths");
+        HIP_TRY(launch_kv_growths(g, lm->kv_add, nullptr), "lm_set_lengths");
         HIP_TRY(lm_reserve(lm, lm->kv_add, n, 0, nullptr, nullptr, nullptr, nullptr), "lm_set_lengths");
-        HIP_TRY(hipDeviceSynchronize(), "lm_set_lengths");
         lm->h_len = lens;
+        HIP_TRY(hipDeviceSynchronize(), "lm_set_lengths");
         return SXQ_OK;
     }
     for (int s = 0; s < n; ++s) lm->h_len[s] = lengths[s];
@@ -1183,7 +1215,11 @@ sxq_status sxq_lm_reset(sxq_lm* lm, int n, void* stream) {
     std::lock_guard<std::mutex> lock(lm->mu);
     DeviceGuard g(lm->device);
     HIP_TRY(g.err, "hipSetDevice");
-    if (lm->paged) {
+    if (lm->paged && lm->kv_lost) {
+        if (n < lm->c.max_batch) return check_lost(lm, "lm_reset");
+        HIP_TRY(empty_pages(lm, (hipStream_t)stream), "lm_reset");
+        lm->kv_lost = false;
+    } else if (lm->paged) {
         HIP_TRY(launch_fill_int(lm->kv_add, n, INT32_MIN, (hipStream_t)stream), "lm_reset");
         HIP_TRY(lm_reserve(lm, lm->kv_add, n, 0, nullptr, nullptr, nullptr, (hipStream_t)stream), "lm_reset");
     } else {
@@ -1224,10 +1260,14 @@ sxq_status sxq_lm_step(sxq_lm* lm, int n, const int32_t* ids, const float* embed
     for (int s = 0; s < n; ++s)
         if (lm->h_len[s] >= lm->c.max_seq)
             return fail(SXQ_ERR_INVALID, "lm_step: stream %d KV cache is full (%d positions)", s, lm->c.max_seq);
+    KvGrowths grow{n, {}};
+    for (int s = 0; s < n; ++s) grow.add[s] = 1;
     if (lm->paged) {
+        sxq_status ok = check_lost(lm, "lm_step");
+        if (ok != SXQ_OK) return ok;
         std::vector<int> lens = lm->h_len;
-        for (int s = 0; s < n; ++s) ++lens[s];
-        const sxq_status ok = check_pages(lm, "lm_step", lens);
+        for (int s = 0; s < n; ++s) lens[s] += grow.add[s];
+        ok = check_pages(lm, "lm_step", lens);
         if (ok != SXQ_OK) return ok;
     }
     DeviceGuard g(lm->device);
@@ -1256,9 +1296,14 @@ sxq_status sxq_lm_step(sxq_lm* lm, int n, const int32_t* ids, const float* embed
         }
         HIP_TRY(hipGraphLaunch(it->second, st), "lm_step: graph launch");
     } else {
-        HIP_TRY(enqueue_step(lm, n, emb, st), "lm_step");
+        lm->kv_moved = false;
+        const hipError_t e = enqueue_step(lm, n, emb, st);
+        if (e != hipSuccess) {
+            lm_undo(lm, grow, st);
+            return hip_fail(e, "lm_step");
+        }
     }
-    for (int s = 0; s < n; ++s) lm->h_len[s] += 1;
+    for (int s = 0; s < n; ++s) lm->h_len[s] += grow.add[s];
     if (logits)
         HIP_TRY(hipMemcpyAsync(logits, lm->logits, sizeof(float) * n * lm->c.vocab, hipMemcpyDeviceToDevice, st), "lm_step: logits");
     if (hidden)
@@ -1362,10 +1407,14 @@ sxq_status sxq_lm_prefill(sxq_lm* lm, int n, const int32_t* counts, const int32_
     DeviceGuard g(lm->device);
     HIP_TRY(g.err, "hipSetDevice");
     hipStream_t st = (hipStream_t)stream;
+    KvGrowths grow{n, {}};
+    for (int s = 0; s < n; ++s) grow.add[s] = counts[s];
     if (lm->paged) {
+        sxq_status ok = check_lost(lm, "lm_prefill");
+        if (ok != SXQ_OK) return ok;
         std::vector<int> lens = lm->h_len;
         for (int s = 0; s < n; ++s) lens[s] += counts[s];
-        const sxq_status ok = check_pages(lm, "lm_prefill", lens);
+        ok = check_pages(lm, "lm_prefill", lens);
         if (ok != SXQ_OK) return ok;
     }
     const PfLayout P = pf_layout(lm, (int)T, pm);
@@ -1379,9 +1428,13 @@ sxq_status sxq_lm_prefill(sxq_lm* lm, int n, const int32_t* counts, const int32_
     }
     const bool all = (flags & SXQ_LM_ALL_LOGITS) != 0;
     if (all && !logits) return fail(SXQ_ERR_INVALID, "lm_prefill: SXQ_LM_ALL_LOGITS needs a logits buffer");
-    HIP_TRY(enqueue_prefill(lm, pm, (int)T, ids, embeds, all ? logits : nullptr, all ? hidden : nullptr,
-                            (flags & SXQ_LM_EXACT) != 0, trace, st),
-            "lm_prefill");
+    lm->kv_moved = false;
+    const hipError_t e = enqueue_prefill(lm, pm, (int)T, ids, embeds, all ? logits : nullptr, all ? hidden : nullptr,
+                                         (flags & SXQ_LM_EXACT) != 0, trace, st);
+    if (e != hipSuccess) {
+        lm_undo(lm, grow, st);
+        return hip_fail(e, "lm_prefill");
+    }
     for (int s = 0; s < n; ++s) lm->h_len[s] += counts[s];
     if (logits && !all)
         HIP_TRY(hipMemcpyAsync(logits, lm->logits, sizeof(float) * n * c.vocab, hipMemcpyDeviceToDevice, st),

@@ -461,8 +461,8 @@ __global__ __launch_bounds__(256) void k_kv_stack(int32_t* __restrict__ free_lis
     if (i < n) free_list[i] = n - 1 - i;
 }
 
-__global__ __launch_bounds__(64) void k_kv_counts(const PrefillMeta pm, int32_t* __restrict__ add) {
-    if ((int)threadIdx.x < pm.n) add[threadIdx.x] = pm.counts[threadIdx.x];
+__global__ __launch_bounds__(64) void k_kv_growths(const KvGrowths g, int32_t* __restrict__ add) {
+    if ((int)threadIdx.x < g.n) add[threadIdx.x] = g.add[threadIdx.x];
 }
 
 __global__ __launch_bounds__(256) void k_f32_to_bf16(const float* __restrict__ x, int64_t n, __bf16* __restrict__ y) {
@@ -477,17 +477,21 @@ bool pow2_page(int p) { return p >= 16 && p <= 1024 && (p & (p - 1)) == 0; }
 
 namespace sxq {
 
-hipError_t launch_kv_reserve(const KvReserve& a, hipStream_t s) {
+hipError_t launch_kv_reserve(const KvReserve& a, hipStream_t s, bool* moved) {
     const bool wave = a.n_rows <= 64;
-    const int mode = a.capacity <= (wave ? 256 : 2048) ? kAllInline : wave || a.capacity <= a.n_rows ? kMapApart : kPagesApart;
-    if (wave) hipLaunchKernelGGL((k_kv_reserve<64, 1>), dim3(1), dim3(64), 0, s, a, mode);
-    else if (a.n_rows <= 1024) hipLaunchKernelGGL((k_kv_reserve<1024, 1>), dim3(1), dim3(1024), 0, s, a, mode);
-    else hipLaunchKernelGGL((k_kv_reserve<1024, 4>), dim3(1), dim3(1024), 0, s, a, mode);
-    if (mode == kPagesApart)
-        hipLaunchKernelGGL(k_kv_pages, dim3(std::min(256, (a.n_pages + kPagesPer - 1) / kPagesPer)), dim3(kPagesPer), 0, s, a);
-    if (mode != kAllInline)
-        hipLaunchKernelGGL(k_kv_map, dim3((a.capacity + kMapTokens - 1) / kMapTokens), dim3(256), 0, s, a);
-    return hipGetLastError();
+    int mode = a.capacity <= (wave ? 256 : 2048) ? kAllInline : wave || a.capacity <= a.n_rows ? kMapApart : kPagesApart;
+    // (each launch's own result: `moved` may not depend on an error that an earlier call left)
+    auto launch = [&](const void* kernel, int grid, int block, void** args) {
+        return hipLaunchKernel(kernel, dim3(grid), dim3(block), args, 0, s);
+    };
+    void *both[] = {(void*)&a, &mode}, *one[] = {(void*)&a};
+    hipError_t e = wave ? launch((const void*)k_kv_reserve<64, 1>, 1, 64, both)
+                        : launch(a.n_rows <= 1024 ? (const void*)k_kv_reserve<1024, 1> : (const void*)k_kv_reserve<1024, 4>, 1, 1024, both);
+    if (e == hipSuccess && moved) *moved = true;
+    if (e == hipSuccess && mode == kPagesApart)
+        e = launch((const void*)k_kv_pages, std::min(256, (a.n_pages + kPagesPer - 1) / kPagesPer), kPagesPer, one);
+    if (e == hipSuccess && mode != kAllInline) e = launch((const void*)k_kv_map, (a.capacity + kMapTokens - 1) / kMapTokens, 256, one);
+    return e;
 }
 
 hipError_t launch_kv_append(const KvAppend& a, const KvPool& p, hipStream_t s) {
@@ -514,8 +518,8 @@ hipError_t launch_kv_stack(int32_t* free_list, int n, hipStream_t s) {
     return hipGetLastError();
 }
 
-hipError_t launch_kv_counts(const PrefillMeta& pm, int32_t* add, hipStream_t s) {
-    hipLaunchKernelGGL(k_kv_counts, dim3(1), dim3(64), 0, s, pm, add);
+hipError_t launch_kv_growths(const KvGrowths& g, int32_t* add, hipStream_t s) {
+    hipLaunchKernelGGL(k_kv_growths, dim3(1), dim3(64), 0, s, g, add);
     return hipGetLastError();
 }
 

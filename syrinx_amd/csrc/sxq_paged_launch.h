@@ -14,7 +14,9 @@ struct KvReserve {
     const int32_t* add;
     int32_t *lens, *table, *free_list, *free_count, *cu, *slots, *pos, *rows, *status;
 };
-hipError_t launch_kv_reserve(const KvReserve& a, hipStream_t s);
+// moved (or null): set once the launch that moves lengths (and, up to 64 rows, pages) is made,
+// which a later one of the call that fails does not take back.
+hipError_t launch_kv_reserve(const KvReserve& a, hipStream_t s, bool* moved = nullptr);
 
 struct KvAppend {
     const void* qkv;
@@ -52,9 +54,11 @@ hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table
                             hipStream_t s);
 // A free stack of pages 0 .. n - 1, page 0 on top.
 hipError_t launch_kv_stack(int32_t* free_list, int n, hipStream_t s);
-// add[i] = pm.counts[i], i < pm.n (a prompt's growths).
-struct PrefillMeta;
-hipError_t launch_kv_counts(const PrefillMeta& pm, int32_t* add, hipStream_t s);
+// The growths of an engine's streams, written to its device array.
+struct KvGrowths {
+    int n, add[16];
+};
+hipError_t launch_kv_growths(const KvGrowths& g, int32_t* add, hipStream_t s);
 // bf16 (round to nearest even) of n f32 values.
 hipError_t launch_f32_to_bf16(const float* x, int64_t n, uint16_t* y, hipStream_t s);
 

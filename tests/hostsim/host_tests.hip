@@ -92,10 +92,10 @@ void page_kernels() {
         const int n = *(int*)args[1], v = *(int*)args[2];
         return [=] { for (int i = 0; i < n; ++i) y[i] = v; };
     });
-    sim::kernel("k_kv_counts", [](void** args) {
-        const PrefillMeta pm = *(const PrefillMeta*)args[0];
+    sim::kernel("k_kv_growths", [](void** args) {
+        const KvGrowths g = *(const KvGrowths*)args[0];
         int32_t* add = *(int32_t**)args[1];
-        return [=] { for (int i = 0; i < pm.n; ++i) add[i] = pm.counts[i]; };
+        return [=] { for (int i = 0; i < g.n; ++i) add[i] = g.add[i]; };
     });
 }
 
@@ -178,8 +178,67 @@ void error_of_one_call() {
     EXPECT((e.lengths() == std::vector<int32_t>{6, 21, 0, 0}));
 }
 
+// Whichever of a call's launches and copies fails, the call can be made again: lengths, pages
+// and the map stay as the host has them.  Steps (eager, captured, replayed) and prompts.
+void failed_calls() {
+    for (const char* kind : {"step", "graph", "replay", "prompt"}) {
+        const std::string k = kind;
+        for (int at = 0;; ++at) {
+            Engine e(60, 2000);
+            EXPECT(e.prefill({15, 33, 1}) == SXQ_OK && e.step(3) == SXQ_OK);
+            if (k == "replay") EXPECT(e.step(3, SXQ_LM_GRAPH) == SXQ_OK);
+            e.consistent();
+            const std::vector<int32_t> before = e.lengths();
+            auto call = [&] { return k == "prompt" ? e.prefill({300, 2, 17}) : e.step(3, k == "step" ? 0 : SXQ_LM_GRAPH); };
+            sim::state().fail_in = at;
+            const sxq_status st = call();
+            const bool all_passed = sim::state().fail_in >= 0;  // fewer calls than that: nothing failed
+            sim::state().fail_in = -1;
+            e.consistent();
+            if (all_passed) {
+                EXPECT(st == SXQ_OK && at > (k == "replay" ? 1 : 9));
+                break;
+            }
+            EXPECT(st == SXQ_ERR_DEVICE);
+            if (e.lengths() != before) continue;  // what failed was a copy out, after the work
+            EXPECT(call() == SXQ_OK);
+            e.consistent();
+            for (int s = 0; s < 3; ++s) EXPECT(e.lengths()[s] == before[s] + (k == "prompt" ? (int[]){300, 2, 17}[s] : 1));
+        }
+    }
+}
+
+// Where the pages cannot be put back either (the device is lost, say), later calls say so
+// instead of running on lengths that the host does not know, until the streams are emptied.
+void failed_undo() {
+    Engine e(60, 2000);
+    EXPECT(e.prefill({15, 33, 1}) == SXQ_OK);
+    sim::State& s = sim::state();
+    const int before = s.calls;
+    EXPECT(e.step(3) == SXQ_OK);
+    const int per_step = s.calls - before;
+    s.fail_in = per_step / 2;
+    s.fail_times = 100;
+    EXPECT(e.step(3) == SXQ_ERR_DEVICE);
+    s.fail_in = -1;
+    s.fail_times = 1;
+    for (int again = 0; again < 2; ++again) {
+        EXPECT(e.step(3) == SXQ_ERR_INVALID && std::strstr(sxq_last_error(), "reset"));
+        EXPECT(e.prefill({4}) == SXQ_ERR_INVALID);
+        const int32_t one = 3;
+        EXPECT(sxq_lm_set_lengths(e.lm, &one, 1) == SXQ_ERR_INVALID);
+        EXPECT(sxq_lm_reset(e.lm, 2, nullptr) == SXQ_ERR_INVALID);  // not all of them
+    }
+    EXPECT(sxq_lm_reset(e.lm, e.n, nullptr) == SXQ_OK);
+    e.consistent();
+    EXPECT(e.free_pages() == 60 && e.prefill({15, 33, 1}) == SXQ_OK && e.step(3) == SXQ_OK);
+    e.consistent();
+}
+
 const std::map<std::string, void (*)()> kTests = {
     {"error_of_one_call", error_of_one_call},
+    {"failed_calls", failed_calls},
+    {"failed_undo", failed_undo},
 };
 
 }  // namespace

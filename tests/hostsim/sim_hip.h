@@ -20,6 +20,7 @@ struct Launch {
 };
 struct State {
     int fail_in = -1;             // this many more calls of the kinds below succeed, then one fails (-1: none)
+    int fail_times = 1;           // and as many after it
     int calls = 0;                // kernel launches, async copies, graph launches
     size_t malloc_limit = (size_t)-1;  // a larger hipMalloc is out of memory
     std::vector<size_t> mallocs;  // sizes, in order

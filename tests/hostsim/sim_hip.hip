@@ -29,7 +29,9 @@ bool fails() {
     sim::State& s = sim::state();
     ++s.calls;
     if (s.fail_in < 0) return false;
-    return s.fail_in-- == 0;
+    if (s.fail_in > 0) return --s.fail_in, false;
+    if (--s.fail_times == 0) s.fail_in = -1, s.fail_times = 1;
+    return true;
 }
 void enqueue(hipStream_t s, Work w) {
     if (capture && s == captured_stream) capture->push_back(std::move(w));

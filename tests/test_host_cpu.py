@@ -9,7 +9,7 @@ import pytest
 
 HERE = os.path.join(os.path.dirname(os.path.abspath(__file__)), "hostsim")
 
-TESTS = ["error_of_one_call"]
+TESTS = ["error_of_one_call", "failed_calls", "failed_undo"]
 
 
 @pytest.fixture(scope="module")
