@@ -118,7 +118,7 @@ struct sxq_lm {
     void* pf = nullptr;  // prefill workspace, grown to the largest prompt batch so far
     size_t pf_size = 0;
     std::vector<void*> allocs;
-    std::mutex mu;
+    mutable std::mutex mu;
 };
 
 namespace {
@@ -991,6 +991,7 @@ sxq_status sxq_lm_create_paged(int device, const sxq_lm_config* cfg, int kv_dtyp
 sxq_status sxq_lm_free_pages(const sxq_lm* lm, int* free_pages) {
     if (!lm || !free_pages) return fail(SXQ_ERR_INVALID, "lm_free_pages: null pointer");
     if (!lm->paged) return fail(SXQ_ERR_INVALID, "lm_free_pages: not a paged engine");
+    std::lock_guard<std::mutex> lock(lm->mu);
     int used = 0;
     for (int len : lm->h_len) used += kv_blocks(len, lm->pool.shift);
     *free_pages = lm->pool.n_pages - used;
@@ -1232,6 +1233,7 @@ sxq_status sxq_lm_reset(sxq_lm* lm, int n, void* stream) {
 sxq_status sxq_lm_get_lengths(const sxq_lm* lm, int32_t* lengths, int n) {
     if (!lm || !lengths) return fail(SXQ_ERR_INVALID, "lm_get_lengths: null pointer");
     if (n < 1 || n > lm->c.max_batch) return fail(SXQ_ERR_INVALID, "lm_get_lengths: bad stream count");
+    std::lock_guard<std::mutex> lock(lm->mu);
     for (int s = 0; s < n; ++s) lengths[s] = lm->h_len[s];
     return SXQ_OK;
 }

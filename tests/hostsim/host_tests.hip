@@ -3,11 +3,14 @@
 //   host_tests NAME      runs one test, prints "ok"
 #include <hip/hip_runtime.h>
 
+#include <atomic>
+#include <chrono>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <thread>
 
 #include "../../include/sxq.h"
 #include "sim_hip.h"
@@ -235,10 +238,38 @@ void failed_undo() {
     e.consistent();
 }
 
+// A thread that asks for the free pages or the lengths waits for a call that is changing them.
+void lengths_are_read_under_the_lock() {
+    Engine e(60, 2000);
+    const int32_t lens[2] = {40, 3}, more[2] = {100, 90};
+    EXPECT(sxq_lm_set_lengths(e.lm, lens, 2) == SXQ_OK);
+    for (int what = 0; what < 2; ++what) {
+        std::atomic<bool> returned{false}, during{false};
+        std::thread reader;
+        sim::state().on_sync = [&] {
+            if (reader.joinable()) return;
+            reader = std::thread([&] {
+                int32_t v[2] = {0, 0};
+                int pages = 0;
+                if (what) EXPECT(sxq_lm_get_lengths(e.lm, v, 2) == SXQ_OK);
+                else EXPECT(sxq_lm_free_pages(e.lm, &pages) == SXQ_OK);
+                returned = true;
+            });
+            for (int i = 0; i < 200 && !returned; ++i) std::this_thread::sleep_for(std::chrono::milliseconds(1));
+            during = returned.load();
+        };
+        EXPECT(sxq_lm_set_lengths(e.lm, what ? lens : more, 2) == SXQ_OK);
+        reader.join();
+        sim::state().on_sync = nullptr;
+        EXPECT(!during && returned);
+    }
+}
+
 const std::map<std::string, void (*)()> kTests = {
     {"error_of_one_call", error_of_one_call},
     {"failed_calls", failed_calls},
     {"failed_undo", failed_undo},
+    {"lengths_are_read_under_the_lock", lengths_are_read_under_the_lock},
 };
 
 }  // namespace
