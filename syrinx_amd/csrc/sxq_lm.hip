@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -127,8 +128,9 @@ namespace {
 int64_t embed_rows(const sxq_lm_config& c) { return c.embed_rows > 0 && !c.tied_embedding ? c.embed_rows : c.vocab; }
 
 hipError_t dalloc(sxq_lm* lm, void** p, size_t bytes) {
+    lm->allocs.push_back(nullptr);  // (its place first: nothing is lost if there is none)
     hipError_t e = hipMalloc(p, bytes ? bytes : 1);
-    if (e == hipSuccess) lm->allocs.push_back(*p);
+    if (e == hipSuccess) lm->allocs.back() = *p;
     return e;
 }
 
@@ -331,11 +333,11 @@ hipError_t fill_cache(void* p, int64_t n, int dtype, uint64_t seed) {
     return e;
 }
 
-// Pages of all streams at these lengths; refuses what the pool does not hold.
-sxq_status check_pages(const sxq_lm* lm, const char* who, const std::vector<int>& lens) {
+// Pages of all streams once these have grown; refuses what the pool does not hold.
+sxq_status check_pages(const sxq_lm* lm, const char* who, const KvGrowths& g) {
     if (!lm->paged) return SXQ_OK;
     int64_t need = 0;
-    for (int len : lens) need += kv_blocks(len, lm->pool.shift);
+    for (int s = 0; s < lm->c.max_batch; ++s) need += kv_blocks(lm->h_len[s] + (s < g.n ? g.add[s] : 0), lm->pool.shift);
     if (need > lm->pool.n_pages)
         return fail(SXQ_ERR_OOM, "%s: the streams need %lld KV pages of %d", who, (long long)need, lm->pool.n_pages);
     return SXQ_OK;
@@ -537,7 +539,8 @@ void destroy_lm(sxq_lm* lm) {
     for (auto& kv : lm->expand_graphs) (void)hipGraphExecDestroy(kv.second);
     if (lm->pf) (void)hipFree(lm->pf);
     if (lm->cap) (void)hipStreamDestroy(lm->cap);
-    for (void* p : lm->allocs) (void)hipFree(p);
+    for (void* p : lm->allocs)
+        if (p) (void)hipFree(p);
     delete lm;
 }
 
@@ -792,7 +795,8 @@ struct PageConfig {
     int dtype, page_size, n_pages;
 };
 
-sxq_status lm_create(int device, const sxq_lm_config* cfg, const PageConfig* pages, sxq_lm** out) {
+// (made: the engine as soon as it exists, for who has to free it; null again on an error)
+sxq_status lm_build(int device, const sxq_lm_config* cfg, const PageConfig* pages, sxq_lm** out, sxq_lm*& made) {
     if (!out) return fail(SXQ_ERR_INVALID, "lm_create: null output handle");
     *out = nullptr;
     sxq_status st = check_config(cfg, pages != nullptr);
@@ -814,7 +818,7 @@ sxq_status lm_create(int device, const sxq_lm_config* cfg, const PageConfig* pag
     }
     DeviceGuard g(device);
     HIP_TRY(g.err, "hipSetDevice");
-    sxq_lm* lm = new sxq_lm();
+    sxq_lm* lm = made = new sxq_lm();
     lm->device = device;
     lm->c = *cfg;
     const sxq_lm_config& c = lm->c;
@@ -906,6 +910,7 @@ sxq_status lm_create(int device, const sxq_lm_config* cfg, const PageConfig* pag
         A((void**)&lm->rope_row, sizeof(float) * 256);
     if (e != hipSuccess) {
         destroy_lm(lm);
+        made = nullptr;
         return hip_fail(e, "lm_create: allocation");
     }
     // RoPE tables, computed on the host with the reference's f32 formula:
@@ -969,11 +974,22 @@ sxq_status lm_create(int device, const sxq_lm_config* cfg, const PageConfig* pag
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         destroy_lm(lm);
+        made = nullptr;
         return hip_fail(e, "lm_create: initialisation");
     }
     lm->h_len.assign(MB, 0);
     *out = lm;
     return SXQ_OK;
+}
+
+sxq_status lm_create(int device, const sxq_lm_config* cfg, const PageConfig* pages, sxq_lm** out) {
+    sxq_lm* made = nullptr;
+    try {
+        return lm_build(device, cfg, pages, out, made);
+    } catch (const std::bad_alloc&) {  // (a paged engine's RoPE tables pass through a gigabyte of host memory at most)
+        if (made) destroy_lm(made);
+        return fail(SXQ_ERR_OOM, "lm_create: out of host memory");
+    }
 }
 
 }  // namespace
@@ -1191,17 +1207,13 @@ sxq_status sxq_lm_set_lengths(sxq_lm* lm, const int32_t* lengths, int n) {
     if (lm->paged) {  // pages given back or taken (those of added positions hold what they held)
         sxq_status st = check_lost(lm, "lm_set_lengths");
         if (st != SXQ_OK) return st;
-        std::vector<int> lens = lm->h_len;
         KvGrowths g{n, {}};
-        for (int s = 0; s < n; ++s) {
-            g.add[s] = lengths[s] - lens[s];
-            lens[s] = lengths[s];
-        }
-        st = check_pages(lm, "lm_set_lengths", lens);
+        for (int s = 0; s < n; ++s) g.add[s] = lengths[s] - lm->h_len[s];
+        st = check_pages(lm, "lm_set_lengths", g);
         if (st != SXQ_OK) return st;
         HIP_TRY(launch_kv_growths(g, lm->kv_add, nullptr), "lm_set_lengths");
         HIP_TRY(lm_reserve(lm, lm->kv_add, n, 0, nullptr, nullptr, nullptr, nullptr), "lm_set_lengths");
-        lm->h_len = lens;
+        for (int s = 0; s < n; ++s) lm->h_len[s] = lengths[s];
         HIP_TRY(hipDeviceSynchronize(), "lm_set_lengths");
         return SXQ_OK;
     }
@@ -1267,9 +1279,7 @@ sxq_status sxq_lm_step(sxq_lm* lm, int n, const int32_t* ids, const float* embed
     if (lm->paged) {
         sxq_status ok = check_lost(lm, "lm_step");
         if (ok != SXQ_OK) return ok;
-        std::vector<int> lens = lm->h_len;
-        for (int s = 0; s < n; ++s) lens[s] += grow.add[s];
-        ok = check_pages(lm, "lm_step", lens);
+        ok = check_pages(lm, "lm_step", grow);
         if (ok != SXQ_OK) return ok;
     }
     DeviceGuard g(lm->device);
@@ -1414,9 +1424,7 @@ sxq_status sxq_lm_prefill(sxq_lm* lm, int n, const int32_t* counts, const int32_
     if (lm->paged) {
         sxq_status ok = check_lost(lm, "lm_prefill");
         if (ok != SXQ_OK) return ok;
-        std::vector<int> lens = lm->h_len;
-        for (int s = 0; s < n; ++s) lens[s] += counts[s];
-        ok = check_pages(lm, "lm_prefill", lens);
+        ok = check_pages(lm, "lm_prefill", grow);
         if (ok != SXQ_OK) return ok;
     }
     const PfLayout P = pf_layout(lm, (int)T, pm);

@@ -10,6 +10,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <new>
 #include <thread>
 
 #include "../../include/sxq.h"
@@ -19,6 +20,19 @@
 #include "sxq_paged_launch.h"
 
 using namespace sxq;
+
+// Host allocations that still succeed before one fails (-1: all do).
+thread_local int allocations = -1;
+void* operator new(size_t n) {
+    if (allocations == 0) {
+        allocations = -1;
+        throw std::bad_alloc();
+    }
+    if (allocations > 0) --allocations;
+    return std::malloc(n ? n : 1);
+}
+void operator delete(void* p) noexcept { std::free(p); }
+void operator delete(void* p, size_t) noexcept { std::free(p); }
 
 #define EXPECT(c)                                                                                            \
     do {                                                                                                     \
@@ -265,7 +279,49 @@ void lengths_are_read_under_the_lock() {
     }
 }
 
+// What a step or a prompt checks before its first HIP call takes no host memory: an exception
+// would leave through the C entry.
+void checks_allocate_nothing() {
+    Engine e(10, 2000);
+    EXPECT(e.prefill({30, 50}) == SXQ_OK);
+    sim::state().on_call = [] { allocations = -1; };
+    allocations = 0;
+    EXPECT(e.step(2) == SXQ_OK);
+    const int32_t big[2] = {300, 5};
+    for (int i = 0; i < 2; ++i) {
+        allocations = 0;
+        EXPECT(i ? e.step(2) == SXQ_OK
+                 : sxq_lm_prefill(e.lm, 2, big, nullptr, e.embeds.data(), nullptr, nullptr, nullptr, 0, nullptr, 0, nullptr) == SXQ_ERR_OOM);
+    }
+    allocations = -1;
+    sim::state().on_call = nullptr;
+    e.consistent();
+}
+
+// Creation runs out of host memory at each of its allocations in turn: an error, every device
+// allocation given back.
+void creation_out_of_host_memory() {
+    const sxq_lm_config c = config(3000, 4);
+    for (int paged = 0; paged < 2; ++paged)
+        for (int at = 0;; ++at) {
+            sxq_lm* lm = nullptr;
+            const int held = sim::state().held;
+            allocations = at;
+            const sxq_status st = paged ? sxq_lm_create_paged(0, &c, SXQ_F32, 16, 100, &lm) : sxq_lm_create(0, &c, &lm);
+            const bool enough = allocations > 0;
+            allocations = -1;
+            EXPECT(st == (lm ? SXQ_OK : SXQ_ERR_OOM) && (lm || sim::state().held == held));
+            if (lm) {
+                sxq_lm_destroy(lm);
+                EXPECT(sim::state().held == held);
+            }
+            if (enough) break;
+        }
+}
+
 const std::map<std::string, void (*)()> kTests = {
+    {"checks_allocate_nothing", checks_allocate_nothing},
+    {"creation_out_of_host_memory", creation_out_of_host_memory},
     {"error_of_one_call", error_of_one_call},
     {"failed_calls", failed_calls},
     {"failed_undo", failed_undo},

@@ -23,8 +23,10 @@ struct State {
     int fail_times = 1;           // and as many after it
     int calls = 0;                // kernel launches, async copies, graph launches
     size_t malloc_limit = (size_t)-1;  // a larger hipMalloc is out of memory
+    int held = 0;                 // allocations not yet freed
     std::vector<size_t> mallocs;  // sizes, in order
     std::vector<Launch> launches;
+    std::function<void()> on_call;  // in hipGetDevice, the first HIP call of an entry point
     std::function<void()> on_sync;  // in hipDeviceSynchronize
 };
 State& state();

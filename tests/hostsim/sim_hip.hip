@@ -8,6 +8,8 @@
 
 #include "sim_hip.h"
 
+extern thread_local int allocations;  // host_tests.hip
+
 namespace {
 
 using Work = std::function<void()>;
@@ -83,6 +85,11 @@ hipError_t hipLaunchKernel(const void* f, dim3 grid, dim3 block, void** args, si
     const unsigned g[3] = {grid.x, grid.y, grid.z}, b[3] = {block.x, block.y, block.z};
     for (int d = 0; d < 3; ++d)
         if (!g[d] || (uint64_t)g[d] * b[d] > 0xFFFFFFFFull || (d && g[d] > 65535)) return ret(hipErrorInvalidConfiguration);
+    struct Free {  // the records take no part in a test's count
+        int all = allocations;
+        Free() { allocations = -1; }
+        ~Free() { allocations = all; }
+    } records;
     const std::string& name = names()[f];
     sim::state().launches.push_back({name, {g[0], g[1], g[2]}, {b[0], b[1], b[2]}});
     for (auto& k : bodies)
@@ -105,6 +112,7 @@ hipError_t hipGetDeviceCount(int* n) {
     return hipSuccess;
 }
 hipError_t hipGetDevice(int* d) {
+    if (sim::state().on_call) sim::state().on_call();
     *d = 0;
     return hipSuccess;
 }
@@ -120,17 +128,21 @@ hipError_t hipDeviceSynchronize() {
 
 hipError_t hipMalloc(void** p, size_t n) {
     if (n > sim::state().malloc_limit) return ret(hipErrorOutOfMemory);
-    sim::state().mallocs.push_back(n);
     // (zero pages on demand: 256-byte aligned within a block of its own)
     char* raw = (char*)calloc(1, n + 512);
     if (!raw) return ret(hipErrorOutOfMemory);
     char* at = (char*)(((uintptr_t)raw + 256 + sizeof(void*)) & ~(uintptr_t)255);
     ((void**)at)[-1] = raw;
     *p = at;
+    ++sim::state().held;
+    const int all = allocations;
+    allocations = -1;  // (the records' own memory)
+    sim::state().mallocs.push_back(n);
+    allocations = all;
     return hipSuccess;
 }
 hipError_t hipFree(void* p) {
-    if (p) free(((void**)p)[-1]);
+    if (p) free(((void**)p)[-1]), --sim::state().held;
     return hipSuccess;
 }
 hipError_t hipMallocAsync(void** p, size_t n, hipStream_t) { return hipMalloc(p, n); }
