@@ -417,6 +417,12 @@ sxq_status sxq_lm_reset(sxq_lm *lm, int n_streams, void *stream);
  * launch, so at capture for a graph) keeps every projection bit-identical. */
 sxq_status sxq_lm_step(sxq_lm *lm, int n_streams, const int32_t *ids, const float *embeds, float *logits,
                        float *hidden, int32_t *next_ids, unsigned flags, void *stream);
+/* The step of a paged engine in which only some of its streams take part: active host int32
+ * [n_streams] (NULL: all).  A stream whose entry is 0 keeps its length and its pages -- one
+ * that has stopped, in a batch that goes on -- and takes none; its input row is still read,
+ * its output rows mean nothing.  Refused with an entry of 0 for an engine that is not paged. */
+sxq_status sxq_lm_step_active(sxq_lm *lm, int n_streams, const int32_t *active, const int32_t *ids, const float *embeds,
+                              float *logits, float *hidden, int32_t *next_ids, unsigned flags, void *stream);
 /* sxq_lm_prefill flags */
 #define SXQ_LM_EXACT 2u      /* Q4_K projections through Candle's integer vec-dot (bit-identical) rather than the
                                 f16 MFMA GEMM; Q8_0 / Q4_0 are bit-identical either way */

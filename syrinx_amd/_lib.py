@@ -79,6 +79,7 @@ _SIGS = {
     "sxq_kv_attention_workspace": (_I, [_P, _I, _I, _P]),
     "sxq_kv_attention": (_I, [_I, _P, _I, _P, _I64, _I, _I, _P, _P, _I, _P, _I64, _I, _F, _P, _I64, _P, _SZ, _P]),
     "sxq_lm_step": (_I, [_P, _I, _P, _P, _P, _P, _P, _U, _P]),
+    "sxq_lm_step_active": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _U, _P]),
     "sxq_lm_read_kv": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _P]),
     "sxq_lm_prefill": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _U, _P, _SZ, _P]),
     "sxq_lm_prefill_trace_floats": (_I, [_P, _I64, _P]),

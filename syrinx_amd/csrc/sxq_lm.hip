@@ -47,8 +47,10 @@ struct GraphKey {
     bool embeds;
     const float* trace;
     int splits;  // attention splits per (stream, KV head) in the grid
+    bool some;   // only some of the streams take part (paged)
     bool operator<(const GraphKey& o) const {
         if (n != o.n) return n < o.n;
+        if (some != o.some) return some < o.some;
         if (embeds != o.embeds) return embeds < o.embeds;
         if (splits != o.splits) return splits < o.splits;
         return trace < o.trace;
@@ -112,6 +114,7 @@ struct sxq_lm {
     int32_t *kv_table = nullptr, *kv_free = nullptr, *kv_free_count = nullptr;
     int32_t *kv_add = nullptr, *kv_ones = nullptr;  // growths of a call; one token each
     int32_t *kv_cu = nullptr, *kv_status = nullptr, *kv_slots = nullptr, *kv_pos = nullptr, *kv_rows = nullptr;
+    int32_t* kv_map = nullptr;  // slots and positions of a step's tokens where some streams have none [2][max_batch]
     float* kv_ctx = nullptr;  // context rows of a step [max_batch][n_heads * head_dim]
     void* kv_ws = nullptr;    // the attention's workspace
     bool kv_moved = false;    // the call being enqueued has moved lengths and pages
@@ -343,7 +346,8 @@ sxq_status check_pages(const sxq_lm* lm, const char* who, const KvGrowths& g) {
     return SXQ_OK;
 }
 
-hipError_t enqueue_step(sxq_lm* lm, int n, bool from_embeds, hipStream_t s) {
+// some (paged): the growths are kv_add's zeros and ones, else one token each.
+hipError_t enqueue_step(sxq_lm* lm, int n, bool from_embeds, hipStream_t s, bool some = false) {
     const sxq_lm_config& c = lm->c;
     hipError_t e = hipSuccess;
 #define STEP(x)                      \
@@ -362,7 +366,11 @@ hipError_t enqueue_step(sxq_lm* lm, int n, bool from_embeds, hipStream_t s) {
         tr += floats;
         return p;
     };
-    if (lm->paged) STEP(lm_reserve(lm, lm->kv_ones, n, n, lm->kv_slots, lm->kv_pos, lm->kv_rows, s));
+    if (lm->paged && !some) STEP(lm_reserve(lm, lm->kv_ones, n, n, lm->kv_slots, lm->kv_pos, lm->kv_rows, s));
+    if (some) {  // the map holds the tokens there are; the step's rows are the streams
+        STEP(lm_reserve(lm, lm->kv_add, n, n, lm->kv_map, lm->kv_map + c.max_batch, lm->kv_rows, s));
+        STEP(launch_kv_by_row(lm->kv_cu, lm->kv_map, lm->kv_map + c.max_batch, n, lm->kv_slots, lm->kv_pos, s));
+    }
     // one stream through the fused attention: the embedding kernel also copies the step's
     // RoPE row, so that the attention splits issue their loads before the length returns
     const bool spec = lm->rope_row && n == 1 && lm->wo_fused && !from_embeds && !lm->embed_scheme;
@@ -871,6 +879,7 @@ sxq_status lm_build(int device, const sxq_lm_config* cfg, const PageConfig* page
         for (int32_t** p : {&lm->kv_add, &lm->kv_ones, &lm->kv_status, &lm->kv_slots, &lm->kv_pos, &lm->kv_rows})
             A((void**)p, sizeof(int32_t) * MB);
         A((void**)&lm->kv_cu, sizeof(int32_t) * (MB + 1));
+        A((void**)&lm->kv_map, sizeof(int32_t) * 2 * MB);
         A((void**)&lm->kv_ctx, sizeof(float) * (size_t)MB * lm->ctx);
         A(&lm->kv_ws, kv_attend_workspace(pool, MB, c.n_heads));
     } else {
@@ -953,6 +962,8 @@ sxq_status lm_build(int device, const sxq_lm_config* cfg, const PageConfig* page
     if (e == hipSuccess && pages) {
         e = empty_pages(lm, nullptr);
         if (e == hipSuccess) e = launch_fill_int(lm->kv_ones, MB, 1, nullptr);
+        // (the queries of a stream that has sat out since the start: finite)
+        if (e == hipSuccess) e = hipMemset(lm->qbuf, 0, sizeof(float) * (size_t)MB * lm->ctx);
         if (e == hipSuccess) e = hipMemset(lm->kv_ws, 0, kv_attend_workspace(pool, MB, c.n_heads));
     }
     lm->attn_fused = !pages && getenv("SXQ_ATTN_UNFUSED") == nullptr && attn_decode_fits(lm->vdt, c.n_heads, c.n_kv_heads, hd, lm->max_splits);
@@ -1267,15 +1278,25 @@ sxq_status sxq_lm_kv_fill_random(sxq_lm* lm, const int32_t* lengths, int n, uint
 
 sxq_status sxq_lm_step(sxq_lm* lm, int n, const int32_t* ids, const float* embeds, float* logits, float* hidden,
                        int32_t* next_ids, unsigned flags, void* stream) {
+    return sxq_lm_step_active(lm, n, nullptr, ids, embeds, logits, hidden, next_ids, flags, stream);
+}
+
+sxq_status sxq_lm_step_active(sxq_lm* lm, int n, const int32_t* active, const int32_t* ids, const float* embeds,
+                              float* logits, float* hidden, int32_t* next_ids, unsigned flags, void* stream) {
     if (!lm) return fail(SXQ_ERR_INVALID, "lm_step: null handle");
     if (n < 1 || n > lm->c.max_batch) return fail(SXQ_ERR_INVALID, "lm_step: %d streams (max %d)", n, lm->c.max_batch);
     if (flags & ~SXQ_LM_GRAPH) return fail(SXQ_ERR_INVALID, "lm_step: unknown flags 0x%x", flags);
     std::lock_guard<std::mutex> lock(lm->mu);
-    for (int s = 0; s < n; ++s)
-        if (lm->h_len[s] >= lm->c.max_seq)
-            return fail(SXQ_ERR_INVALID, "lm_step: stream %d KV cache is full (%d positions)", s, lm->c.max_seq);
     KvGrowths grow{n, {}};
-    for (int s = 0; s < n; ++s) grow.add[s] = 1;
+    bool some = false;
+    for (int s = 0; s < n; ++s) {
+        grow.add[s] = !active || active[s] ? 1 : 0;
+        some |= !grow.add[s];
+    }
+    if (some && !lm->paged) return fail(SXQ_ERR_INVALID, "lm_step: only a paged engine's streams can sit out");
+    for (int s = 0; s < n; ++s)
+        if (grow.add[s] && lm->h_len[s] >= lm->c.max_seq)
+            return fail(SXQ_ERR_INVALID, "lm_step: stream %d KV cache is full (%d positions)", s, lm->c.max_seq);
     if (lm->paged) {
         sxq_status ok = check_lost(lm, "lm_step");
         if (ok != SXQ_OK) return ok;
@@ -1288,9 +1309,10 @@ sxq_status sxq_lm_step(sxq_lm* lm, int n, const int32_t* ids, const float* embed
     const bool emb = embeds != nullptr;
     if (ids) HIP_TRY(hipMemcpyAsync(lm->d_ids, ids, sizeof(int) * n * lm->ids_per, hipMemcpyDeviceToDevice, st), "lm_step: ids");
     if (emb) HIP_TRY(hipMemcpyAsync(lm->h, embeds, sizeof(float) * n * lm->c.dim, hipMemcpyDeviceToDevice, st), "lm_step: embeds");
+    if (some) HIP_TRY(launch_kv_growths(grow, lm->kv_add, st), "lm_step: growths");
     lm->grid_splits = lm->paged ? 0 : step_grid_splits(lm, n);
     if (flags & SXQ_LM_GRAPH) {
-        const GraphKey key{n, emb, lm->trace, lm->grid_splits};
+        const GraphKey key{n, emb, lm->trace, lm->grid_splits, some};
         auto it = lm->graphs.find(key);
         if (it == lm->graphs.end()) {
             // Capture on the library's own stream (the legacy default stream cannot capture).
@@ -1298,7 +1320,7 @@ sxq_status sxq_lm_step(sxq_lm* lm, int n, const int32_t* ids, const float* embed
             hipGraphExec_t exec = nullptr;
             HIP_TRY(hipStreamSynchronize(st), "lm_step: sync before capture");
             HIP_TRY(hipStreamBeginCapture(lm->cap, hipStreamCaptureModeThreadLocal), "lm_step: begin capture");
-            hipError_t e = enqueue_step(lm, n, emb, lm->cap);
+            hipError_t e = enqueue_step(lm, n, emb, lm->cap, some);
             hipError_t e2 = hipStreamEndCapture(lm->cap, &graph);
             if (e == hipSuccess) e = e2;
             if (e == hipSuccess) e = hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0);
@@ -1309,7 +1331,7 @@ sxq_status sxq_lm_step(sxq_lm* lm, int n, const int32_t* ids, const float* embed
         HIP_TRY(hipGraphLaunch(it->second, st), "lm_step: graph launch");
     } else {
         lm->kv_moved = false;
-        const hipError_t e = enqueue_step(lm, n, emb, st);
+        const hipError_t e = enqueue_step(lm, n, emb, st, some);
         if (e != hipSuccess) {
             lm_undo(lm, grow, st);
             return hip_fail(e, "lm_step");

@@ -465,6 +465,17 @@ __global__ __launch_bounds__(64) void k_kv_growths(const KvGrowths g, int32_t* _
     if ((int)threadIdx.x < g.n) add[threadIdx.x] = g.add[threadIdx.x];
 }
 
+__global__ __launch_bounds__(64) void k_kv_by_row(const int32_t* __restrict__ cu, const int32_t* __restrict__ map_slots,
+                                                  const int32_t* __restrict__ map_pos, int rows, int32_t* __restrict__ slots,
+                                                  int32_t* __restrict__ pos) {
+    const int r = threadIdx.x;
+    if (r >= rows) return;
+    const int t = cu[r];
+    const bool has = cu[r + 1] > t;
+    slots[r] = has ? map_slots[t] : -1;
+    pos[r] = has ? map_pos[t] : 0;
+}
+
 __global__ __launch_bounds__(256) void k_f32_to_bf16(const float* __restrict__ x, int64_t n, __bf16* __restrict__ y) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i < n) y[i] = (__bf16)x[i];
@@ -520,6 +531,12 @@ hipError_t launch_kv_stack(int32_t* free_list, int n, hipStream_t s) {
 
 hipError_t launch_kv_growths(const KvGrowths& g, int32_t* add, hipStream_t s) {
     hipLaunchKernelGGL(k_kv_growths, dim3(1), dim3(64), 0, s, g, add);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_by_row(const int32_t* cu, const int32_t* map_slots, const int32_t* map_pos, int rows, int32_t* slots,
+                            int32_t* pos, hipStream_t s) {
+    hipLaunchKernelGGL(k_kv_by_row, dim3(1), dim3(64), 0, s, cu, map_slots, map_pos, rows, slots, pos);
     return hipGetLastError();
 }
 

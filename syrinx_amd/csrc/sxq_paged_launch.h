@@ -59,6 +59,9 @@ struct KvGrowths {
     int n, add[16];
 };
 hipError_t launch_kv_growths(const KvGrowths& g, int32_t* add, hipStream_t s);
+// Row r's slot and position (-1 and 0 without a token) from a map of at most one token a row.
+hipError_t launch_kv_by_row(const int32_t* cu, const int32_t* map_slots, const int32_t* map_pos, int rows, int32_t* slots,
+                            int32_t* pos, hipStream_t s);
 // bf16 (round to nearest even) of n f32 values.
 hipError_t launch_f32_to_bf16(const float* x, int64_t n, uint16_t* y, hipStream_t s);
 

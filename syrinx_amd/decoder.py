@@ -137,6 +137,7 @@ class DecoderLM:
         self.device = torch.device(device)
         self._h = ctypes.c_void_p()
         self._c = cfg.to_c()
+        self.paged = kv_pages is not None
         if kv_pages is None:
             check(lib().sxq_lm_create(self._dev(), ctypes.byref(self._c), ctypes.byref(self._h)))
         else:
@@ -215,12 +216,14 @@ class DecoderLM:
 
     # -- step ---------------------------------------------------------------------------
     def step(self, ids: torch.Tensor = None, embeds: torch.Tensor = None, n: int = None, graph: bool = False,
-             want_logits: bool = True, want_hidden: bool = False, out=None):
+             want_logits: bool = True, want_hidden: bool = False, out=None, active=None):
         """One token for n streams.  ids int32 [n, 1 + n_codebooks] (or [n]) or embeds
         f32 [n, dim]; None for both reuses the previous argmax.  Returns (logits, next_ids),
         or (logits, next_ids, hidden) with want_hidden (the post-final-RMSNorm state).
         out = (logits, next_ids, hidden) writes into those device tensors instead (fixed
-        buffers for a loop whose later launches are captured on their addresses)."""
+        buffers for a loop whose later launches are captured on their addresses).
+        active (paged engines): n flags on the host; a stream whose flag is 0 keeps its length
+        and pages, its output rows mean nothing (sxq_lm_step_active)."""
         if ids is not None:
             ids = ids.to(device=self.device, dtype=torch.int32).reshape(-1, self.ids_per).contiguous()
             n = ids.shape[0]
@@ -240,8 +243,13 @@ class DecoderLM:
             nxt = torch.empty((n,), dtype=torch.int32, device=self.device)
             hidden = torch.empty((n, self.cfg.dim), dtype=torch.float32, device=self.device) if want_hidden else None
         P = lambda t: ctypes.c_void_p(t.data_ptr()) if t is not None else None  # noqa: E731
-        check(lib().sxq_lm_step(self._h, n, P(ids), P(embeds), P(logits), P(hidden), P(nxt), LM_GRAPH if graph else 0,
-                                torch.cuda.current_stream(self.device).cuda_stream))
+        some = None
+        if active is not None:
+            if len(active) != n:
+                raise ValueError(f"step: {len(active)} active flags for {n} streams")
+            some = (ctypes.c_int32 * n)(*(1 if a else 0 for a in active))
+        check(lib().sxq_lm_step_active(self._h, n, some, P(ids), P(embeds), P(logits), P(hidden), P(nxt),
+                                       LM_GRAPH if graph else 0, torch.cuda.current_stream(self.device).cuda_stream))
         return (logits, nxt, hidden) if want_hidden else (logits, nxt)
 
     def prefill(self, prompts=None, embeds=None, exact: bool = False, all_logits: bool = False, trace: bool = False):
@@ -384,16 +392,16 @@ class SlowAr(DecoderLM):
         self._last_argmax = nxt
         return logits[0], self._fast_hidden(hidden).reshape(1, 1, -1)
 
-    def slow_step_batch(self, frames, graph: bool = True, out=None):
+    def slow_step_batch(self, frames, graph: bool = True, out=None, active=None):
         """frames: [n, 1 + num_codebooks]; ragged cache lengths need no left padding
         (slow_ar.rs:456-499).  Returns (semantic_logits [n, vocab], hidden [n, 1, hidden_dim]);
-        out = (logits, next_ids, hidden) as for step() (hidden [n, hidden_dim])."""
+        out = (logits, next_ids, hidden) and active as for step() (hidden [n, hidden_dim])."""
         hid_out = None
         if out is not None and self.project_in is not None:  # the step writes the raw hidden first
             raw = torch.empty((out[0].shape[0], self.cfg.dim), dtype=torch.float32, device=self.device)
             out, hid_out = (out[0], out[1], raw), out[2]
         logits, nxt, hidden = self.step(ids=torch.as_tensor(frames, dtype=torch.int32), graph=graph, want_hidden=True,
-                                        out=out)
+                                        out=out, active=active)
         self._last_argmax = nxt
         return logits, self._fast_hidden(hidden, hid_out).reshape(-1, 1, self.hidden_dim)
 

@@ -79,7 +79,8 @@ def generate_frames(slow: SlowAr, fast: FastAr, sampler: FishSampler, logits0, h
     cache length.  Returns the frames [n, 1 + n_cb] of every pass and the streams' active
     flags after each pass's semantic draw (device tensors; the host has synchronised).
     `active` / `frame` may be passed to keep their buffers (and the captured expansion)
-    across calls."""
+    across calls.  On a paged slow engine a stream that the host has seen stop sits out of the
+    steps that follow: it takes no more pages."""
     c = slow.cfg
     n_cb = c.n_codebooks
     n = logits0.shape[0]
@@ -95,6 +96,7 @@ def generate_frames(slow: SlowAr, fast: FastAr, sampler: FishSampler, logits0, h
     frames, flags = [], []
     flag_host = torch.empty(n, dtype=torch.int32, pin_memory=True)
     done = torch.cuda.Event()
+    live = active.tolist() if slow.paged else None
     for _ in range(max_new_frames):
         # 1. each active stream's semantic draw (a stop freezes the stream); 2. the frame
         sampler.sample_semantic(logits, out=frame[:, 0], out_stride=1 + n_cb, active=active)
@@ -106,10 +108,12 @@ def generate_frames(slow: SlowAr, fast: FastAr, sampler: FishSampler, logits0, h
         if len(frames) >= max_new_frames or pos + 1 >= c.max_seq:
             break
         # 4. feed the frame back (enqueued before the host looks at the flags)
-        slow.slow_step_batch(frame, out=(logits, nxt, hidden))
+        slow.slow_step_batch(frame, out=(logits, nxt, hidden), active=live)
         pos += 1
         done.synchronize()
         if not bool(flag_host.any()):
             break
+        if live is not None:
+            live = flag_host.tolist()
     torch.cuda.current_stream(dev).synchronize()
     return frames, flags

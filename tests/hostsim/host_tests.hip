@@ -93,11 +93,29 @@ void reserve_rows(const KvReserve& a) {
     for (; t < a.capacity; ++t) a.slots[t] = a.pos[t] = a.rows[t] = -1;
 }
 
+std::vector<int> stored;  // the slots of the last append, by row
+
 // Bodies of the kernels that keep an engine's lengths and pages.
 void page_kernels() {
     sim::kernel("k_kv_reserve", [](void** args) {
         const KvReserve a = *(const KvReserve*)args[0];
         return [a] { reserve_rows(a); };
+    });
+    sim::kernel("k_kv_by_row", [](void** args) {
+        const int32_t *cu = *(int32_t**)args[0], *ms = *(int32_t**)args[1], *mp = *(int32_t**)args[2];
+        const int rows = *(int*)args[3];
+        int32_t *slots = *(int32_t**)args[4], *pos = *(int32_t**)args[5];
+        return [=] {
+            for (int r = 0; r < rows; ++r) {
+                const bool has = cu[r + 1] > cu[r];
+                slots[r] = has ? ms[cu[r]] : -1;
+                pos[r] = has ? mp[cu[r]] : 0;
+            }
+        };
+    });
+    sim::kernel("k_kv_append", [](void** args) {
+        const KvAppend a = *(const KvAppend*)args[0];
+        return [a] { stored.assign(a.slots, a.slots + a.n_tokens); };
     });
     sim::kernel("k_kv_stack", [](void** args) {
         int32_t* list = *(int32_t**)args[0];
@@ -319,6 +337,66 @@ void creation_out_of_host_memory() {
         }
 }
 
+// Steps in which some streams sit out: those keep lengths and pages, the others' rows get their
+// own slots; eager, captured and replayed, each failing at each of its calls.
+void streams_that_sit_out() {
+    for (unsigned flags : {0u, (unsigned)SXQ_LM_GRAPH}) {
+        Engine e(40, 2000);
+        EXPECT(e.prefill({15, 31, 7, 64}) == SXQ_OK);
+        auto some = [&](std::vector<int32_t> active) {
+            return sxq_lm_step_active(e.lm, 4, active.data(), nullptr, e.embeds.data(), e.logits.data(), nullptr, nullptr, flags, nullptr);
+        };
+        std::vector<int32_t> want = e.lengths();
+        for (int turn = 0; turn < 40; ++turn) {
+            std::vector<int32_t> active(4);
+            for (int s = 0; s < 4; ++s) active[s] = (turn >> s & 1) * (turn + 3);  // any value but 0
+            EXPECT(some(active) == SXQ_OK);
+            for (int s = 0; s < 4; ++s) {
+                want[s] += active[s] != 0;
+                const int p = want[s] - 1;
+                EXPECT(stored[s] == (active[s] ? seen.table[s * seen.table_stride + (p >> 4)] * 16 + (p & 15) : -1));
+            }
+            EXPECT(e.lengths() == want);
+            e.consistent();
+            if (turn % 7 == 3) {
+                EXPECT(e.step(4, flags) == SXQ_OK);
+                for (int& v : want) ++v;
+                e.consistent();
+            }
+        }
+        for (int at = 0;; ++at) {
+            sim::state().fail_in = at;
+            const sxq_status st = some({1, 0, 1, 0});
+            const bool all_passed = sim::state().fail_in >= 0;
+            sim::state().fail_in = -1;
+            e.consistent();
+            if (all_passed) break;
+            EXPECT(st == SXQ_ERR_DEVICE);
+        }
+    }
+    // the pool counts only those that take part
+    Engine e(4, 2000, 2);
+    EXPECT(e.prefill({32, 32}) == SXQ_OK);
+    const int32_t one[2] = {0, 1}, none[2] = {0, 0}, small[2] = {16, 32};
+    EXPECT(sxq_lm_step_active(e.lm, 2, one, nullptr, e.embeds.data(), nullptr, nullptr, nullptr, 0, nullptr) == SXQ_ERR_OOM);
+    EXPECT(sxq_lm_step_active(e.lm, 2, none, nullptr, e.embeds.data(), nullptr, nullptr, nullptr, 0, nullptr) == SXQ_OK);
+    EXPECT(sxq_lm_set_lengths(e.lm, small, 2) == SXQ_OK && e.step(2) == SXQ_ERR_OOM);
+    EXPECT(sxq_lm_step_active(e.lm, 2, one, nullptr, e.embeds.data(), nullptr, nullptr, nullptr, 0, nullptr) == SXQ_OK);
+    e.consistent();
+    // nor does a full stream that sits out stop the others
+    Engine f(20, 64, 2);
+    EXPECT(f.prefill({64, 3}) == SXQ_OK && f.step(2) == SXQ_ERR_INVALID);
+    EXPECT(sxq_lm_step_active(f.lm, 2, one, nullptr, f.embeds.data(), nullptr, nullptr, nullptr, 0, nullptr) == SXQ_OK);
+    // a contiguous engine's streams cannot
+    const sxq_lm_config c = config(64, 2);
+    sxq_lm* lm = nullptr;
+    EXPECT(sxq_lm_create(0, &c, &lm) == SXQ_OK);
+    const int32_t all[2] = {1, 1};
+    EXPECT(sxq_lm_step_active(lm, 2, one, nullptr, e.embeds.data(), nullptr, nullptr, nullptr, 0, nullptr) == SXQ_ERR_INVALID);
+    EXPECT(sxq_lm_step_active(lm, 2, all, nullptr, e.embeds.data(), nullptr, nullptr, nullptr, 0, nullptr) == SXQ_OK);
+    EXPECT(sxq_lm_destroy(lm) == SXQ_OK);
+}
+
 const std::map<std::string, void (*)()> kTests = {
     {"checks_allocate_nothing", checks_allocate_nothing},
     {"creation_out_of_host_memory", creation_out_of_host_memory},
@@ -326,6 +404,7 @@ const std::map<std::string, void (*)()> kTests = {
     {"failed_calls", failed_calls},
     {"failed_undo", failed_undo},
     {"lengths_are_read_under_the_lock", lengths_are_read_under_the_lock},
+    {"streams_that_sit_out", streams_that_sit_out},
 };
 
 }  // namespace

@@ -1,0 +1,126 @@
+"""Serving loops on a paged decode engine: streams that have stopped, pages that run out in the
+middle of a generation, long histories under a prompt."""
+import dataclasses
+import functools
+
+import numpy as np
+import pytest
+import torch
+
+import test_gpu_decoder as T
+from syrinx_amd import SxqError, _lib, dualar
+from syrinx_amd import decoder as D
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need a ROCm GPU")
+    return torch.device("cuda:0")
+
+
+# ---- steps in which some streams sit out --------------------------------------------------
+
+PATTERNS = [(1, 1, 1), (1, 0, 1), (0, 0, 1), (0, 1, 0), (1, 1, 1), (1, 0, 0)]
+
+
+@pytest.mark.parametrize("page", [16, 32])
+def test_every_op_of_the_streams_that_take_part_matches_oracle(cuda, ora, page):
+    cfg, lengths = T._fish_small(n_layers=2, max_batch=3), [31, 5, 16]
+    lm, W = T._build(cfg, cuda, 31, 3, cls=functools.partial(D.DecoderLM, kv_pages=12, page_size=page))
+    lm.kv_fill_random(lengths, seed=32)
+    lm.enable_trace()
+    rng = np.random.default_rng(33)
+    for active in PATTERNS:
+        frames = list(T._frames(rng, 3, cfg))
+        logits, _ = lm.step(ids=torch.from_numpy(np.stack(frames)), active=active)
+        tr, got = lm.trace(3), logits.cpu().numpy()
+        for s in range(3):
+            if active[s]:
+                want = T._replay_step(ora, lm, cfg, W, tr, s, lengths[s], frame=frames[s])
+                T._bits_equal(got[s], want, f"{active} stream {s} head projection")
+                lengths[s] += 1
+        assert lm.lengths(3) == lengths and lm.free_pages() == 12 - sum(-(-n // page) for n in lengths)
+
+
+def test_steps_of_some_streams_as_graphs(cuda):
+    """Graph and eager steps of changing patterns, eager work and synchronizations between: the
+    same bits for the streams that take part, the caches of the others as they were."""
+    cfg = T._fish_small(n_layers=2, max_batch=3)
+    a, b = (D.DecoderLM(cfg, device=cuda, kv_pages=18, page_size=16, kv_dtype=torch.bfloat16) for _ in range(2))
+    rng = np.random.default_rng(5)
+    prompts = [torch.from_numpy(T._frames(rng, n, cfg)) for n in (15, 30, 1)]
+    for lm in (a, b):
+        lm.init_random(seed=4)
+        lm.prefill(prompts=prompts)
+    for turn in range(18):
+        active = PATTERNS[turn * 5 % len(PATTERNS)]
+        ids = torch.from_numpy(T._frames(rng, 3, cfg))
+        held = [s for s in range(3) if not active[s]]
+        before = [[x.clone() for x in a.read_kv(1, s, 0, 0, a.lengths(3)[s])] for s in held]
+        x, nx = a.step(ids=ids, graph=True, active=active)
+        y, ny = b.step(ids=ids, graph=False, active=active)
+        if turn % 3 == 1:
+            torch.cuda.synchronize()
+        live = [s for s in range(3) if active[s]]
+        assert torch.equal(x[live], y[live]) and torch.equal(nx[live], ny[live]), (turn, active)
+        assert x.isfinite().all() and a.lengths(3) == b.lengths(3)
+        for s, old in zip(held, before):
+            assert all(torch.equal(u, v) for u, v in zip(a.read_kv(1, s, 0, 0, a.lengths(3)[s]), old))
+    for wrong in ([1, 0], [1, 1, 1, 1]):
+        with pytest.raises(ValueError):
+            a.step(ids=ids, active=wrong)
+    with pytest.raises(SxqError) as e:
+        D.DecoderLM(cfg, device=cuda).step(ids=ids, active=[1, 0, 1])
+    assert e.value.code == _lib.ERR_INVALID
+
+
+# ---- the Fish frame loop ----------------------------------------------------------------
+
+class Scripted(dualar.FishSampler):
+    """A sampler whose stream i stops at its pass stops[i] (from 0)."""
+
+    def __init__(self, stops, semantic, device):
+        super().__init__([1] * len(stops), semantic=semantic, device=device)
+        self.stops, self.turn = stops, 0
+
+    def sample_semantic(self, logits, out=None, out_stride=1, active=None):
+        super().sample_semantic(logits, out=out, out_stride=out_stride, active=active)
+        stop = torch.tensor([self.turn >= s for s in self.stops], device=active.device)
+        active.masked_fill_(stop, 0)
+        self.turn += 1
+
+
+def _loop(cuda, pages, counts, stops, frames, page_size=16, **kw):
+    """The frame loop over prompts of `counts` tokens; the slow engine, the number of passes, and
+    the flags of every pass."""
+    cfg = dataclasses.replace(T._fish_small(n_layers=1, max_batch=len(counts)), max_seq=400)
+    slow = D.SlowAr(cfg, device=cuda, kv_pages=pages, page_size=page_size, **kw)
+    slow.init_random(seed=6)
+    fast = D.FastAr(D.fish_s2_fast_ar_config(n_layers=1, num_codebooks=10, residual_size=64, max_batch=len(counts)), device=cuda)
+    fast.init_random(seed=7)
+    rng = np.random.default_rng(8)
+    logits, hidden = slow.prefill_batch([T._frames(rng, c, cfg).T for c in counts])
+    sampler = Scripted(stops, (cfg.semantic_begin, cfg.semantic_end, -1), cuda)
+    out, flags = dualar.generate_frames(slow, fast, sampler, logits, hidden, frames, max(counts))
+    return slow, out, torch.stack(flags).cpu()
+
+
+def test_streams_that_have_stopped_take_no_pages(cuda):
+    """Three of four streams stop early: the pool holds the live tokens and no more."""
+    stops, counts, frames = [3, 200, 7, 0], [20, 10, 31, 5], 120
+    # stream 1 alone grows to 10 + 119; a stopped one may have had one step more than it needed
+    pages = -(-(10 + 119) // 16) + sum(-(-(c + s + 1) // 16) for c, s in ((20, 3), (31, 7), (5, 0)))
+    slow, out, flags = _loop(cuda, pages, counts, stops, frames)
+    assert len(out) == frames and flags[:, 1].all()
+    assert flags[:, 0].sum() == 3 and flags[:, 2].sum() == 7 and flags[:, 3].sum() == 0
+    lens = slow.lengths(4)
+    assert lens[1] == 10 + 119
+    assert all(c + s <= n <= c + s + 1 for n, c, s in zip((lens[0], lens[2], lens[3]), (20, 31, 5), (3, 7, 0)))
+
+
+def test_every_stream_stopped_ends_the_loop(cuda):
+    slow, out, flags = _loop(cuda, 8, [16, 20], [2, 5], 60)
+    assert len(out) <= 7 and not flags[-1].any()
