@@ -17,7 +17,7 @@ from dataclasses import dataclass, fields
 
 import torch
 
-from ._lib import check, lib
+from ._lib import ERR_OOM, SxqError, check, lib
 from .quantized import GgmlDType, QMatMul
 
 LM_GRAPH = 1
@@ -122,6 +122,11 @@ def fish_s2_fast_ar_config(n_layers=4, num_codebooks=10, residual_size=4096, max
                 tied_embedding=0, embed_rows=residual_size)
     base.update(kw)
     return DecoderConfig(**base)
+
+
+def out_of_pages(e: SxqError) -> bool:
+    """Whether a paged engine's call was refused for want of pages (nothing of it has run)."""
+    return e.code == ERR_OOM and "KV pages" in e.msg
 
 
 class DecoderLM:

@@ -17,7 +17,8 @@ from dataclasses import dataclass, field
 
 import torch
 
-from .decoder import FastAr, SlowAr
+from ._lib import SxqError
+from .decoder import FastAr, SlowAr, out_of_pages
 from .sampling import FishSampler, SamplingParams
 
 
@@ -80,7 +81,8 @@ def generate_frames(slow: SlowAr, fast: FastAr, sampler: FishSampler, logits0, h
     flags after each pass's semantic draw (device tensors; the host has synchronised).
     `active` / `frame` may be passed to keep their buffers (and the captured expansion)
     across calls.  On a paged slow engine a stream that the host has seen stop sits out of the
-    steps that follow: it takes no more pages."""
+    steps that follow: it takes no more pages.  When the pages do not reach for the streams
+    that go on, the loop ends with the frames it has, as it does at max_seq."""
     c = slow.cfg
     n_cb = c.n_codebooks
     n = logits0.shape[0]
@@ -108,7 +110,22 @@ def generate_frames(slow: SlowAr, fast: FastAr, sampler: FishSampler, logits0, h
         if len(frames) >= max_new_frames or pos + 1 >= c.max_seq:
             break
         # 4. feed the frame back (enqueued before the host looks at the flags)
-        slow.slow_step_batch(frame, out=(logits, nxt, hidden), active=live)
+        try:
+            slow.slow_step_batch(frame, out=(logits, nxt, hidden), active=live)
+        except SxqError as e:
+            if live is None or not out_of_pages(e):
+                raise
+            done.synchronize()  # who has stopped in this pass, and leaves its place to the others
+            now = flag_host.tolist()
+            if now == live or not any(now):
+                break
+            live = now
+            try:
+                slow.slow_step_batch(frame, out=(logits, nxt, hidden), active=live)
+            except SxqError as e:
+                if not out_of_pages(e):
+                    raise
+                break
         pos += 1
         done.synchronize()
         if not bool(flag_host.any()):

@@ -121,6 +121,22 @@ def test_streams_that_have_stopped_take_no_pages(cuda):
     assert all(c + s <= n <= c + s + 1 for n, c, s in zip((lens[0], lens[2], lens[3]), (20, 31, 5), (3, 7, 0)))
 
 
+def test_the_loop_ends_with_its_frames_when_pages_run_out(cuda):
+    """Two live streams over a pool for 40 more tokens each: the frames up to there."""
+    slow, out, flags = _loop(cuda, 2 * 3, [8, 8], [500, 500], 300)
+    assert len(out) == 3 * 16 - 8 + 1 and flags.all()  # the last pass has no room for a step
+    assert slow.lengths(2) == [48, 48] and slow.free_pages() == 0
+
+
+def test_a_stream_that_stops_on_the_last_page_leaves_it_to_the_others(cuda):
+    """The step that finds no pages comes before the host has seen who has stopped: it is made
+    again for those that have not."""
+    # both need a page at length 32; stream 0 stops in that very pass, one page is left
+    slow, out, flags = _loop(cuda, 5, [16, 16], [16, 500], 40)
+    assert len(out) == 33 and flags[:, 1].all() and flags[:, 0].sum() == 16
+    assert slow.lengths(2) == [32, 48]
+
+
 def test_every_stream_stopped_ends_the_loop(cuda):
     slow, out, flags = _loop(cuda, 8, [16, 20], [2, 5], 60)
     assert len(out) <= 7 and not flags[-1].any()
