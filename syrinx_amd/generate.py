@@ -25,7 +25,8 @@ from dataclasses import dataclass
 
 import torch
 
-from .decoder import Qwen2Lm
+from ._lib import SxqError
+from .decoder import Qwen2Lm, out_of_pages
 from .embedding import QEmbed
 from .sampling import RasSampler
 
@@ -130,12 +131,20 @@ class CosyVoiceLm:
             smp.sample(logits, ignore_eos=i < min_len, out=tok.view(-1))
             host.copy_(tok.view(-1), non_blocking=True)
             done.record()
+            short = None
             if i + 1 < max_len:  # the next step, enqueued before the host looks at the token
-                lm.step(ids=tok, graph=graph, out=(logits, nxt, None))
+                try:
+                    lm.step(ids=tok, graph=graph, out=(logits, nxt, None))
+                except SxqError as e:
+                    if not out_of_pages(e):
+                        raise
+                    short = e
             done.synchronize()
             t = int(host[0])
             if v.stop_begin <= t < v.stop_end:
                 break
+            if short is not None:  # (after a stop there is no step to make)
+                raise short
             out.append(t)
         torch.cuda.current_stream(dev).synchronize()
         return out

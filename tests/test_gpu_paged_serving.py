@@ -10,6 +10,8 @@ import torch
 import test_gpu_decoder as T
 from syrinx_amd import SxqError, _lib, dualar
 from syrinx_amd import decoder as D
+from syrinx_amd.generate import COSYVOICE2, CosyVoiceLm
+from syrinx_amd.sampling import RasSampler
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +142,41 @@ def test_a_stream_that_stops_on_the_last_page_leaves_it_to_the_others(cuda):
 def test_every_stream_stopped_ends_the_loop(cuda):
     slow, out, flags = _loop(cuda, 8, [16, 20], [2, 5], 60)
     assert len(out) <= 7 and not flags[-1].any()
+
+
+# ---- the CosyVoice loop -----------------------------------------------------------------
+
+class ScriptedRas(RasSampler):
+    """A sampler whose draw number `stop` (from 0) is a stop id."""
+
+    def __init__(self, stop, variant, device):
+        super().__init__([3], eos=(variant.stop_begin, variant.stop_end), device=device)
+        self.stop, self.turn, self.first = stop, 0, variant.stop_begin
+
+    def sample(self, logits, ignore_eos=False, out=None):
+        super().sample(logits, ignore_eos=True, out=out)
+        if self.turn == self.stop:
+            out.fill_(self.first)
+        self.turn += 1
+
+
+@pytest.mark.parametrize("stop,ends", [(0, True), (6, True), (7, True), (8, False), (100, False)])
+def test_a_token_that_stops_needs_no_page_for_the_step_after_it(cuda, stop, ends):
+    """Nine prompt rows in a pool of one page of 16: seven steps have room.  The draw after them may
+    be the stop, whose step (enqueued before the host looks) is not needed; another token's is."""
+    cfg = D.cosyvoice2_lm_config(n_layers=1, max_seq=160)
+    lm = D.Qwen2Lm(cfg, device=cuda, kv_pages=1, page_size=16)
+    lm.init_random(seed=10)
+    text = torch.randn((50, cfg.dim), device=cuda) * 0.5
+    speech = torch.randn((cfg.embed_rows, cfg.dim), device=cuda) * 0.5
+    lm.set_vector(-1, D.EMBED, speech)
+    cv = CosyVoiceLm(lm, text, speech, torch.randn((2, cfg.dim), device=cuda))
+    sampler = ScriptedRas(stop, COSYVOICE2, cuda)
+    run = lambda: cv.generate([1, 2, 3, 4], [5, 6, 7], 0, 40, seed=0, sampler=sampler)  # noqa: E731
+    if ends:
+        assert len(run()) == stop
+    else:
+        with pytest.raises(SxqError) as e:
+            run()
+        assert e.value.code == _lib.ERR_OOM and "KV pages" in str(e.value)
+    assert lm.lengths(1)[0] <= 16
