@@ -364,8 +364,11 @@ sxq_status sxq_lm_create(int device, const sxq_lm_config *cfg, sxq_lm **out);
  * but its RoPE row and table entries.  Steps and prefills take pages as streams grow, and are
  * refused with SXQ_ERR_OOM before any GPU work when there are not enough; sxq_lm_reset and
  * shorter sxq_lm_set_lengths give them back (longer ones take pages that hold what they
- * held).  A prefill also lays one layer's keys and values out as f32 in its workspace.  Every
- * other call is as for sxq_lm_create, except that sxq_fish_fast_expand refuses a paged engine
+ * held).  A prefill also lays one layer's keys and values of its streams -- every position
+ * they hold, old and new -- out as f32 in a workspace that the engine keeps: at most the pool's
+ * positions * n_kv_heads * head_dim * 8 bytes, allocated (with room to grow) when a prefill
+ * needs more than the last, so a prefill may find the pages and still fail with SXQ_ERR_OOM,
+ * nothing done; its cost grows with the history.  Every other call is as for sxq_lm_create, except that sxq_fish_fast_expand refuses a paged engine
  * (its cache is one frame's codes).  Keys and values are rounded once to kv_dtype; the
  * attention's sums are in another order than the contiguous engine's.  A step or prefill that
  * fails gives its pages back, so it can be made again; if the device takes not even that, the

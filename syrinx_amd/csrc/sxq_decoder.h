@@ -94,10 +94,11 @@ hipError_t launch_prefill_attn(const float* q, const float* kc, const float* vc,
 // The token and tile tables of one prefill, built on the device from the per-stream
 // token counts and cache lengths (streams 0 .. n-1, tokens stream-major): tok (2 ints per
 // token), tiles (4 ints per tile, at most T + n tiles), last[s] = row of stream s's last
-// token (-1 without tokens); lengths[s] += counts[s] when `advance` (after the layers).
+// token (-1 without tokens); lengths[s] += counts[s] when `advance` (after the layers).  A tile
+// names its stream by at[s], which the attention multiplies by its kv_stream_stride.
 struct PrefillMeta {
     int n, tile_tokens;
-    int counts[16], lens[16];
+    int counts[16], lens[16], at[16];
 };
 hipError_t launch_prefill_tables(const PrefillMeta& pm, int T, int* tok, int* tiles, int* last, hipStream_t s);
 hipError_t launch_prefill_advance(const PrefillMeta& pm, int* len, hipStream_t s);

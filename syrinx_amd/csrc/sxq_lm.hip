@@ -594,16 +594,10 @@ hipError_t pf_proj(const sxq_lm* lm, const QWeight& w, const float* x, const uin
 // Device buffers of one prefill of T tokens over n streams (offsets into lm->pf).
 struct PfLayout {
     size_t h, hn, qkv, q, cx, gu, af, act, gemm, tok, tiles, last, total;
-    size_t kv_map, kv_k, kv_v;  // paged: the slot map, one layer's keys and values as f32 [n][n_kv][span][hd]
-    int span;
+    // paged: the slot map, one layer's keys and values as f32 [n_kv][positions of all streams][hd]
+    size_t kv_map, kv_k, kv_v, kv_bytes;
+    KvSpans spans;
 };
-
-// The longest stream after a prefill.
-int pf_span(const PrefillMeta& pm) {
-    int m = 0;
-    for (int i = 0; i < pm.n; ++i) m = std::max(m, pm.lens[i] + pm.counts[i]);
-    return m;
-}
 
 PfLayout pf_layout(const sxq_lm* lm, int T, const PrefillMeta& pm) {
     const int n = pm.n;
@@ -642,8 +636,10 @@ PfLayout pf_layout(const sxq_lm* lm, int T, const PrefillMeta& pm) {
     p.tiles = take(sizeof(int) * 4 * (size_t)(T + n));
     p.last = take(sizeof(int) * (size_t)n);
     if (lm->paged) {
-        p.span = pf_span(pm);
-        const size_t kv = sizeof(float) * (size_t)n * c.n_kv_heads * p.span * c.head_dim;
+        p.spans.n = n;
+        for (int i = 0; i < n; ++i) p.spans.start[i + 1] = p.spans.start[i] + pm.lens[i] + pm.counts[i];
+        const size_t kv = sizeof(float) * (size_t)c.n_kv_heads * p.spans.start[n] * c.head_dim;
+        p.kv_bytes = 2 * kv;
         p.kv_map = take(sizeof(int) * 3 * (size_t)T);
         p.kv_k = take(kv);
         p.kv_v = take(kv);
@@ -690,7 +686,6 @@ hipError_t enqueue_prefill(sxq_lm* lm, const PrefillMeta& pm, int T, const int* 
     PF(launch_prefill_tables(pm, T, tok, tiles, last, s));
     int32_t* kv_map = (int32_t*)(base + P.kv_map);
     float *kv_k = (float*)(base + P.kv_k), *kv_v = (float*)(base + P.kv_v);
-    const int64_t kv_stride = (int64_t)c.n_kv_heads * P.span * c.head_dim;
     if (lm->paged) {
         KvGrowths g{n, {}};
         for (int i = 0; i < n; ++i) g.add[i] = pm.counts[i];
@@ -745,8 +740,8 @@ hipError_t enqueue_prefill(sxq_lm* lm, const PrefillMeta& pm, int T, const int* 
             // the prompt's attention reads each stream's positions in one run: the pages, the
             // new tokens' among them (so as later steps read them), laid out so for this layer
             PF(lm_append(lm, l, qkv, T, kv_map, kv_map + T, q, s));
-            PF(launch_kv_gather(layer_pool(lm, l), lm->kv_table, lm->max_blocks, lm->max_blocks, lm->d_len, 0, n, 0,
-                                c.n_kv_heads, 0, P.span, kv_k, kv_v, s));
+            PF(launch_kv_gather(layer_pool(lm, l), lm->kv_table, lm->max_blocks, lm->max_blocks, P.spans, 0, 0,
+                                c.n_kv_heads, 0, kv_k, kv_v, s));
         } else {
             PF(launch_prefill_rope_kv(qkv, T, lm->qkv_n, c.n_heads, c.n_kv_heads, c.head_dim,
                                       c.qk_norm ? L.q_norm : nullptr, c.qk_norm ? L.k_norm : nullptr, c.norm_eps,
@@ -755,7 +750,7 @@ hipError_t enqueue_prefill(sxq_lm* lm, const PrefillMeta& pm, int T, const int* 
         }
         PF(record(q, (size_t)T * lm->ctx));
         PF(launch_prefill_attn(q, lm->paged ? kv_k : kc, lm->paged ? kv_v : vc, tiles, n_tiles, c.n_heads, c.n_kv_heads,
-                               c.head_dim, lm->paged ? P.span : c.max_seq, lm->paged ? kv_stride : lm->kv_stream_stride,
+                               c.head_dim, lm->paged ? P.spans.start[n] : c.max_seq, lm->paged ? c.head_dim : lm->kv_stream_stride,
                                ctx_blocks && !tr ? nullptr : cx, ctx_blocks ? act : nullptr, s));
         PF(record(cx, (size_t)T * lm->ctx));
         if (!f16 && !ctx_blocks) PF(launch_quantize_act(lm->vdt, false, cx, lm->ctx, T, lm->ctx, act, s));
@@ -1429,6 +1424,7 @@ sxq_status sxq_lm_prefill(sxq_lm* lm, int n, const int32_t* counts, const int32_
                         lm->h_len[s], counts[s], c.max_seq);
         pm.counts[s] = counts[s];
         pm.lens[s] = lm->h_len[s];
+        pm.at[s] = s;
         T += counts[s];
     }
     if (T == 0) return SXQ_OK;
@@ -1450,13 +1446,31 @@ sxq_status sxq_lm_prefill(sxq_lm* lm, int n, const int32_t* counts, const int32_
         if (ok != SXQ_OK) return ok;
     }
     const PfLayout P = pf_layout(lm, (int)T, pm);
+    if (lm->paged)  // a tile's stream by its first position
+        for (int s = 0; s < n; ++s) pm.at[s] = P.spans.start[s];
     if (lm->pf_size < P.total) {
         HIP_TRY(hipDeviceSynchronize(), "lm_prefill: sync before regrowing the workspace");
         if (lm->pf) (void)hipFree(lm->pf);
         lm->pf = nullptr;
         lm->pf_size = 0;
-        HIP_TRY(hipMalloc(&lm->pf, P.total), "lm_prefill: workspace");
-        lm->pf_size = P.total;
+        // room for half as many positions again (no more than the pool has), or a conversation
+        // that grows by chunks would allocate at each of them
+        size_t want = P.total;
+        if (lm->paged) {
+            const size_t all = 2 * sizeof(float) * (size_t)lm->pool.n_pages * lm->pool.page * c.n_kv_heads * c.head_dim;
+            want += std::min(P.kv_bytes / 2, all > P.kv_bytes ? all - P.kv_bytes : 0);
+        }
+        hipError_t e = hipMalloc(&lm->pf, want);
+        if (e != hipSuccess && want > P.total) {
+            (void)hipGetLastError();
+            want = P.total;
+            e = hipMalloc(&lm->pf, want);
+        }
+        if (e != hipSuccess) {
+            lm->pf = nullptr;
+            return hip_fail(e, "lm_prefill: workspace");
+        }
+        lm->pf_size = want;
     }
     const bool all = (flags & SXQ_LM_ALL_LOGITS) != 0;
     if (all && !logits) return fail(SXQ_ERR_INVALID, "lm_prefill: SXQ_LM_ALL_LOGITS needs a logits buffer");
@@ -1517,8 +1531,8 @@ sxq_status sxq_lm_read_kv(const sxq_lm* lm, int layer, int s, int g, int pos0, i
     HIP_TRY(gd.err, "hipSetDevice");
     if (lm->paged) {
         if (count == 0) return SXQ_OK;
-        HIP_TRY(launch_kv_gather(layer_pool(lm, layer), lm->kv_table, lm->max_blocks, lm->max_blocks, nullptr, s, 1, g, 1, pos0,
-                                 count, k_out, v_out, (hipStream_t)stream), "lm_read_kv");
+        HIP_TRY(launch_kv_gather(layer_pool(lm, layer), lm->kv_table, lm->max_blocks, lm->max_blocks, KvSpans{1, {0, count}}, s,
+                                 g, 1, pos0, k_out, v_out, (hipStream_t)stream), "lm_read_kv");
         return SXQ_OK;
     }
     const int64_t off = (int64_t)layer * lm->kv_layer_stride + (int64_t)s * lm->kv_stream_stride +

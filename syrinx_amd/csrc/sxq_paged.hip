@@ -431,16 +431,19 @@ void append_by_cache(const KvAppend& a, const KvPool& p, hipStream_t s) {
 // Eight elements of K and of V a thread.
 template <typename TC>
 __global__ __launch_bounds__(256) void k_kv_gather(const KvPool P, const int32_t* __restrict__ table, int64_t table_stride,
-                                                   int max_blocks, const int32_t* __restrict__ lens, int r0, int h0,
-                                                   int heads, int p0, int span, float* __restrict__ k,
-                                                   float* __restrict__ v) {
+                                                   int max_blocks, const KvSpans S, int r0, int h0, int p0,
+                                                   float* __restrict__ k, float* __restrict__ v) {
     const int per = P.hd / 8, i = blockIdx.x * 256 + threadIdx.x, q = i / per, d = 8 * (i - q * per);
-    const int row = blockIdx.y / heads, h = blockIdx.y - row * heads, p = p0 + q;
-    if (q >= span || (lens && p >= kv_clamp_len(lens[r0 + row], max_blocks, P.shift))) return;
-    const int b = p >> P.shift;
+    const int total = S.start[S.n];
+    if (q >= total) return;
+    int row = 0, first = 0;
+#pragma unroll
+    for (int z = 1; z < 16; ++z)
+        if (z < S.n && q >= S.start[z]) row = z, first = S.start[z];
+    const int h = blockIdx.y, p = p0 + q - first, b = p >> P.shift;
     const int slot = b < max_blocks ? kv_slot(table[(r0 + row) * table_stride + b], p, P.shift, P.n_pages) : -1;
     const int64_t from = slot < 0 ? 0 : kv_slot_base(P, slot, h0 + h) + d;
-    const int64_t to = ((int64_t)blockIdx.y * span + q) * P.hd + d;
+    const int64_t to = ((int64_t)h * total + q) * P.hd + d;
 #pragma unroll
     for (int o = 0; o < 8; o += 4) {
         float f[4] = {0.f, 0.f, 0.f, 0.f};
@@ -512,11 +515,10 @@ hipError_t launch_kv_append(const KvAppend& a, const KvPool& p, hipStream_t s) {
     return hipGetLastError();
 }
 
-hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table_stride, int max_blocks,
-                            const int32_t* lens, int r0, int rows, int h0, int heads, int p0, int span, float* k, float* v,
-                            hipStream_t s) {
-    const dim3 grid((unsigned)(((int64_t)span * (p.hd / 8) + 255) / 256), rows * heads);
-#define SXQ_GA(T) hipLaunchKernelGGL(k_kv_gather<T>, grid, dim3(256), 0, s, p, table, table_stride, max_blocks, lens, r0, h0, heads, p0, span, k, v)
+hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table_stride, int max_blocks, const KvSpans& spans,
+                            int r0, int h0, int heads, int p0, float* k, float* v, hipStream_t s) {
+    const dim3 grid((unsigned)(((int64_t)spans.start[spans.n] * (p.hd / 8) + 255) / 256), heads);
+#define SXQ_GA(T) hipLaunchKernelGGL(k_kv_gather<T>, grid, dim3(256), 0, s, p, table, table_stride, max_blocks, spans, r0, h0, p0, k, v)
     if (p.dtype == kF32) SXQ_GA(float);
     else if (p.dtype == kF16) SXQ_GA(_Float16);
     else SXQ_GA(__bf16);

@@ -46,12 +46,14 @@ struct KvAttend {
 size_t kv_attend_workspace(const KvPool& p, int n_q, int nh);
 hipError_t launch_kv_attend(const KvAttend& a, const KvPool& p, hipStream_t s);
 
-// One layer's positions p0 .. p0 + span - 1 of rows r0 .. r0 + rows - 1 and KV heads h0 .. as
-// f32 [row][head][span][hd] (either output may be null): with lens those below the row's length,
-// without it all.  An absent page reads as zeros.
-hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table_stride, int max_blocks,
-                            const int32_t* lens, int r0, int rows, int h0, int heads, int p0, int span, float* k, float* v,
-                            hipStream_t s);
+// Up to 16 rows' positions one after another: row i's are start[i] .. start[i + 1] - 1 of start[n].
+struct KvSpans {
+    int n, start[17];
+};
+// One layer's KV heads h0 .. h0 + heads - 1 of rows r0 .. r0 + n - 1, each row's positions from p0
+// on, as f32 [head][start[n]][hd] (either output may be null).  An absent page reads as zeros.
+hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table_stride, int max_blocks, const KvSpans& spans,
+                            int r0, int h0, int heads, int p0, float* k, float* v, hipStream_t s);
 // A free stack of pages 0 .. n - 1, page 0 on top.
 hipError_t launch_kv_stack(int32_t* free_list, int n, hipStream_t s);
 // The growths of an engine's streams, written to its device array.

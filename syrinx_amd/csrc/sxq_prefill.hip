@@ -85,7 +85,7 @@ SXQ_DEV void pf_zero_rows(float* dst, int wave, int lane, int from) {
 }
 
 // One workgroup (256 threads) per (tile, KV group, share of the tile's rows): a tile is up to
-// kPfRows / G consecutive prompt tokens of one stream (tile = {stream, first token row t0,
+// kPfRows / G consecutive prompt tokens of one stream (tile = {stream's at, first token row t0,
 // count, position p0 of token t0}); its rows are r = i * G + hh (token i, query head
 // g * G + hh).  Keys go through LDS 16 NP at a time, every row keeps an online softmax (running
 // max m, sum l, rescaled accumulator) over blocks of 32 and masks the keys past its own position.
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(256) void k_prefill_tables(PrefillMeta pm, int T, i
                 const int d = kend - (z < s ? 1 : 0) - pm.lens[z];  // its tiles that end at or before
                 rank += nz - (d >= cz ? nz : max(d, 0) / pm.tile_tokens);
             }
-            tiles[rank] = make_int4(s, base + i0, cnt, pm.lens[s] + i0);
+            tiles[rank] = make_int4(pm.at[s], base + i0, cnt, pm.lens[s] + i0);
         }
         if (t == 0) last[s] = c > 0 ? base + c - 1 : -1;
         base += c;

@@ -397,6 +397,57 @@ void streams_that_sit_out() {
     EXPECT(sxq_lm_destroy(lm) == SXQ_OK);
 }
 
+// A prompt's workspace holds f32 keys and values of the positions there are, not of streams times
+// the longest; and a conversation that grows chunk by chunk allocates it a few times, not at
+// every chunk.  Where the headroom does not fit, the bare size does.
+void prompt_workspace() {
+    const size_t row = 2 * 2 * 64 * sizeof(float);  // K and V of a position, two heads of 64
+    const size_t token = 64 << 10;                  // more than the other buffers take for a token
+    {
+        Engine e(16000 / 16 + 40, 20000, 16);
+        std::vector<int32_t> counts(16, 10);
+        counts[3] = 16000;
+        std::vector<size_t>& m = sim::state().mallocs;
+        const size_t before = m.size();
+        EXPECT(e.prefill(counts) == SXQ_OK);
+        std::vector<int32_t> few(16, 1);
+        EXPECT(e.prefill(few) == SXQ_OK);
+        EXPECT(m.size() == before + 1 && m.back() < 1.5 * (16150 + 16) * row + 16150 * token);
+    }
+    {
+        Engine e(1250, 20000, 16);
+        std::vector<size_t>& m = sim::state().mallocs;
+        std::vector<int32_t> small(16, 1), lens(16, 10);
+        lens[3] = 16000;
+        EXPECT(sxq_lm_set_lengths(e.lm, lens.data(), 16) == SXQ_OK);
+        const size_t before = m.size();
+        EXPECT(e.prefill(small) == SXQ_OK && m.size() == before + 1);
+        EXPECT(m.back() < 1.5 * 16200 * row + 16 * token);  // (streams times the longest: 16 * 16001 * row)
+    }
+    {
+        Engine e(1250, 20000, 2);
+        std::vector<size_t>& m = sim::state().mallocs;
+        const size_t before = m.size();
+        int calls = 0;
+        for (; e.lengths()[0] < 19000; ++calls) EXPECT(e.prefill({64, 2}) == SXQ_OK);
+        EXPECT(calls > 290 && m.size() - before <= 16);
+        const size_t last = m.back();
+        const int32_t lens[2] = {0, 10};
+        EXPECT(last <= 1250 * 16 * row + 66 * token);  // never for more positions than the pool has
+        EXPECT(sxq_lm_set_lengths(e.lm, lens, 2) == SXQ_OK && e.prefill({64, 2}) == SXQ_OK && m.back() == last);
+    }
+    {
+        Engine e(1250, 20000, 2);
+        const int32_t lens[2] = {9000, 9000};
+        EXPECT(sxq_lm_set_lengths(e.lm, lens, 2) == SXQ_OK);
+        sim::state().malloc_limit = 18200 * row + 10 * token;  // no room for more
+        EXPECT(e.prefill({4, 4}) == SXQ_OK);
+        EXPECT(e.step(2) == SXQ_OK);
+        e.consistent();
+        sim::state().malloc_limit = (size_t)-1;
+    }
+}
+
 const std::map<std::string, void (*)()> kTests = {
     {"checks_allocate_nothing", checks_allocate_nothing},
     {"creation_out_of_host_memory", creation_out_of_host_memory},
@@ -404,6 +455,7 @@ const std::map<std::string, void (*)()> kTests = {
     {"failed_calls", failed_calls},
     {"failed_undo", failed_undo},
     {"lengths_are_read_under_the_lock", lengths_are_read_under_the_lock},
+    {"prompt_workspace", prompt_workspace},
     {"streams_that_sit_out", streams_that_sit_out},
 };
 

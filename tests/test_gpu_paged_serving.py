@@ -180,3 +180,39 @@ def test_a_token_that_stops_needs_no_page_for_the_step_after_it(cuda, stop, ends
             run()
         assert e.value.code == _lib.ERR_OOM and "KV pages" in str(e.value)
     assert lm.lengths(1)[0] <= 16
+
+
+# ---- prompts over long histories ----------------------------------------------------------
+
+@pytest.mark.parametrize("kv_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lens,counts,page", [([17000, 5, 300], [40, 33, 1], 32), ([0, 20000], [3, 70], 64),
+                                              ([100, 0, 17], [1, 50, 130], 16)])
+def test_a_prompt_attends_over_its_own_history(cuda, kv_dtype, lens, counts, page):
+    """Streams of unlike lengths (past the contiguous engine's limit too): the traced context of a
+    prompt's rows against 64-bit attention over what the pages hold of the row's own stream."""
+    n, cfg = len(lens), dataclasses.replace(T._fish_small(n_layers=2, max_batch=len(lens)), max_seq=24000)
+    pages = sum(-(-(a + b) // page) for a, b in zip(lens, counts))
+    lm = D.DecoderLM(cfg, device=cuda, kv_pages=pages, page_size=page, kv_dtype=kv_dtype)
+    lm.init_random(seed=11)
+    lm.kv_fill_random(lens, seed=12)
+    rng = np.random.default_rng(13)
+    *_, tr = lm.prefill(prompts=[torch.from_numpy(T._frames(rng, c, cfg)) for c in counts], exact=True, trace=True)
+    assert lm.free_pages() == 0
+    nh, nkv, hd = cfg.n_heads, cfg.n_kv_heads, cfg.head_dim
+    G, first, u = nh // nkv, 0, 2.0 ** -24
+    for s in range(n):
+        for i in sorted({0, counts[s] // 2, counts[s] - 1}):
+            L = lens[s] + i + 1
+            for l in range(2):
+                q = torch.from_numpy(tr["layers"][l]["q"][first + i].copy()).to(cuda).view(nh, hd).double()
+                got = torch.from_numpy(tr["layers"][l]["ctx"][first + i].copy()).to(cuda).view(nh, hd).double()
+                for g in range(nkv):
+                    k, v = (x.double() for x in lm.read_kv(l, s, g, 0, L))
+                    qq = q[g * G:(g + 1) * G]
+                    w = torch.softmax(qq @ k.t().contiguous() * hd ** -0.5, -1)
+                    S = (qq.abs() @ k.abs().t().contiguous()).amax(-1, keepdim=True) * hd ** -0.5
+                    # hd products and sums a score, exp of it and its rescalings, L weighted terms
+                    rel = 2 * (hd + 3) * u * S + 2 * S * u + (8 + 4 * (L / 16 + 2) + 2 * L) * u
+                    err = (got[g * G:(g + 1) * G] - w @ v).abs()
+                    assert bool((err <= 2 * rel * (w @ v.abs())).all()), (s, i, l, g)
+        first += counts[s]

@@ -10,7 +10,7 @@ import pytest
 HERE = os.path.join(os.path.dirname(os.path.abspath(__file__)), "hostsim")
 
 TESTS = ["checks_allocate_nothing", "creation_out_of_host_memory", "error_of_one_call", "failed_calls", "failed_undo", "lengths_are_read_under_the_lock",
-         "streams_that_sit_out"]
+         "prompt_workspace", "streams_that_sit_out"]
 
 
 @pytest.fixture(scope="module")
