@@ -520,8 +520,7 @@ hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table
     const dim3 grid((unsigned)(((int64_t)spans.start[spans.n] * (p.hd / 8) + 255) / 256), heads);
 #define SXQ_GA(T) hipLaunchKernelGGL(k_kv_gather<T>, grid, dim3(256), 0, s, p, table, table_stride, max_blocks, spans, r0, h0, p0, k, v)
     if (p.dtype == kF32) SXQ_GA(float);
-    else if (p.dtype == kF16) SXQ_GA(_Float16);
-    else SXQ_GA(__bf16);
+    else SXQ_GA(__bf16);  // (an engine's pages are f32 or bf16)
 #undef SXQ_GA
     return hipGetLastError();
 }
