@@ -368,11 +368,12 @@ sxq_status sxq_lm_create(int device, const sxq_lm_config *cfg, sxq_lm **out);
  * they hold, old and new -- out as f32 in a workspace that the engine keeps: at most the pool's
  * positions * n_kv_heads * head_dim * 8 bytes, allocated (with room to grow) when a prefill
  * needs more than the last, so a prefill may find the pages and still fail with SXQ_ERR_OOM,
- * nothing done; its cost grows with the history.  Every other call is as for sxq_lm_create, except that sxq_fish_fast_expand refuses a paged engine
- * (its cache is one frame's codes).  Keys and values are rounded once to kv_dtype; the
- * attention's sums are in another order than the contiguous engine's.  A step or prefill that
- * fails gives its pages back, so it can be made again; if the device takes not even that, the
- * following calls are refused until sxq_lm_reset has emptied all max_batch streams. */
+ * nothing done; its cost grows with the history.  Every other call is as for sxq_lm_create,
+ * except that sxq_fish_fast_expand refuses a paged engine (its cache is one frame's codes).
+ * Keys and values are rounded once to kv_dtype; the attention's sums are in another order than
+ * the contiguous engine's.  A step or prefill that fails gives its pages back, so it can be
+ * made again; if the device takes not even that, the following calls are refused until
+ * sxq_lm_reset has emptied all max_batch streams. */
 sxq_status sxq_lm_create_paged(int device, const sxq_lm_config *cfg, int kv_dtype, int page_size, int n_pages,
                                sxq_lm **out);
 /* Pages that no stream of a paged engine holds. */

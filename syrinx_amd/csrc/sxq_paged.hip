@@ -508,11 +508,22 @@ hipError_t launch_kv_reserve(const KvReserve& a, hipStream_t s, bool* moved) {
     return e;
 }
 
-hipError_t launch_kv_append(const KvAppend& a, const KvPool& p, hipStream_t s) {
-    if (a.dtype == kF32) append_by_cache<float>(a, p, s);
-    else if (a.dtype == kF16) append_by_cache<_Float16>(a, p, s);
-    else append_by_cache<__bf16>(a, p, s);
-    return hipGetLastError();
+hipError_t launch_kv_append(const KvAppend& all, const KvPool& p, hipStream_t s) {
+    constexpr int kMost = 1 << 23;  // tokens a launch: its grid may not pass 2^32 threads
+    const size_t e = type_size(all.dtype);
+    for (int64_t t0 = 0; t0 < all.n_tokens; t0 += kMost) {
+        KvAppend a = all;
+        a.n_tokens = (int)std::min<int64_t>(kMost, all.n_tokens - t0);
+        a.qkv = (const char*)all.qkv + t0 * all.row_stride * e;
+        if (all.pos) a.pos = all.pos + t0;
+        a.slots = all.slots + t0;
+        if (all.q_out) a.q_out = (char*)all.q_out + t0 * all.nh * p.hd * e;
+        if (a.dtype == kF32) append_by_cache<float>(a, p, s);
+        else if (a.dtype == kF16) append_by_cache<_Float16>(a, p, s);
+        else append_by_cache<__bf16>(a, p, s);
+        if (const hipError_t err = hipGetLastError(); err != hipSuccess) return err;
+    }
+    return hipSuccess;
 }
 
 hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table_stride, int max_blocks, const KvSpans& spans,

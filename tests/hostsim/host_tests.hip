@@ -94,6 +94,7 @@ void reserve_rows(const KvReserve& a) {
 }
 
 std::vector<int> stored;  // the slots of the last append, by row
+std::vector<KvAppend> appends;
 
 // Bodies of the kernels that keep an engine's lengths and pages.
 void page_kernels() {
@@ -115,7 +116,10 @@ void page_kernels() {
     });
     sim::kernel("k_kv_append", [](void** args) {
         const KvAppend a = *(const KvAppend*)args[0];
-        return [a] { stored.assign(a.slots, a.slots + a.n_tokens); };
+        return [a] {
+            appends.push_back(a);
+            stored.assign(a.slots, a.slots + a.n_tokens);
+        };
     });
     sim::kernel("k_kv_stack", [](void** args) {
         int32_t* list = *(int32_t**)args[0];
@@ -448,7 +452,37 @@ void prompt_workspace() {
     }
 }
 
+// Tokens beyond what one launch's grid may hold (2^32 threads): in parts, each at its own rows.
+void append_of_many_tokens() {
+    const int n = (1 << 24) + 5, width = 3 * 8;
+    sxq_kv_pages p{};
+    p.dtype = SXQ_F16;
+    p.n_kv_heads = 1;
+    p.head_dim = 8;
+    p.page_size = 16;
+    p.n_pages = 4;
+    p.k = p.v = (void*)4096;
+    p.pos_stride = 8;
+    p.head_stride = 128;
+    p.page_stride = 128;
+    std::vector<int32_t> slots(n, -1), pos(n, 0);
+    uint16_t* const qkv = (uint16_t*)(uintptr_t)(1 << 20);
+    uint16_t* const out = (uint16_t*)((uintptr_t)1 << 40);
+    float tables[8] = {};
+    EXPECT(sxq_kv_append(0, &p, SXQ_F16, qkv, width + 8, n, 1, nullptr, nullptr, 1e-6f, tables, tables, 2, 0, pos.data(),
+                         slots.data(), out, nullptr) == SXQ_OK);
+    int64_t at = 0;
+    size_t i = sim::state().launches.size() - appends.size();
+    for (const KvAppend& a : appends) {
+        EXPECT(a.slots == slots.data() + at && a.pos == pos.data() + at && a.qkv == qkv + at * (width + 8) && a.q_out == out + at * 8);
+        EXPECT(a.n_tokens > 0 && sim::state().launches[i++].grid[0] == (unsigned)a.n_tokens);
+        at += a.n_tokens;
+    }
+    EXPECT(at == n && appends.size() > 1);
+}
+
 const std::map<std::string, void (*)()> kTests = {
+    {"append_of_many_tokens", append_of_many_tokens},
     {"checks_allocate_nothing", checks_allocate_nothing},
     {"creation_out_of_host_memory", creation_out_of_host_memory},
     {"error_of_one_call", error_of_one_call},

@@ -9,8 +9,9 @@ import pytest
 
 HERE = os.path.join(os.path.dirname(os.path.abspath(__file__)), "hostsim")
 
-TESTS = ["checks_allocate_nothing", "creation_out_of_host_memory", "error_of_one_call", "failed_calls", "failed_undo", "lengths_are_read_under_the_lock",
-         "prompt_workspace", "streams_that_sit_out"]
+TESTS = ["append_of_many_tokens", "checks_allocate_nothing", "creation_out_of_host_memory", "error_of_one_call", "failed_calls",
+         "failed_undo", "lengths_are_read_under_the_lock", "prompt_workspace",
+         "streams_that_sit_out"]
 
 
 @pytest.fixture(scope="module")
