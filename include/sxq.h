@@ -260,13 +260,18 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
  * over KV head h / (n_heads / n_kv_heads) (n_heads a multiple of n_kv_heads).  q and out:
  * rows of n_heads * head_dim, q_stride / out_stride elements apart (multiples of 16 bytes,
  * 16-byte aligned), q_dtype the pages' type, or SXQ_F32 over SXQ_BF16 pages; out has q's type.
- * Scores, softmax and sums are f32.  rows int32 [n_q]: the table row of each query (NULL: b);
+ * Scores, softmax statistics and sums are f32; over 16-bit pages a weight is carried in parts
+ * of the pages' type, off by at most 2^-18 of itself (16-bit queries over bf16) or 2^-22 (f16;
+ * f32 queries), below the output's own rounding.  rows int32 [n_q]: the table row of each query (NULL: b);
  * a query whose row lies outside 0 .. n_rows - 1 leaves its out row as it was.  A request
  * without positions (or whose pages are all absent) gives zeros.  max_blocks * page_size at
  * most 2^30, n_q times that at most 2^35, n_q at most 2^20.  What lies past a request's
- * length, in its last page or elsewhere, may hold anything; a key or value of its own that is
- * not finite makes the outputs that read it not finite.  Two calls on the same inputs give
- * the same bits.
+ * length, in its last page or elsewhere, may hold anything.  Its own keys and values act as in
+ * the formula: a score of -inf has no weight (a head all whose scores are -inf gives zeros, as
+ * a request without positions does), one of +inf or NaN makes the head's output NaN, and a value
+ * that is not finite makes its column of the output not finite.  Over bf16 pages an f32 query
+ * element beyond bf16's range counts as infinite.  Two calls on the same inputs give the same
+ * bits.
  * workspace: sxq_kv_attention_workspace bytes, 256-byte aligned, of which the caller zeroes
  * the first SXQ_KV_COUNTER_BYTES before its first use; every call leaves them zero, and the
  * workspace good for any call that needs no more bytes.  Calls that share one must not

@@ -552,6 +552,31 @@ __global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv_
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[h][i] = c[i] * scale2;
         }
+        if constexpr (QP > 1) {
+            // A query's lower part that is zero, or of the other sign, makes NaN of an infinite
+            // key where the whole query gives an infinite score: the first part's product has it
+            // (and is NaN where the score is).
+            float sum = 0.0f;
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum += x[h][i];
+            if (__any(sum != sum)) {
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    v4f c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const v4u kk = {kreg[h][s][0], kreg[h][s][1], kreg[h][s][2], kreg[h][s][3]};
+                        const v4u qq = {qreg[0][s][0], qreg[0][s][1], qreg[0][s][2], qreg[0][s][3]};
+                        c = O::mfma(__builtin_bit_cast(typename O::V8, kk), __builtin_bit_cast(typename O::V8, qq), c);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (x[h][i] != x[h][i]) x[h][i] = c[i] * scale2;
+                }
+            }
+        }
         const bool cut = (t + H) * 16 > it.len;  // some position lies past the end
         bool absent = false;
 #pragma unroll
