@@ -1,9 +1,11 @@
 """What the paged attention does with keys, values and queries that are not finite, for every
-pair of types."""
+pair of types, and a decode loop held to derived bounds at each of its steps."""
 import pytest
 import torch
 
-from test_gpu_paged import DT, F64, TYPES, U32, _close, _filled
+from syrinx_amd.paged import RELEASE, PagedKvCache
+from test_gpu_paged import (DT, F64, TYPES, U32, _append_reference, _attend_reference, _close, _filled, _half_step,
+                            _tables)
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +78,67 @@ def test_infinite_queries_and_values(cuda, qt, ct):
     q = torch.zeros((3, 2, 64), device=cuda, dtype=DT[qt])
     q[:, :, :] = float("-inf")
     assert not bool(cache.attend(0, q)[:2].any())
+
+
+class Stored:
+    """Requests' rows in 64 bits as the definition gives them, before the pages' rounding, with the
+    bound of the f32 arithmetic that made them."""
+
+    def __init__(self, rows):
+        self.k, self.v, self.kb = ([[] for _ in range(rows)] for _ in range(3))
+
+
+@pytest.mark.parametrize("it,ct", TYPES)
+def test_decode_loop_step_by_step(cuda, it, ct):
+    """Prompts admitted, decode steps with requests joining, pausing, rewinding and leaving.  Each
+    step is held to two derived bounds: every row that the pages hold, read through the table,
+    against the row's own values (one rounding of the pages' type); and the context against
+    64-bit attention over what is stored."""
+    rows, nh, nkv, hd, page = 6, 8, 2, 64, 16
+    cache = PagedKvCache(1, nkv, hd, n_pages=40, page_size=page, max_rows=rows, max_len=120, dtype=DT[ct], device=cuda)
+    want = Stored(rows)
+    tables = _tables(cache.max_len, hd, cuda, 1e4)
+    g = torch.Generator(device=cuda).manual_seed(23)
+    w = 1 + 0.1 * torch.randn(hd, generator=g, device=cuda)
+    rel = (hd / 2 + 9) * U32  # as for the append alone
+    tiny = torch.finfo(DT[ct]).smallest_normal * torch.finfo(DT[ct]).eps
+    steps = [[30, 0, 17, 1, 0, 0], [1, 0, 1, 1, 0, 0], [1, 45, 0, 1, 0, 0], [1, 1, 1, 1, 100, 0], [RELEASE, 1, 1, 1, 1, 0],
+             [16, 1, RELEASE, 1, 1, 64], [1, 1, 31, 1, 1, 1], [1, -20, 1, 1, 1, 1], [1, 1, 1, 1, 1, 1], [1, 12, 0, -3, 1, 1]]
+    for step, add in enumerate(steps):
+        m = cache.reserve(add)
+        assert not bool(m.status.any())
+        for r, a in enumerate(add):
+            if a < 0:
+                keep = max(0, len(want.k[r]) + a)
+                for rows_of in (want.k, want.v, want.kb):
+                    del rows_of[r][keep:]
+        n = m.slots.numel()
+        qkv = torch.randn((n, (nh + 2 * nkv) * hd), generator=g, device=cuda).to(DT[it])
+        q = cache.append(0, qkv, m, n_heads=nh, q_norm=w, k_norm=w, rope=tables)
+        ref, mag = _append_reference(qkv, nh, nkv, hd, w, w, 1e-6, tables, m.pos.long(), False)
+        for t, r in enumerate(m.rows.tolist()):
+            want.k[r].append(ref[t, nh:nh + nkv])
+            want.kb[r].append(rel * mag[t, nh:nh + nkv])
+            want.v[r].append(ref[t, nh + nkv:])
+        assert cache.lens.tolist() == [len(k) for k in want.k]
+        held = set()
+        for r in range(rows):
+            L = len(want.k[r])
+            if L == 0:
+                continue
+            p = torch.arange(L, device=cuda)
+            ids = cache.table[r].long()[p // page]
+            mine = set(ids.tolist())
+            assert not held & mine and min(mine) >= 0  # no page belongs to two
+            held |= mine
+            half = _half_step(DT[ct])
+            k, v = (pool[0, ids, :, p % page].to(F64) for pool in (cache.k, cache.v))
+            k64, kb = torch.stack(want.k[r]), torch.stack(want.kb[r])
+            assert bool(((k - k64).abs() <= kb + half * (k64.abs() + kb) + tiny).all()), (step, r, "keys")
+            v64 = torch.stack(want.v[r])
+            assert bool(((v - v64).abs() <= half * v64.abs() + tiny).all()), (step, r, "values")
+        last = [int(c) - 1 for c, a in zip(m.cu.tolist()[1:], add) if a > 0]
+        qs, of = q.view(n, nh, hd)[last].contiguous(), m.rows[last].contiguous()
+        ctx = cache.attend(0, qs, rows=of)
+        exact, bound = _attend_reference(qs, cache.k[0], cache.v[0], cache.table, cache.lens, of.tolist(), hd ** -0.5)
+        _close(ctx, exact, bound, DT[it], f"step {step}")
