@@ -132,14 +132,14 @@ def out_of_pages(e: SxqError) -> bool:
 class DecoderLM:
     """A decode-step engine (sxq_lm) on one GPU.
 
-    With kv_pages, its cache is paged (sxq_lm_create_paged): that many pages of page_size (32)
-    positions a layer, of kv_dtype (torch.float32, the default, or torch.bfloat16), shared by all
-    streams, instead of max_seq f32 positions reserved for each."""
+    With kv_pages, its cache is paged (sxq_lm_create_paged): that many pages of page_size
+    positions a layer, of kv_dtype (torch.float32 or torch.bfloat16), shared by all streams,
+    instead of max_seq f32 positions reserved for each."""
 
-    def __init__(self, cfg: DecoderConfig, device="cuda:0", kv_pages: int = None, page_size: int = None,
-                 kv_dtype: torch.dtype = None):
-        if kv_pages is None and (page_size is not None or kv_dtype is not None):
-            raise ValueError("page_size and kv_dtype are a paged cache's: give kv_pages too")
+    def __init__(self, cfg: DecoderConfig, device="cuda:0", kv_pages: int = None, page_size: int = 32,
+                 kv_dtype: torch.dtype = torch.float32):
+        if kv_pages is None and kv_dtype != torch.float32:
+            raise ValueError(f"kv_dtype {kv_dtype} is a paged cache's: give kv_pages too (the contiguous cache is f32)")
         self.cfg = cfg
         self.device = torch.device(device)
         self._h = ctypes.c_void_p()
@@ -148,9 +148,8 @@ class DecoderLM:
         if kv_pages is None:
             check(lib().sxq_lm_create(self._dev(), ctypes.byref(self._c), ctypes.byref(self._h)))
         else:
-            code = {None: 0, torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(kv_dtype, -1)
-            check(lib().sxq_lm_create_paged(self._dev(), ctypes.byref(self._c), code,
-                                            32 if page_size is None else int(page_size), int(kv_pages),
+            code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(kv_dtype, -1)
+            check(lib().sxq_lm_create_paged(self._dev(), ctypes.byref(self._c), code, int(page_size), int(kv_pages),
                                             ctypes.byref(self._h)))
         self.ids_per = 1 + cfg.n_codebooks
 

@@ -9,9 +9,8 @@ CFG = D.cosyvoice2_lm_config(n_layers=1, max_seq=64)
 
 
 @pytest.mark.parametrize("cls", [D.DecoderLM, D.SlowAr, D.Qwen2Lm])
-@pytest.mark.parametrize("kw", [dict(kv_dtype=torch.bfloat16), dict(kv_dtype=torch.float32), dict(page_size=16),
-                                dict(page_size=32, kv_dtype=torch.bfloat16)])
-def test_a_cache_that_is_not_paged_takes_no_page_arguments(cls, kw):
+@pytest.mark.parametrize("kw", [dict(kv_dtype=torch.bfloat16), dict(kv_dtype=torch.float16), dict(page_size=64, kv_dtype=torch.bfloat16)])
+def test_a_cache_that_is_not_paged_holds_f32(cls, kw):
     with pytest.raises(ValueError, match="kv_pages"):
         cls(CFG, **kw)
 
