@@ -229,11 +229,11 @@ typedef struct {
  *     requests' included) exceed the free ones, 3 if the tokens asked for up to and with it
  *     exceed `capacity`; otherwise status 0.
  * A call that refuses nothing is undone exactly -- table, stack and lengths -- by the call
- * with add negated (and a capacity for what grows back), if no request shrank below 0.  cu int32 [n_rows + 1]: the first token of each accepted request, then their
- * number T; token t < T of the map: slots[t], pos[t] (its position) and rows[t] (its
- * request), requests ascending; entries T .. capacity - 1 are -1.  capacity may be 0 (the
- * three maps are then not touched).  n_rows * max_blocks and max_blocks * page_size < 2^31,
- * capacity at most 2^30. */
+ * with add negated (and a capacity for what grows back), if no request shrank below 0.
+ * cu int32 [n_rows + 1]: the first token of each accepted request, then their number T; token
+ * t < T of the map: slots[t], pos[t] (its position) and rows[t] (its request), requests
+ * ascending; entries T .. capacity - 1 are -1.  capacity may be 0 (the three maps are then not
+ * touched).  n_rows * max_blocks and max_blocks * page_size < 2^31, capacity at most 2^30. */
 sxq_status sxq_kv_reserve(int device, int page_size, int n_pages, int n_rows, int max_blocks, const int32_t *add,
                           int32_t *lens, int32_t *table, int64_t table_stride, int32_t *free_list,
                           int32_t *free_count, int capacity, int32_t *cu, int32_t *slots, int32_t *pos,
@@ -257,7 +257,9 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
 /* Attention of one new token per query row over its request's pages (decode: nn.rs:340-352,
  * attention.rs:67-76):
  *   out[b][h] = sum_j p_j v_j,  p = softmax_j(scale * q[b][h] . k_j),  j < lens[rows[b]],
- * over KV head h / (n_heads / n_kv_heads) (n_heads a multiple of n_kv_heads).  q and out:
+ * over KV head h / (n_heads / n_kv_heads) (n_heads a multiple of n_kv_heads).  Every query sees
+ * its whole request, also positions that were reserved together with its own: of several new
+ * tokens of a request this is a decoder's attention of the last one only.  q and out:
  * rows of n_heads * head_dim, q_stride / out_stride elements apart (multiples of 16 bytes,
  * 16-byte aligned), q_dtype the pages' type, or SXQ_F32 over SXQ_BF16 pages; out has q's type.
  * Scores, softmax statistics and sums are f32; over 16-bit pages a weight is carried in parts

@@ -4,11 +4,17 @@ stream, so that a server holds as many requests as their lengths allow.
 ``PagedKvCache`` owns the pools of every layer, the block tables, the lengths and the stack of
 free pages.  One decode step of a batch is
 
-    m = cache.reserve(add, capacity)                  # pages, slots, positions: on the GPU
+    m = cache.reserve(add, capacity)                  # add: 0 or 1 a request; pages, slots, positions
     q = cache.append(layer, qkv, m, n_heads=..., rope=..., ...)   # per layer
     ctx = cache.attend(layer, q, rows=m.rows)
 
-with no copy to the host; every call enqueues on the current stream of the cache's device and
+A query of ``attend`` sees every position of its request, those reserved together with it too:
+right for the one new token of a decode step, and for the last of a prompt's tokens, not for the
+tokens before it.  A map of several tokens a request (a prompt's) is for ``append``; a prompt's
+tokens, each over its own prefix, are attended to by a paged engine (``DecoderLM.prefill``), and
+of such a map ``attend`` takes the last token of each request, at m.cu[r + 1] - 1.
+
+Nothing is copied to the host; every call enqueues on the current stream of the cache's device and
 may be captured into a graph.  The reference keeps one growing tensor per stream
 (KvCache, crates/syrinx-fish/src/s2/nn.rs:221-254); append is its QK-norm + RoPE + cache append
 (nn.rs:325-339, crates/syrinx-lm/src/cv2/attention.rs:50-66) and attend its attention of one new
@@ -43,7 +49,7 @@ class KvPages(ctypes.Structure):
 class SlotMap:
     """Where new tokens go: token t is at slot slots[t] and position pos[t] of request rows[t]
     (int32, -1 past the last token).  cu[r] is request r's first token, status[r] why it was
-    refused (0: it was not; 1 out of pages, 2 longer than max_len, 3 over the map's capacity)."""
+    refused (0: it was not; 1 out of pages, 2 longer than max_len's pages, 3 over the map's capacity)."""
     slots: torch.Tensor
     pos: torch.Tensor
     rows: torch.Tensor
@@ -60,8 +66,8 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 class PagedKvCache:
-    """Keys and values of up to max_rows requests of up to max_len positions in n_pages pages
-    of page_size positions (a power of two, 16..1024).
+    """Keys and values of up to max_rows requests of up to max_len positions (rounded up to whole
+    pages) in n_pages pages of page_size positions (a power of two, 16..1024).
 
     k, v: [n_layers, n_pages, n_kv_heads, page_size, head_dim]; table: int32 [max_rows, blocks];
     lens: int32 [max_rows]; free: int32 [n_pages], of which the first free_count[0] are free (to
@@ -125,7 +131,8 @@ class PagedKvCache:
         rest 0; copied from the host, so not under capture).  capacity: the map's length (with
         a sequence: by default its tokens).  out: a map of an earlier call of this capacity, to
         write into.  Pages go to requests in order; a request that cannot get them stays as it
-        was (status)."""
+        was (status), and what it asked for counts against the requests after it: new prompts
+        belong in the last rows, or in a call after the running requests' own."""
         if not torch.is_tensor(add):
             add = [int(a) for a in add]
             if len(add) > self.max_rows:
@@ -244,7 +251,8 @@ class PagedKvCache:
                out: torch.Tensor = None, workspace: torch.Tensor = None) -> torch.Tensor:
         """softmax(scale q k^T) v of one new token per row of q [n, n_heads, head_dim] (or
         [n, n_heads * head_dim]) over the cache of request rows[n] (int32; None: request n) up to
-        its length.  q: the pages' type, or f32 over bf16 pages.  scale: 1 / sqrt(head_dim) by
+        its length, whatever the query's own position: of several new tokens of a request only
+        the last is attended as a decoder does.  q: the pages' type, or f32 over bf16 pages.  scale: 1 / sqrt(head_dim) by
         default.  A row of no request (rows[n] < 0) leaves out[n] as it was (without `out`:
         unset); an empty request gives zeros.  workspace: `workspace(n, n_heads)`, to keep its
         zeroing out of a captured graph."""

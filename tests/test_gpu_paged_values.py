@@ -142,3 +142,25 @@ def test_decode_loop_step_by_step(cuda, it, ct):
         ctx = cache.attend(0, qs, rows=of)
         exact, bound = _attend_reference(qs, cache.k[0], cache.v[0], cache.table, cache.lens, of.tolist(), hd ** -0.5)
         _close(ctx, exact, bound, DT[it], f"step {step}")
+
+
+def test_every_query_sees_its_whole_request(cuda):
+    """Maps with several tokens of a request: each query reads the request to its end, later tokens
+    included, so that a decoder's attention is that of the last one; picked by cu, those equal
+    the calls of one token."""
+    nh, nkv, hd = 4, 2, 64
+    cache = PagedKvCache(1, nkv, hd, n_pages=20, page_size=16, max_rows=3, max_len=100, dtype=torch.float32, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(5)
+    m = cache.reserve([40, 0, 3])
+    q = cache.append(0, torch.randn((43, (nh + 2 * nkv) * hd), generator=g, device=cuda), m, n_heads=nh)
+    q = q.view(43, nh, hd)
+    got = cache.attend(0, q, rows=m.rows)
+    want, bound = _attend_reference(q, cache.k[0], cache.v[0], cache.table, cache.lens, m.rows.tolist(), hd ** -0.5)
+    _close(got, want, bound, torch.float32)
+    grew = m.cu[1:] > m.cu[:-1]
+    last = (m.cu[1:] - 1).clamp(min=0).long()
+    rows = torch.where(grew, torch.arange(3, device=cuda), -1).int()
+    out = torch.full((3, nh, hd), 7.0, device=cuda)
+    cache.attend(0, q[last].contiguous(), rows=rows, out=out)
+    assert bool((out[1] == 7).all())
+    _close(out[[0, 2]], want[[39, 42]], bound[[39, 42]], torch.float32)
