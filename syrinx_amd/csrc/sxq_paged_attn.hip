@@ -361,10 +361,10 @@ struct Shape {
 // cores' time at 5.4 TB/s), so the bound is HBM, or latency for little work.  Measured
 // (32 / 8 heads of 128, bf16, us): 64 requests of 1000..16384 positions (1.44 GB) 268, 5.4 TB/s
 // where a plain read of 3 GB reaches 6.2; one of 131071 (537 MB) 104; 16 of 256..2040 with f32
-// queries (74 MB) 18.2; HBM traffic 1.01 of the bytes asked for.  Of the 18 about 3 are the
-// launch and the loads of lengths and table in turn, 4 the end: partials out, an atomic, the
-// join's loads.  Two tiles ahead rather than one (registers for two workgroups a CU either way)
-// changed nothing.
+// queries (74 MB) 18.2; HBM traffic 1.012, 1.005 and 1.05 of the bytes asked for.  Of the 18
+// about 3 are the launch and the loads of lengths and table in turn, 4 the end: partials out, an
+// atomic, the join's loads.  Two tiles ahead rather than one (registers for two workgroups a CU
+// either way) changed nothing.
 // {m, l} and the sum: m is the maximum of scale * log2(e) * score (or
 // 0 where none is above -inf), l and the sum carry the weights 2^(x - m + kWeightShift).
 template <typename TQ, typename T, int HDP, bool FULL>
