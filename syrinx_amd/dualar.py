@@ -64,6 +64,8 @@ def drive_batch(slow: SlowAr, fast: FastAr, prompts, stop_id: int, params: Drive
     slow.reset(n)
     logits0, hidden0 = slow.prefill_batch(prompts)
     frames, flags = generate_frames(slow, fast, sampler, logits0, hidden0, params.max_new_frames, tmax)
+    if slow.paged:  # the batch is over: its pages are the next one's, whatever streams that has
+        slow.reset(n)
     f = torch.stack(frames)      # [T, n, 1 + n_cb]
     a = torch.stack(flags)       # [T, n]: the frame of step t counts for stream i when still active
     out = []

@@ -216,3 +216,22 @@ def test_a_prompt_attends_over_its_own_history(cuda, kv_dtype, lens, counts, pag
                     err = (got[g * G:(g + 1) * G] - w @ v).abs()
                     assert bool((err <= 2 * rel * (w @ v.abs())).all()), (s, i, l, g)
         first += counts[s]
+
+
+def test_a_finished_batch_holds_no_pages(cuda):
+    """A batch of three, then one stream that needs the pages of all: drive_batch gives back what
+    its streams held."""
+    cfg = T._fish_small(n_layers=1, max_batch=3)
+    slow = D.SlowAr(cfg, device=cuda, kv_pages=6, page_size=16)
+    slow.init_random(seed=6)
+    fast = D.FastAr(D.fish_s2_fast_ar_config(n_layers=1, num_codebooks=10, residual_size=64, max_batch=3), device=cuda)
+    fast.init_random(seed=7)
+    rng = np.random.default_rng(8)
+    prompts = [T._frames(rng, c, cfg).T for c in (12, 20, 5)]
+    params = dualar.DriveParams(max_new_frames=6)
+    first = dualar.drive_batch(slow, fast, prompts, stop_id=-1, params=params)
+    assert slow.free_pages() == 6
+    long = dualar.drive_batch(slow, fast, [T._frames(rng, 80, cfg).T], stop_id=-1, params=params)
+    assert long[0].shape[1] == 6 and slow.free_pages() == 6
+    again = dualar.drive_batch(slow, fast, prompts, stop_id=-1, params=params)
+    assert all(torch.equal(x, y) for x, y in zip(first, again))
