@@ -431,7 +431,9 @@ sxq_status sxq_lm_step(sxq_lm *lm, int n_streams, const int32_t *ids, const floa
 /* The step of a paged engine in which only some of its streams take part: active host int32
  * [n_streams] (NULL: all).  A stream whose entry is 0 keeps its length and its pages -- one
  * that has stopped, in a batch that goes on -- and takes none; its input row is still read,
- * its output rows mean nothing.  Refused with an entry of 0 for an engine that is not paged. */
+ * its output rows mean nothing (the argmax that a step without ids would feed it among them:
+ * one that comes back is given its id).  Refused with an entry of 0 for an engine that is not
+ * paged. */
 sxq_status sxq_lm_step_active(sxq_lm *lm, int n_streams, const int32_t *active, const int32_t *ids, const float *embeds,
                               float *logits, float *hidden, int32_t *next_ids, unsigned flags, void *stream);
 /* sxq_lm_prefill flags */
