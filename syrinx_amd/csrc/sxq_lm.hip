@@ -993,7 +993,10 @@ sxq_status lm_create(int device, const sxq_lm_config* cfg, const PageConfig* pag
     try {
         return lm_build(device, cfg, pages, out, made);
     } catch (const std::bad_alloc&) {  // (a paged engine's RoPE tables pass through a gigabyte of host memory at most)
-        if (made) destroy_lm(made);
+        if (made) {
+            DeviceGuard g(device);
+            destroy_lm(made);
+        }
         return fail(SXQ_ERR_OOM, "lm_create: out of host memory");
     }
 }
