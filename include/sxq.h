@@ -56,7 +56,9 @@ typedef enum {
     SXQ_Q8_0 = 8,
     SXQ_Q4K = 12,
     SXQ_Q8K = 15,
+    SXQ_I8 = 24,      /* cache pages only (sxq_kv_*): int8 codes with a scale a block */
     SXQ_BF16 = 30,
+    SXQ_E4M3 = 0x101, /* cache pages only: float8 e4m3 codes (no infinities, 448 the largest); not a GGML type */
 } sxq_dtype;
 
 /* sxq_qmm_forward flags */
@@ -205,16 +207,33 @@ sxq_status sxq_embed_gather(int device, int scheme, const uint8_t *q, const floa
  * row outside its range as no token, a length outside 0 .. max_blocks * page_size as the
  * nearest of the two. */
 typedef struct {
-    int32_t dtype;     /* SXQ_F32, SXQ_F16 or SXQ_BF16 */
+    int32_t dtype;     /* SXQ_F32, SXQ_F16, SXQ_BF16, or 8 bits with scales: SXQ_I8, SXQ_E4M3 */
     int32_t n_kv_heads;
-    int32_t head_dim;  /* a multiple of 8, 8..256 */
+    int32_t head_dim;  /* a multiple of 8 (8-bit pages: of 16), up to 256 */
     int32_t page_size; /* positions per page: a power of two, 16..1024 */
     int32_t n_pages;   /* n_pages * page_size < 2^31 */
     void *k, *v;       /* the pools, 16-byte aligned, laid out alike: */
     int64_t page_stride, head_stride, pos_stride; /* elements, multiples of 16 bytes, at least head_dim; a
                                                      head's row at one position is contiguous; pos_stride
                                                      at most 2^24 */
+    /* 8-bit pages only (else not read): the scale of the SXQ_KV_SCALE_BLOCK positions from b *
+     * SXQ_KV_SCALE_BLOCK on of a page and head is k_scale[page * scale_page_stride + head *
+     * scale_head_stride + b]; strides in floats, at least page_size / SXQ_KV_SCALE_BLOCK */
+    float *k_scale, *v_scale;
+    int64_t scale_page_stride, scale_head_stride;
 } sxq_kv_pages;
+
+/* 8-bit pages: a code c of a block with scale s stands for c * s.  Keys and values have scales of
+ * their own, for every 16 positions (from a multiple of 16 on) of a KV head.  sxq_kv_append sets
+ * them: a token whose position in its page is a multiple of 16 begins its block anew; the scale is
+ * the smallest power of two 2^e, e >= -100, with |x| <= Q 2^e for the finite elements x that the
+ * call writes to the block (Q: 127 for SXQ_I8, 448 for SXQ_E4M3), or the scale that the block has
+ * if that is larger (and the block is not begun anew); then the block's earlier codes, those before
+ * the first that the call writes, are rescaled to it.  A code is x / s rounded to nearest, ties to
+ * even; infinities become the largest code of their sign, a NaN becomes the e4m3 NaN, or int8's 0.
+ * Rescaling by powers of two is exact for e4m3, but for values below 2^-6 of the scale, and rounds
+ * int8 codes once more. */
+#define SXQ_KV_SCALE_BLOCK 16
 
 /* Block tables and slot maps from the requests' lengths.  Request r of n_rows holds lens[r]
  * positions in the pages table[r][0 .. ceil(lens[r] / page_size)) (table row stride
@@ -248,7 +267,10 @@ sxq_status sxq_kv_reserve(int device, int page_size, int n_pages, int n_rows, in
  * rotation), pairs (2i, 2i+1) if interleaved, else (i, i + head_dim / 2).  Keys and values go to
  * slots[t] of the pages, queries to q_out [n_tokens][n_heads * head_dim] in in_dtype (NULL:
  * not computed).  Arithmetic in f32, one rounding at each store.  A token whose slot lies
- * outside the pool writes nothing.  Tokens with one slot write it in no particular order. */
+ * outside the pool writes nothing.  Tokens with one slot write it in no particular order.
+ * 8-bit pages (above): the tokens that fall in one block of 16 positions follow one another in the
+ * map, in the order of their positions and without a gap between these, as sxq_kv_reserve lays them
+ * (of a block that comes up in two places of the map the codes and scale are unspecified). */
 sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, const void *qkv, int64_t row_stride,
                          int n_tokens, int n_heads, const float *q_norm, const float *k_norm, float eps,
                          const float *cos, const float *sin, int max_pos, int interleaved, const int32_t *pos,
@@ -261,10 +283,12 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
  * its whole request, also positions that were reserved together with its own: of several new
  * tokens of a request this is a decoder's attention of the last one only.  q and out:
  * rows of n_heads * head_dim, q_stride / out_stride elements apart (multiples of 16 bytes,
- * 16-byte aligned), q_dtype the pages' type, or SXQ_F32 over SXQ_BF16 pages; out has q's type.
+ * 16-byte aligned), q_dtype the pages' type, SXQ_F32 over SXQ_BF16 pages, any over 8-bit ones; out has q's type.
  * Scores, softmax statistics and sums are f32; over 16-bit pages a weight is carried in parts
  * of the pages' type, off by at most 2^-18 of itself (16-bit queries over bf16) or 2^-22 (f16;
- * f32 queries), below the output's own rounding.  rows int32 [n_q]: the table row of each query (NULL: b);
+ * f32 queries), below the output's own rounding.  Over 8-bit pages q may be of any of the three
+ * types: a code takes part exactly, an f32 query in three bf16 parts, a weight (times its value's
+ * scale) in bf16 parts, off by at most 2^-17 of itself (16-bit queries) or 2^-22.  rows int32 [n_q]: the table row of each query (NULL: b);
  * a query whose row lies outside 0 .. n_rows - 1 leaves its out row as it was.  A request
  * without positions (or whose pages are all absent) gives zeros.  max_blocks * page_size at
  * most 2^30, n_q times that at most 2^35, n_q at most 2^20.  What lies past a request's
@@ -284,6 +308,30 @@ sxq_status sxq_kv_attention(int device, const sxq_kv_pages *pages, int q_dtype, 
                             int n_q, int n_heads, const int32_t *rows, const int32_t *lens, int n_rows,
                             const int32_t *table, int64_t table_stride, int max_blocks, float scale, void *out,
                             int64_t out_stride, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Attention of new tokens each over its own prefix (a prompt's chunk, drafted tokens to verify),
+ * over 8-bit pages: as sxq_kv_attention, but query i sees the positions 0 .. pos[i] of its request
+ * (no more than it has; none if pos[i] < 0: zeros).  rows (not NULL) and pos are those of
+ * sxq_kv_reserve's map: queries of one request that follow one another share its keys' loads,
+ * whatever their positions; any other order is as right.  A weight is rounded to bf16 (2^-8 of
+ * itself) for bf16 queries, is off by at most 2^-17 for f16 and 2^-22 for f32 ones.  A workspace holds nothing between
+ * calls; calls that share one must not overlap. */
+sxq_status sxq_kv_prefix_attention_workspace(const sxq_kv_pages *pages, int n_q, int n_heads, size_t *bytes);
+sxq_status sxq_kv_prefix_attention(int device, const sxq_kv_pages *pages, int q_dtype, const void *q, int64_t q_stride,
+                                   int n_q, int n_heads, const int32_t *rows, const int32_t *pos, const int32_t *lens,
+                                   int n_rows, const int32_t *table, int64_t table_stride, int max_blocks, float scale,
+                                   void *out, int64_t out_stride, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Keys and values read back, of pages of any type: entry t of k and v, cu[i] <= t < cu[i + 1], is
+ * position start[i] + t - cu[i] of request rows[i], as n_kv_heads rows of head_dim elements of
+ * out_dtype (SXQ_F32, SXQ_F16 or SXQ_BF16; code times scale, rounded once), entries out_stride
+ * elements apart (a multiple of 16 bytes, both arrays 16-byte aligned).  cu int32 [n_ranges + 1]
+ * ascends from 0; rows may be NULL (request i), start too (0).  At most `total` entries are
+ * written, and none from cu[n_ranges] on.  A position outside 0 .. lens - 1, a request outside 0 ..
+ * n_rows - 1 and an absent page read as zeros. */
+sxq_status sxq_kv_read(int device, const sxq_kv_pages *pages, const int32_t *cu, const int32_t *rows, const int32_t *start,
+                       int n_ranges, int total, const int32_t *lens, int n_rows, const int32_t *table, int64_t table_stride,
+                       int max_blocks, int out_dtype, void *k, void *v, int64_t out_stride, void *stream);
 
 /* ---- Decoder step: the callers of QMatMul in one autoregressive LM token ------------
  *

@@ -78,6 +78,10 @@ _SIGS = {
     "sxq_kv_append": (_I, [_I, _P, _I, _P, _I64, _I, _I, _P, _P, _F, _P, _P, _I, _I, _P, _P, _P, _P]),
     "sxq_kv_attention_workspace": (_I, [_P, _I, _I, _P]),
     "sxq_kv_attention": (_I, [_I, _P, _I, _P, _I64, _I, _I, _P, _P, _I, _P, _I64, _I, _F, _P, _I64, _P, _SZ, _P]),
+    "sxq_kv_prefix_attention_workspace": (_I, [_P, _I, _I, _P]),
+    "sxq_kv_prefix_attention": (_I, [_I, _P, _I, _P, _I64, _I, _I, _P, _P, _P, _I, _P, _I64, _I, _F, _P, _I64, _P, _SZ,
+                                     _P]),
+    "sxq_kv_read": (_I, [_I, _P, _P, _P, _P, _I, _I, _P, _I, _P, _I64, _I, _I, _P, _P, _I64, _P]),
     "sxq_lm_step": (_I, [_P, _I, _P, _P, _P, _P, _P, _U, _P]),
     "sxq_lm_step_active": (_I, [_P, _I, _P, _P, _P, _P, _P, _P, _U, _P]),
     "sxq_lm_read_kv": (_I, [_P, _I, _I, _I, _I, _I, _P, _P, _P]),

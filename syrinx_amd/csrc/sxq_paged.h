@@ -22,7 +22,11 @@ struct KvPool {
     void *k, *v;
     int64_t page_stride, head_stride, pos_stride;
     int32_t dtype, nkv, hd, page, shift, n_pages;
+    // 8-bit pages: a scale for every kScaleBlock positions of a page and head.  Strides in floats.
+    float *k_scale, *v_scale;
+    int64_t scale_page_stride, scale_head_stride;
 };
+constexpr int kScaleShift = 4, kScaleBlock = 1 << kScaleShift;
 
 SXQ_PG_HD int kv_blocks(int len, int shift) { return (int)(((int64_t)len + (1 << shift) - 1) >> shift); }
 // A stored length as the kernels take it: 0 .. the positions its table row can hold.
@@ -40,6 +44,12 @@ SXQ_PG_HD int64_t kv_page_base(const KvPool& p, int id, int head) {
 // Element offset of head `head` at a slot (which lies in the pool).
 SXQ_PG_HD int64_t kv_slot_base(const KvPool& p, int slot, int head) {
     return kv_page_base(p, slot >> p.shift, head) + (int64_t)(slot & (p.page - 1)) * p.pos_stride;
+}
+
+// Offset of the scale of head `head` at a slot (which lies in the pool).
+SXQ_PG_HD int64_t kv_scale_at(const KvPool& p, int slot, int head) {
+    return (int64_t)(slot >> p.shift) * p.scale_page_stride + (int64_t)head * p.scale_head_stride +
+           ((slot & (p.page - 1)) >> kScaleShift);
 }
 
 }  // namespace sxq

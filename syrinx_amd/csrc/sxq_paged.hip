@@ -8,6 +8,7 @@
 #include "sxq_abi.h"
 #include "sxq_decoder.h"
 #include "sxq_paged.h"
+#include "sxq_paged_dev.h"
 #include "sxq_paged_launch.h"
 
 using namespace sxq;
@@ -52,37 +53,6 @@ SXQ_DEV Sums block_scan(Sums mine, Sums* red, Sums& total) {
     }
     total = sum;
     return lower + before;
-}
-
-// The last i with first[i] <= j, over n ascending firsts (first[0] <= j); for U values of j at
-// once, so that the steps' LDS (or L2) reads overlap.
-template <int U>
-SXQ_DEV void owners(const int* first, int n, const int (&j)[U], int (&i)[U]) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) i[u] = 0;
-    for (int step = n > 1 ? 1 << (31 - __builtin_clz(n - 1)) : 0; step; step >>= 1)
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            if (i[u] + step < n && first[i[u] + step] <= j[u]) i[u] += step;
-}
-SXQ_DEV int owner(const int* first, int n, int j) {
-    const int jj[1] = {j};
-    int i[1];
-    owners(first, n, jj, i);
-    return i[0];
-}
-
-// The same by a whole wave for one j: 64 offsets a step.
-SXQ_DEV int wave_owner(const int* first, int n, int j) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0;
-    while (n > 1) {
-        const int step = (n + 63) / 64, at = lane * step;
-        const int k = __builtin_popcountll(__ballot(at < n && first[lo + min(at, n - 1)] <= j)) - 1;
-        lo += k * step;
-        n = min(step, n - k * step);
-    }
-    return lo;
 }
 
 // How much of a call one workgroup does by itself.
@@ -337,23 +307,6 @@ __global__ __launch_bounds__(256) void k_kv_map(const KvReserve A) {
 }
 
 // ---------------------------------------------------------------------------- append
-// Four consecutive elements as f32, at any element's alignment, and back.
-template <typename T>
-SXQ_DEV void load4(const T* p, float* f) {
-    typedef T v4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    const v4 v = *(const v4*)p;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = to_f32(v[e]);
-}
-template <typename T>
-SXQ_DEV void store4(T* p, const float* f) {
-    typedef T v4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    v4 v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(f[e]);
-    *(v4*)p = v;
-}
-
 // Eight elements of a head a lane -- four RoPE pairs, as two vectors of four: (8 j, 8 j + 4)
 // interleaved, (4 j, hd / 2 + 4 j) in halves -- so that a head takes hd / 8 lanes (rounded up
 // to a power of two, LH), a wave 64 / LH heads of one token, the norm's sum stays among
@@ -562,7 +515,8 @@ namespace abi {
 
 sxq_status kv_pool(const char* who, const sxq_kv_pages* g, bool pointers, KvPool* out) {
     if (!g) return fail(SXQ_ERR_INVALID, "%s: null pages", who);
-    if (!kv_dtype(g->dtype)) return fail(SXQ_ERR_DTYPE, "%s: page dtype %d (f32, f16 or bf16)", who, g->dtype);
+    const bool is8 = kv_is8(g->dtype);
+    if (!kv_dtype(g->dtype) && !is8) return fail(SXQ_ERR_DTYPE, "%s: page dtype %d (f32, f16, bf16, int8 or e4m3)", who, g->dtype);
     if (!pow2_page(g->page_size))
         return fail(SXQ_ERR_INVALID, "%s: page_size %d is not a power of two in 16..1024", who, g->page_size);
     if (g->n_pages < 1 || (int64_t)g->n_pages * g->page_size > 0x7FFFFFFF)
@@ -571,7 +525,8 @@ sxq_status kv_pool(const char* who, const sxq_kv_pages* g, bool pointers, KvPool
         return fail(SXQ_ERR_INVALID, "%s: n_kv_heads %d", who, g->n_kv_heads);
     if (g->head_dim < 8 || g->head_dim > 256 || g->head_dim % 8)
         return fail(SXQ_ERR_SHAPE, "%s: head_dim %d is not a multiple of 8 in 8..256", who, g->head_dim);
-    const int64_t unit = 16 / type_size(g->dtype), most = (int64_t)1 << 50;
+    if (is8 && g->head_dim % 16) return fail(SXQ_ERR_SHAPE, "%s: head_dim %d of 8-bit pages is not a multiple of 16", who, g->head_dim);
+    const int64_t unit = 16 / kv_elem_size(g->dtype), most = (int64_t)1 << 50;
     for (int64_t st : {g->page_stride, g->head_stride, g->pos_stride})
         if (st < g->head_dim || st % unit || st > most)
             return fail(SXQ_ERR_SHAPE, "%s: page strides (%lld, %lld, %lld) must be multiples of %lld elements, at least head_dim",
@@ -579,6 +534,14 @@ sxq_status kv_pool(const char* who, const sxq_kv_pages* g, bool pointers, KvPool
     if (g->pos_stride > 1 << 24) return fail(SXQ_ERR_SHAPE, "%s: pos_stride %lld above 2^24 elements", who, (long long)g->pos_stride);
     if (pointers && (!g->k || !g->v)) return fail(SXQ_ERR_INVALID, "%s: null page pool", who);
     if (((uintptr_t)g->k | (uintptr_t)g->v) & 15) return fail(SXQ_ERR_INVALID, "%s: the page pools must be 16-byte aligned", who);
+    if (is8) {
+        for (int64_t st : {g->scale_page_stride, g->scale_head_stride})
+            if (st < g->page_size / kScaleBlock || st > most)
+                return fail(SXQ_ERR_SHAPE, "%s: scale strides (%lld, %lld) of pages of %d blocks", who,
+                            (long long)g->scale_page_stride, (long long)g->scale_head_stride, g->page_size / kScaleBlock);
+        if (pointers && (!g->k_scale || !g->v_scale)) return fail(SXQ_ERR_INVALID, "%s: null scales of 8-bit pages", who);
+        if (((uintptr_t)g->k_scale | (uintptr_t)g->v_scale) & 3) return fail(SXQ_ERR_INVALID, "%s: the scales must be 4-byte aligned", who);
+    }
     out->k = g->k;
     out->v = g->v;
     out->page_stride = g->page_stride;
@@ -590,6 +553,10 @@ sxq_status kv_pool(const char* who, const sxq_kv_pages* g, bool pointers, KvPool
     out->page = g->page_size;
     out->shift = __builtin_ctz((unsigned)g->page_size);
     out->n_pages = g->n_pages;
+    out->k_scale = is8 ? g->k_scale : nullptr;
+    out->v_scale = is8 ? g->v_scale : nullptr;
+    out->scale_page_stride = is8 ? g->scale_page_stride : 0;
+    out->scale_head_stride = is8 ? g->scale_head_stride : 0;
     return SXQ_OK;
 }
 
@@ -668,7 +635,7 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages* pages, int in_dtype, co
     a.pos = pos;
     a.slots = slots;
     a.q_out = q_out;
-    HIP_TRY(launch_kv_append(a, p, (hipStream_t)stream), "kv_append");
+    HIP_TRY(kv_is8(p.dtype) ? launch_kv8_append(a, p, (hipStream_t)stream) : launch_kv_append(a, p, (hipStream_t)stream), "kv_append");
     return SXQ_OK;
 }
 

@@ -830,16 +830,55 @@ hipError_t launch_kv_attend(const KvAttend& a, const KvPool& p, hipStream_t s) {
 
 }  // namespace sxq
 
+namespace {
+
+// What sxq_kv_attention and sxq_kv_prefix_attention take alike, checked.
+sxq_status check_attend(const char* who, const KvPool& p, const KvAttend& a, size_t need, size_t workspace_bytes) {
+    const bool known = a.q_dtype == kF32 || a.q_dtype == kF16 || a.q_dtype == kBF16;
+    if (kv_is8(p.dtype) ? !known : a.q_dtype != p.dtype && !(a.q_dtype == kF32 && p.dtype == kBF16))
+        return fail(SXQ_ERR_DTYPE, "%s: queries of dtype %d over pages of dtype %d", who, a.q_dtype, p.dtype);
+    if (a.n_q < 0 || a.n_q > 1 << 20 || a.nh < 1 || a.nh > 16384 || a.nh % p.nkv)
+        return fail(SXQ_ERR_SHAPE, "%s: %d queries of %d heads over %d KV heads", who, a.n_q, a.nh, p.nkv);
+    const int64_t width = (int64_t)a.nh * p.hd, unit = 16 / type_size(a.q_dtype);
+    if (a.q_stride < width || a.out_stride < width || a.q_stride % unit || a.out_stride % unit)
+        return fail(SXQ_ERR_SHAPE, "%s: q_stride %lld, out_stride %lld (multiples of %lld elements, rows of %lld)", who,
+                    (long long)a.q_stride, (long long)a.out_stride, (long long)unit, (long long)width);
+    if (a.n_rows < 1 || a.max_blocks < 1 || a.table_stride < a.max_blocks || (int64_t)a.max_blocks * p.page > 1 << 30)
+        return fail(SXQ_ERR_INVALID, "%s: a table of %d rows of %d blocks, stride %lld", who, a.n_rows, a.max_blocks, (long long)a.table_stride);
+    if ((int64_t)a.n_q * a.max_blocks * p.page > (int64_t)1 << 35)
+        return fail(SXQ_ERR_INVALID, "%s: %d queries of up to %lld positions", who, a.n_q, (long long)a.max_blocks * p.page);
+    if (!(a.scale - a.scale == 0.0f)) return fail(SXQ_ERR_INVALID, "%s: scale is not finite", who);
+    if (a.n_q == 0) return SXQ_OK;
+    if (!a.q || !a.lens || !a.table || !a.out || !a.ws) return fail(SXQ_ERR_INVALID, "%s: null pointer", who);
+    if (((uintptr_t)a.q | (uintptr_t)a.out) & 15) return fail(SXQ_ERR_INVALID, "%s: q and out must be 16-byte aligned", who);
+    if ((uintptr_t)a.ws & 255) return fail(SXQ_ERR_INVALID, "%s: the workspace must be 256-byte aligned", who);
+    if (workspace_bytes < need)
+        return fail(SXQ_ERR_INVALID, "%s: a workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
+    return SXQ_OK;
+}
+
+sxq_status workspace_of(const char* who, const sxq_kv_pages* pages, int n_q, int n_heads, bool prefix, size_t* bytes) {
+    if (!bytes) return fail(SXQ_ERR_INVALID, "%s: null output", who);
+    KvPool p;
+    if (sxq_status st = kv_pool(who, pages, false, &p)) return st;
+    if (prefix && !kv_is8(p.dtype)) return fail(SXQ_ERR_DTYPE, "%s: pages of dtype %d (int8 or e4m3)", who, p.dtype);
+    if (n_q < 0 || n_q > 1 << 20 || n_heads < 1 || n_heads > 16384 || n_heads % p.nkv)
+        return fail(SXQ_ERR_SHAPE, "%s: %d queries of %d heads over %d KV heads", who, n_q, n_heads, p.nkv);
+    *bytes = prefix ? kv8_prefix_workspace(p, n_q, n_heads)
+             : kv_is8(p.dtype) ? kv8_attend_workspace(p, n_q, n_heads) : kv_attend_workspace(p, n_q, n_heads);
+    return SXQ_OK;
+}
+
+}  // namespace
+
 extern "C" {
 
 sxq_status sxq_kv_attention_workspace(const sxq_kv_pages* pages, int n_q, int n_heads, size_t* bytes) {
-    if (!bytes) return fail(SXQ_ERR_INVALID, "kv_attention_workspace: null output");
-    KvPool p;
-    if (sxq_status st = kv_pool("kv_attention_workspace", pages, false, &p)) return st;
-    if (n_q < 0 || n_q > 1 << 20 || n_heads < 1 || n_heads > 16384 || n_heads % p.nkv)
-        return fail(SXQ_ERR_SHAPE, "kv_attention_workspace: %d queries of %d heads over %d KV heads", n_q, n_heads, p.nkv);
-    *bytes = kv_attend_workspace(p, n_q, n_heads);
-    return SXQ_OK;
+    return workspace_of("kv_attention_workspace", pages, n_q, n_heads, false, bytes);
+}
+
+sxq_status sxq_kv_prefix_attention_workspace(const sxq_kv_pages* pages, int n_q, int n_heads, size_t* bytes) {
+    return workspace_of("kv_prefix_attention_workspace", pages, n_q, n_heads, true, bytes);
 }
 
 sxq_status sxq_kv_attention(int device, const sxq_kv_pages* pages, int q_dtype, const void* q, int64_t q_stride,
@@ -848,46 +887,35 @@ sxq_status sxq_kv_attention(int device, const sxq_kv_pages* pages, int q_dtype, 
                             int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
     KvPool p;
     if (sxq_status st = kv_pool("kv_attention", pages, n_q > 0, &p)) return st;
-    if (q_dtype != p.dtype && !(q_dtype == kF32 && p.dtype == kBF16))
-        return fail(SXQ_ERR_DTYPE, "kv_attention: queries of dtype %d over pages of dtype %d", q_dtype, p.dtype);
-    if (n_q < 0 || n_q > 1 << 20 || n_heads < 1 || n_heads > 16384 || n_heads % p.nkv)
-        return fail(SXQ_ERR_SHAPE, "kv_attention: %d queries of %d heads over %d KV heads", n_q, n_heads, p.nkv);
-    const int64_t width = (int64_t)n_heads * p.hd, unit = 16 / type_size(q_dtype);
-    if (q_stride < width || out_stride < width || q_stride % unit || out_stride % unit)
-        return fail(SXQ_ERR_SHAPE, "kv_attention: q_stride %lld, out_stride %lld (multiples of %lld elements, rows of %lld)",
-                    (long long)q_stride, (long long)out_stride, (long long)unit, (long long)width);
-    if (n_rows < 1 || max_blocks < 1 || table_stride < max_blocks || (int64_t)max_blocks * p.page > 1 << 30)
-        return fail(SXQ_ERR_INVALID, "kv_attention: a table of %d rows of %d blocks, stride %lld", n_rows, max_blocks, (long long)table_stride);
-    if ((int64_t)n_q * max_blocks * p.page > (int64_t)1 << 35)
-        return fail(SXQ_ERR_INVALID, "kv_attention: %d queries of up to %lld positions", n_q, (long long)max_blocks * p.page);
+    const KvAttend a = {q,      q_stride,     q_dtype, n_q, n_heads,    rows,     lens, table, n_rows, max_blocks,
+                        table_stride, scale, out,     out_stride, workspace};
+    const bool is8 = kv_is8(p.dtype), sized = n_q > 0 && n_q <= 1 << 20 && n_heads > 0 && n_heads <= 16384 && n_heads % p.nkv == 0;
+    const size_t need = !sized ? 0 : is8 ? kv8_attend_workspace(p, n_q, n_heads) : kv_attend_workspace(p, n_q, n_heads);
+    if (sxq_status st = check_attend("kv_attention", p, a, need, workspace_bytes)) return st;
     if (!rows && n_q > n_rows) return fail(SXQ_ERR_SHAPE, "kv_attention: %d queries over %d table rows", n_q, n_rows);
-    if (!(scale - scale == 0.0f)) return fail(SXQ_ERR_INVALID, "kv_attention: scale is not finite");
     if (n_q == 0) return SXQ_OK;
-    if (!q || !lens || !table || !out || !workspace) return fail(SXQ_ERR_INVALID, "kv_attention: null pointer");
-    if (((uintptr_t)q | (uintptr_t)out) & 15) return fail(SXQ_ERR_INVALID, "kv_attention: q and out must be 16-byte aligned");
-    if ((uintptr_t)workspace & 255) return fail(SXQ_ERR_INVALID, "kv_attention: the workspace must be 256-byte aligned");
-    const size_t need = kv_attend_workspace(p, n_q, n_heads);
-    if (workspace_bytes < need)
-        return fail(SXQ_ERR_INVALID, "kv_attention: a workspace of %zu bytes, %zu needed", workspace_bytes, need);
     DeviceGuard g(device);
     HIP_TRY(g.err, "hipSetDevice");
-    KvAttend a;
-    a.q = q;
-    a.q_stride = q_stride;
-    a.q_dtype = q_dtype;
-    a.n_q = n_q;
-    a.nh = n_heads;
-    a.rows = rows;
-    a.lens = lens;
-    a.table = table;
-    a.n_rows = n_rows;
-    a.max_blocks = max_blocks;
-    a.table_stride = table_stride;
-    a.scale = scale;
-    a.out = out;
-    a.out_stride = out_stride;
-    a.ws = workspace;
-    HIP_TRY(launch_kv_attend(a, p, (hipStream_t)stream), "kv_attention");
+    HIP_TRY(is8 ? launch_kv8_attend(a, p, (hipStream_t)stream) : launch_kv_attend(a, p, (hipStream_t)stream), "kv_attention");
+    return SXQ_OK;
+}
+
+sxq_status sxq_kv_prefix_attention(int device, const sxq_kv_pages* pages, int q_dtype, const void* q, int64_t q_stride,
+                                   int n_q, int n_heads, const int32_t* rows, const int32_t* pos, const int32_t* lens,
+                                   int n_rows, const int32_t* table, int64_t table_stride, int max_blocks, float scale,
+                                   void* out, int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+    KvPool p;
+    if (sxq_status st = kv_pool("kv_prefix_attention", pages, n_q > 0, &p)) return st;
+    if (!kv_is8(p.dtype)) return fail(SXQ_ERR_DTYPE, "kv_prefix_attention: pages of dtype %d (int8 or e4m3)", p.dtype);
+    const KvAttend a = {q,      q_stride,     q_dtype, n_q, n_heads,    rows,     lens, table, n_rows, max_blocks,
+                        table_stride, scale, out,     out_stride, workspace};
+    const bool sized = n_q > 0 && n_q <= 1 << 20 && n_heads > 0 && n_heads <= 16384 && n_heads % p.nkv == 0;
+    if (sxq_status st = check_attend("kv_prefix_attention", p, a, sized ? kv8_prefix_workspace(p, n_q, n_heads) : 0, workspace_bytes)) return st;
+    if (n_q == 0) return SXQ_OK;
+    if (!rows || !pos) return fail(SXQ_ERR_INVALID, "kv_prefix_attention: null pointer");
+    DeviceGuard g(device);
+    HIP_TRY(g.err, "hipSetDevice");
+    HIP_TRY(launch_kv8_prefix(a, pos, p, (hipStream_t)stream), "kv_prefix_attention");
     return SXQ_OK;
 }
 

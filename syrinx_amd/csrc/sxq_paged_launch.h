@@ -46,6 +46,28 @@ struct KvAttend {
 size_t kv_attend_workspace(const KvPool& p, int n_q, int nh);
 hipError_t launch_kv_attend(const KvAttend& a, const KvPool& p, hipStream_t s);
 
+// The same over 8-bit pages (sxq_paged8*.hip); with pos (a position a query, or null) query i sees
+// the positions 0 .. pos[i] only.
+hipError_t launch_kv8_append(const KvAppend& a, const KvPool& p, hipStream_t s);
+size_t kv8_attend_workspace(const KvPool& p, int n_q, int nh);
+hipError_t launch_kv8_attend(const KvAttend& a, const KvPool& p, hipStream_t s);
+size_t kv8_prefix_workspace(const KvPool& p, int n_q, int nh);
+hipError_t launch_kv8_prefix(const KvAttend& a, const int32_t* pos, const KvPool& p, hipStream_t s);
+
+// sxq_kv_read, of pages of any type.
+struct KvRead {
+    const int32_t *cu, *rows, *start, *lens, *table;
+    int n_ranges, total, n_rows, max_blocks;
+    int64_t table_stride;
+    int out_dtype;
+    void *k, *v;
+    int64_t out_stride;
+};
+hipError_t launch_kv_read(const KvRead& a, const KvPool& p, hipStream_t s);
+
+inline bool kv_is8(int dtype) { return dtype == kI8 || dtype == kE4M3; }
+inline int kv_elem_size(int dtype) { return kv_is8(dtype) ? 1 : type_size(dtype); }
+
 // Up to 16 rows' positions one after another: row i's are start[i] .. start[i + 1] - 1 of start[n].
 struct KvSpans {
     int n, start[17];

@@ -10,9 +10,15 @@ free pages.  One decode step of a batch is
 
 A query of ``attend`` sees every position of its request, those reserved together with it too:
 right for the one new token of a decode step, and for the last of a prompt's tokens, not for the
-tokens before it.  A map of several tokens a request (a prompt's) is for ``append``; a prompt's
-tokens, each over its own prefix, are attended to by a paged engine (``DecoderLM.prefill``), and
-of such a map ``attend`` takes the last token of each request, at m.cu[r + 1] - 1.
+tokens before it.  Over pages of 8 bits ``attend`` takes the map's positions too (pos=m.pos), and each
+token of a map of several a request (a prompt's chunk, drafted tokens) then sees its own prefix.
+Over other pages such a map is for ``append``: a prompt's tokens are attended to by a paged engine
+(``DecoderLM.prefill``), and of such a map ``attend`` takes the last token of each request, at
+m.cu[r + 1] - 1.
+
+Pages of 8 bits (int8 or float8 e4m3) hold codes, and k_scale / v_scale a power of two for every
+SCALE_BLOCK positions of a KV head: ``append`` quantizes as it writes, ``attend`` computes with the
+values that the codes stand for, and ``read`` gives them back, of pages of any type.
 
 Nothing is copied to the host; every call enqueues on the current stream of the cache's device and
 may be captured into a graph.  The reference keeps one growing tensor per stream
@@ -33,16 +39,20 @@ import torch
 from ._lib import check, lib
 
 RELEASE = -(1 << 31)  # an `add` that empties any request
+SCALE_BLOCK = 16  # SXQ_KV_SCALE_BLOCK: positions of a page that share a scale (8-bit pages)
 _COUNTER_BYTES = 262144  # SXQ_KV_COUNTER_BYTES: the part of a workspace that starts as zeros
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+_DTYPES_8 = {torch.int8: 24, torch.float8_e4m3fn: 0x101}  # SXQ_I8, SXQ_E4M3: of pages only
 _P = ctypes.c_void_p
 
 
 class KvPages(ctypes.Structure):
     _fields_ = [("dtype", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
                 ("page_size", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("k", _P), ("v", _P),
-                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("pos_stride", ctypes.c_int64)]
+                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("pos_stride", ctypes.c_int64),
+                ("k_scale", _P), ("v_scale", _P), ("scale_page_stride", ctypes.c_int64),
+                ("scale_head_stride", ctypes.c_int64)]
 
 
 @dataclass
@@ -67,16 +77,19 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 class PagedKvCache:
     """Keys and values of up to max_rows requests of up to max_len positions (rounded up to whole
-    pages) in n_pages pages of page_size positions (a power of two, 16..1024).
+    pages) in n_pages pages of page_size positions (a power of two, 16..1024).  dtype: float32,
+    float16, bfloat16, or int8 / float8_e4m3fn with scales (head_dim then a multiple of 16).
 
-    k, v: [n_layers, n_pages, n_kv_heads, page_size, head_dim]; table: int32 [max_rows, blocks];
+    k, v: [n_layers, n_pages, n_kv_heads, page_size, head_dim]; of 8 bits also k_scale, v_scale: f32
+    [n_layers, n_pages, n_kv_heads, page_size / SCALE_BLOCK]; table: int32 [max_rows, blocks];
     lens: int32 [max_rows]; free: int32 [n_pages], of which the first free_count[0] are free (to
     be written in place, never replaced)."""
 
     def __init__(self, n_layers, n_kv_heads, head_dim, *, n_pages, page_size=32, max_rows, max_len,
                  dtype=torch.bfloat16, device="cuda:0"):
-        if dtype not in _DTYPES:
-            raise ValueError(f"PagedKvCache: dtype {dtype} (float32, float16 or bfloat16)")
+        self.is8 = dtype in _DTYPES_8
+        if dtype not in _DTYPES and not self.is8:
+            raise ValueError(f"PagedKvCache: dtype {dtype} (float32, float16, bfloat16, int8 or float8_e4m3fn)")
         if min(n_layers, max_rows, max_len) < 1:
             raise ValueError(f"PagedKvCache: {n_layers} layers, {max_rows} rows of {max_len} positions")
         device = torch.device(device)
@@ -86,7 +99,7 @@ class PagedKvCache:
         self.n_layers, self.n_kv_heads, self.head_dim = int(n_layers), int(n_kv_heads), int(head_dim)
         self.n_pages, self.page_size = int(n_pages), int(page_size)
         self.max_rows, self.max_len = int(max_rows), int(max_len)
-        probe = self._pages(None, None)
+        probe = self._pages(None, None, None, None)
         need = ctypes.c_size_t()
         check(lib().sxq_kv_attention_workspace(ctypes.byref(probe), 0, self.n_kv_heads, ctypes.byref(need)))
         if device.type != "cuda":
@@ -95,7 +108,14 @@ class PagedKvCache:
         shape = (self.n_layers, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim)
         self.k = torch.empty(shape, dtype=dtype, device=device)
         self.v = torch.empty(shape, dtype=dtype, device=device)
-        self._layers = [self._pages(self.k[i], self.v[i]) for i in range(self.n_layers)]
+        self.k_scale = self.v_scale = None
+        scales = [(None, None)] * self.n_layers
+        if self.is8:
+            shape = (self.n_layers, self.n_pages, self.n_kv_heads, self.page_size // SCALE_BLOCK)
+            self.k_scale = torch.zeros(shape, dtype=torch.float32, device=device)
+            self.v_scale = torch.zeros(shape, dtype=torch.float32, device=device)
+            scales = [(self.k_scale[i], self.v_scale[i]) for i in range(self.n_layers)]
+        self._layers = [self._pages(self.k[i], self.v[i], *scales[i]) for i in range(self.n_layers)]
         self._layer_refs = [ctypes.byref(p) for p in self._layers]
         self.table = torch.full((self.max_rows, self.max_blocks), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(self.max_rows, dtype=torch.int32, device=device)
@@ -104,10 +124,11 @@ class PagedKvCache:
         self.free_count = torch.full((1,), self.n_pages, dtype=torch.int32, device=device)
         self._need, self._ws = {}, {}
 
-    def _pages(self, k, v):
-        unit = self.head_dim * self.page_size
-        return KvPages(_DTYPES[self.dtype], self.n_kv_heads, self.head_dim, self.page_size, self.n_pages, _ptr(k),
-                       _ptr(v), unit * self.n_kv_heads, unit, self.head_dim)
+    def _pages(self, k, v, k_scale, v_scale):
+        unit, blocks = self.head_dim * self.page_size, self.page_size // SCALE_BLOCK
+        return KvPages(_DTYPES_8[self.dtype] if self.is8 else _DTYPES[self.dtype], self.n_kv_heads, self.head_dim,
+                       self.page_size, self.n_pages, _ptr(k), _ptr(v), unit * self.n_kv_heads, unit, self.head_dim,
+                       _ptr(k_scale), _ptr(v_scale), blocks * self.n_kv_heads, blocks)
 
     def _stream(self):
         return _raw_stream(self._index) if _raw_stream else torch.cuda.current_stream(self.device).cuda_stream
@@ -174,7 +195,10 @@ class PagedKvCache:
         bf16; any row stride), token t to slot_map.slots[t]: QK-RMSNorm by q_norm / k_norm (f32
         [head_dim]) and RoPE by rope = (cos, sin) (f32 [positions, head_dim / 2]), keys and
         values into the layer's pages, the queries returned [T, n_heads * head_dim] in qkv's
-        type.  A token without a slot leaves its row of out as it was."""
+        type.  A token without a slot leaves its row of out as it was.  Into pages of 8 bits the
+        map's tokens must be in the order in which `reserve` lays them (a block's next to one
+        another): each block of SCALE_BLOCK positions gets the smallest power of two that holds what
+        it is given, or keeps a larger one, and its earlier codes follow."""
         hd, dev, dtype, shape = self.head_dim, self.device, qkv.dtype, qkv.shape
         width = (n_heads + 2 * self.n_kv_heads) * hd
         code = _DTYPES.get(dtype)
@@ -215,20 +239,56 @@ class PagedKvCache:
                                   out.data_ptr(), self._stream()))
         return out
 
+    # -- back from the pages ----------------------------------------------------------------
+    def read(self, layer: int, cu: torch.Tensor, total: int, *, rows: torch.Tensor = None, start: torch.Tensor = None,
+             dtype: torch.dtype = torch.bfloat16, out=None):
+        """Keys and values of ranges of positions, one range after another: entry t of the two
+        tensors [total, n_kv_heads, head_dim], cu[i] <= t < cu[i + 1], is position start[i] + t - cu[i]
+        of request rows[i].  cu: int32 [n + 1], ascending from 0; rows: int32 [n] (None: request i);
+        start: int32 [n] (None: 0).  What a request does not hold reads as zeros; entries from cu[n] on
+        are left as they were (without `out`: unset).  dtype: float32, float16 or bfloat16; out: a
+        pair of tensors to write into (their dtype counts)."""
+        self._want("cu", cu, torch.int32)
+        n, total = cu.numel() - 1, int(total)
+        if n < 0 or total < 0:
+            raise ValueError(f"PagedKvCache.read: cu holds {n + 1} elements, total {total}")
+        shape = (total, self.n_kv_heads, self.head_dim)
+        if out is None:
+            if dtype not in _DTYPES:
+                raise ValueError(f"PagedKvCache.read: dtype {dtype} (float32, float16 or bfloat16)")
+            out = tuple(torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+        k, v = out
+        width = self.n_kv_heads * self.head_dim
+        for what, t in (("k", k), ("v", v)):
+            if (t.dtype not in _DTYPES or t.dtype is not k.dtype or t.device != self.device or t.shape != shape
+                    or (total > 0 and (t[0].is_contiguous() is False or t.stride(0) != k.stride(0)))):
+                raise ValueError(f"PagedKvCache.read: out's {what} must be f32, f16 or bf16 {shape} on {self.device}, entries "
+                                 f"contiguous, both alike, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        for what, t in (("rows", rows), ("start", start)):
+            if t is not None:
+                self._want(what, t, torch.int32, n)
+        stride = k.stride(0) if total > 1 else width
+        check(lib().sxq_kv_read(self._index, self._layer(layer), cu.data_ptr(), _ptr(rows), _ptr(start), n, total,
+                                self.lens.data_ptr(), self.max_rows, self.table.data_ptr(), self.max_blocks, self.max_blocks,
+                                _DTYPES[k.dtype], k.data_ptr(), v.data_ptr(), stride, self._stream()))
+        return k, v
+
     # -- attention ------------------------------------------------------------------------
-    def workspace(self, n_q: int, n_heads: int) -> torch.Tensor:
-        """A workspace, ready for use, of attend over n_q queries of n_heads heads: one for every
-        captured graph, kept while the graph lives."""
-        need = self._need.get((n_q, n_heads))
+    def workspace(self, n_q: int, n_heads: int, prefix: bool = False) -> torch.Tensor:
+        """A workspace, ready for use, of attend over n_q queries of n_heads heads (prefix: with
+        positions): one for every captured graph, kept while the graph lives."""
+        need = self._need.get((n_q, n_heads, prefix))
         if need is None:
             size = ctypes.c_size_t()
-            check(lib().sxq_kv_attention_workspace(self._layer_refs[0], n_q, n_heads, ctypes.byref(size)))
-            need = self._need[(n_q, n_heads)] = int(size.value)
+            ask = lib().sxq_kv_prefix_attention_workspace if prefix else lib().sxq_kv_attention_workspace
+            check(ask(self._layer_refs[0], n_q, n_heads, ctypes.byref(size)))
+            need = self._need[(n_q, n_heads, prefix)] = int(size.value)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        ws[:_COUNTER_BYTES].zero_()
+        if not prefix:
+            ws[:_COUNTER_BYTES].zero_()
         return ws
 
-    def _kept_workspace(self, n_q, n_heads):
+    def _kept_workspace(self, n_q, n_heads, prefix=False):
         """Eager calls: one workspace per stream, kept.  Under capture: a fresh one, owned by
         the graph, its zeroing recorded."""
         if torch.cuda.current_device() == self._index:
@@ -237,25 +297,27 @@ class PagedKvCache:
             with torch.cuda.device(self._index):
                 capturing = torch.cuda.is_current_stream_capturing()
         if capturing:
-            return self.workspace(n_q, n_heads)
-        stream = self._stream()
-        ws = self._ws.get(stream)
-        need = self._need.get((n_q, n_heads))
+            return self.workspace(n_q, n_heads, prefix)
+        key = (self._stream(), prefix)
+        ws = self._ws.get(key)
+        need = self._need.get((n_q, n_heads, prefix))
         if ws is None or need is None or ws.numel() < need:
-            fresh = self.workspace(n_q, n_heads)
+            fresh = self.workspace(n_q, n_heads, prefix)
             if ws is None or ws.numel() < fresh.numel():
-                ws = self._ws[stream] = fresh
+                ws = self._ws[key] = fresh
         return ws
 
-    def attend(self, layer: int, q: torch.Tensor, *, rows: torch.Tensor = None, scale: float = None,
-               out: torch.Tensor = None, workspace: torch.Tensor = None) -> torch.Tensor:
+    def attend(self, layer: int, q: torch.Tensor, *, rows: torch.Tensor = None, pos: torch.Tensor = None,
+               scale: float = None, out: torch.Tensor = None, workspace: torch.Tensor = None) -> torch.Tensor:
         """softmax(scale q k^T) v of one new token per row of q [n, n_heads, head_dim] (or
         [n, n_heads * head_dim]) over the cache of request rows[n] (int32; None: request n) up to
         its length, whatever the query's own position: of several new tokens of a request only
-        the last is attended as a decoder does.  q: the pages' type, or f32 over bf16 pages.  scale: 1 / sqrt(head_dim) by
-        default.  A row of no request (rows[n] < 0) leaves out[n] as it was (without `out`:
-        unset); an empty request gives zeros.  workspace: `workspace(n, n_heads)`, to keep its
-        zeroing out of a captured graph."""
+        the last is attended as a decoder does.  pos (int32 [n], over pages of 8 bits, with rows):
+        query i sees positions 0 .. pos[i] only; queries of one request that follow one another are
+        computed together.  q: the pages' type, f32 over bf16 pages, or f32, f16 or bf16 over pages of
+        8 bits.  scale: 1 / sqrt(head_dim) by default.  A row of no request (rows[n] < 0) leaves out[n] as it was (without `out`:
+        unset); an empty request gives zeros.  workspace: `workspace(n, n_heads)` (with positions:
+        `workspace(n, n_heads, prefix=True)`), to keep its zeroing out of a captured graph."""
         hd, dev, dtype, shape = self.head_dim, self.device, q.dtype, q.shape
         code, dims = _DTYPES.get(dtype), len(shape)
         if code is None or q.device != dev or dims not in (2, 3) or (dims == 3 and shape[2] != hd):
@@ -275,6 +337,10 @@ class PagedKvCache:
             if st[-1] != 1 or (dims == 3 and shape[1] > 1 and st[1] != hd):
                 raise ValueError(f"PagedKvCache.attend: each row of {what} must be contiguous, got strides {st}")
             strides.append(st[0] if n > 1 else width)
+        if pos is not None:
+            if rows is None or not self.is8:
+                raise ValueError(f"PagedKvCache.attend: positions take rows, and pages of 8 bits (these are {self.dtype})")
+            self._want("pos", pos, torch.int32, n)
         if rows is not None:
             self._want("rows", rows, torch.int32, n)
             rows = rows.data_ptr()
@@ -283,9 +349,16 @@ class PagedKvCache:
         if n == 0:
             return out
         if workspace is None:
-            workspace = self._kept_workspace(n, n_heads)
+            workspace = self._kept_workspace(n, n_heads, pos is not None)
         else:
             self._want("workspace", workspace, torch.uint8)
+        if pos is not None:
+            check(lib().sxq_kv_prefix_attention(self._index, self._layer(layer), code, q.data_ptr(), strides[0], n, n_heads,
+                                                rows, pos.data_ptr(), self.lens.data_ptr(), self.max_rows,
+                                                self.table.data_ptr(), self.max_blocks, self.max_blocks, scale,
+                                                out.data_ptr(), strides[1], workspace.data_ptr(), workspace.numel(),
+                                                self._stream()))
+            return out
         check(lib().sxq_kv_attention(self._index, self._layer(layer), code, q.data_ptr(), strides[0], n, n_heads, rows,
                                      self.lens.data_ptr(), self.max_rows, self.table.data_ptr(), self.max_blocks,
                                      self.max_blocks, scale, out.data_ptr(), strides[1], workspace.data_ptr(),
