@@ -9,11 +9,403 @@
 #include "sxq_abi.h"
 #include "sxq_paged.h"
 #include "sxq_paged_dev.h"
+#include "sxq_paged_split.h"
 
 using namespace sxq;
 using namespace sxq::abi;
 
 namespace {
+
+// ---- codes as matrix operands ------------------------------------------------------------
+// Both codes are exact in bf16 (int8: seven bits and a sign; e4m3: four bits) and in f16.
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
+template <typename C, typename M>
+struct Operand;
+template <>
+struct Operand<E4M3, __bf16> {
+    // elements 2 hi and 2 hi + 1 of w
+    template <bool HI>
+    static SXQ_DEV uint32_t two(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, (v2bf)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+    }
+    static SXQ_DEV v4u eight(uint32_t a, uint32_t b) { return (v4u){two<false>(a), two<true>(a), two<false>(b), two<true>(b)}; }
+    // out[c]: byte c of a (lower half) and of b
+    static SXQ_DEV void columns(uint32_t a, uint32_t b, uint32_t* out) {
+        const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400), hi = __builtin_amdgcn_perm(b, a, 0x07030602);
+        out[0] = two<false>(lo), out[1] = two<true>(lo), out[2] = two<false>(hi), out[3] = two<true>(hi);
+    }
+};
+template <>
+struct Operand<E4M3, _Float16> {
+    template <bool HI>
+    static SXQ_DEV uint32_t two(uint32_t w) {
+        return __builtin_bit_cast(uint32_t, (v2h)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+    }
+    static SXQ_DEV v4u eight(uint32_t a, uint32_t b) { return (v4u){two<false>(a), two<true>(a), two<false>(b), two<true>(b)}; }
+};
+template <>
+struct Operand<I8, __bf16> {
+    template <int E>
+    static SXQ_DEV uint32_t bits(uint32_t w) {
+        return __float_as_uint((float)(int8_t)(w >> (8 * E)));
+    }
+    // (the upper halves of two f32, exact)
+    static SXQ_DEV uint32_t pack(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302); }
+    static SXQ_DEV v4u eight(uint32_t a, uint32_t b) {
+        return (v4u){pack(bits<0>(a), bits<1>(a)), pack(bits<2>(a), bits<3>(a)), pack(bits<0>(b), bits<1>(b)), pack(bits<2>(b), bits<3>(b))};
+    }
+    static SXQ_DEV void columns(uint32_t a, uint32_t b, uint32_t* out) {
+        out[0] = pack(bits<0>(a), bits<0>(b)), out[1] = pack(bits<1>(a), bits<1>(b));
+        out[2] = pack(bits<2>(a), bits<2>(b)), out[3] = pack(bits<3>(a), bits<3>(b));
+    }
+};
+template <>
+struct Operand<I8, _Float16> {
+    // 0x6400 | b is 1024 + b: with the code's sign bit turned, b - 128 is the code
+    static SXQ_DEV uint32_t two(uint32_t w, uint32_t sel) {
+        const v2h v = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, w, sel));
+        return __builtin_bit_cast(uint32_t, v - (v2h){(_Float16)1152.0f, (_Float16)1152.0f});
+    }
+    static SXQ_DEV v4u eight(uint32_t a, uint32_t b) {
+        a ^= 0x80808080u, b ^= 0x80808080u;
+        return (v4u){two(a, 0x04010400), two(a, 0x04030402), two(b, 0x04010400), two(b, 0x04030402)};
+    }
+};
+
+SXQ_DEV v4f mfma(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+SXQ_DEV v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// A query's matrix type, and into how many bf16 parts its elements and the weights are cut.
+template <typename TQ>
+struct Query {
+    typedef TQ M;
+    static constexpr int kQP = 1, kWP = 2;
+};
+template <>
+struct Query<float> {
+    typedef __bf16 M;
+    static constexpr int kQP = 3, kWP = 3;
+};
+template <typename M>
+struct Vec8;
+template <>
+struct Vec8<__bf16> {
+    typedef v8bf T;
+};
+template <>
+struct Vec8<_Float16> {
+    typedef v8h T;
+};
+
+// Eight elements of a query as QP operands of 8 (parts of an f32 element sum to it exactly; what
+// passes bf16's range is infinite, its further parts zero).
+template <typename TQ, int QP>
+SXQ_DEV void query_parts(const TQ* src, bool in, v4u (&out)[QP]) {
+    if constexpr (QP == 1) {
+        const v4u v = *(const v4u*)src;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[0][e] = in ? v[e] : 0;
+    } else {
+        float f[8];
+        *(v4f*)f = *(const v4f*)src;
+        *(v4f*)(f + 4) = *(const v4f*)(src + 4);
+#pragma unroll
+        for (int q = 0; q < QP; ++q) {
+            v8bf part;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                part[e] = (__bf16)(in ? f[e] : 0.0f);
+                const float p = (float)part[e];
+                f[e] = fabsf(p) < INFINITY ? f[e] - p : p == p ? 0.0f : p;
+            }
+            out[q] = __builtin_bit_cast(v4u, part);
+        }
+    }
+}
+
+constexpr int kHalves = 2;  // 16-position halves of a wave's tile
+constexpr int kTile = 16 * kHalves;
+inline int attend_places(int hd) { return hd <= 64 ? 1024 : hd <= 128 ? 512 : 256; }
+
+// One item of 16 query heads (or fewer) of one KV head, as k_kv_attend: one pass over its keys and
+// values, four waves each with its own running maximum, sum and weighted values in registers.
+// Scores: A = 16 keys x 32 head elements, B = the queries' elements x 16 heads; the sum over
+// elements may take them in any order, so lane (r = lane % 16, g = lane / 16) loads 16 codes of key r
+// and makes two operands of them.  A half tile of 16 positions has one scale of keys and one of
+// values, the same for all lanes: the first goes into the factor of the scores, the second into the
+// weights before these are cut into bf16 parts.  Lane (r, g) of the result holds head r at
+// positions 4 g + i; the weights are used in those registers, so the lane loads HDP / 16 columns of
+// the values 4 g + i, two of a column meeting in a register by byte permutes before they are widened.
+template <typename TQ, typename C, int HDP, bool FULL>
+__global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv8_attend(const KvAttend A, const KvPool P,
+                                                                                         int target) {
+    typedef typename Query<TQ>::M M;
+    typedef typename Vec8<M>::T V8;
+    typedef Operand<C, M> KeyOp;
+    typedef Operand<C, __bf16> ValueOp;
+    constexpr int H = kHalves, KS = HDP / 64, D = HDP / 16, VD = D / 4;  // VD: dwords of a lane's columns
+    constexpr int QP = Query<TQ>::kQP, WP = Query<TQ>::kWP;
+    __shared__ EndShared<HDP> end;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int hd = FULL ? HDP : P.hd, G = A.nh / P.nkv;
+    const int ht = attend_head_tiles(A.nh, P.nkv);
+    const int kh = blockIdx.y / ht, h0 = kh * G + (blockIdx.y - kh * ht) * 16;
+    const int heads = min(16, (kh + 1) * G - h0);
+    const float scale2 = A.scale * 1.44269504088896340736f;
+    const uint32_t ps = (uint32_t)P.pos_stride;
+    const uint32_t kcol = 16 * g, koff = r * ps, vcol = D * r;
+    const bool vin = FULL || (int)vcol < hd;
+    uint32_t voff[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) voff[i] = (4 * g + i) * ps + (vin ? vcol : 0);
+    const char* kpool = (const char*)P.k + (int64_t)kh * P.head_stride;
+    const char* vpool = (const char*)P.v + (int64_t)kh * P.head_stride;
+    const float* kscale = P.k_scale + (int64_t)kh * P.scale_head_stride;
+    const float* vscale = P.v_scale + (int64_t)kh * P.scale_head_stride;
+
+    Item it;
+    if (!(A.n_q > kScanMax ? planned_item<kTile>(A, P, blockIdx.x, it) : find_item<kTile>(A, P, target, blockIdx.x, it))) return;
+
+    // the queries: B operands, in the element order of the key loads
+    const TQ* qrow = (const TQ*)A.q + (int64_t)it.b * A.q_stride + (int64_t)(h0 + min(r, heads - 1)) * hd;
+    V8 qreg[QP][KS][2];
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+            const int col = 64 * s + 16 * g + 8 * f;
+            const bool in = FULL || col < hd;
+            v4u parts[QP];
+            query_parts<TQ, QP>(qrow + (in ? col : 0), in, parts);
+#pragma unroll
+            for (int q = 0; q < QP; ++q) qreg[q][s][f] = __builtin_bit_cast(V8, parts[q]);
+        }
+
+    const int32_t* table = A.table + (int64_t)it.row * A.table_stride;
+    const int t_last = (it.len + 15) / 16 - 1;  // the last half tile (16 positions) with a position
+    const int t_end = min((it.first + it.tiles) * H, t_last + 1);
+    // Wave w takes the tiles w, w + 4, ... of the segment.  Lane j holds the page (-1: absent) and the
+    // scales of the wave's half tile j of a batch of 64, so that a tile waits for no load of theirs;
+    // the next batch's pages are loaded when one begins, its scales two tiles later.
+    const int t0 = it.first * H + wave * H, log_p = P.shift - 4, block_mask = (P.page >> kScaleShift) - 1;
+    auto tile_of = [&](int batch) { return t0 + (batch * 64 + lane) / H * (kWaves * H) + (lane & (H - 1)); };
+    auto page_batch = [&](int batch) {
+        const int t = tile_of(batch);
+        int id = -1;
+        if (t < t_end) id = table[t >> log_p];
+        return kv_page_ok(id, P.n_pages) ? id : -1;
+    };
+    auto scale_batch = [&](const float* scales, int batch, int id) {
+        float s = 0.0f;
+        if (id >= 0) s = scales[(int64_t)id * P.scale_page_stride + (tile_of(batch) & block_mask)];
+        return s;
+    };
+    int pages = page_batch(0), pages_next = -1;
+    float ks_lane = scale_batch(kscale, 0, pages), vs_lane = scale_batch(vscale, 0, pages), ks_next = 0.0f, vs_next = 0.0f;
+
+    v4f acc[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) acc[d] = (v4f){0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.0f;
+
+    uint32_t kreg[H][KS][4], vreg[H][4][VD];
+    int id[H];
+    float ks[H], vs[H];
+    int64_t at[H];
+    auto place = [&](int t) {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+            at[h] = max(id[h], 0) * P.page_stride + (int64_t)((uint32_t)(((t + h) * 16) & (P.page - 1)) * (uint64_t)ps);
+    };
+    auto load_k = [&]() {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                v4u v;
+                if constexpr (FULL) v = *(const v4u*)(kpool + at[h] + 64 * s + (koff + kcol));
+                else v = *(const v4u*)(kpool + at[h] + (koff + ((int)(64 * s + kcol) < hd ? 64 * s + kcol : 0)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kreg[h][s][e] = v[e];
+            }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                typedef uint32_t vec __attribute__((ext_vector_type(VD == 1 ? 2 : VD)));
+                const char* src = vpool + at[h] + voff[i];
+                if constexpr (VD == 1) vreg[h][i][0] = *(const uint32_t*)src;
+                else {
+                    const vec v = *(const vec*)src;
+#pragma unroll
+                    for (int e = 0; e < VD; ++e) vreg[h][i][e] = v[e];
+                }
+            }
+    };
+
+    int t = t0, k = 0;  // the tile's first half, its number in the batch
+    if (t < t_end) {
+        // the first tile's pages by scalar loads, which do not queue behind the card's other
+        // vector loads
+        typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
+        const scalar_ptr st = (scalar_ptr)(uintptr_t)table;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            const int page = st[min(t + h, t_last) >> log_p];
+            id[h] = t + h <= t_last && kv_page_ok(page, P.n_pages) ? page : -1;
+        }
+        place(t);
+        load_k();
+        load_v();
+        if (t + 64 / H * (kWaves * H) < t_end) pages_next = page_batch(1);
+    }
+    int batch = 1;
+    while (t < t_end) {
+        const int next = t + kWaves * H;
+        const bool more = next < t_end;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            ks[h] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks_lane), k * H + h));
+            vs[h] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs_lane), k * H + h));
+        }
+        // scores
+        float x[H][4];
+        int okh[H];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            okh[h] = id[h] >= 0;
+            v4f c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if constexpr (!FULL) {
+                    const bool in = (int)(64 * s + kcol) < hd;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) kreg[h][s][e] = in ? kreg[h][s][e] : 0;
+                }
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    const V8 key = __builtin_bit_cast(V8, KeyOp::eight(kreg[h][s][2 * f], kreg[h][s][2 * f + 1]));
+#pragma unroll
+                    for (int q = QP - 1; q >= 0; --q) c = mfma(key, qreg[q][s][f], c);  // the small parts first
+                }
+            }
+            const float factor = scale2 * ks[h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[h][i] = c[i] * factor;
+        }
+        const bool cut = (t + H) * 16 > it.len;  // some position lies past the end
+        bool absent = false;
+#pragma unroll
+        for (int h = 0; h < H; ++h) absent |= !okh[h];
+        const bool partial = cut || absent;
+        if (partial)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!okh[h] || (t + h) * 16 + 4 * g + i >= it.len) x[h][i] = -INFINITY;
+        if (more) {
+            if (++k == 64 / H) {
+                k = 0;
+                pages = pages_next;
+                ks_lane = ks_next;
+                vs_lane = vs_next;
+                pages_next = page_batch(++batch);
+            } else if (k == 2) {
+                ks_next = scale_batch(kscale, batch, pages_next);
+                vs_next = scale_batch(vscale, batch, pages_next);
+            }
+#pragma unroll
+            for (int h = 0; h < H; ++h) id[h] = __builtin_amdgcn_readlane(pages, k * H + h);
+            place(next);
+            load_k();
+        }
+        // the running maximum moves only where a score passes it
+        float mx = x[0][0];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[h][i]);
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, head_max(mx));
+            const float al = m > -INFINITY ? exp2_fast(m - mn) : 1.0f;  // nothing but zeros before
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < D; ++d) acc[d] *= al;
+            m = mn;
+        }
+        const float base = m > -INFINITY ? m : 0.0f;
+        float w[H][4];
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[h][i] = exp2_fast(x[h][i] - base);
+                l += w[h][i];
+                w[h][i] *= vs[h];
+            }
+        // values that no weight belongs to may hold anything: zeros in their place
+        if (partial)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = okh[h] && (t + h) * 16 + 4 * g + i < it.len;
+#pragma unroll
+                    for (int e = 0; e < VD; ++e) vreg[h][i][e] = in ? vreg[h][i][e] : 0;
+                }
+#pragma unroll
+        for (int hh = 0; hh < H; hh += 2) {
+            v8bf part[WP];
+#pragma unroll
+            for (int p = 0; p < WP; ++p)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float& v = w[hh + (j >> 2)][j & 3];
+                    part[p][j] = (__bf16)v;
+                    v -= (float)part[p][j];
+                }
+#pragma unroll
+            for (int q = 0; q < VD; ++q) {
+                uint32_t col[4][4];  // [pair of positions][column]
+#pragma unroll
+                for (int j = 0; j < 4; ++j)  // positions 2 j and 2 j + 1 of the lane's eight
+                    ValueOp::columns(vreg[hh + (j >> 1)][2 * (j & 1)][q], vreg[hh + (j >> 1)][2 * (j & 1) + 1][q], col[j]);
+#pragma unroll
+                for (int p = WP - 1; p >= 0; --p)  // the small parts first
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        acc[4 * q + c] = mfma(__builtin_bit_cast(v8bf, (v4u){col[0][c], col[1][c], col[2][c], col[3][c]}), part[p], acc[4 * q + c]);
+            }
+        }
+        if (more) load_v();
+        t = next;
+    }
+    finish_item<TQ, HDP, D, 1>(A, it, hd, h0, heads, acc, m, l, end);
+}
+
+template <typename TQ, typename C>
+void attend_by_width(const KvAttend& a, const KvPool& p, dim3 grid, int target, hipStream_t s) {
+#define SXQ_AT(HDP, FULL) hipLaunchKernelGGL((k_kv8_attend<TQ, C, HDP, FULL>), grid, dim3(256), 0, s, a, p, target)
+    if (p.hd == 64) SXQ_AT(64, true);
+    else if (p.hd == 128) SXQ_AT(128, true);
+    else if (p.hd == 256) SXQ_AT(256, true);
+    else if (p.hd < 64) SXQ_AT(64, false);
+    else if (p.hd < 128) SXQ_AT(128, false);
+    else SXQ_AT(256, false);
+#undef SXQ_AT
+}
+template <typename TQ>
+void attend_by_code(const KvAttend& a, const KvPool& p, dim3 grid, int target, hipStream_t s) {
+    if (p.dtype == kI8) attend_by_width<TQ, I8>(a, p, grid, target, s);
+    else attend_by_width<TQ, E4M3>(a, p, grid, target, s);
+}
 
 // A wave a query and head, 64 positions at a time: a lane's dot product with its key, a running
 // maximum and sum, then the weighted values, a lane a column (and every 64th after it).
@@ -89,10 +481,23 @@ void attend_plain(const KvAttend& a, const int32_t* pos, const KvPool& p, hipStr
 
 namespace sxq {
 
-size_t kv8_attend_workspace(const KvPool& p, int n_q, int nh) { return SXQ_KV_COUNTER_BYTES; }
+size_t kv8_attend_workspace(const KvPool& p, int n_q, int nh) {
+    return kCountBytes + attend_plan_bytes(n_q) +
+           2 * (size_t)attend_target_max(nh, p.nkv, attend_places(p.hd)) * nh * attend_part_floats(p.hd) * sizeof(float);
+}
 size_t kv8_prefix_workspace(const KvPool& p, int n_q, int nh) { return 256; }
 
-hipError_t launch_kv8_attend(const KvAttend& a, const KvPool& p, hipStream_t s) { return launch_kv8_prefix(a, nullptr, p, s); }
+hipError_t launch_kv8_attend(const KvAttend& a, const KvPool& p, hipStream_t s) {
+    const int target = attend_target(a.n_q, a.nh, p.nkv, attend_places(p.hd));
+    // (no more items than the table's width allows: workgroups that find none cost time)
+    const int64_t widest = (int64_t)a.n_q * (((int64_t)a.max_blocks * p.page + kTile * kMinTiles - 1) / (kTile * kMinTiles));
+    const dim3 grid((unsigned)std::min<int64_t>(target + a.n_q, widest), p.nkv * attend_head_tiles(a.nh, p.nkv));
+    if (a.n_q > kScanMax) hipLaunchKernelGGL(k_kv_attend_plan<kTile>, dim3(1), dim3(1024), 0, s, a, p, target);
+    if (a.q_dtype == kF32) attend_by_code<float>(a, p, grid, target, s);
+    else if (a.q_dtype == kF16) attend_by_code<_Float16>(a, p, grid, target, s);
+    else attend_by_code<__bf16>(a, p, grid, target, s);
+    return hipGetLastError();
+}
 hipError_t launch_kv8_prefix(const KvAttend& a, const int32_t* pos, const KvPool& p, hipStream_t s) {
     if (a.q_dtype == kF32) attend_plain<float>(a, pos, p, s);
     else if (a.q_dtype == kF16) attend_plain<_Float16>(a, pos, p, s);
