@@ -1,6 +1,5 @@
-// sxq_paged8_attn.hip -- attention over the 8-bit paged cache: one new token per request
-// (sxq_kv_attention), and several, each over its own prefix (sxq_kv_prefix_attention).
-// include/sxq.h states both.
+// sxq_paged8_attn.hip -- attention of one new token per request over the 8-bit paged cache
+// (sxq_kv_attention over SXQ_I8 and SXQ_E4M3; include/sxq.h states it).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -8,7 +7,7 @@
 #include "../../include/sxq.h"
 #include "sxq_abi.h"
 #include "sxq_paged.h"
-#include "sxq_paged_dev.h"
+#include "sxq_paged8_dev.h"
 #include "sxq_paged_split.h"
 
 using namespace sxq;
@@ -16,114 +15,8 @@ using namespace sxq::abi;
 
 namespace {
 
-// ---- codes as matrix operands ------------------------------------------------------------
-// Both codes are exact in bf16 (int8: seven bits and a sign; e4m3: four bits) and in f16.
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-
-template <typename C, typename M>
-struct Operand;
-template <>
-struct Operand<E4M3, __bf16> {
-    // elements 2 hi and 2 hi + 1 of w
-    template <bool HI>
-    static SXQ_DEV uint32_t two(uint32_t w) {
-        return __builtin_bit_cast(uint32_t, (v2bf)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
-    }
-    static SXQ_DEV v4u eight(uint32_t a, uint32_t b) { return (v4u){two<false>(a), two<true>(a), two<false>(b), two<true>(b)}; }
-    // out[c]: byte c of a (lower half) and of b
-    static SXQ_DEV void columns(uint32_t a, uint32_t b, uint32_t* out) {
-        const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x05010400), hi = __builtin_amdgcn_perm(b, a, 0x07030602);
-        out[0] = two<false>(lo), out[1] = two<true>(lo), out[2] = two<false>(hi), out[3] = two<true>(hi);
-    }
-};
-template <>
-struct Operand<E4M3, _Float16> {
-    template <bool HI>
-    static SXQ_DEV uint32_t two(uint32_t w) {
-        return __builtin_bit_cast(uint32_t, (v2h)__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
-    }
-    static SXQ_DEV v4u eight(uint32_t a, uint32_t b) { return (v4u){two<false>(a), two<true>(a), two<false>(b), two<true>(b)}; }
-};
-template <>
-struct Operand<I8, __bf16> {
-    template <int E>
-    static SXQ_DEV uint32_t bits(uint32_t w) {
-        return __float_as_uint((float)(int8_t)(w >> (8 * E)));
-    }
-    // (the upper halves of two f32, exact)
-    static SXQ_DEV uint32_t pack(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302); }
-    static SXQ_DEV v4u eight(uint32_t a, uint32_t b) {
-        return (v4u){pack(bits<0>(a), bits<1>(a)), pack(bits<2>(a), bits<3>(a)), pack(bits<0>(b), bits<1>(b)), pack(bits<2>(b), bits<3>(b))};
-    }
-    static SXQ_DEV void columns(uint32_t a, uint32_t b, uint32_t* out) {
-        out[0] = pack(bits<0>(a), bits<0>(b)), out[1] = pack(bits<1>(a), bits<1>(b));
-        out[2] = pack(bits<2>(a), bits<2>(b)), out[3] = pack(bits<3>(a), bits<3>(b));
-    }
-};
-template <>
-struct Operand<I8, _Float16> {
-    // 0x6400 | b is 1024 + b: with the code's sign bit turned, b - 128 is the code
-    static SXQ_DEV uint32_t two(uint32_t w, uint32_t sel) {
-        const v2h v = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, w, sel));
-        return __builtin_bit_cast(uint32_t, v - (v2h){(_Float16)1152.0f, (_Float16)1152.0f});
-    }
-    static SXQ_DEV v4u eight(uint32_t a, uint32_t b) {
-        a ^= 0x80808080u, b ^= 0x80808080u;
-        return (v4u){two(a, 0x04010400), two(a, 0x04030402), two(b, 0x04010400), two(b, 0x04030402)};
-    }
-};
-
 SXQ_DEV v4f mfma(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 SXQ_DEV v4f mfma(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-
-// A query's matrix type, and into how many bf16 parts its elements and the weights are cut.
-template <typename TQ>
-struct Query {
-    typedef TQ M;
-    static constexpr int kQP = 1, kWP = 2;
-};
-template <>
-struct Query<float> {
-    typedef __bf16 M;
-    static constexpr int kQP = 3, kWP = 3;
-};
-template <typename M>
-struct Vec8;
-template <>
-struct Vec8<__bf16> {
-    typedef v8bf T;
-};
-template <>
-struct Vec8<_Float16> {
-    typedef v8h T;
-};
-
-// Eight elements of a query as QP operands of 8 (parts of an f32 element sum to it exactly; what
-// passes bf16's range is infinite, its further parts zero).
-template <typename TQ, int QP>
-SXQ_DEV void query_parts(const TQ* src, bool in, v4u (&out)[QP]) {
-    if constexpr (QP == 1) {
-        const v4u v = *(const v4u*)src;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[0][e] = in ? v[e] : 0;
-    } else {
-        float f[8];
-        *(v4f*)f = *(const v4f*)src;
-        *(v4f*)(f + 4) = *(const v4f*)(src + 4);
-#pragma unroll
-        for (int q = 0; q < QP; ++q) {
-            v8bf part;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                part[e] = (__bf16)(in ? f[e] : 0.0f);
-                const float p = (float)part[e];
-                f[e] = fabsf(p) < INFINITY ? f[e] - p : p == p ? 0.0f : p;
-            }
-            out[q] = __builtin_bit_cast(v4u, part);
-        }
-    }
-}
 
 constexpr int kHalves = 2;  // 16-position halves of a wave's tile
 constexpr int kTile = 16 * kHalves;
@@ -407,76 +300,6 @@ void attend_by_code(const KvAttend& a, const KvPool& p, dim3 grid, int target, h
     else attend_by_width<TQ, E4M3>(a, p, grid, target, s);
 }
 
-// A wave a query and head, 64 positions at a time: a lane's dot product with its key, a running
-// maximum and sum, then the weighted values, a lane a column (and every 64th after it).
-template <typename TQ, typename C>
-__global__ __launch_bounds__(256) void k_kv8_attend_plain(const KvAttend A, const int32_t* pos, const KvPool P) {
-    __shared__ float s_q[4][256], s_p[4][64];
-    __shared__ int s_slot[4][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, hd = P.hd;
-    const int b = blockIdx.x, h = blockIdx.y * 4 + wave, kh = min(h, A.nh - 1) / (A.nh / P.nkv);
-    const int row = A.rows ? A.rows[b] : b;
-    if ((uint32_t)row >= (uint32_t)A.n_rows) return;
-    int len = kv_clamp_len(A.lens[row], A.max_blocks, P.shift);
-    if (pos) len = min(len, max(pos[b], -1) + 1);
-    const bool live = h < A.nh;
-    for (int d = lane; d < hd; d += 64) s_q[wave][d] = live ? to_f32(((const TQ*)A.q)[(int64_t)b * A.q_stride + (int64_t)h * hd + d]) : 0.0f;
-    float m = -INFINITY, l = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int p0 = 0; p0 < len; p0 += 64) {
-        const int p = p0 + lane;
-        const int slot = p < len ? kv_slot(A.table[(int64_t)row * A.table_stride + (p >> P.shift)], p, P.shift, P.n_pages) : -1;
-        __syncthreads();
-        float x = -INFINITY;
-        if (slot >= 0) {
-            const uint32_t* w = (const uint32_t*)((const uint8_t*)P.k + kv_slot_base(P, slot, kh));
-            float dot = 0.0f;
-            for (int d = 0; d < hd; d += 4) {
-                float f[4];
-                C::unpack(w[d / 4], f);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) dot += f[e] * s_q[wave][d + e];
-            }
-            x = dot * P.k_scale[kv_scale_at(P, slot, kh)] * A.scale;
-        }
-        float top = x == x ? x : INFINITY;
-        for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        const float mn = fmaxf(m, top), up = m > -INFINITY ? expf(m - mn) : 1.0f;
-        float e = mn > -INFINITY ? expf(x - mn) : 0.0f, sum = e;
-        for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        l = l * up + sum;
-        m = mn;
-        s_p[wave][lane] = slot >= 0 ? e * P.v_scale[kv_scale_at(P, slot, kh)] : 0.0f;
-        s_slot[wave][lane] = slot;
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int d = lane + 64 * q;
-            if (d >= hd) break;
-            float a = acc[q] * up;
-            for (int k = 0; k < 64; ++k) {
-                if (s_slot[wave][k] < 0) continue;
-                float f[4];
-                C::unpack(((const uint8_t*)P.v)[kv_slot_base(P, s_slot[wave][k], kh) + d], f);
-                a += s_p[wave][k] * f[0];
-            }
-            acc[q] = a;
-        }
-    }
-    if (!live) return;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int d = lane + 64 * q;
-        if (d < hd) ((TQ*)A.out)[(int64_t)b * A.out_stride + (int64_t)h * hd + d] = from_f32<TQ>(l == 0.0f ? 0.0f : acc[q] / l);
-    }
-}
-
-template <typename TQ>
-void attend_plain(const KvAttend& a, const int32_t* pos, const KvPool& p, hipStream_t s) {
-    const dim3 grid(a.n_q, (a.nh + 3) / 4);
-    if (p.dtype == kI8) hipLaunchKernelGGL((k_kv8_attend_plain<TQ, I8>), grid, dim3(256), 0, s, a, pos, p);
-    else hipLaunchKernelGGL((k_kv8_attend_plain<TQ, E4M3>), grid, dim3(256), 0, s, a, pos, p);
-}
-
 }  // namespace
 
 namespace sxq {
@@ -485,7 +308,6 @@ size_t kv8_attend_workspace(const KvPool& p, int n_q, int nh) {
     return kCountBytes + attend_plan_bytes(n_q) +
            2 * (size_t)attend_target_max(nh, p.nkv, attend_places(p.hd)) * nh * attend_part_floats(p.hd) * sizeof(float);
 }
-size_t kv8_prefix_workspace(const KvPool& p, int n_q, int nh) { return 256; }
 
 hipError_t launch_kv8_attend(const KvAttend& a, const KvPool& p, hipStream_t s) {
     const int target = attend_target(a.n_q, a.nh, p.nkv, attend_places(p.hd));
@@ -496,12 +318,6 @@ hipError_t launch_kv8_attend(const KvAttend& a, const KvPool& p, hipStream_t s) 
     if (a.q_dtype == kF32) attend_by_code<float>(a, p, grid, target, s);
     else if (a.q_dtype == kF16) attend_by_code<_Float16>(a, p, grid, target, s);
     else attend_by_code<__bf16>(a, p, grid, target, s);
-    return hipGetLastError();
-}
-hipError_t launch_kv8_prefix(const KvAttend& a, const int32_t* pos, const KvPool& p, hipStream_t s) {
-    if (a.q_dtype == kF32) attend_plain<float>(a, pos, p, s);
-    else if (a.q_dtype == kF16) attend_plain<_Float16>(a, pos, p, s);
-    else attend_plain<__bf16>(a, pos, p, s);
     return hipGetLastError();
 }
 

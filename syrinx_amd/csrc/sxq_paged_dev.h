@@ -55,6 +55,7 @@ SXQ_DEV void store4(T* p, const float* f) {
 
 // ---- 8-bit codes ---------------------------------------------------------------------------
 struct I8 {
+    static constexpr bool kNan = false;
     static constexpr float kTop = 127.0f;
     static constexpr int kTopExp = 6;           // 127 = 1.984375 * 2^6
     static constexpr uint32_t kTopMant = 0x7E0000u;
@@ -76,6 +77,7 @@ struct I8 {
     }
 };
 struct E4M3 {
+    static constexpr bool kNan = true;
     static constexpr float kTop = 448.0f;
     static constexpr int kTopExp = 8;           // 448 = 1.75 * 2^8
     static constexpr uint32_t kTopMant = 0x600000u;

@@ -585,7 +585,11 @@ def test_attention_of_codes_that_are_nan(cuda, prefix):
         assert bool(got[0, 2:, 9].isnan().all())
         cols = [c for c in range(64) if c != 9]
         assert torch.equal(got[0, 2:][:, cols], clean[0, 2:][:, cols])
-        if prefix:  # queries that do not see them
+        if prefix:  # queries that do not see them, beside others that do
+            both = torch.cat([q, q]).view(2, 3, 4, 64).transpose(0, 1).reshape(6, 4, 64).contiguous()
+            two = torch.tensor([0, 0, 1, 1, 2, 2], dtype=torch.int32, device=cuda)
+            got = cache.attend(0, both, rows=two, pos=torch.tensor([38, 39, 34, 99, 16, 16], dtype=torch.int32, device=cuda))
+            assert bool(got[0::2].isfinite().all()) and torch.equal(got[5], clean[2])
             got = cache.attend(0, q, rows=rows, pos=torch.tensor([38, 34, 16], dtype=torch.int32, device=cuda))
             assert bool(got.isfinite().all())
         cache.k[0, t[1][1], 0, 3, 5], cache.v[0, t[0][1], 1, 7, 9] = was
@@ -612,6 +616,29 @@ def test_attention_over_absent_pages(cuda, ct, prefix):
     else:
         got = cache.attend(0, q, rows=rows)
     assert not bool(got[0].any()) and not bool(got[2].any())
+
+
+def test_prefix_queries_before_a_nan(cuda):
+    """Queries of one tile before and after a NaN key and a NaN value: those that do not see it are as
+    without it, the others NaN (of the value: in its column)."""
+    cache, g = _filled(cuda, 2, 64, 16, [300], "e4m3", 3)
+    nan = torch.tensor(float("nan")).to(torch.float8_e4m3fn).to(cuda)
+    rows = torch.zeros(300, dtype=torch.int32, device=cuda)
+    pos = torch.arange(300, dtype=torch.int32, device=cuda)
+    for qt in ("f32", "bf16", "f16"):
+        q = _queries(g, cuda, 300, 4, 64, qt)
+        clean = cache.attend(0, q, rows=rows, pos=pos).clone()
+        at_v, at_k = int(cache.table[0, 70 // 16]), int(cache.table[0, 200 // 16])
+        was = cache.v[0, at_v, 1, 70 % 16, 9].clone(), cache.k[0, at_k, 0, 200 % 16, 0].clone()
+        cache.v[0, at_v, 1, 70 % 16, 9] = nan
+        cache.k[0, at_k, 0, 200 % 16, 0] = nan
+        got = cache.attend(0, q, rows=rows, pos=pos)
+        cols = [c for c in range(64) if c != 9]
+        assert torch.equal(got[:70], clean[:70]) and torch.equal(got[:200, :2], clean[:200, :2])
+        assert bool(got[70:, 2:, 9].isnan().all()) and bool(got[200:, :2].isnan().all())
+        want, bound = _reference(q, cache, [0] * 300, list(range(1, 301)), 0.125, split=PREFIX_SPLIT[qt])
+        _close(got[70:, 2:][:, :, cols], want[70:, 2:][:, :, cols], bound[70:, 2:][:, :, cols], DT[qt])
+        cache.v[0, at_v, 1, 70 % 16, 9], cache.k[0, at_k, 0, 200 % 16, 0] = was
 
 
 def test_offsets_past_32_bits(cuda):
