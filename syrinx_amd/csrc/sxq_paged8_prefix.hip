@@ -18,26 +18,32 @@ namespace {
 typedef float v16f __attribute__((ext_vector_type(16)));
 
 // ---- how the work is split ---------------------------------------------------------------
-// Consecutive queries of one request make tiles of whole tokens, kRows rows (a token and a head of
-// the KV head's group) or fewer; a group of more heads than that is cut into parts of kRows heads,
-// a token a tile.  A unit is a KV head and such a part.  A tile's keys are taken kKeys at a time;
-// where there are fewer tiles than the card has places, the longer ones are cut along their keys,
-// into pieces whose results a launch of its own joins.  A launch of one workgroup writes the tiles
-// and pieces ("items") down, and the attention's workgroups go through them.
-constexpr int kRows = 128;
-constexpr int kKeys = 64;
-constexpr int kMinPiece = 4;  // tiles of keys
+// Consecutive queries of one request make tiles of whole tokens, `rows` rows (a token and a head of the
+// KV head's group) or fewer; a group of more heads than that is cut into parts of so many heads, a
+// token a tile.  A unit is a KV head and such a part.  A tile's keys are taken `keys` at a time; where
+// there are fewer tiles than the card has places, the longer ones are cut along their keys, into
+// pieces whose results a launch of its own joins.  A launch of one workgroup writes the tiles and
+// pieces ("items") down, and the attention's workgroups go through them.
+// Two kernels: `wide` tiles of 128 rows, whose waves share the keys through LDS, and `few` of 32, whose
+// waves share the rows and divide the keys.
+constexpr int kWideRows = 128, kFewRows = 32;
+constexpr int kFewKeys = 128;  // a tile of keys: 32 a wave
+SXQ_HD constexpr int keys_a_tile(int hd) { return hd <= 128 ? 64 : 32; }  // wide (registers)
 
 struct Geometry {
+    int rows, keys;                   // of a tile
     int group, parts, units, tokens;  // heads a KV head; parts of a group; units; tokens a tile
-    int places;                       // items of one unit that the card holds at once
-    SXQ_HD Geometry(int nh, int nkv, int hd) {
+    int places, min_piece;            // items of one unit that the card holds at once; tiles of keys
+    SXQ_HD Geometry(int nh, int nkv, int hd, bool f32, bool few) {
+        rows = few ? kFewRows : kWideRows;
+        keys = few ? kFewKeys : keys_a_tile(hd);
         group = nh / nkv;
-        parts = (group + kRows - 1) / kRows;
+        parts = (group + rows - 1) / rows;
         units = nkv * parts;
-        tokens = group < kRows ? kRows / group : 1;
-        const int all = hd <= 128 ? 512 : 256;
+        tokens = group < rows ? rows / group : 1;
+        const int all = hd <= (f32 ? 64 : 128) ? 512 : 256;
         places = units < all ? all / units : 1;
+        min_piece = few ? 1 : 4;
     }
 };
 
@@ -48,11 +54,10 @@ struct TileItem {
     int part, pieces;       // where its result goes, of how many pieces (1: out)
 };
 
-// The workspace: counts {tiles, items}; the tiles' first queries; items; the tiles that are cut
+// The workspace: counts {items, tiles that are cut}; items; the tiles that are cut
 // {first item, pieces}; partials: per part and unit, {m, l} of each row, then the weighted sums.
 struct PrefixPlan {
     int* counts;
-    int* tile;
     TileItem* item;
     int2* cut;
     float* partial;
@@ -63,17 +68,15 @@ struct PrefixPlan {
         const int most = n_q + g.places;  // items: a tile each, and pieces up to the places
         counts = (int*)p;
         p += 256;
-        tile = (int*)p;
-        p += up(sizeof(int) * (size_t)n_q);
         item = (TileItem*)p;
         p += up(sizeof(TileItem) * (size_t)most);
         cut = (int2*)p;
         p += up(sizeof(int2) * (size_t)g.places);
         partial = (float*)p;
-        p += (size_t)g.places * g.units * part_floats(hd) * sizeof(float);
+        p += (size_t)g.places * g.units * part_floats(g.rows, hd) * sizeof(float);
         bytes = (size_t)(p - (char*)ws);
     }
-    SXQ_HD static size_t part_floats(int hd) { return (size_t)kRows * (hd + 2); }
+    SXQ_HD static size_t part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 };
 
 // The positions that query t sees, and whether it has a request.
@@ -82,78 +85,86 @@ SXQ_DEV int seen(const KvAttend& A, const int32_t* pos, const KvPool& P, int t, 
     return min(len, max(pos[t], -1) + 1);
 }
 
+// A thousand queries at a time, a thread each: where its run began and which of the chunk's tiles it is
+// in by ballots, the tiles' counts and limits in LDS.  Two loads in turn and three barriers a chunk.
 __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, const int32_t* pos, const KvPool P, const Geometry g,
                                                           bool may_cut) {
-    __shared__ int red[16], s_cut;
+    __shared__ int s_wave[2][16], s_limit[1025], s_count[1025], s_token[1025], s_row[1025], s_cut;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const PrefixPlan plan(A.ws, A.n_q, P.hd, g);
-    // Over the workgroup's threads up to this one: the sum, or the largest.
-    auto scan = [&](int v, bool largest, int& all) {
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(v, o, 64);
-            if (lane >= o) v = largest ? max(v, u) : v + u;
-        }
-        __syncthreads();
-        if (lane == 63) red[wave] = v;
-        __syncthreads();
-        int before = largest ? INT32_MIN : 0;
-        all = before;
-        for (int w = 0; w < 16; ++w) {
-            if (w == wave) before = all;
-            all = largest ? max(all, red[w]) : all + red[w];
-        }
-        return largest ? max(v, before) : v + before;
-    };
-    // 1. the tiles' first queries
+    const uint64_t upto = ~(uint64_t)0 >> (63 - lane);
+    if (tid == 0) s_cut = 0;
     int tiles = 0, run = 0;  // so far; where the run that reaches into the chunk began
     for (int c0 = 0; c0 < A.n_q; c0 += 1024) {
         const int t = c0 + tid;
-        const int row = t < A.n_q ? A.rows[t] : -1;
+        const int row = t < A.n_q ? A.rows[t] : -1, before = t > 0 && t < A.n_q ? A.rows[t - 1] : -1;
         const bool live = (uint32_t)row < (uint32_t)A.n_rows;
-        const bool begins = t < A.n_q && (t == 0 || A.rows[t - 1] != row);
-        int last, count;
-        const int start = max(run, scan(begins ? t : -1, true, last));
-        const bool first = live && (t - start) % g.tokens == 0;
-        const int at = scan(first ? 1 : 0, false, count);
-        if (first) plan.tile[tiles + at - 1] = t;
-        tiles += count;
-        run = max(run, last);
-    }
-    __syncthreads();
-    // 2. each tile's queries and keys
-    int work = 0;
-    for (int i0 = 0; i0 < tiles; i0 += 1024) {
-        const int i = i0 + tid;
-        int keys = 0, all;
-        if (i < tiles) {
-            const int t = plan.tile[i], row = A.rows[t];
-            int n = 1, limit = seen(A, pos, P, t, row);
-            while (n < g.tokens && t + n < A.n_q && A.rows[t + n] == row) limit = max(limit, seen(A, pos, P, t + n, row)), ++n;
-            keys = (limit + kKeys - 1) / kKeys;
-            plan.item[i] = TileItem{t, n, row, limit, 0, keys, 0, 1};
-        }
-        scan(keys, false, all);
-        work += all;
-    }
-    if (tid == 0) s_cut = 0;
-    __syncthreads();
-    // 3. pieces: at most g.places items in all where there are fewer tiles than that
-    const bool cutting = may_cut && tiles < g.places;
-    int items = tiles;
-    if (cutting) {
-        const int piece = max(kMinPiece, (work + g.places - tiles - 1) / (g.places - tiles));
-        TileItem mine{};  // (tiles < 1024: one a thread)
-        int n = 0, all;
-        if (tid < tiles) {
-            mine = plan.item[tid];
-            n = max(1, (mine.end + piece - 1) / piece);
-        }
-        const int at = scan(n, false, all) - n;
-        items = all;
+        const int limit = live ? seen(A, pos, P, t, row) : 0;
+        for (int i = tid; i < 1025; i += 1024) s_limit[i] = s_count[i] = 0;
+        const uint64_t begins = __ballot(t < A.n_q && (t == 0 || before != row));
+        if (lane == 0) s_wave[0][wave] = begins ? c0 + 64 * wave + 63 - __builtin_clzll(begins) : -1;
         __syncthreads();
+        int start = run;
+        for (int w = 0; w < wave; ++w) start = max(start, s_wave[0][w]);
+        if (begins & upto) start = c0 + 64 * wave + 63 - __builtin_clzll(begins & upto);
+        const bool first = live && (t - start) % g.tokens == 0;
+        const uint64_t firsts = __ballot(first);
+        if (lane == 0) s_wave[1][wave] = __builtin_popcountll(firsts);
+        for (int w = 0; w < 16; ++w) run = max(run, s_wave[0][w]);
+        __syncthreads();
+        int at = __builtin_popcountll(firsts & upto), count = 0;  // tiles of the chunk up to this query (0: the last chunk's last)
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) at += s_wave[1][w];
+            count += s_wave[1][w];
+        }
+        if (live) {
+            atomicMax(&s_limit[at], limit);
+            atomicAdd(&s_count[at], 1);
+        }
+        if (first) {
+            s_token[at] = t;
+            s_row[at] = row;
+        }
+        __syncthreads();
+        for (int i = tid; i <= count; i += 1024) {
+            if (i > 0) {
+                plan.item[tiles + i - 1] = TileItem{s_token[i], s_count[i], s_row[i], s_limit[i], 0, (s_limit[i] + g.keys - 1) / g.keys, 0, 1};
+            } else if (s_count[0] > 0) {
+                TileItem& last = plan.item[tiles - 1];
+                last.count += s_count[0];
+                last.limit = max(last.limit, s_limit[0]);
+                last.end = (last.limit + g.keys - 1) / g.keys;
+            }
+        }
+        tiles += count;
+        __syncthreads();
+    }
+    // pieces: at most g.places items in all where there are fewer tiles than that (a tile a thread)
+    int items = tiles;
+    if (may_cut && tiles < g.places) {
+        TileItem mine{};
+        if (tid < tiles) {
+            if (A.n_q <= 1024) mine = TileItem{s_token[tid + 1], s_count[tid + 1], s_row[tid + 1], s_limit[tid + 1], 0, (s_limit[tid + 1] + g.keys - 1) / g.keys, 0, 1};
+            else mine = plan.item[tid];
+        }
+        auto scan = [&](int v, int turn, int& all) {  // the sum over the threads up to this one
+            v = wave_scan(v);
+            if (lane == 63) s_wave[turn][wave] = v;
+            __syncthreads();
+            int lower = 0;
+            all = 0;
+            for (int w = 0; w < 16; ++w) {
+                if (w == wave) lower = all;
+                all += s_wave[turn][w];
+            }
+            return v + lower;
+        };
+        int work;
+        scan(mine.end, 0, work);
+        const int piece = max(g.min_piece, (work + g.places - tiles - 1) / (g.places - tiles));
+        const int keys = mine.end, n = tid < tiles ? max(1, (keys + piece - 1) / piece) : 0;
+        const int at = scan(n, 1, items) - n;
         if (n > 1) plan.cut[atomicAdd(&s_cut, 1)] = make_int2(at, n);
-        const int keys = mine.end;
         for (int k = 0; k < n; ++k) {
             mine.first = (int)((int64_t)keys * k / n);
             mine.end = (int)((int64_t)keys * (k + 1) / n);
@@ -173,6 +184,9 @@ __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, cons
 SXQ_DEV v16f mfma32(v8bf a, v8bf b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 SXQ_DEV v16f mfma32(v8h a, v8h b, v16f c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
+SXQ_DEV v4f mfma16(v8bf a, v8bf b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+SXQ_DEV v4f mfma16(v8h a, v8h b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
 // The other half of the wave's value.
 SXQ_DEV float other_half(float v) {
     float a = v, b = v;
@@ -190,10 +204,11 @@ constexpr int kWeightParts<float> = 3;
 
 template <int HDP>
 struct Stage {
+    static constexpr int kKeys = keys_a_tile(HDP), kBlocks = kKeys / kScaleBlock;
     __attribute__((aligned(16))) uint16_t k[kKeys * HDP];  // [key][element], 16-byte pieces exchanged within a row
     __attribute__((aligned(16))) uint16_t v[HDP * kKeys];  // [column][key], the same
-    float ks[4], vs[4];                                     // scales of the four blocks of 16 keys
-    int absent[4];                                          // whether each block is
+    float ks[kBlocks], vs[kBlocks];                         // scales of the blocks of 16 keys
+    int absent[kBlocks];                                          // whether each block is
 };
 
 // The first key of each column whose value is NaN.
@@ -207,18 +222,23 @@ template <int HDP>
 SXQ_DEV int k_piece(int key, int piece) {
     return HDP == 64 ? piece ^ ((key >> 1) & 7) : piece ^ (key & 15);
 }
-SXQ_DEV int v_piece(int col, int piece) { return piece ^ ((col >> 1) & 7) ^ ((col >> 4) & 1); }
+template <int HDP>
+SXQ_DEV int v_piece(int col, int piece) {
+    return keys_a_tile(HDP) == 64 ? piece ^ ((col >> 1) & 7) ^ ((col >> 4) & 1) : piece ^ ((col >> 2) & 3);
+}
 
 template <typename TQ, typename C, int HDP, bool FULL>
-__global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const KvAttend A, const int32_t* pos, const KvPool P,
+__global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) void k_kv8_prefix(const KvAttend A, const int32_t* pos, const KvPool P,
                                                                        const Geometry geo) {
     typedef typename Query<TQ>::M M;
     typedef typename Vec8<M>::T V8;
     constexpr int QP = Query<TQ>::kQP, WP = kWeightParts<TQ>;
     constexpr int KS = HDP / 16, CT = HDP / 32;             // steps over the head's elements, tiles of 32 columns
+    constexpr int kKeys = Stage<HDP>::kKeys, NB = Stage<HDP>::kBlocks, KT = kKeys / 32;
     constexpr int KP = kKeys * HDP / 16 / 256;              // 16-code pieces of keys a thread stages
-    constexpr int VP = 8 * (HDP / 4) / 256 > 0 ? 8 * (HDP / 4) / 256 : 1;  // 8-key x 4-column pieces of values a thread
-    constexpr bool VALL = 8 * (HDP / 4) >= 256;
+    constexpr int VPieces = kKeys / 8 * (HDP / 4);          // 8-key x 4-column pieces of values
+    constexpr int VP = VPieces > 256 ? VPieces / 256 : 1;   // a thread's
+    constexpr bool VALL = VPieces >= 256;
     __shared__ Stage<HDP> stage[2];
     __shared__ Nans<HDP> s_nans[2];  // of this item and the last
 
@@ -242,8 +262,8 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
             if (tid < HDP) nans->first[tid] = INT32_MAX;
             if (tid == 0) nans->any = 0;
         }
-        const int unit = (int)(w % geo.units), kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * kRows;
-        const int heads = min(min(kRows, geo.group), (kh + 1) * geo.group - h0);
+        const int unit = (int)(w % geo.units), kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
+        const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0);
         const TileItem it = plan.item[items - 1 - (int)(w / geo.units)];
         const int n_rows = it.count * heads;
         const int32_t* table = A.table + (int64_t)it.row * A.table_stride;
@@ -293,12 +313,14 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
         int kid[KP], vid[VP], sid = -1;  // pages of the next tile to load
         auto load_ids = [&](int tile) {
 #pragma unroll
-            for (int j = 0; j < KP; ++j) kid[j] = page_of(tile * 4 + (tid + 256 * j) / (HDP / 16) / 16);
+            for (int j = 0; j < KP; ++j) kid[j] = page_of(tile * NB + (tid + 256 * j) / (HDP / 16) / 16);
 #pragma unroll
-            for (int j = 0; j < VP; ++j) vid[j] = page_of(tile * 4 + ((tid + 256 * j) / (HDP / 4) & 7) / 2);
-            if (tid < 8) sid = page_of(tile * 4 + (tid & 3));
+            for (int j = 0; j < VP; ++j) vid[j] = page_of(tile * NB + ((tid + 256 * j) / (HDP / 4) & (2 * NB - 1)) / 2);
+            if (tid < 2 * NB) sid = page_of(tile * NB + (tid & (NB - 1)));
         };
         auto load_codes = [&](int tile) {
+            int tid = threadIdx.x;
+            asm volatile("" : "+v"(tid));
             const int key0 = tile * kKeys;
 #pragma unroll
             for (int j = 0; j < KP; ++j) {
@@ -311,7 +333,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
             }
 #pragma unroll
             for (int j = 0; j < VP; ++j) {
-                const int piece = tid + 256 * j, c = 4 * (piece % (HDP / 4)), o = piece / (HDP / 4) & 7;  // o = 2 u + f
+                const int piece = tid + 256 * j, c = 4 * (piece % (HDP / 4)), o = piece / (HDP / 4) & (2 * NB - 1);  // o = 2 u + f
                 const int key = 16 * (o >> 1) + 4 * (o & 1), off = (key0 + key) & (P.page - 1);
                 const bool in = vid[j] >= 0 && (FULL || c < hd);
                 const char* src = vpool + (int64_t)max(vid[j], 0) * P.page_stride + (uint64_t)off * ps + (in ? c : 0);
@@ -323,11 +345,13 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
                 }
             }
             block_id = sid;
-            if (tid < 8 && sid >= 0)
-                sc = (tid < 4 ? P.k_scale : P.v_scale)[(int64_t)sid * P.scale_page_stride + (int64_t)kh * P.scale_head_stride +
-                                                       ((tile * 4 + (tid & 3)) & block_mask)];
+            if (tid < 2 * NB && sid >= 0)
+                sc = (tid < NB ? P.k_scale : P.v_scale)[(int64_t)sid * P.scale_page_stride + (int64_t)kh * P.scale_head_stride +
+                                                       ((tile * NB + (tid & (NB - 1))) & block_mask)];
         };
         auto store_stage = [&](Stage<HDP>& S, int tile) {
+            int tid = threadIdx.x;
+            asm volatile("" : "+v"(tid));
 #pragma unroll
             for (int j = 0; j < KP; ++j) {
                 const int piece = tid + 256 * j, key = piece / (HDP / 16), c = 2 * (piece % (HDP / 16));
@@ -346,7 +370,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
                 if (found & 0x80808080u) {
 #pragma unroll
                     for (int j = 0; j < VP; ++j) {
-                        const int piece = tid + 256 * j, c = 4 * (piece % (HDP / 4)), o = piece / (HDP / 4) & 7;
+                        const int piece = tid + 256 * j, c = 4 * (piece % (HDP / 4)), o = piece / (HDP / 4) & (2 * NB - 1);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
 #pragma unroll
@@ -362,19 +386,19 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
 #pragma unroll
             for (int j = 0; j < VP; ++j) {
                 const int piece = tid + 256 * j, c = 4 * (piece % (HDP / 4)), o = piece / (HDP / 4);
-                if (!VALL && o >= 8) break;
+                if (!VALL && o >= 2 * NB) break;
                 uint32_t out[4][4];  // [pair of keys][column]
 #pragma unroll
                 for (int e = 0; e < 4; ++e) Operand<C, __bf16>::columns(vcode[j][2 * e], vcode[j][2 * e + 1], out[e]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    *(v4u*)(S.v + (c + e) * kKeys + 8 * v_piece(c + e, o)) = (v4u){out[0][e], out[1][e], out[2][e], out[3][e]};
+                    *(v4u*)(S.v + (c + e) * kKeys + 8 * v_piece<HDP>(c + e, o)) = (v4u){out[0][e], out[1][e], out[2][e], out[3][e]};
             }
-            if (tid < 4) {
+            if (tid < NB) {
                 S.ks[tid] = block_id >= 0 ? sc : 0.0f;
                 S.absent[tid] = block_id < 0;
-            } else if (tid < 8) {
-                S.vs[tid - 4] = block_id >= 0 ? sc : 0.0f;
+            } else if (tid < 2 * NB) {
+                S.vs[tid - NB] = block_id >= 0 ? sc : 0.0f;
             }
         };
 
@@ -401,25 +425,42 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
                 if (tile + 2 < it.end) load_ids(tile + 2);
             }
             const int key0 = tile * kKeys;
+            int col32 = lane & 31, hf = lane >> 5;
+            asm volatile("" : "+v"(col32), "+v"(hf));
             if (!idle && key0 < most) {
-                v16f c[2];
+                v16f c[KT];
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt) {
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) c[kt][i] = 0.0f;
-                    const int key = 32 * kt + col32;
-                    const uint16_t* row = S.k + key * HDP;
+                {
+                    // operands four ahead, and no further: the scheduler would take them all at once,
+                    // and spill
+                    V8 a[2][4];
+                    auto fetch = [&](int n) {
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        const V8 a = *(const V8*)(row + 8 * k_piece<HDP>(key, 2 * s + hf));
+                        for (int j = 0; j < 4; ++j) {
+                            const int kt = (4 * n + j) / KS, st = (4 * n + j) % KS, key = 32 * kt + col32;
+                            a[n & 1][j] = *(const V8*)(S.k + key * HDP + 8 * k_piece<HDP>(key, 2 * st + hf));
+                        }
+                    };
+                    fetch(0);
 #pragma unroll
-                        for (int p = QP - 1; p >= 0; --p) c[kt] = mfma32(a, qreg[p][s], c[kt]);  // the small parts first
+                    for (int n = 0; n < KT * KS / 4; ++n) {
+                        if (n + 1 < KT * KS / 4) fetch(n + 1);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int kt = (4 * n + j) / KS, st = (4 * n + j) % KS;
+#pragma unroll
+                            for (int p = QP - 1; p >= 0; --p) c[kt] = mfma32(a[n & 1][j], qreg[p][st], c[kt]);  // the small parts first
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                float factor[4], vs[4];
+                float factor[NB], vs[NB];
                 int absent = 0;
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
+                for (int b = 0; b < NB; ++b) {
                     factor[b] = scale2 * S.ks[b];
                     vs[b] = S.vs[b];
                     absent |= S.absent[b];
@@ -427,7 +468,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
                 float mx = -INFINITY;
                 if (key0 + kKeys > least || __builtin_amdgcn_readfirstlane(absent)) {
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt)
+                    for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int key = key0 + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3);
@@ -436,10 +477,10 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
                             mx = fmaxf(mx, c[kt][i]);
                         }
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) factor[b] = 1.0f;
+                    for (int b = 0; b < NB; ++b) factor[b] = 1.0f;
                 } else {
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
+                    for (int b = 0; b < NB; ++b) {
                         float top = c[b >> 1][8 * (b & 1)];
 #pragma unroll
                         for (int i = 1; i < 8; ++i) top = fmaxf(top, c[b >> 1][8 * (b & 1) + i]);
@@ -456,9 +497,9 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
                     m = mn;
                 }
                 const float base = m > -INFINITY ? m : 0.0f;
-                v8bf part[WP][4];
+                v8bf part[WP][NB];
 #pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
+                for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int b = 2 * kt + (i >> 3);
@@ -471,16 +512,21 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
                             w -= (float)part[p][b][i & 7];
                         }
                     }
+                v8bf a[2][NB];
+                auto fetch = [&](int d) {
+                    const int col = 32 * d + col32;
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) a[d & 1][u] = *(const v8bf*)(S.v + col * kKeys + 8 * v_piece<HDP>(col, 2 * u + hf));
+                };
+                fetch(0);
 #pragma unroll
                 for (int d = 0; d < CT; ++d) {
-                    const int col = 32 * d + col32;
-                    const uint16_t* row = S.v + col * kKeys;
+                    if (d + 1 < CT) fetch(d + 1);
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const v8bf a = *(const v8bf*)(row + 8 * v_piece(col, 2 * u + hf));
+                    for (int u = 0; u < NB; ++u)
 #pragma unroll
-                        for (int p = WP - 1; p >= 0; --p) acc[d] = mfma32(a, part[p][u], acc[d]);
-                    }
+                        for (int p = WP - 1; p >= 0; --p) acc[d] = mfma32(a[d & 1][u], part[p][u], acc[d]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (more) store_stage(stage[(tile + 1 - it.first) & 1], tile + 1);
@@ -497,9 +543,9 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
         if (idle || wave * 32 + col32 >= n_rows) continue;
         const bool alone = it.pieces == 1;
         const float inv = alone ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-        float* part = plan.partial + ((size_t)it.part * geo.units + unit) * PrefixPlan::part_floats(hd);
+        float* part = plan.partial + ((size_t)it.part * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
         if (!alone && hf == 0) *(float2*)(part + 2 * rho) = make_float2(m, l);
-        float* sums = part + 2 * kRows + (size_t)rho * hd;
+        float* sums = part + 2 * geo.rows + (size_t)rho * hd;
         TQ* out = (TQ*)A.out + (int64_t)tok * A.out_stride + (int64_t)head * hd;
 #pragma unroll
         for (int d = 0; d < CT; ++d)
@@ -516,38 +562,374 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
     }
 }
 
-// The pieces of each cut tile, joined: a wave a row and unit at a time, four columns a lane.
+// ---- few rows ------------------------------------------------------------------------------
+// One item of up to 32 rows: the waves go through the keys as those of k_kv8_attend do, 32 each of every
+// 128, keys and values straight into registers, two tiles of 16 rows on each operand; then the four
+// waves' sums are added up through LDS.  What bounds it is the keys' bytes, or latency.
+template <typename TQ, typename C, int HDP, bool FULL>
+__global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(const KvAttend A, const int32_t* pos, const KvPool P,
+                                                                          const Geometry geo) {
+    typedef typename Query<TQ>::M M;
+    typedef typename Vec8<M>::T V8;
+    constexpr int H = 2, NR = 2, KS = HDP / 64, D = HDP / 16, VD = D / 4;
+    constexpr int QP = Query<TQ>::kQP, WP = kWeightParts<TQ>;
+    __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ __attribute__((aligned(16))) float s_acc[4][16][HDP + 4];
+    __shared__ Nans<HDP> nans;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 15, g = lane >> 4;
+    const int hd = FULL ? HDP : P.hd;
+    const PrefixPlan plan(A.ws, A.n_q, hd, geo);
+    const int w = blockIdx.x / geo.units, unit = blockIdx.x - w * geo.units;
+    if (w >= plan.counts[0]) return;
+    const TileItem it = plan.item[w];
+    const int kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
+    const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0), n_rows = it.count * heads;
+    const float scale2 = A.scale * 1.44269504088896340736f;
+    if constexpr (C::kNan) {
+        if (tid < HDP) nans.first[tid] = INT32_MAX;
+        if (tid == 0) nans.any = 0;
+        __syncthreads();
+    }
+
+    // this lane's rows (those past the last repeat it)
+    int limit[NR], least = INT32_MAX;
+    V8 qreg[QP][NR][KS][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const int rho = min(16 * n + r, n_rows - 1), tok = it.token + rho / heads, head = h0 + rho % heads;
+        limit[n] = seen(A, pos, P, tok, it.row);
+        least = min(least, limit[n]);
+        const TQ* q = (const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                const int col = 64 * s + 16 * g + 8 * f;
+                const bool in = FULL || col < hd;
+                v4u parts[QP];
+                query_parts<TQ, QP>(q + (in ? col : 0), in, parts);
+#pragma unroll
+                for (int p = 0; p < QP; ++p) qreg[p][n][s][f] = __builtin_bit_cast(V8, parts[p]);
+            }
+    }
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
+    least = __builtin_amdgcn_readfirstlane(least);
+
+    const uint32_t ps = (uint32_t)P.pos_stride;
+    const uint32_t kcol = 16 * g, koff = r * ps, vcol = D * r;
+    const bool vin = FULL || (int)vcol < hd;
+    uint32_t voff[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) voff[i] = (4 * g + i) * ps + (vin ? vcol : 0);
+    const char* kpool = (const char*)P.k + (int64_t)kh * P.head_stride;
+    const char* vpool = (const char*)P.v + (int64_t)kh * P.head_stride;
+    const float* kscale = P.k_scale + (int64_t)kh * P.scale_head_stride;
+    const float* vscale = P.v_scale + (int64_t)kh * P.scale_head_stride;
+
+    const int32_t* table = A.table + (int64_t)it.row * A.table_stride;
+    const int t_last = (it.limit + 15) / 16 - 1;  // the last half tile (16 positions) with a position
+    const int t_end = min(it.end * (kFewKeys / 16), t_last + 1);
+    // lane j: the page (-1: absent) and scales of the wave's half tile j of a batch of 64
+    const int t0 = it.first * (kFewKeys / 16) + wave * H, log_p = P.shift - kScaleShift, block_mask = (P.page >> kScaleShift) - 1;
+    auto tile_of = [&](int batch) { return t0 + (batch * 64 + lane) / H * (4 * H) + (lane & (H - 1)); };
+    auto page_batch = [&](int batch) {
+        const int t = tile_of(batch);
+        int id = -1;
+        if (t < t_end) id = table[t >> log_p];
+        return kv_page_ok(id, P.n_pages) ? id : -1;
+    };
+    auto scale_batch = [&](const float* scales, int batch, int id) {
+        float s = 0.0f;
+        if (id >= 0) s = scales[(int64_t)id * P.scale_page_stride + (tile_of(batch) & block_mask)];
+        return s;
+    };
+    int pages = page_batch(0), pages_next = -1;
+    float ks_lane = scale_batch(kscale, 0, pages), vs_lane = scale_batch(vscale, 0, pages), ks_next = 0.0f, vs_next = 0.0f;
+
+    v4f acc[NR][D];
+    float m[NR], l[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < D; ++d) acc[n][d] = (v4f){0.f, 0.f, 0.f, 0.f};
+    }
+    uint32_t kreg[H][KS][4], vreg[H][4][VD];
+    int id[H];
+    int64_t at[H];
+    auto place = [&](int t, int k) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            id[h] = __builtin_amdgcn_readlane(pages, k * H + h);
+            at[h] = max(id[h], 0) * P.page_stride + (int64_t)((uint32_t)(((t + h) * 16) & (P.page - 1)) * (uint64_t)ps);
+        }
+    };
+    auto load_k = [&]() {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                v4u v;
+                if constexpr (FULL) v = *(const v4u*)(kpool + at[h] + 64 * s + (koff + kcol));
+                else v = *(const v4u*)(kpool + at[h] + (koff + ((int)(64 * s + kcol) < hd ? 64 * s + kcol : 0)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kreg[h][s][e] = v[e];
+            }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                typedef uint32_t vec __attribute__((ext_vector_type(VD == 1 ? 2 : VD)));
+                const char* src = vpool + at[h] + voff[i];
+                if constexpr (VD == 1) vreg[h][i][0] = *(const uint32_t*)src;
+                else {
+                    const vec v = *(const vec*)src;
+#pragma unroll
+                    for (int e = 0; e < VD; ++e) vreg[h][i][e] = v[e];
+                }
+            }
+    };
+    int t = t0, k = 0;  // the tile's first half, its number in the batch
+    if (t < t_end) {
+        place(t, 0);
+        load_k();
+        load_v();
+        if (t + 64 / H * (4 * H) < t_end) pages_next = page_batch(1);
+    }
+    int batch = 1;
+    while (t < t_end) {
+        const int next = t + 4 * H;
+        const bool more = next < t_end;
+        float ks[H], vs[H];
+        bool okh[H], absent = false;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            ks[h] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks_lane), k * H + h));
+            vs[h] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs_lane), k * H + h));
+            okh[h] = id[h] >= 0;
+            absent |= !okh[h];
+        }
+        const bool partial = (t + H) * 16 > least || absent;  // some row does not see some position
+        float x[NR][H][4];
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            v4f c[NR];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) c[n] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if constexpr (!FULL) {
+                    const bool in = (int)(64 * s + kcol) < hd;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) kreg[h][s][e] = in ? kreg[h][s][e] : 0;
+                }
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    const V8 key = __builtin_bit_cast(V8, Operand<C, M>::eight(kreg[h][s][2 * f], kreg[h][s][2 * f + 1]));
+#pragma unroll
+                    for (int p = QP - 1; p >= 0; --p)  // the small parts first
+#pragma unroll
+                        for (int n = 0; n < NR; ++n) c[n] = mfma16(key, qreg[p][n][s][f], c[n]);
+                }
+            }
+            const float factor = scale2 * ks[h];
+#pragma unroll
+            for (int n = 0; n < NR; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[n][h][i] = c[n][i] * factor;
+                    if (partial && (!okh[h] || (t + h) * 16 + 4 * g + i >= limit[n])) x[n][h][i] = -INFINITY;
+                }
+        }
+        const int t_now = t;
+        if (more) {
+            if (++k == 64 / H) {
+                k = 0;
+                pages = pages_next;
+                ks_lane = ks_next;
+                vs_lane = vs_next;
+                pages_next = page_batch(++batch);
+            } else if (k == 2) {
+                ks_next = scale_batch(kscale, batch, pages_next);
+                vs_next = scale_batch(vscale, batch, pages_next);
+            }
+            place(next, k);
+            load_k();
+        }
+        // values that no row of the item sees may hold anything, and a NaN belongs to the rows that see
+        // its position (a weight of zero would not keep it from the others): zeros in their place, and
+        // a column's first NaN noted
+        if (partial)
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int p = (t_now + h) * 16 + 4 * g + i;
+                    const bool in = okh[h] && p < it.limit && vin;
+#pragma unroll
+                    for (int e = 0; e < VD; ++e) {
+                        uint32_t& v = vreg[h][i][e];
+                        v = in ? v : 0;
+                        if constexpr (C::kNan)
+                            if (((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u)
+                                for (int b = 0; b < 32; b += 8)
+                                    if ((v >> b & 0x7F) == 0x7F) {
+                                        v &= ~(0xFFu << b);
+                                        atomicMin(&nans.first[vcol + 4 * e + b / 8], p);
+                                        nans.any = 1;
+                                    }
+                    }
+                }
+        v8bf part[NR][WP];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            float mx = x[n][0][0];
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[n][h][i]);
+            if (__any(mx > m[n])) {
+                const float mn = fmaxf(m[n], head_max(mx));
+                const float al = m[n] > -INFINITY ? exp2_fast(m[n] - mn) : 1.0f;  // nothing but zeros before
+                l[n] *= al;
+#pragma unroll
+                for (int d = 0; d < D; ++d) acc[n][d] *= al;
+                m[n] = mn;
+            }
+            const float base = m[n] > -INFINITY ? m[n] : 0.0f;
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = exp2_fast(x[n][h][i] - base);
+                    l[n] += v;
+                    v *= vs[h];
+#pragma unroll
+                    for (int p = 0; p < WP; ++p) {
+                        part[n][p][4 * h + i] = (__bf16)v;
+                        v -= (float)part[n][p][4 * h + i];
+                    }
+                }
+        }
+#pragma unroll
+        for (int q = 0; q < VD; ++q) {
+            uint32_t col[4][4];  // [pair of positions][column]
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // positions 2 j and 2 j + 1 of the lane's eight
+                Operand<C, __bf16>::columns(vreg[j >> 1][2 * (j & 1)][q], vreg[j >> 1][2 * (j & 1) + 1][q], col[j]);
+#pragma unroll
+            for (int p = WP - 1; p >= 0; --p)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int n = 0; n < NR; ++n)
+                        acc[n][4 * q + c] = mfma16(__builtin_bit_cast(v8bf, (v4u){col[0][c], col[1][c], col[2][c], col[3][c]}), part[n][p], acc[n][4 * q + c]);
+        }
+        if (more) load_v();
+        t = next;
+    }
+
+    // the four waves' sums, 16 rows at a time
+    const bool alone = it.pieces == 1;
+    float* to = plan.partial + ((size_t)it.part * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        if (16 * n >= n_rows) break;
+        if (n) __syncthreads();
+        l[n] = head_sum(l[n]);
+        if (g == 0) {
+            s_m[wave][r] = m[n];
+            s_l[wave][r] = l[n];
+        }
+        __syncthreads();
+        float M = s_m[0][r];
+#pragma unroll
+        for (int w2 = 1; w2 < 4; ++w2) M = fmaxf(M, s_m[w2][r]);
+        const float f = m[n] > -INFINITY ? exp2_fast(m[n] - M) : 1.0f;  // (no weights, or NaN: as they are)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < D; ++e) s_acc[wave][r][(4 * g + i) * D + e] = acc[n][e][i] * f;
+        __syncthreads();
+        const int per = hd / 4;
+        for (int o = tid; o < min(16, n_rows - 16 * n) * per; o += 256) {
+            const int row = o / per, c = 4 * (o - row * per), rho = 16 * n + row, tok = it.token + rho / heads;
+            float top = s_m[0][row], sum = 0.0f;
+#pragma unroll
+            for (int w2 = 1; w2 < 4; ++w2) top = fmaxf(top, s_m[w2][row]);
+            v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w2 = 0; w2 < 4; ++w2) {
+                sum += s_l[w2][row] * (s_m[w2][row] > -INFINITY ? exp2_fast(s_m[w2][row] - top) : 1.0f);
+                v += *(const v4f*)&s_acc[w2][row][c];
+            }
+            if constexpr (C::kNan)
+                if (nans.any) {
+                    const int lim = seen(A, pos, P, tok, it.row);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (nans.first[c + e] < lim) v[e] = NAN;
+                }
+            if (alone) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const float out[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+                store4((TQ*)A.out + (int64_t)tok * A.out_stride + (int64_t)(h0 + rho % heads) * hd + c, out);
+            } else {
+                *(v4f*)(to + 2 * geo.rows + (size_t)rho * hd + c) = v;
+                if (c == 0) *(float2*)(to + 2 * rho) = make_float2(top, sum);
+            }
+        }
+    }
+}
+
+// ---- the join ------------------------------------------------------------------------------
+// The pieces of each cut tile, in their order, four columns of a row a thread, four pieces' loads at
+// a time.
 template <typename TQ>
 __global__ __launch_bounds__(256) void k_kv8_prefix_join(const KvAttend A, const KvPool P, const Geometry geo) {
     const PrefixPlan plan(A.ws, A.n_q, P.hd, geo);
-    const int cuts = plan.counts[1], lane = threadIdx.x & 63, hd = P.hd;
-    const int waves = gridDim.x * 4, mine = blockIdx.x * 4 + (threadIdx.x >> 6);
-    for (int64_t w = mine; w < (int64_t)cuts * geo.units * kRows; w += waves) {
-        const int row = (int)(w % kRows), unit = (int)(w / kRows % geo.units);
-        const int2 cut = plan.cut[w / kRows / geo.units];
+    const int cuts = plan.counts[1], hd = P.hd, per = hd / 4, at_once = 256 / per;  // rows a workgroup takes at once
+    const int steps = (geo.rows + at_once - 1) / at_once;
+    const int sub = threadIdx.x / per, col = 4 * (threadIdx.x - sub * per);
+    for (int w = blockIdx.x; w < cuts * geo.units * steps; w += gridDim.x) {
+        const int step = w % steps, unit = w / steps % geo.units, row = step * at_once + sub;
+        const int2 cut = plan.cut[w / steps / geo.units];
         const TileItem it = plan.item[cut.x];
-        const int kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * kRows;
-        const int heads = min(min(kRows, geo.group), (kh + 1) * geo.group - h0);
-        if (row >= it.count * heads) continue;
-        const float* part = plan.partial + ((size_t)cut.x * geo.units + unit) * PrefixPlan::part_floats(hd);
-        const size_t step = (size_t)geo.units * PrefixPlan::part_floats(hd);
-        float m = -INFINITY;
-        for (int k = lane; k < cut.y; k += 64) m = fmaxf(m, part[k * step + 2 * row]);
-        for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-        float l = 0.0f;
+        const int kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
+        const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0);
+        if (sub >= at_once || row >= it.count * heads) continue;
+        const float* part = plan.partial + ((size_t)cut.x * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
+        const size_t stride = (size_t)geo.units * PrefixPlan::part_floats(geo.rows, hd);
+        float m = -INFINITY, l = 0.0f;
         v4f v = {0.f, 0.f, 0.f, 0.f};
-        const int col = 4 * lane;
-        for (int k = 0; k < cut.y; ++k) {
-            const float2 ml = *(const float2*)(part + k * step + 2 * row);
-            const float f = ml.x > -INFINITY ? exp2_fast(ml.x - m) : 1.0f;  // (no weights, or NaN: as they are)
-            l += ml.y * f;
-            if (col < hd) v += *(const v4f*)(part + k * step + 2 * kRows + (size_t)row * hd + col) * f;
-        }
-        if (col >= hd) continue;
-        float f[4];
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int k0 = 0; k0 < cut.y; k0 += 4) {
+            float2 ml[4];
+            v4f x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = v[e] * inv;
+            for (int u = 0; u < 4; ++u) {
+                const float* p = part + min(k0 + u, cut.y - 1) * stride;
+                ml[u] = *(const float2*)(p + 2 * row);
+                x[u] = *(const v4f*)(p + 2 * geo.rows + (size_t)row * hd + col);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (k0 + u >= cut.y) break;
+                const float mn = fmaxf(m, ml[u].x);
+                const float up = m > -INFINITY ? exp2_fast(m - mn) : 1.0f;  // (no weights, or NaN: as they are)
+                const float f = ml[u].x > -INFINITY ? exp2_fast(ml[u].x - mn) : 1.0f;
+                l = l * up + ml[u].y * f;
+                v = v * up + x[u] * f;
+                m = mn;
+            }
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float f[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
         store4((TQ*)A.out + (int64_t)(it.token + row / heads) * A.out_stride + (int64_t)(h0 + row % heads) * hd + col, f);
     }
 }
@@ -555,8 +937,12 @@ __global__ __launch_bounds__(256) void k_kv8_prefix_join(const KvAttend A, const
 template <typename TQ, typename C, int HDP, bool FULL>
 hipError_t prefix_launch(const KvAttend& a, const int32_t* pos, const KvPool& p, const Geometry& g, hipStream_t s) {
     const int64_t most = ((int64_t)a.n_q + g.places) * g.units;
-    const int grid = (int)std::min<int64_t>(most, HDP <= 128 ? 512 : 256);
-    hipLaunchKernelGGL((k_kv8_prefix<TQ, C, HDP, FULL>), dim3(grid), dim3(256), 0, s, a, pos, p, g);
+    if (g.rows == kFewRows) {
+        hipLaunchKernelGGL((k_kv8_prefix_few<TQ, C, HDP, FULL>), dim3((unsigned)most), dim3(256), 0, s, a, pos, p, g);
+    } else {
+        const int grid = (int)std::min<int64_t>(most, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 512 : 256);
+        hipLaunchKernelGGL((k_kv8_prefix<TQ, C, HDP, FULL>), dim3(grid), dim3(256), 0, s, a, pos, p, g);
+    }
     return hipGetLastError();
 }
 template <typename TQ, typename C>
@@ -572,8 +958,9 @@ template <typename TQ>
 hipError_t prefix_by_code(const KvAttend& a, const int32_t* pos, const KvPool& p, const Geometry& g, bool may_cut, hipStream_t s) {
     const hipError_t e = p.dtype == kI8 ? prefix_by_width<TQ, I8>(a, pos, p, g, s) : prefix_by_width<TQ, E4M3>(a, pos, p, g, s);
     if (e != hipSuccess || !may_cut) return e;
-    const int64_t waves = (int64_t)g.places * g.units * kRows;
-    hipLaunchKernelGGL((k_kv8_prefix_join<TQ>), dim3((unsigned)std::min<int64_t>(1024, (waves + 3) / 4)), dim3(256), 0, s, a, p, g);
+    const int at_once = 256 / (p.hd / 4), steps = (g.rows + at_once - 1) / at_once;
+    const int64_t all = (int64_t)(g.places / 2) * g.units * steps;  // (a cut tile has two pieces at least)
+    hipLaunchKernelGGL((k_kv8_prefix_join<TQ>), dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(1024, all))), dim3(256), 0, s, a, p, g);
     return hipGetLastError();
 }
 
@@ -582,11 +969,16 @@ hipError_t prefix_by_code(const KvAttend& a, const int32_t* pos, const KvPool& p
 namespace sxq {
 
 size_t kv8_prefix_workspace(const KvPool& p, int n_q, int nh) {
-    return PrefixPlan(nullptr, n_q, p.hd, Geometry(nh, p.nkv, p.hd)).bytes;
+    size_t most = 0;
+    for (int form = 0; form < 4; ++form) most = std::max(most, PrefixPlan(nullptr, n_q, p.hd, Geometry(nh, p.nkv, p.hd, form & 1, form & 2)).bytes);
+    return most;
 }
 
 hipError_t launch_kv8_prefix(const KvAttend& a, const int32_t* pos, const KvPool& p, hipStream_t s) {
-    const Geometry g(a.nh, p.nkv, p.hd);
+    const int group = a.nh / p.nkv;
+    // Drafted tokens and the like, 32 rows a request or fewer on average: the few-row kernel.
+    const bool few = (int64_t)a.n_q * group <= (int64_t)kFewRows * std::min(a.n_rows, 64) || a.n_q * group <= kFewRows;
+    const Geometry g(a.nh, p.nkv, p.hd, a.q_dtype == kF32, few);
     // (as many tiles as places, whatever the map: nothing is cut)
     const bool may_cut = (a.n_q + g.tokens - 1) / g.tokens < g.places;
     hipLaunchKernelGGL(k_kv8_prefix_plan, dim3(1), dim3(1024), 0, s, a, pos, p, g, may_cut);
