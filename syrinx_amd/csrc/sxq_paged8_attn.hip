@@ -28,7 +28,7 @@ inline int attend_places(int hd) { return hd <= 64 ? 1024 : hd <= 128 ? 512 : 25
 // elements may take them in any order, so lane (r = lane % 16, g = lane / 16) loads 16 codes of key r
 // and makes two operands of them.  A half tile of 16 positions has one scale of keys and one of
 // values, the same for all lanes: the first goes into the factor of the scores, the second into the
-// weights before these are cut into bf16 parts.  Lane (r, g) of the result holds head r at
+// weights before these are cut into bf16 parts (three under f32 queries, else two).  Lane (r, g) of the result holds head r at
 // positions 4 g + i; the weights are used in those registers, so the lane loads HDP / 16 columns of
 // the values 4 g + i, two of a column meeting in a register by byte permutes before they are widened.
 template <typename TQ, typename C, int HDP, bool FULL>
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv8
     typedef Operand<C, M> KeyOp;
     typedef Operand<C, __bf16> ValueOp;
     constexpr int H = kHalves, KS = HDP / 64, D = HDP / 16, VD = D / 4;  // VD: dwords of a lane's columns
-    constexpr int QP = Query<TQ>::kQP, WP = Query<TQ>::kWP;
+    constexpr int QP = Query<TQ>::kQP, WP = sizeof(TQ) == 4 ? 3 : 2;  // parts of a query, of a weight
     __shared__ EndShared<HDP> end;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -65,18 +65,15 @@ __global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv8
 
     // the queries: B operands, in the element order of the key loads
     const TQ* qrow = (const TQ*)A.q + (int64_t)it.b * A.q_stride + (int64_t)(h0 + min(r, heads - 1)) * hd;
-    V8 qreg[QP][KS][2];
+    V8 qreg[QP][2 * KS];
+    int qcol[2 * KS];
+    bool qin[2 * KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-            const int col = 64 * s + 16 * g + 8 * f;
-            const bool in = FULL || col < hd;
-            v4u parts[QP];
-            query_parts<TQ, QP>(qrow + (in ? col : 0), in, parts);
-#pragma unroll
-            for (int q = 0; q < QP; ++q) qreg[q][s][f] = __builtin_bit_cast(V8, parts[q]);
-        }
+    for (int s = 0; s < 2 * KS; ++s) {
+        qcol[s] = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+        qin[s] = FULL || qcol[s] < hd;
+    }
+    const float row_scale = scale2 * load_query<TQ>(qrow, qcol, qin, qreg, [](float v) { return head_max(v); });
 
     const int32_t* table = A.table + (int64_t)it.row * A.table_stride;
     const int t_last = (it.len + 15) / 16 - 1;  // the last half tile (16 positions) with a position
@@ -185,10 +182,10 @@ __global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv8
                 for (int f = 0; f < 2; ++f) {
                     const V8 key = __builtin_bit_cast(V8, KeyOp::eight(kreg[h][s][2 * f], kreg[h][s][2 * f + 1]));
 #pragma unroll
-                    for (int q = QP - 1; q >= 0; --q) c = mfma(key, qreg[q][s][f], c);  // the small parts first
+                    for (int q = QP - 1; q >= 0; --q) c = mfma(key, qreg[q][2 * s + f], c);  // the small parts first
                 }
             }
-            const float factor = scale2 * ks[h];
+            const float factor = row_scale * ks[h];
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[h][i] = c[i] * factor;
         }

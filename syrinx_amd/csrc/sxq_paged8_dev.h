@@ -68,16 +68,18 @@ struct Operand<I8, _Float16> {
     }
 };
 
-// A query's matrix type, and into how many bf16 parts its elements and the weights are cut.
+// A query's matrix type, and into how many parts its elements are cut: an f32 row, times the power of two
+// that takes its largest element to 2^14 .. 2^15, into two of f16 (off by at most 2^-22 of the element, or
+// 2^-39 of the row's largest).
 template <typename TQ>
 struct Query {
     typedef TQ M;
-    static constexpr int kQP = 1, kWP = 2;
+    static constexpr int kQP = 1;
 };
 template <>
 struct Query<float> {
-    typedef __bf16 M;
-    static constexpr int kQP = 3, kWP = 3;
+    typedef _Float16 M;
+    static constexpr int kQP = 2;
 };
 template <typename M>
 struct Vec8;
@@ -90,29 +92,49 @@ struct Vec8<_Float16> {
     typedef v8h T;
 };
 
-// Eight elements of a query as QP operands of 8 (parts of an f32 element sum to it exactly; what
-// passes bf16's range is infinite, its further parts zero).
-template <typename TQ, int QP>
-SXQ_DEV void query_parts(const TQ* src, bool in, v4u (&out)[QP]) {
-    if constexpr (QP == 1) {
-        const v4u v = *(const v4u*)src;
+// The operands of one lane's share of a row, N times eight elements from q + cols[i] on (in[i]: within the
+// head), and what the row's products are to be multiplied by.  all_lanes takes a lane's largest to the
+// row's.
+template <typename TQ, int N, typename V8, typename Reduce>
+SXQ_DEV float load_query(const TQ* q, const int (&cols)[N], const bool (&in)[N], V8 (&out)[Query<TQ>::kQP][N], Reduce all_lanes) {
+    if constexpr (Query<TQ>::kQP == 1) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) out[0][e] = in ? v[e] : 0;
+        for (int i = 0; i < N; ++i) {
+            v4u v = *(const v4u*)(q + (in[i] ? cols[i] : 0));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = in[i] ? v[e] : 0;
+            out[0][i] = __builtin_bit_cast(V8, v);
+        }
+        return 1.0f;
     } else {
-        float f[8];
-        *(v4f*)f = *(const v4f*)src;
-        *(v4f*)(f + 4) = *(const v4f*)(src + 4);
+        float f[N][8], most = 0.0f;
 #pragma unroll
-        for (int q = 0; q < QP; ++q) {
-            v8bf part;
+        for (int i = 0; i < N; ++i) {
+            const TQ* src = q + (in[i] ? cols[i] : 0);
+            *(v4f*)f[i] = *(const v4f*)src;
+            *(v4f*)(f[i] + 4) = *(const v4f*)(src + 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                part[e] = (__bf16)(in ? f[e] : 0.0f);
-                const float p = (float)part[e];
-                f[e] = fabsf(p) < INFINITY ? f[e] - p : p == p ? 0.0f : p;
+                f[i][e] = in[i] ? f[i][e] : 0.0f;
+                const float a = fabsf(f[i][e]);
+                most = a < INFINITY ? fmaxf(most, a) : most;
             }
-            out[q] = __builtin_bit_cast(v4u, part);
         }
+        most = all_lanes(most);
+        // 2^(14 - E) of the largest, 2^E and up (E at least -112, which 2^126 takes to 2^14)
+        const int up = 14 - max((int)(__float_as_uint(most) >> 23) - 127, -112);
+        const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float v = f[i][e] * by;
+                const _Float16 hi = (_Float16)v;
+                out[0][i][e] = hi;
+                const float rest = v - (float)hi;
+                out[1][i][e] = (_Float16)(rest == rest ? rest : 0.0f);  // (an infinity has none)
+            }
+        return __uint_as_float((uint32_t)(127 - up) << 23);
     }
 }
 

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/sxq.h"
 #include "sxq_abi.h"
@@ -202,14 +203,25 @@ constexpr int kWeightParts<_Float16> = 2;
 template <>
 constexpr int kWeightParts<float> = 3;
 
+// A tile of keys and values in LDS, 16-bit: keys [key][element], values [column][key], the 16-byte pieces of
+// a row exchanged so that those of neighbouring rows lie on different banks.
 template <int HDP>
 struct Stage {
     static constexpr int kKeys = keys_a_tile(HDP), kBlocks = kKeys / kScaleBlock;
-    __attribute__((aligned(16))) uint16_t k[kKeys * HDP];  // [key][element], 16-byte pieces exchanged within a row
-    __attribute__((aligned(16))) uint16_t v[HDP * kKeys];  // [column][key], the same
-    float ks[kBlocks], vs[kBlocks];                         // scales of the blocks of 16 keys
-    int absent[kBlocks];                                          // whether each block is
+    __attribute__((aligned(16))) uint16_t k[kKeys * HDP], v[HDP * kKeys];
 };
+template <int HDP>
+SXQ_DEV int k_swap(int key) {
+    return HDP == 64 ? key >> 1 & 7 : key & 15;
+}
+template <int HDP>
+SXQ_DEV int v_swap(int col) {
+    return keys_a_tile(HDP) == 64 ? (col >> 1 & 7) ^ (col >> 4 & 1) : col >> 2 & 3;
+}
+
+// Whether a scale may go into its weights' exponents: they then stay above what is flushed to zero down
+// to 2^-66 of the largest, and below infinity.
+SXQ_DEV bool plain_scale(float s) { return s >= 0x1p-60f && s < 0x1p100f; }
 
 // The first key of each column whose value is NaN.
 template <int HDP>
@@ -217,28 +229,24 @@ struct Nans {
     int first[HDP], any;
 };
 
-// Where a 16-byte piece of a row lies: the pieces of neighbouring rows on different banks.
-template <int HDP>
-SXQ_DEV int k_piece(int key, int piece) {
-    return HDP == 64 ? piece ^ ((key >> 1) & 7) : piece ^ (key & 15);
-}
-template <int HDP>
-SXQ_DEV int v_piece(int col, int piece) {
-    return keys_a_tile(HDP) == 64 ? piece ^ ((col >> 1) & 7) ^ ((col >> 4) & 1) : piece ^ ((col >> 2) & 3);
-}
-
+// Tiles of 128 rows: a wave has 32 of them, its queries and weighted values in registers; the keys and
+// values of a tile of keys are widened to 16 bits once for all of them, through LDS, two stages in turn,
+// the next tile's codes under way in registers meanwhile.  Scores: A = 32 keys x 16 elements, B = the
+// queries' elements x 32 rows, so that a lane has one row's scores for half of the keys (8 (i / 4) +
+// 4 (lane / 32) + i % 4) and the softmax of a row is two lanes'; weighted values: A = 32 columns x 16 keys,
+// B = the weights in the registers that the scores came in, the values' keys laid out in LDS to match.
+// What bounds it: the matrix cores' products and the lanes' work on the weights (an exponential, the
+// maximum, the sum, the rounding) take turns on a SIMD's two waves.
 template <typename TQ, typename C, int HDP, bool FULL>
-__global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) void k_kv8_prefix(const KvAttend A, const int32_t* pos, const KvPool P,
-                                                                       const Geometry geo) {
+__global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) void k_kv8_prefix(const KvAttend A, const int32_t* pos,
+                                                                                                 const KvPool P, const Geometry geo) {
     typedef typename Query<TQ>::M M;
     typedef typename Vec8<M>::T V8;
     constexpr int QP = Query<TQ>::kQP, WP = kWeightParts<TQ>;
-    constexpr int KS = HDP / 16, CT = HDP / 32;             // steps over the head's elements, tiles of 32 columns
+    constexpr int KS = HDP / 16, CT = HDP / 32;  // steps over the head's elements, tiles of 32 columns
     constexpr int kKeys = Stage<HDP>::kKeys, NB = Stage<HDP>::kBlocks, KT = kKeys / 32;
-    constexpr int KP = kKeys * HDP / 16 / 256;              // 16-code pieces of keys a thread stages
-    constexpr int VPieces = kKeys / 8 * (HDP / 4);          // 8-key x 4-column pieces of values
-    constexpr int VP = VPieces > 256 ? VPieces / 256 : 1;   // a thread's
-    constexpr bool VALL = VPieces >= 256;
+    constexpr int kRowPieces = HDP / 16, KP = kKeys * kRowPieces / 256;  // pieces of 16 codes a key; a thread's
+    constexpr int VE = HDP == 64 ? 4 : 8;                                // keys of a thread's piece of values (by 4 columns)
     __shared__ Stage<HDP> stage[2];
     __shared__ Nans<HDP> s_nans[2];  // of this item and the last
 
@@ -246,7 +254,7 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
     const int col32 = lane & 31, hf = lane >> 5;
     const int hd = FULL ? HDP : P.hd;
     const PrefixPlan plan(A.ws, A.n_q, hd, geo);
-    const int items = plan.counts[0];
+    const int items = __builtin_amdgcn_readfirstlane(plan.counts[0]);
     // (a negative scale is the positive one over negated queries: the running maximum wants factors
     // of 0 or more)
     const float scale2 = fabsf(A.scale) * 1.44269504088896340736f;
@@ -254,8 +262,19 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
     const uint32_t ps = (uint32_t)P.pos_stride;
     const int log_p = P.shift - kScaleShift, block_mask = (P.page >> kScaleShift) - 1;
 
-    // long items first: of one request the last queries see the most
+    // What this thread stages.  Keys: 16 codes of keys kkey + 32 j (256 threads to 64, 32 or 16 keys at
+    // once), of a block of 16 keys that is the wave's; values: 4 columns of VE keys of one block, those of
+    // an operand's piece (16 u + 4 f + {0..3, 8..11}) or half of it.
+    const int kkey = tid / kRowPieces, kc = 16 * (tid % kRowPieces);
+    constexpr int kStep = 256 / kRowPieces;  // keys between a thread's pieces
+    const int kblock = wave * (64 / kRowPieces) / 16;
+    const int vu = HDP == 256 ? wave >> 1 : wave, vf = HDP == 256 ? wave & 1 : HDP == 128 ? hf : lane >> 4 & 1;
+    const int vc = 4 * (HDP == 256 ? lane : HDP == 128 ? col32 : lane & 15), vhalf = HDP == 64 ? hf : 0;
+    const bool kin = FULL || kc < hd, vin = FULL || vc < hd;
+    const uint32_t koff = (uint32_t)(kkey & 15) * ps + (kin ? kc : 0), voff = (uint32_t)(4 * vf + 8 * vhalf) * ps + (vin ? vc : 0);
+
     int turn = 0;
+    // long items first: of one request the last queries see the most
     for (int64_t w = blockIdx.x; w < (int64_t)items * geo.units; w += gridDim.x) {
         Nans<HDP>* const nans = &s_nans[turn++ & 1];
         if constexpr (C::kNan) {  // (its readers were done before the last item's first barrier)
@@ -264,11 +283,17 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
         }
         const int unit = (int)(w % geo.units), kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
         const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0);
-        const TileItem it = plan.item[items - 1 - (int)(w / geo.units)];
-        const int n_rows = it.count * heads;
+        TileItem it = plan.item[items - 1 - (int)(w / geo.units)];
+        it.row = __builtin_amdgcn_readfirstlane(it.row);
+        it.limit = __builtin_amdgcn_readfirstlane(it.limit);
+        it.first = __builtin_amdgcn_readfirstlane(it.first);
+        it.end = __builtin_amdgcn_readfirstlane(it.end);
+        const int n_rows = __builtin_amdgcn_readfirstlane(it.count) * heads;
         const int32_t* table = A.table + (int64_t)it.row * A.table_stride;
         const char* kpool = (const char*)P.k + (int64_t)kh * P.head_stride;
         const char* vpool = (const char*)P.v + (int64_t)kh * P.head_stride;
+        const float* kscale = P.k_scale + (int64_t)kh * P.scale_head_stride;
+        const float* vscale = P.v_scale + (int64_t)kh * P.scale_head_stride;
 
         // this lane's row of the wave's 32: its query, head and limit
         const int rho = min(wave * 32 + col32, n_rows - 1), tok = it.token + rho / heads, head = h0 + rho % heads;
@@ -284,121 +309,132 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
         const bool idle = wave * 32 >= n_rows;
 
         V8 qreg[QP][KS];
+        float row_scale;
         {
-            const TQ* q = (const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd;
+            int qcol[KS];
+            bool qin[KS];
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                const int col = 16 * s + 8 * hf;
-                const bool in = FULL || col < hd;
-                v4u parts[QP];
-                query_parts<TQ, QP>(q + (in ? col : 0), in, parts);
-#pragma unroll
-                for (int p = 0; p < QP; ++p) {
-                    parts[p] ^= flip;
-                    qreg[p][s] = __builtin_bit_cast(V8, parts[p]);
-                }
+                qcol[s] = 16 * s + 8 * hf;
+                qin[s] = FULL || qcol[s] < hd;
             }
+            row_scale = scale2 * load_query<TQ>((const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd, qcol, qin, qreg,
+                                                [](float v) { return fmaxf(v, other_half(v)); });
+#pragma unroll
+            for (int p = 0; p < QP; ++p)
+#pragma unroll
+                for (int s = 0; s < KS; ++s) qreg[p][s] = __builtin_bit_cast(V8, __builtin_bit_cast(v4u, qreg[p][s]) ^ flip);
         }
 
-        // what this thread stages of a tile of keys: pieces of 16 codes of one key, and of 4 columns
-        // by the 8 keys of one operand piece (keys 16 u + 4 f + {0..3, 8..11})
-        uint32_t kcode[KP][4], vcode[VP][8];
-        float sc = 0.0f;
-        int block_id = -1;
-        auto page_of = [&](int block) {  // of a block of 16 keys
+        // Lane j: the page (-1: absent) and scales of block j of a batch of 64 blocks of 16 keys, so that a
+        // tile's addresses are scalar and wait for no load; the next batch is loaded when one begins.
+        const int blocks = (it.limit + kScaleBlock - 1) >> kScaleShift, b0 = it.first * NB;
+        auto page_batch = [&](int batch) {
+            const int b = b0 + 64 * batch + lane;
             int id = -1;
-            if (block * 16 < it.limit) id = table[block >> log_p];
+            if (b < blocks) id = table[b >> log_p];
             return kv_page_ok(id, P.n_pages) ? id : -1;
         };
-        int kid[KP], vid[VP], sid = -1;  // pages of the next tile to load
-        auto load_ids = [&](int tile) {
-#pragma unroll
-            for (int j = 0; j < KP; ++j) kid[j] = page_of(tile * NB + (tid + 256 * j) / (HDP / 16) / 16);
-#pragma unroll
-            for (int j = 0; j < VP; ++j) vid[j] = page_of(tile * NB + ((tid + 256 * j) / (HDP / 4) & (2 * NB - 1)) / 2);
-            if (tid < 2 * NB) sid = page_of(tile * NB + (tid & (NB - 1)));
+        auto scale_batch = [&](const float* scales, int batch, int id) {
+            float s = 1.0f;
+            if (id >= 0) s = scales[(int64_t)id * P.scale_page_stride + ((b0 + 64 * batch + lane) & block_mask)];
+            return s;
         };
+        int pages = page_batch(0), pages_next = -1, batch = 0, at = 0;  // at: the next tile's first block in the batch
+        float ks_lane = scale_batch(kscale, 0, pages), vs_lane = scale_batch(vscale, 0, pages), ks_next = 1.0f, vs_next = 1.0f;
+        if (blocks > b0 + 64) pages_next = page_batch(1);  // (later ones: -1 past the last block)
+
+        uint32_t kcode[KP][4], vcode[VE];
+        float ks[NB], vs[NB], ks_load[NB], vs_load[NB];  // of the tile at hand, and of the one that is loaded
+        float value_scale = 1.0f;  // of the block whose values this thread stages
+        int absent = 0, absent_load = 0;
+        // Codes of a tile under way.  Absent blocks' keys are masked, their values have to be zeros.
         auto load_codes = [&](int tile) {
-            int tid = threadIdx.x;
-            asm volatile("" : "+v"(tid));
-            const int key0 = tile * kKeys;
+            if (at == 64) {
+                at = 0;
+                ++batch;
+                pages = pages_next;
+                ks_lane = ks_next;
+                vs_lane = vs_next;
+                pages_next = page_batch(batch + 1);
+            } else if (at == 2 * NB) {
+                ks_next = scale_batch(kscale, batch + 1, pages_next);
+                vs_next = scale_batch(vscale, batch + 1, pages_next);
+            }
+            auto page = [&](int b) { return __builtin_amdgcn_readlane(pages, at + b); };
+            auto offset = [&](int b, int id) {
+                return (int64_t)max(id, 0) * P.page_stride + (int64_t)((uint32_t)((tile * NB + b) & block_mask) * (uint64_t)(kScaleBlock * ps));
+            };
 #pragma unroll
             for (int j = 0; j < KP; ++j) {
-                const int piece = tid + 256 * j, key = piece / (HDP / 16), c = 16 * (piece % (HDP / 16));
-                const int off = (key0 + key) & (P.page - 1);
-                v4u v = {0, 0, 0, 0};
-                if (kid[j] >= 0 && (FULL || c < hd)) v = *(const v4u*)(kpool + (int64_t)kid[j] * P.page_stride + (uint64_t)off * ps + c);
+                const int b = kblock + j * kStep / 16;
+                const v4u v = *(const v4u*)(kpool + offset(b, page(b)) + koff);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) kcode[j][e] = v[e];
             }
+            const int id = page(vu);
+            const char* src = vpool + offset(vu, id);
 #pragma unroll
-            for (int j = 0; j < VP; ++j) {
-                const int piece = tid + 256 * j, c = 4 * (piece % (HDP / 4)), o = piece / (HDP / 4) & (2 * NB - 1);  // o = 2 u + f
-                const int key = 16 * (o >> 1) + 4 * (o & 1), off = (key0 + key) & (P.page - 1);
-                const bool in = vid[j] >= 0 && (FULL || c < hd);
-                const char* src = vpool + (int64_t)max(vid[j], 0) * P.page_stride + (uint64_t)off * ps + (in ? c : 0);
+            for (int e = 0; e < VE; ++e) vcode[e] = *(const uint32_t*)(src + ((e & 3) + 8 * (e >> 2)) * ps + voff);
+            absent_load = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int d = (e & 3) + 8 * (e >> 2);
-                    // what no query of the item sees may hold anything: zeros
-                    vcode[j][e] = in && key0 + key + d < it.limit ? *(const uint32_t*)(src + d * ps) : 0;
-                }
+            for (int b = 0; b < NB; ++b) {
+                ks_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks_lane), at + b));
+                vs_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs_lane), at + b));
+                if (b == vu) value_scale = vs_load[b];
+                if (!plain_scale(vs_load[b])) vs_load[b] = 1.0f;
+                absent_load |= page(b) < 0 ? 1 << b : 0;
             }
-            block_id = sid;
-            if (tid < 2 * NB && sid >= 0)
-                sc = (tid < NB ? P.k_scale : P.v_scale)[(int64_t)sid * P.scale_page_stride + (int64_t)kh * P.scale_head_stride +
-                                                       ((tile * NB + (tid & (NB - 1))) & block_mask)];
+            at += NB;
         };
         auto store_stage = [&](Stage<HDP>& S, int tile) {
-            int tid = threadIdx.x;
-            asm volatile("" : "+v"(tid));
 #pragma unroll
             for (int j = 0; j < KP; ++j) {
-                const int piece = tid + 256 * j, key = piece / (HDP / 16), c = 2 * (piece % (HDP / 16));
-                uint16_t* row = S.k + key * HDP;
-                *(v4u*)(row + 8 * k_piece<HDP>(key, c)) = Operand<C, M>::eight(kcode[j][0], kcode[j][1]);
-                *(v4u*)(row + 8 * k_piece<HDP>(key, c + 1)) = Operand<C, M>::eight(kcode[j][2], kcode[j][3]);
+                const int key = kkey + kStep * j;
+                if constexpr (!FULL)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) kcode[j][e] = kin ? kcode[j][e] : 0;
+                const int piece = kc / 8;
+                *(v4u*)(S.k + key * HDP + 8 * (piece ^ k_swap<HDP>(key))) = Operand<C, M>::eight(kcode[j][0], kcode[j][1]);
+                *(v4u*)(S.k + key * HDP + 8 * ((piece + 1) ^ k_swap<HDP>(key))) = Operand<C, M>::eight(kcode[j][2], kcode[j][3]);
             }
+            if (absent_load >> vu & 1 || !vin)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) vcode[e] = 0;
             if constexpr (C::kNan) {
                 // A NaN belongs to the rows that see its key, and a weight of zero would not keep it
                 // from the others: a zero in its place, and its column's first such key noted.
                 uint32_t found = 0;  // (0x7F is the only byte that one more takes to 0x80)
 #pragma unroll
-                for (int j = 0; j < VP; ++j)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) found |= (vcode[j][e] & 0x7F7F7F7Fu) + 0x01010101u;
+                for (int e = 0; e < VE; ++e) found |= (vcode[e] & 0x7F7F7F7Fu) + 0x01010101u;
                 if (found & 0x80808080u) {
 #pragma unroll
-                    for (int j = 0; j < VP; ++j) {
-                        const int piece = tid + 256 * j, c = 4 * (piece % (HDP / 4)), o = piece / (HDP / 4) & (2 * NB - 1);
+                    for (int e = 0; e < VE; ++e)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-#pragma unroll
-                            for (int b = 0; b < 4; ++b)
-                                if ((vcode[j][e] >> (8 * b) & 0x7F) == 0x7F) {
-                                    vcode[j][e] &= ~(0xFFu << (8 * b));
-                                    atomicMin(&nans->first[c + b], tile * kKeys + 16 * (o >> 1) + 4 * (o & 1) + (e & 3) + 8 * (e >> 2));
-                                    nans->any = 1;
-                                }
-                    }
+                        for (int b = 0; b < 4; ++b)
+                            if ((vcode[e] >> (8 * b) & 0x7F) == 0x7F) {
+                                vcode[e] &= ~(0xFFu << (8 * b));
+                                atomicMin(&nans->first[vc + b], tile * kKeys + 16 * vu + 4 * vf + 8 * vhalf + (e & 3) + 8 * (e >> 2));
+                                nans->any = 1;
+                            }
                 }
             }
+            uint32_t out[VE / 2][4];  // [pair of keys][column]
 #pragma unroll
-            for (int j = 0; j < VP; ++j) {
-                const int piece = tid + 256 * j, c = 4 * (piece % (HDP / 4)), o = piece / (HDP / 4);
-                if (!VALL && o >= 2 * NB) break;
-                uint32_t out[4][4];  // [pair of keys][column]
+            for (int e = 0; e < VE / 2; ++e) Operand<C, __bf16>::columns(vcode[2 * e], vcode[2 * e + 1], out[e]);
+            if (!plain_scale(value_scale))  // into the values instead
 #pragma unroll
-                for (int e = 0; e < 4; ++e) Operand<C, __bf16>::columns(vcode[j][2 * e], vcode[j][2 * e + 1], out[e]);
+                for (int e = 0; e < VE / 2; ++e)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    *(v4u*)(S.v + (c + e) * kKeys + 8 * v_piece<HDP>(c + e, o)) = (v4u){out[0][e], out[1][e], out[2][e], out[3][e]};
-            }
-            if (tid < NB) {
-                S.ks[tid] = block_id >= 0 ? sc : 0.0f;
-                S.absent[tid] = block_id < 0;
-            } else if (tid < 2 * NB) {
-                S.vs[tid - NB] = block_id >= 0 ? sc : 0.0f;
+                    for (int c = 0; c < 4; ++c) {
+                        const float lo = __uint_as_float(out[e][c] << 16) * value_scale, hi = __uint_as_float(out[e][c] & 0xFFFF0000u) * value_scale;
+                        out[e][c] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302);
+                    }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint16_t* to = S.v + (vc + c) * kKeys + 8 * ((2 * vu + vf) ^ v_swap<HDP>(vc + c)) + 4 * vhalf;
+                if constexpr (VE == 8) *(v4u*)to = (v4u){out[0][c], out[1][c], out[2][c], out[3][c]};
+                else *(v2u*)to = (v2u){out[0][c], out[1][c]};
             }
         };
 
@@ -409,128 +445,128 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
             for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
         float m = -INFINITY, l = 0.0f;
 
-        if (it.first < it.end) {
-            load_ids(it.first);
-            load_codes(it.first);
-            if (it.first + 1 < it.end) load_ids(it.first + 1);
-        }
-        __syncthreads();  // the last item's readers are done with the stages
-        if (it.first < it.end) store_stage(stage[0], it.first);
-        __syncthreads();
-        for (int tile = it.first; tile < it.end; ++tile) {
-            const Stage<HDP>& S = stage[(tile - it.first) & 1];
-            const bool more = tile + 1 < it.end;
-            if (more) {
-                load_codes(tile + 1);
-                if (tile + 2 < it.end) load_ids(tile + 2);
-            }
-            const int key0 = tile * kKeys;
-            int col32 = lane & 31, hf = lane >> 5;
-            asm volatile("" : "+v"(col32), "+v"(hf));
-            if (!idle && key0 < most) {
-                v16f c[KT];
+        auto take = [&]() {  // the tile that was loaded is the one at hand
+            absent = absent_load;
 #pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
+            for (int b = 0; b < NB; ++b) ks[b] = ks_load[b], vs[b] = vs_load[b];
+        };
+        auto compute = [&](const Stage<HDP>& S, int key0) {
+            v16f c[KT];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) c[kt][i] = 0.0f;
-                {
-                    // operands four ahead, and no further: the scheduler would take them all at once,
-                    // and spill
-                    V8 a[2][4];
-                    auto fetch = [&](int n) {
+            for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int kt = (4 * n + j) / KS, st = (4 * n + j) % KS, key = 32 * kt + col32;
-                            a[n & 1][j] = *(const V8*)(S.k + key * HDP + 8 * k_piece<HDP>(key, 2 * st + hf));
-                        }
-                    };
-                    fetch(0);
+                for (int i = 0; i < 16; ++i) c[kt][i] = 0.0f;
+            const uint16_t* krow = S.k + col32 * HDP;  // (32 keys on, the same exchange)
+            const int kx = k_swap<HDP>(col32) ^ hf;
+            {
+                // operands four ahead and no further: the scheduler would take them all at once, and spill
+                V8 a[2][4];
+                auto fetch = [&](int n) {
 #pragma unroll
-                    for (int n = 0; n < KT * KS / 4; ++n) {
-                        if (n + 1 < KT * KS / 4) fetch(n + 1);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int kt = (4 * n + j) / KS, st = (4 * n + j) % KS;
-#pragma unroll
-                            for (int p = QP - 1; p >= 0; --p) c[kt] = mfma32(a[n & 1][j], qreg[p][st], c[kt]);  // the small parts first
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
+                    for (int j = 0; j < 4; ++j) {
+                        const int s = (4 * n + j) / KT, kt = (4 * n + j) % KT;
+                        a[n & 1][j] = *(const V8*)(krow + 32 * kt * HDP + 8 * (kx ^ (2 * s)));
                     }
-                }
-                float factor[NB], vs[NB];
-                int absent = 0;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    factor[b] = scale2 * S.ks[b];
-                    vs[b] = S.vs[b];
-                    absent |= S.absent[b];
-                }
-                float mx = -INFINITY;
-                if (key0 + kKeys > least || __builtin_amdgcn_readfirstlane(absent)) {
-#pragma unroll
-                    for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int key = key0 + 32 * kt + 8 * (i >> 2) + 4 * hf + (i & 3);
-                            const float x = c[kt][i] * factor[2 * kt + (i >> 3)];
-                            c[kt][i] = key < limit && !S.absent[2 * kt + (i >> 3)] ? x : -INFINITY;
-                            mx = fmaxf(mx, c[kt][i]);
-                        }
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) factor[b] = 1.0f;
-                } else {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        float top = c[b >> 1][8 * (b & 1)];
-#pragma unroll
-                        for (int i = 1; i < 8; ++i) top = fmaxf(top, c[b >> 1][8 * (b & 1) + i]);
-                        mx = fmaxf(mx, top * factor[b]);
-                    }
-                }
-                // the running maximum moves only where a score passes it
-                if (__any(mx > m)) {
-                    const float mn = fmaxf(m, fmaxf(mx, other_half(mx)));
-                    const float al = m > -INFINITY ? exp2_fast(m - mn) : 1.0f;  // nothing but zeros before
-                    l *= al;
-#pragma unroll
-                    for (int d = 0; d < CT; ++d) acc[d] *= al;
-                    m = mn;
-                }
-                const float base = m > -INFINITY ? m : 0.0f;
-                v8bf part[WP][NB];
-#pragma unroll
-                for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int b = 2 * kt + (i >> 3);
-                        float w = exp2_fast(fmaf(c[kt][i], factor[b], -base));
-                        l += w;
-                        w *= vs[b];
-#pragma unroll
-                        for (int p = 0; p < WP; ++p) {
-                            part[p][b][i & 7] = (__bf16)w;
-                            w -= (float)part[p][b][i & 7];
-                        }
-                    }
-                v8bf a[2][NB];
-                auto fetch = [&](int d) {
-                    const int col = 32 * d + col32;
-#pragma unroll
-                    for (int u = 0; u < NB; ++u) a[d & 1][u] = *(const v8bf*)(S.v + col * kKeys + 8 * v_piece<HDP>(col, 2 * u + hf));
                 };
                 fetch(0);
 #pragma unroll
-                for (int d = 0; d < CT; ++d) {
-                    if (d + 1 < CT) fetch(d + 1);
+                for (int n = 0; n < KS * KT / 4; ++n) {
+                    if (n + 1 < KS * KT / 4) fetch(n + 1);
 #pragma unroll
-                    for (int u = 0; u < NB; ++u)
+                    for (int p = QP - 1; p >= 0; --p)  // the small part first
 #pragma unroll
-                        for (int p = WP - 1; p >= 0; --p) acc[d] = mfma32(a[d & 1][u], part[p][u], acc[d]);
+                        for (int j = 0; j < 4; ++j) c[(4 * n + j) % KT] = mfma32(a[n & 1][j], qreg[p][(4 * n + j) / KT], c[(4 * n + j) % KT]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (more) store_stage(stage[(tile + 1 - it.first) & 1], tile + 1);
+            float factor[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) factor[b] = row_scale * ks[b];
+            float mx = -INFINITY;
+            if (key0 + kKeys > least || absent) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int key = key0 + 16 * b + 8 * (i >> 2) + 4 * hf + (i & 3);
+                        const float x = c[b >> 1][8 * (b & 1) + i] * factor[b];
+                        c[b >> 1][8 * (b & 1) + i] = key < limit && !(absent >> b & 1) ? x : -INFINITY;
+                        mx = fmaxf(mx, c[b >> 1][8 * (b & 1) + i]);
+                    }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) factor[b] = 1.0f;
+            } else {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float top = c[b >> 1][8 * (b & 1)];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) top = fmaxf(top, c[b >> 1][8 * (b & 1) + i]);
+                    mx = fmaxf(mx, top * factor[b]);
+                }
+            }
+            // the running maximum moves only where a score passes it
+            if (__any(mx > m)) {
+                const float mn = fmaxf(m, fmaxf(mx, other_half(mx)));
+                const float al = m > -INFINITY ? exp2_fast(m - mn) : 1.0f;  // nothing but zeros before
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < CT; ++d) acc[d] *= al;
+                m = mn;
+            }
+            const float base = m > -INFINITY ? m : 0.0f;
+            const uint16_t* vrow = S.v + col32 * kKeys;  // (32 columns on, the same exchange)
+            const int vx = v_swap<HDP>(col32) ^ hf;
+            v8bf a[2][CT];
+            auto fetch = [&](int u) {
+#pragma unroll
+                for (int d = 0; d < CT; ++d) a[u & 1][d] = *(const v8bf*)(vrow + 32 * d * kKeys + 8 * (vx ^ (2 * u)));
+            };
+            fetch(0);
+#pragma unroll
+            for (int u = 0; u < NB; ++u) {
+                if (u + 1 < NB) fetch(u + 1);
+                // the weights of a block of 16 keys times its values' scale, which goes into the exponent;
+                // the row's sum takes it out again
+                const float back = base - __builtin_amdgcn_logf(vs[u]);
+                v8bf part[WP];
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float x = exp2_fast(fmaf(c[u >> 1][8 * (u & 1) + j], factor[u], -back));
+                    sum += x;
+#pragma unroll
+                    for (int p = 0; p < WP; ++p) {
+                        part[p][j] = (__bf16)x;
+                        x -= (float)part[p][j];
+                    }
+                }
+                l = fmaf(sum, __builtin_amdgcn_rcpf(vs[u]), l);
+#pragma unroll
+                for (int p = WP - 1; p >= 0; --p)
+#pragma unroll
+                    for (int d = 0; d < CT; ++d) acc[d] = mfma32(a[u & 1][d], part[p], acc[d]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+
+        if (it.first < it.end) load_codes(it.first);
+        __syncthreads();  // the last item's readers are done with the stages
+        if (it.first < it.end) store_stage(stage[0], it.first);
+        take();
+        __syncthreads();
+        auto step = [&](const Stage<HDP>& S, Stage<HDP>& next, int tile) {
+            const bool more = tile + 1 < it.end;
+            if (more) load_codes(tile + 1);
+            if (!idle && tile * kKeys < most) compute(S, tile * kKeys);
+            if (more) {
+                store_stage(next, tile + 1);
+                take();
+            }
             __syncthreads();
+        };
+        for (int tile = it.first; tile < it.end; tile += 2) {
+            step(stage[0], stage[1], tile);
+            if (tile + 1 < it.end) step(stage[1], stage[0], tile + 1);
         }
         l += other_half(l);
         if constexpr (C::kNan)
@@ -594,25 +630,22 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(cons
     }
 
     // this lane's rows (those past the last repeat it)
-    int limit[NR], least = INT32_MAX;
-    V8 qreg[QP][NR][KS][2];
+    int limit[NR], least = INT32_MAX, qcol[2 * KS];
+    bool qin[2 * KS];
+#pragma unroll
+    for (int s = 0; s < 2 * KS; ++s) {
+        qcol[s] = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+        qin[s] = FULL || qcol[s] < hd;
+    }
+    V8 qreg[NR][QP][2 * KS];
+    float row_scale[NR];
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
         const int rho = min(16 * n + r, n_rows - 1), tok = it.token + rho / heads, head = h0 + rho % heads;
         limit[n] = seen(A, pos, P, tok, it.row);
         least = min(least, limit[n]);
-        const TQ* q = (const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd;
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-                const int col = 64 * s + 16 * g + 8 * f;
-                const bool in = FULL || col < hd;
-                v4u parts[QP];
-                query_parts<TQ, QP>(q + (in ? col : 0), in, parts);
-#pragma unroll
-                for (int p = 0; p < QP; ++p) qreg[p][n][s][f] = __builtin_bit_cast(V8, parts[p]);
-            }
+        row_scale[n] = scale2 * load_query<TQ>((const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd, qcol, qin, qreg[n],
+                                               [](float v) { return head_max(v); });
     }
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
@@ -735,15 +768,14 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(cons
 #pragma unroll
                     for (int p = QP - 1; p >= 0; --p)  // the small parts first
 #pragma unroll
-                        for (int n = 0; n < NR; ++n) c[n] = mfma16(key, qreg[p][n][s][f], c[n]);
+                        for (int n = 0; n < NR; ++n) c[n] = mfma16(key, qreg[n][p][2 * s + f], c[n]);
                 }
             }
-            const float factor = scale2 * ks[h];
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[n][h][i] = c[n][i] * factor;
+                    x[n][h][i] = c[n][i] * (row_scale[n] * ks[h]);
                     if (partial && (!okh[h] || (t + h) * 16 + 4 * g + i >= limit[n])) x[n][h][i] = -INFINITY;
                 }
         }
