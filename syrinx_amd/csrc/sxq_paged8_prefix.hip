@@ -31,6 +31,8 @@ constexpr int kWideRows = 128, kFewRows = 32;
 constexpr int kFewKeys = 128;  // a tile of keys: 32 a wave
 SXQ_HD constexpr int keys_a_tile(int hd) { return hd <= 128 ? 64 : 32; }  // wide (registers)
 
+constexpr int kRounds = 4;  // with so many tiles a place, or more, none is cut
+
 struct Geometry {
     int rows, keys;                   // of a tile
     int group, parts, units, tokens;  // heads a KV head; parts of a group; units; tokens a tile
@@ -42,7 +44,7 @@ struct Geometry {
         parts = (group + rows - 1) / rows;
         units = nkv * parts;
         tokens = group < rows ? rows / group : 1;
-        const int all = hd <= (f32 ? 64 : 128) ? 512 : 256;
+        const int all = hd <= 128 ? 512 : 256;
         places = units < all ? all / units : 1;
         min_piece = few ? 1 : 4;
     }
@@ -66,7 +68,7 @@ struct PrefixPlan {
     SXQ_HD static size_t up(size_t v) { return (v + 255) / 256 * 256; }
     SXQ_HD PrefixPlan(void* ws, int n_q, int hd, const Geometry& g) {
         char* p = (char*)ws;
-        const int most = n_q + g.places;  // items: a tile each, and pieces up to the places
+        const int most = n_q + 2 * g.places;  // items: a tile each, and the pieces of cut ones
         counts = (int*)p;
         p += 256;
         item = (TileItem*)p;
@@ -74,20 +76,20 @@ struct PrefixPlan {
         cut = (int2*)p;
         p += up(sizeof(int2) * (size_t)g.places);
         partial = (float*)p;
-        p += (size_t)g.places * g.units * part_floats(g.rows, hd) * sizeof(float);
+        p += 2 * (size_t)g.places * g.units * part_floats(g.rows, hd) * sizeof(float);
         bytes = (size_t)(p - (char*)ws);
     }
     SXQ_HD static size_t part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 };
 
-// The positions that query t sees, and whether it has a request.
+// The positions that a query sees, of its request's length and its position.
+SXQ_DEV int seen_of(int len, int pos, int max_blocks, int shift) { return min(kv_clamp_len(len, max_blocks, shift), max(pos, -1) + 1); }
 SXQ_DEV int seen(const KvAttend& A, const int32_t* pos, const KvPool& P, int t, int row) {
-    const int len = kv_clamp_len(A.lens[row], A.max_blocks, P.shift);
-    return min(len, max(pos[t], -1) + 1);
+    return seen_of(A.lens[row], pos[t], A.max_blocks, P.shift);
 }
 
-// A thousand queries at a time, a thread each: where its run began and which of the chunk's tiles it is
-// in by ballots, the tiles' counts and limits in LDS.  Two loads in turn and three barriers a chunk.
+// A thousand queries at a time, a thread each (the next chunk's under way): where its run began and
+// which of the chunk's tiles it is in by ballots, the tiles' counts and limits in LDS.
 __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, const int32_t* pos, const KvPool P, const Geometry g,
                                                           bool may_cut) {
     __shared__ int s_wave[2][16], s_limit[1025], s_count[1025], s_token[1025], s_row[1025], s_cut;
@@ -96,11 +98,16 @@ __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, cons
     const uint64_t upto = ~(uint64_t)0 >> (63 - lane);
     if (tid == 0) s_cut = 0;
     int tiles = 0, run = 0;  // so far; where the run that reaches into the chunk began
+    int row_next = tid < A.n_q ? A.rows[tid] : -1, before_next = tid > 0 && tid < A.n_q ? A.rows[tid - 1] : -1;
+    int pos_next = tid < A.n_q ? pos[tid] : -1;
     for (int c0 = 0; c0 < A.n_q; c0 += 1024) {
-        const int t = c0 + tid;
-        const int row = t < A.n_q ? A.rows[t] : -1, before = t > 0 && t < A.n_q ? A.rows[t - 1] : -1;
+        const int t = c0 + tid, row = row_next, before = before_next, at_pos = pos_next;
         const bool live = (uint32_t)row < (uint32_t)A.n_rows;
-        const int limit = live ? seen(A, pos, P, t, row) : 0;
+        const int len = live ? A.lens[row] : 0;
+        const int t2 = t + 1024;
+        row_next = t2 < A.n_q ? A.rows[t2] : -1;
+        before_next = t2 < A.n_q ? A.rows[t2 - 1] : -1;
+        pos_next = t2 < A.n_q ? pos[t2] : -1;
         for (int i = tid; i < 1025; i += 1024) s_limit[i] = s_count[i] = 0;
         const uint64_t begins = __ballot(t < A.n_q && (t == 0 || before != row));
         if (lane == 0) s_wave[0][wave] = begins ? c0 + 64 * wave + 63 - __builtin_clzll(begins) : -1;
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, cons
             count += s_wave[1][w];
         }
         if (live) {
-            atomicMax(&s_limit[at], limit);
+            atomicMax(&s_limit[at], seen_of(len, at_pos, A.max_blocks, P.shift));
             atomicAdd(&s_count[at], 1);
         }
         if (first) {
@@ -140,9 +147,10 @@ __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, cons
         tiles += count;
         __syncthreads();
     }
-    // pieces: at most g.places items in all where there are fewer tiles than that (a tile a thread)
+    // Pieces: where there are not many more tiles than places, those longer than a place's share are cut
+    // into such shares (a tile a thread).  No more than 2 * places pieces are of cut tiles.
     int items = tiles;
-    if (may_cut && tiles < g.places) {
+    if (may_cut && tiles <= 1024 && tiles < kRounds * g.places) {
         TileItem mine{};
         if (tid < tiles) {
             if (A.n_q <= 1024) mine = TileItem{s_token[tid + 1], s_count[tid + 1], s_row[tid + 1], s_limit[tid + 1], 0, (s_limit[tid + 1] + g.keys - 1) / g.keys, 0, 1};
@@ -160,16 +168,19 @@ __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, cons
             }
             return v + lower;
         };
-        int work;
-        scan(mine.end, 0, work);
-        const int piece = max(g.min_piece, (work + g.places - tiles - 1) / (g.places - tiles));
-        const int keys = mine.end, n = tid < tiles ? max(1, (keys + piece - 1) / piece) : 0;
-        const int at = scan(n, 1, items) - n;
+        int work, both;
+        scan(mine.end, 0, work);  // (2^30 positions a tile at most, 2^35 of all: 2^29 tiles of keys)
+        const int piece = max(g.min_piece, (work + g.places - 1) / g.places);
+        // (half as much again stays whole)
+        const int keys = mine.end, n = tid >= tiles ? 0 : 2 * keys > 3 * piece ? (keys + piece - 1) / piece : 1;
+        const int upto_me = scan(n + (n > 1 ? n << 16 : 0), 1, both);  // items, and those of cut tiles
+        items = both & 0xFFFF;
+        const int at = (upto_me & 0xFFFF) - n, part = (upto_me >> 16) - n;
         if (n > 1) plan.cut[atomicAdd(&s_cut, 1)] = make_int2(at, n);
         for (int k = 0; k < n; ++k) {
             mine.first = (int)((int64_t)keys * k / n);
             mine.end = (int)((int64_t)keys * (k + 1) / n);
-            mine.part = at + k;
+            mine.part = n > 1 ? part + k : 0;
             mine.pieces = n;
             plan.item[at + k] = mine;
         }
@@ -238,7 +249,7 @@ struct Nans {
 // What bounds it: the matrix cores' products and the lanes' work on the weights (an exponential, the
 // maximum, the sum, the rounding) take turns on a SIMD's two waves.
 template <typename TQ, typename C, int HDP, bool FULL>
-__global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) void k_kv8_prefix(const KvAttend A, const int32_t* pos,
+__global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const KvAttend A, const int32_t* pos,
                                                                                                  const KvPool P, const Geometry geo) {
     typedef typename Query<TQ>::M M;
     typedef typename Vec8<M>::T V8;
@@ -295,37 +306,6 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
         const float* kscale = P.k_scale + (int64_t)kh * P.scale_head_stride;
         const float* vscale = P.v_scale + (int64_t)kh * P.scale_head_stride;
 
-        // this lane's row of the wave's 32: its query, head and limit
-        const int rho = min(wave * 32 + col32, n_rows - 1), tok = it.token + rho / heads, head = h0 + rho % heads;
-        const int limit = seen(A, pos, P, tok, it.row);
-        int least = limit, most = limit;
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) {
-            least = min(least, __shfl_xor(least, o, 64));
-            most = max(most, __shfl_xor(most, o, 64));
-        }
-        least = __builtin_amdgcn_readfirstlane(least);
-        most = __builtin_amdgcn_readfirstlane(most);
-        const bool idle = wave * 32 >= n_rows;
-
-        V8 qreg[QP][KS];
-        float row_scale;
-        {
-            int qcol[KS];
-            bool qin[KS];
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                qcol[s] = 16 * s + 8 * hf;
-                qin[s] = FULL || qcol[s] < hd;
-            }
-            row_scale = scale2 * load_query<TQ>((const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd, qcol, qin, qreg,
-                                                [](float v) { return fmaxf(v, other_half(v)); });
-#pragma unroll
-            for (int p = 0; p < QP; ++p)
-#pragma unroll
-                for (int s = 0; s < KS; ++s) qreg[p][s] = __builtin_bit_cast(V8, __builtin_bit_cast(v4u, qreg[p][s]) ^ flip);
-        }
-
         // Lane j: the page (-1: absent) and scales of block j of a batch of 64 blocks of 16 keys, so that a
         // tile's addresses are scalar and wait for no load; the next batch is loaded when one begins.
         const int blocks = (it.limit + kScaleBlock - 1) >> kScaleShift, b0 = it.first * NB;
@@ -340,13 +320,23 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
             if (id >= 0) s = scales[(int64_t)id * P.scale_page_stride + ((b0 + 64 * batch + lane) & block_mask)];
             return s;
         };
+        // (loads that wait for each other first, so that the others are under way with them)
         int pages = page_batch(0), pages_next = -1, batch = 0, at = 0;  // at: the next tile's first block in the batch
         float ks_lane = scale_batch(kscale, 0, pages), vs_lane = scale_batch(vscale, 0, pages), ks_next = 1.0f, vs_next = 1.0f;
+        // the exponent that a value scale puts on its weights, and what takes it out of their sum
+        float lift_lane = 0.0f, back_lane = 1.0f;
+        bool odd_scales = false;
+        auto scales_at_hand = [&]() {
+            const bool plain = plain_scale(vs_lane);
+            lift_lane = plain ? __builtin_amdgcn_logf(vs_lane) : 0.0f;
+            back_lane = plain ? __builtin_amdgcn_rcpf(vs_lane) : 1.0f;
+            odd_scales = __any(!plain);
+        };
         if (blocks > b0 + 64) pages_next = page_batch(1);  // (later ones: -1 past the last block)
 
         uint32_t kcode[KP][4], vcode[VE];
-        float ks[NB], vs[NB], ks_load[NB], vs_load[NB];  // of the tile at hand, and of the one that is loaded
-        float value_scale = 1.0f;  // of the block whose values this thread stages
+        float ks[NB], lift[NB], back[NB], ks_load[NB], lift_load[NB], back_load[NB];  // of the tile at hand, and of the one that is loaded
+        float value_scale = 1.0f;  // what the values that this thread stages are to be multiplied by
         int absent = 0, absent_load = 0;
         // Codes of a tile under way.  Absent blocks' keys are masked, their values have to be zeros.
         auto load_codes = [&](int tile) {
@@ -357,6 +347,7 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
                 ks_lane = ks_next;
                 vs_lane = vs_next;
                 pages_next = page_batch(batch + 1);
+                scales_at_hand();
             } else if (at == 2 * NB) {
                 ks_next = scale_batch(kscale, batch + 1, pages_next);
                 vs_next = scale_batch(vscale, batch + 1, pages_next);
@@ -380,10 +371,14 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 ks_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks_lane), at + b));
-                vs_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs_lane), at + b));
-                if (b == vu) value_scale = vs_load[b];
-                if (!plain_scale(vs_load[b])) vs_load[b] = 1.0f;
+                lift_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lift_lane), at + b));
+                back_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(back_lane), at + b));
                 absent_load |= page(b) < 0 ? 1 << b : 0;
+            }
+            value_scale = 1.0f;
+            if (odd_scales) {
+                const float v = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs_lane), at + vu));
+                if (!plain_scale(v)) value_scale = v;
             }
             at += NB;
         };
@@ -422,7 +417,7 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
             uint32_t out[VE / 2][4];  // [pair of keys][column]
 #pragma unroll
             for (int e = 0; e < VE / 2; ++e) Operand<C, __bf16>::columns(vcode[2 * e], vcode[2 * e + 1], out[e]);
-            if (!plain_scale(value_scale))  // into the values instead
+            if (value_scale != 1.0f)
 #pragma unroll
                 for (int e = 0; e < VE / 2; ++e)
 #pragma unroll
@@ -438,6 +433,40 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
             }
         };
 
+        scales_at_hand();
+        if (it.first < it.end) load_codes(it.first);
+        // this lane's row of the wave's 32: its query, head and limit
+        const int rho = min(wave * 32 + col32, n_rows - 1), tok = it.token + rho / heads, head = h0 + rho % heads;
+        V8 qreg[QP][KS];
+        float row_scale;
+        {
+            int qcol[KS];
+            bool qin[KS];
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qcol[s] = 16 * s + 8 * hf;
+                qin[s] = FULL || qcol[s] < hd;
+            }
+            row_scale = scale2 * load_query<TQ>((const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd, qcol, qin, qreg,
+                                                [](float v) { return fmaxf(v, other_half(v)); });
+#pragma unroll
+            for (int p = 0; p < QP; ++p)
+#pragma unroll
+                for (int s = 0; s < KS; ++s) qreg[p][s] = __builtin_bit_cast(V8, __builtin_bit_cast(v4u, qreg[p][s]) ^ flip);
+        }
+
+        const int limit = seen(A, pos, P, tok, it.row);
+        int least = limit, most = limit;
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+            least = min(least, __shfl_xor(least, o, 64));
+            most = max(most, __shfl_xor(most, o, 64));
+        }
+        least = __builtin_amdgcn_readfirstlane(least);
+        most = __builtin_amdgcn_readfirstlane(most);
+        const bool idle = wave * 32 >= n_rows;
+
+
         v16f acc[CT];
 #pragma unroll
         for (int d = 0; d < CT; ++d)
@@ -448,7 +477,7 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
         auto take = [&]() {  // the tile that was loaded is the one at hand
             absent = absent_load;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) ks[b] = ks_load[b], vs[b] = vs_load[b];
+            for (int b = 0; b < NB; ++b) ks[b] = ks_load[b], lift[b] = lift_load[b], back[b] = back_load[b];
         };
         auto compute = [&](const Stage<HDP>& S, int key0) {
             v16f c[KT];
@@ -527,12 +556,12 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
                 if (u + 1 < NB) fetch(u + 1);
                 // the weights of a block of 16 keys times its values' scale, which goes into the exponent;
                 // the row's sum takes it out again
-                const float back = base - __builtin_amdgcn_logf(vs[u]);
+                const float down = base - lift[u];
                 v8bf part[WP];
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    float x = exp2_fast(fmaf(c[u >> 1][8 * (u & 1) + j], factor[u], -back));
+                    float x = exp2_fast(fmaf(c[u >> 1][8 * (u & 1) + j], factor[u], -down));
                     sum += x;
 #pragma unroll
                     for (int p = 0; p < WP; ++p) {
@@ -540,7 +569,7 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
                         x -= (float)part[p][j];
                     }
                 }
-                l = fmaf(sum, __builtin_amdgcn_rcpf(vs[u]), l);
+                l = fmaf(sum, back[u], l);
 #pragma unroll
                 for (int p = WP - 1; p >= 0; --p)
 #pragma unroll
@@ -549,7 +578,6 @@ __global__ __launch_bounds__(256, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 2 : 1) v
             }
         };
 
-        if (it.first < it.end) load_codes(it.first);
         __syncthreads();  // the last item's readers are done with the stages
         if (it.first < it.end) store_stage(stage[0], it.first);
         take();
@@ -628,28 +656,6 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(cons
         if (tid == 0) nans.any = 0;
         __syncthreads();
     }
-
-    // this lane's rows (those past the last repeat it)
-    int limit[NR], least = INT32_MAX, qcol[2 * KS];
-    bool qin[2 * KS];
-#pragma unroll
-    for (int s = 0; s < 2 * KS; ++s) {
-        qcol[s] = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-        qin[s] = FULL || qcol[s] < hd;
-    }
-    V8 qreg[NR][QP][2 * KS];
-    float row_scale[NR];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        const int rho = min(16 * n + r, n_rows - 1), tok = it.token + rho / heads, head = h0 + rho % heads;
-        limit[n] = seen(A, pos, P, tok, it.row);
-        least = min(least, limit[n]);
-        row_scale[n] = scale2 * load_query<TQ>((const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd, qcol, qin, qreg[n],
-                                               [](float v) { return head_max(v); });
-    }
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
-    least = __builtin_amdgcn_readfirstlane(least);
 
     const uint32_t ps = (uint32_t)P.pos_stride;
     const uint32_t kcol = 16 * g, koff = r * ps, vcol = D * r;
@@ -735,6 +741,28 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(cons
         load_v();
         if (t + 64 / H * (4 * H) < t_end) pages_next = page_batch(1);
     }
+    // this lane's rows (those past the last repeat it)
+    int limit[NR], least = INT32_MAX, qcol[2 * KS];
+    bool qin[2 * KS];
+#pragma unroll
+    for (int s = 0; s < 2 * KS; ++s) {
+        qcol[s] = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+        qin[s] = FULL || qcol[s] < hd;
+    }
+    V8 qreg[NR][QP][2 * KS];
+    float row_scale[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        const int rho = min(16 * n + r, n_rows - 1), tok = it.token + rho / heads, head = h0 + rho % heads;
+        limit[n] = seen(A, pos, P, tok, it.row);
+        least = min(least, limit[n]);
+        row_scale[n] = scale2 * load_query<TQ>((const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd, qcol, qin, qreg[n],
+                                               [](float v) { return head_max(v); });
+    }
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
+    least = __builtin_amdgcn_readfirstlane(least);
+
     int batch = 1;
     while (t < t_end) {
         const int next = t + 4 * H;
@@ -936,7 +964,7 @@ __global__ __launch_bounds__(256) void k_kv8_prefix_join(const KvAttend A, const
         const int kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
         const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0);
         if (sub >= at_once || row >= it.count * heads) continue;
-        const float* part = plan.partial + ((size_t)cut.x * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
+        const float* part = plan.partial + ((size_t)it.part * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
         const size_t stride = (size_t)geo.units * PrefixPlan::part_floats(geo.rows, hd);
         float m = -INFINITY, l = 0.0f;
         v4f v = {0.f, 0.f, 0.f, 0.f};
@@ -968,11 +996,11 @@ __global__ __launch_bounds__(256) void k_kv8_prefix_join(const KvAttend A, const
 
 template <typename TQ, typename C, int HDP, bool FULL>
 hipError_t prefix_launch(const KvAttend& a, const int32_t* pos, const KvPool& p, const Geometry& g, hipStream_t s) {
-    const int64_t most = ((int64_t)a.n_q + g.places) * g.units;
+    const int64_t most = ((int64_t)a.n_q + 2 * g.places) * g.units;
     if (g.rows == kFewRows) {
         hipLaunchKernelGGL((k_kv8_prefix_few<TQ, C, HDP, FULL>), dim3((unsigned)most), dim3(256), 0, s, a, pos, p, g);
     } else {
-        const int grid = (int)std::min<int64_t>(most, HDP <= (sizeof(TQ) == 4 ? 64 : 128) ? 512 : 256);
+        const int grid = (int)std::min<int64_t>(most, HDP <= 128 ? 512 : 256);
         hipLaunchKernelGGL((k_kv8_prefix<TQ, C, HDP, FULL>), dim3(grid), dim3(256), 0, s, a, pos, p, g);
     }
     return hipGetLastError();
@@ -991,7 +1019,7 @@ hipError_t prefix_by_code(const KvAttend& a, const int32_t* pos, const KvPool& p
     const hipError_t e = p.dtype == kI8 ? prefix_by_width<TQ, I8>(a, pos, p, g, s) : prefix_by_width<TQ, E4M3>(a, pos, p, g, s);
     if (e != hipSuccess || !may_cut) return e;
     const int at_once = 256 / (p.hd / 4), steps = (g.rows + at_once - 1) / at_once;
-    const int64_t all = (int64_t)(g.places / 2) * g.units * steps;  // (a cut tile has two pieces at least)
+    const int64_t all = (int64_t)g.places * g.units * steps;  // (a cut tile has two pieces at least)
     hipLaunchKernelGGL((k_kv8_prefix_join<TQ>), dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(1024, all))), dim3(256), 0, s, a, p, g);
     return hipGetLastError();
 }
@@ -1011,8 +1039,8 @@ hipError_t launch_kv8_prefix(const KvAttend& a, const int32_t* pos, const KvPool
     // Drafted tokens and the like, 32 rows a request or fewer on average: the few-row kernel.
     const bool few = (int64_t)a.n_q * group <= (int64_t)kFewRows * std::min(a.n_rows, 64) || a.n_q * group <= kFewRows;
     const Geometry g(a.nh, p.nkv, p.hd, a.q_dtype == kF32, few);
-    // (as many tiles as places, whatever the map: nothing is cut)
-    const bool may_cut = (a.n_q + g.tokens - 1) / g.tokens < g.places;
+    // (many more tiles than places, whatever the map: nothing is cut)
+    const bool may_cut = (a.n_q + g.tokens - 1) / g.tokens < kRounds * g.places;
     hipLaunchKernelGGL(k_kv8_prefix_plan, dim3(1), dim3(1024), 0, s, a, pos, p, g, may_cut);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (a.q_dtype == kF32) return prefix_by_code<float>(a, pos, p, g, may_cut, s);
