@@ -414,7 +414,7 @@ enum {
 
 sxq_status sxq_lm_create(int device, const sxq_lm_config *cfg, sxq_lm **out);
 /* The same engine over a paged cache (the operators above): every layer's keys and values in
- * n_pages pages of page_size positions, of kv_dtype SXQ_F32 or SXQ_BF16, shared by all
+ * n_pages pages of page_size positions, of kv_dtype SXQ_F32, SXQ_BF16 or SXQ_E4M3 (with scales), shared by all
  * streams -- a stream holds the pages of its length, so max_seq (up to 2^20) reserves nothing
  * but its RoPE row and table entries.  Steps and prefills take pages as streams grow, and are
  * refused with SXQ_ERR_OOM before any GPU work when there are not enough; sxq_lm_reset and
@@ -425,7 +425,7 @@ sxq_status sxq_lm_create(int device, const sxq_lm_config *cfg, sxq_lm **out);
  * needs more than the last, so a prefill may find the pages and still fail with SXQ_ERR_OOM,
  * nothing done; its cost grows with the history.  Every other call is as for sxq_lm_create,
  * except that sxq_fish_fast_expand refuses a paged engine (its cache is one frame's codes).
- * Keys and values are rounded once to kv_dtype; the attention's sums are in another order than
+ * Keys and values are rounded once to kv_dtype (e4m3: as sxq_kv_append says); the attention's sums are in another order than
  * the contiguous engine's.  A step or prefill that fails gives its pages back, so it can be
  * made again; if the device takes not even that, the following calls are refused until
  * sxq_lm_reset has emptied all max_batch streams. */

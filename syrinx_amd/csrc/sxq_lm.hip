@@ -260,11 +260,18 @@ sxq_status check_lost(const sxq_lm* lm, const char* who) {
     return fail(SXQ_ERR_INVALID, "%s: an earlier call failed with its pages taken; reset all %d streams", who, lm->c.max_batch);
 }
 
+// Scales of all layers' keys (or values).
+int64_t scale_count(const sxq_lm* lm) { return lm->pool.scale_page_stride * lm->pool.n_pages * lm->c.n_layers; }
+
 KvPool layer_pool(const sxq_lm* lm, int l) {
     KvPool p = lm->pool;
-    const size_t off = (size_t)l * lm->pool_layer * type_size(p.dtype);
+    const size_t off = (size_t)l * lm->pool_layer * kv_elem_size(p.dtype);
     p.k = (uint8_t*)p.k + off;
     p.v = (uint8_t*)p.v + off;
+    if (p.k_scale) {
+        p.k_scale += (size_t)l * p.scale_page_stride * p.n_pages;
+        p.v_scale += (size_t)l * p.scale_page_stride * p.n_pages;
+    }
     return p;
 }
 
@@ -288,7 +295,8 @@ hipError_t lm_append(sxq_lm* lm, int l, const float* qkv, int T, const int32_t* 
     a.pos = pos;
     a.slots = slots;
     a.q_out = q;
-    return launch_kv_append(a, layer_pool(lm, l), s);
+    const KvPool p = layer_pool(lm, l);
+    return kv_is8(p.dtype) ? launch_kv8_append(a, p, s) : launch_kv_append(a, p, s);
 }
 
 hipError_t lm_attend(sxq_lm* lm, int l, const float* q, int n, float* ctx, hipStream_t s) {
@@ -306,7 +314,11 @@ hipError_t lm_attend(sxq_lm* lm, int l, const float* q, int n, float* ctx, hipSt
     a.scale = (float)(1.0 / sqrt((double)lm->c.head_dim));
     a.out = ctx;
     a.ws = lm->kv_ws;
-    return launch_kv_attend(a, layer_pool(lm, l), s);
+    const KvPool p = layer_pool(lm, l);
+    return kv_is8(p.dtype) ? launch_kv8_attend(a, p, s) : launch_kv_attend(a, p, s);
+}
+size_t lm_attend_workspace(const KvPool& p, int n_q, int nh) {
+    return kv_is8(p.dtype) ? kv8_attend_workspace(p, n_q, nh) : kv_attend_workspace(p, n_q, nh);
 }
 
 // Every stream empty, every page free.
@@ -318,7 +330,8 @@ hipError_t empty_pages(sxq_lm* lm, hipStream_t s) {
     return e;
 }
 
-// N(0, 1) into n elements of a cache.
+// N(0, 1) into n elements of a cache (e4m3: at one scale, which holds 7).
+constexpr float kFillScale = 0x1p-6f;
 hipError_t fill_cache(void* p, int64_t n, int dtype, uint64_t seed) {
     if (dtype == kF32) return launch_fill_normal((float*)p, n, seed, 0.0f, 1.0f, nullptr);
     const int64_t chunk = std::min<int64_t>(n, (int64_t)16 << 20);
@@ -327,7 +340,9 @@ hipError_t fill_cache(void* p, int64_t n, int dtype, uint64_t seed) {
     for (int64_t at = 0; at < n && e == hipSuccess; at += chunk) {
         const int64_t m = std::min(chunk, n - at);
         e = launch_fill_normal(tmp, m, seed * 1000003ull + (uint64_t)at, 0.0f, 1.0f, nullptr);
-        if (e == hipSuccess) e = launch_f32_to_bf16(tmp, m, (uint16_t*)p + at, nullptr);
+        if (e == hipSuccess)
+            e = dtype == kE4M3 ? launch_f32_to_e4m3(tmp, m, 1.0f / kFillScale, (uint8_t*)p + at, nullptr)
+                               : launch_f32_to_bf16(tmp, m, (uint16_t*)p + at, nullptr);
     }
     if (tmp) {
         (void)hipDeviceSynchronize();
@@ -793,7 +808,7 @@ hipError_t enqueue_prefill(sxq_lm* lm, const PrefillMeta& pm, int T, const int* 
     return hipSuccess;
 }
 
-// A paged engine's pages: `dtype` f32 or bf16.
+// A paged engine's pages: `dtype` f32, bf16 or e4m3.
 struct PageConfig {
     int dtype, page_size, n_pages;
 };
@@ -815,9 +830,12 @@ sxq_status lm_build(int device, const sxq_lm_config* cfg, const PageConfig* page
         k.pos_stride = cfg->head_dim;
         k.head_stride = (int64_t)k.pos_stride * k.page_size;
         k.page_stride = k.head_stride * k.n_kv_heads;
+        k.scale_head_stride = k.page_size / SXQ_KV_SCALE_BLOCK;
+        k.scale_page_stride = k.scale_head_stride * k.n_kv_heads;
         st = kv_pool("lm_create_paged", &k, false, &pool);
         if (st != SXQ_OK) return st;
-        if (pool.dtype == kF16) return fail(SXQ_ERR_DTYPE, "lm_create_paged: pages of f32 or bf16 (the queries are f32)");
+        // (int8 codes round again whenever their block's scale grows, which token by token it does)
+        if (pool.dtype == kF16 || pool.dtype == kI8) return fail(SXQ_ERR_DTYPE, "lm_create_paged: pages of f32, bf16 or e4m3");
     }
     DeviceGuard g(device);
     HIP_TRY(g.err, "hipSetDevice");
@@ -865,9 +883,11 @@ sxq_status lm_build(int device, const sxq_lm_config* cfg, const PageConfig* page
     A((void**)&lm->rope_cos, sizeof(float) * (size_t)c.max_seq * (hd / 2));
     A((void**)&lm->rope_sin, sizeof(float) * (size_t)c.max_seq * (hd / 2));
     if (pages) {
-        const size_t bytes = (size_t)lm->pool_layer * c.n_layers * type_size(pool.dtype);
+        const size_t bytes = (size_t)lm->pool_layer * c.n_layers * kv_elem_size(pool.dtype);
         A(&lm->pool.k, bytes);
         A(&lm->pool.v, bytes);
+        if (kv_is8(pool.dtype))
+            for (float** p : {&lm->pool.k_scale, &lm->pool.v_scale}) A((void**)p, sizeof(float) * (size_t)scale_count(lm));
         A((void**)&lm->kv_table, sizeof(int32_t) * (size_t)MB * lm->max_blocks);
         A((void**)&lm->kv_free, sizeof(int32_t) * (size_t)pool.n_pages);
         A((void**)&lm->kv_free_count, sizeof(int32_t));
@@ -876,7 +896,7 @@ sxq_status lm_build(int device, const sxq_lm_config* cfg, const PageConfig* page
         A((void**)&lm->kv_cu, sizeof(int32_t) * (MB + 1));
         A((void**)&lm->kv_map, sizeof(int32_t) * 2 * MB);
         A((void**)&lm->kv_ctx, sizeof(float) * (size_t)MB * lm->ctx);
-        A(&lm->kv_ws, kv_attend_workspace(pool, MB, c.n_heads));
+        A(&lm->kv_ws, lm_attend_workspace(pool, MB, c.n_heads));
     } else {
         A((void**)&lm->kc, sizeof(float) * (size_t)lm->kv_layer_stride * c.n_layers);
         A((void**)&lm->vc, sizeof(float) * (size_t)lm->kv_layer_stride * c.n_layers);
@@ -959,7 +979,10 @@ sxq_status lm_build(int device, const sxq_lm_config* cfg, const PageConfig* page
         if (e == hipSuccess) e = launch_fill_int(lm->kv_ones, MB, 1, nullptr);
         // (the queries of a stream that has sat out since the start: finite)
         if (e == hipSuccess) e = hipMemset(lm->qbuf, 0, sizeof(float) * (size_t)MB * lm->ctx);
-        if (e == hipSuccess) e = hipMemset(lm->kv_ws, 0, kv_attend_workspace(pool, MB, c.n_heads));
+        if (e == hipSuccess) e = hipMemset(lm->kv_ws, 0, lm_attend_workspace(pool, MB, c.n_heads));
+        if (kv_is8(pool.dtype))
+            for (float* p : {lm->pool.k_scale, lm->pool.v_scale})
+                if (e == hipSuccess) e = launch_fill_f32(p, scale_count(lm), 1.0f, nullptr);
     }
     lm->attn_fused = !pages && getenv("SXQ_ATTN_UNFUSED") == nullptr && attn_decode_fits(lm->vdt, c.n_heads, c.n_kv_heads, hd, lm->max_splits);
     lm->swiglu = getenv("SXQ_SWIGLU_UNFUSED") == nullptr && swiglu_pair_fits(lm->layers[0].w13.w, lm->layers[0].w2.w);
@@ -1269,6 +1292,8 @@ sxq_status sxq_lm_kv_fill_random(sxq_lm* lm, const int32_t* lengths, int n, uint
         const int dt = lm->paged ? lm->pool.dtype : (int)kF32;
         HIP_TRY(fill_cache(lm->paged ? lm->pool.k : lm->kc, total, dt, seed * 2 + 11), "lm_kv_fill_random");
         HIP_TRY(fill_cache(lm->paged ? lm->pool.v : lm->vc, total, dt, seed * 2 + 12), "lm_kv_fill_random");
+        if (dt == kE4M3)
+            for (float* p : {lm->pool.k_scale, lm->pool.v_scale}) HIP_TRY(launch_fill_f32(p, scale_count(lm), kFillScale, nullptr), "lm_kv_fill_random");
         HIP_TRY(hipDeviceSynchronize(), "lm_kv_fill_random");
     }
     return lengths ? sxq_lm_set_lengths(lm, lengths, n) : SXQ_OK;

@@ -382,6 +382,18 @@ void append_by_cache(const KvAppend& a, const KvPool& p, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------- gather
+// Four elements of a pool as f32.
+template <typename TC>
+SXQ_DEV void pool4(const void* pool, int64_t at, float, float* f) {
+    load4((const TC*)pool + at, f);
+}
+template <>
+SXQ_DEV void pool4<E4M3>(const void* pool, int64_t at, float scale, float* f) {
+    E4M3::unpack(*(const uint32_t*)((const uint8_t*)pool + at), f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] *= scale;
+}
+
 // Eight elements of K and of V a thread.
 template <typename TC>
 __global__ __launch_bounds__(256) void k_kv_gather(const KvPool P, const int32_t* __restrict__ table, int64_t table_stride,
@@ -398,15 +410,18 @@ __global__ __launch_bounds__(256) void k_kv_gather(const KvPool P, const int32_t
     const int slot = b < max_blocks ? kv_slot(table[(r0 + row) * table_stride + b], p, P.shift, P.n_pages) : -1;
     const int64_t from = slot < 0 ? 0 : kv_slot_base(P, slot, h0 + h) + d;
     const int64_t to = ((int64_t)h * total + q) * P.hd + d;
+    float ks = 1.0f, vs = 1.0f;
+    if constexpr (sizeof(TC) == 1)
+        if (slot >= 0) ks = P.k_scale[kv_scale_at(P, slot, h0 + h)], vs = P.v_scale[kv_scale_at(P, slot, h0 + h)];
 #pragma unroll
     for (int o = 0; o < 8; o += 4) {
         float f[4] = {0.f, 0.f, 0.f, 0.f};
         if (k) {
-            if (slot >= 0) load4((const TC*)P.k + from + o, f);
+            if (slot >= 0) pool4<TC>(P.k, from + o, ks, f);
             store4(k + to + o, f);
         }
         if (v) {
-            if (slot >= 0) load4((const TC*)P.v + from + o, f);
+            if (slot >= 0) pool4<TC>(P.v, from + o, vs, f);
             store4(v + to + o, f);
         }
     }
@@ -436,6 +451,21 @@ __global__ __launch_bounds__(64) void k_kv_by_row(const int32_t* __restrict__ cu
 __global__ __launch_bounds__(256) void k_f32_to_bf16(const float* __restrict__ x, int64_t n, __bf16* __restrict__ y) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i < n) y[i] = (__bf16)x[i];
+}
+
+__global__ __launch_bounds__(256) void k_f32_to_e4m3(const float* __restrict__ x, int64_t n, float inv, uint32_t* __restrict__ y) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (4 * i >= n) return;
+    float f[4];
+    load4(x + 4 * i, f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] *= inv;
+    y[i] = E4M3::pack(f);
+}
+
+__global__ __launch_bounds__(256) void k_fill_f32(float* __restrict__ y, int64_t n, float v) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) y[i] = v;
 }
 
 bool kv_dtype(int dt) { return dt == kF32 || dt == kF16 || dt == kBF16; }
@@ -485,7 +515,8 @@ hipError_t launch_kv_gather(const KvPool& p, const int32_t* table, int64_t table
     const dim3 grid((unsigned)(((int64_t)spans.start[spans.n] * (p.hd / 8) + 255) / 256), heads);
 #define SXQ_GA(T) hipLaunchKernelGGL(k_kv_gather<T>, grid, dim3(256), 0, s, p, table, table_stride, max_blocks, spans, r0, h0, p0, k, v)
     if (p.dtype == kF32) SXQ_GA(float);
-    else SXQ_GA(__bf16);  // (an engine's pages are f32 or bf16)
+    else if (p.dtype == kE4M3) SXQ_GA(E4M3);
+    else SXQ_GA(__bf16);  // (an engine's pages are f32, bf16 or e4m3)
 #undef SXQ_GA
     return hipGetLastError();
 }
@@ -508,6 +539,16 @@ hipError_t launch_kv_by_row(const int32_t* cu, const int32_t* map_slots, const i
 
 hipError_t launch_f32_to_bf16(const float* x, int64_t n, uint16_t* y, hipStream_t s) {
     hipLaunchKernelGGL(k_f32_to_bf16, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, x, n, (__bf16*)y);
+    return hipGetLastError();
+}
+
+hipError_t launch_f32_to_e4m3(const float* x, int64_t n, float inv, uint8_t* y, hipStream_t s) {
+    hipLaunchKernelGGL(k_f32_to_e4m3, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, x, n, inv, (uint32_t*)y);
+    return hipGetLastError();
+}
+
+hipError_t launch_fill_f32(float* y, int64_t n, float v, hipStream_t s) {
+    hipLaunchKernelGGL(k_fill_f32, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, y, n, v);
     return hipGetLastError();
 }
 

@@ -88,6 +88,9 @@ hipError_t launch_kv_by_row(const int32_t* cu, const int32_t* map_slots, const i
                             int32_t* pos, hipStream_t s);
 // bf16 (round to nearest even) of n f32 values.
 hipError_t launch_f32_to_bf16(const float* x, int64_t n, uint16_t* y, hipStream_t s);
+// e4m3 codes of n f32 values times inv (n a multiple of 4).
+hipError_t launch_f32_to_e4m3(const float* x, int64_t n, float inv, uint8_t* y, hipStream_t s);
+hipError_t launch_fill_f32(float* y, int64_t n, float v, hipStream_t s);
 
 namespace abi {
 // The checks every entry point makes of its pages, and their kernel form.

@@ -133,8 +133,9 @@ class DecoderLM:
     """A decode-step engine (sxq_lm) on one GPU.
 
     With kv_pages, its cache is paged (sxq_lm_create_paged): that many pages of page_size
-    positions a layer, of kv_dtype (torch.float32 or torch.bfloat16), shared by all streams,
-    instead of max_seq f32 positions reserved for each."""
+    positions a layer, of kv_dtype (torch.float32, torch.bfloat16, or torch.float8_e4m3fn with a
+    scale for every 16 positions of a KV head), shared by all streams, instead of max_seq f32
+    positions reserved for each."""
 
     def __init__(self, cfg: DecoderConfig, device="cuda:0", kv_pages: int = None, page_size: int = 32,
                  kv_dtype: torch.dtype = torch.float32):
@@ -148,7 +149,8 @@ class DecoderLM:
         if kv_pages is None:
             check(lib().sxq_lm_create(self._dev(), ctypes.byref(self._c), ctypes.byref(self._h)))
         else:
-            code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}.get(kv_dtype, -1)
+            code = {torch.float32: 0, torch.float16: 1, torch.int8: 24, torch.bfloat16: 30,
+                    torch.float8_e4m3fn: 0x101}.get(kv_dtype, -1)
             check(lib().sxq_lm_create_paged(self._dev(), ctypes.byref(self._c), code, int(page_size), int(kv_pages),
                                             ctypes.byref(self._h)))
         self.ids_per = 1 + cfg.n_codebooks
