@@ -232,7 +232,8 @@ typedef struct {
  * the first that the call writes, are rescaled to it.  A code is x / s rounded to nearest, ties to
  * even; infinities become the largest code of their sign, a NaN becomes the e4m3 NaN, or int8's 0.
  * Rescaling by powers of two is exact for e4m3, but for values below 2^-6 of the scale, and rounds
- * int8 codes once more. */
+ * int8 codes once more.  Dropping positions (sxq_kv_reserve) leaves scales as they are: a block that
+ * is written on from its middle keeps the scale that the dropped ones asked for. */
 #define SXQ_KV_SCALE_BLOCK 16
 
 /* Block tables and slot maps from the requests' lengths.  Request r of n_rows holds lens[r]
@@ -287,8 +288,9 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
  * Scores, softmax statistics and sums are f32; over 16-bit pages a weight is carried in parts
  * of the pages' type, off by at most 2^-18 of itself (16-bit queries over bf16) or 2^-22 (f16;
  * f32 queries), below the output's own rounding.  Over 8-bit pages q may be of any of the three
- * types: a code takes part exactly, an f32 query in three bf16 parts, a weight (times its value's
- * scale) in bf16 parts, off by at most 2^-17 of itself (16-bit queries) or 2^-22.  rows int32 [n_q]: the table row of each query (NULL: b);
+ * types: a code takes part exactly, an f32 query element in two f16 parts, off by at most 2^-22 of itself
+ * or 2^-39 of its head's largest finite one, a weight (times its value's scale) in bf16 parts, off by
+ * at most 2^-17 of itself (16-bit queries) or 2^-22.  rows int32 [n_q]: the table row of each query (NULL: b);
  * a query whose row lies outside 0 .. n_rows - 1 leaves its out row as it was.  A request
  * without positions (or whose pages are all absent) gives zeros.  max_blocks * page_size at
  * most 2^30, n_q times that at most 2^35, n_q at most 2^20.  What lies past a request's

@@ -1037,7 +1037,7 @@ size_t kv8_prefix_workspace(const KvPool& p, int n_q, int nh) {
 hipError_t launch_kv8_prefix(const KvAttend& a, const int32_t* pos, const KvPool& p, hipStream_t s) {
     const int group = a.nh / p.nkv;
     // Drafted tokens and the like, 32 rows a request or fewer on average: the few-row kernel.
-    const bool few = (int64_t)a.n_q * group <= (int64_t)kFewRows * std::min(a.n_rows, 64) || a.n_q * group <= kFewRows;
+    const bool few = (int64_t)a.n_q * group <= (int64_t)kFewRows * std::min(a.n_rows, 64) || (int64_t)a.n_q * group <= kFewRows;
     const Geometry g(a.nh, p.nkv, p.hd, a.q_dtype == kF32, few);
     // (many more tiles than places, whatever the map: nothing is cut)
     const bool may_cut = (a.n_q + g.tokens - 1) / g.tokens < kRounds * g.places;

@@ -139,7 +139,8 @@ class PagedKvCache:
         return self._layer_refs[layer]
 
     def _want(self, what, t, dtype, numel=None):
-        if (t.dtype is not dtype or t.device != self.device or not t.is_contiguous()
+        # get_device: the index without building a device object (every call checks several tensors)
+        if (t.dtype is not dtype or t.get_device() != self._index or not t.is_contiguous()
                 or (numel is not None and t.numel() != numel)):
             size = f" of {numel} elements" if numel else ""
             raise ValueError(f"PagedKvCache: {what} must be a contiguous {dtype} tensor{size} on {self.device}, got "
@@ -202,7 +203,7 @@ class PagedKvCache:
         hd, dev, dtype, shape = self.head_dim, self.device, qkv.dtype, qkv.shape
         width = (n_heads + 2 * self.n_kv_heads) * hd
         code = _DTYPES.get(dtype)
-        if code is None or qkv.device != dev or len(shape) != 2 or shape[1] != width or qkv.stride(1) != 1:
+        if code is None or qkv.get_device() != self._index or len(shape) != 2 or shape[1] != width or qkv.stride(1) != 1:
             raise ValueError(f"PagedKvCache.append: qkv must be [T, {width}] f32, f16 or bf16 rows on {dev}, got "
                              f"{dtype} {tuple(shape)} on {qkv.device}")
         tokens = shape[0]
@@ -226,8 +227,8 @@ class PagedKvCache:
             c, s = rope
             positions = c.shape[0]
             for name, t in (("cos", c), ("sin", s)):
-                self._want(name, t, torch.float32, positions * (hd // 2))
-                if t.dim() != 2 or t.shape[1] != hd // 2 or positions < 1:
+                self._want(name, t, torch.float32)
+                if t.shape != (positions, hd // 2) or positions < 1:
                     raise ValueError(f"PagedKvCache.append: {name} must be [positions, {hd // 2}], got {tuple(t.shape)}")
             cos, sin = c.data_ptr(), s.data_ptr()
         if out is None:
@@ -258,19 +259,21 @@ class PagedKvCache:
                 raise ValueError(f"PagedKvCache.read: dtype {dtype} (float32, float16 or bfloat16)")
             out = tuple(torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
         k, v = out
-        width = self.n_kv_heads * self.head_dim
+        hd, width = self.head_dim, self.n_kv_heads * self.head_dim
+        kind, step = _DTYPES.get(k.dtype), k.stride()[0] if k.dim() else 0
         for what, t in (("k", k), ("v", v)):
-            if (t.dtype not in _DTYPES or t.dtype is not k.dtype or t.device != self.device or t.shape != shape
-                    or (total > 0 and (t[0].is_contiguous() is False or t.stride(0) != k.stride(0)))):
+            st = t.stride()
+            if (kind is None or t.dtype is not k.dtype or t.get_device() != self._index or t.shape != shape
+                    or (total > 0 and (st[0] != step or st[2] != 1 or (st[1] != hd and self.n_kv_heads > 1)))):
                 raise ValueError(f"PagedKvCache.read: out's {what} must be f32, f16 or bf16 {shape} on {self.device}, entries "
                                  f"contiguous, both alike, got {t.dtype} {tuple(t.shape)} on {t.device}")
         for what, t in (("rows", rows), ("start", start)):
             if t is not None:
                 self._want(what, t, torch.int32, n)
-        stride = k.stride(0) if total > 1 else width
+        stride = step if total > 1 else width
         check(lib().sxq_kv_read(self._index, self._layer(layer), cu.data_ptr(), _ptr(rows), _ptr(start), n, total,
                                 self.lens.data_ptr(), self.max_rows, self.table.data_ptr(), self.max_blocks, self.max_blocks,
-                                _DTYPES[k.dtype], k.data_ptr(), v.data_ptr(), stride, self._stream()))
+                                kind, k.data_ptr(), v.data_ptr(), stride, self._stream()))
         return k, v
 
     # -- attention ------------------------------------------------------------------------
@@ -320,7 +323,7 @@ class PagedKvCache:
         `workspace(n, n_heads, prefix=True)`), to keep its zeroing out of a captured graph."""
         hd, dev, dtype, shape = self.head_dim, self.device, q.dtype, q.shape
         code, dims = _DTYPES.get(dtype), len(shape)
-        if code is None or q.device != dev or dims not in (2, 3) or (dims == 3 and shape[2] != hd):
+        if code is None or q.get_device() != self._index or dims not in (2, 3) or (dims == 3 and shape[2] != hd):
             raise ValueError(f"PagedKvCache.attend: q must be [n, heads, {hd}] f32, f16 or bf16 on {dev}, got "
                              f"{dtype} {tuple(shape)} on {q.device}")
         n, width = shape[0], shape[1] * hd if dims == 3 else shape[1]
@@ -329,7 +332,7 @@ class PagedKvCache:
         n_heads = width // hd
         if out is None:
             out = torch.empty(shape, dtype=dtype, device=dev)
-        elif out.device != dev or out.dtype is not dtype or out.shape != shape:
+        elif out.get_device() != self._index or out.dtype is not dtype or out.shape != shape:
             raise ValueError(f"PagedKvCache.attend: out must be {dtype} {tuple(shape)} on {dev}")
         strides = []
         for what, t in (("q", q), ("out", out)):

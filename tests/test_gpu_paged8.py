@@ -343,7 +343,8 @@ def _reference(q, cache, rows, seen, scale, layer=0, split=None):
     """Outputs [n, nh, hd] in 64 bits over positions 0 .. seen[i] - 1 of request rows[i], and each
     element's error bound before the output's rounding, u = 2^-24, S the largest scale sum |q_d k_d| of
     a head: a score is off by (hd + 4) u S (hd products and sums, the scales, which are exact powers
-    of two but for `scale` itself; f32 queries' three bf16 parts are exact), a weight by twice that
+    of two but for `scale` itself), an f32 query's two f16 parts leave out 2^-22 = 4 u of an element (and
+    2^-39 of the row's largest, far below that for these queries), a weight is off by twice that
     relative, by |s - m| u <= 2 S u for its argument, 4 u for exp and 4 u for each rescaling; `split`
     is what the weights' parts leave out; sums of len terms len u each."""
     n, nh, hd = q.shape
@@ -354,6 +355,7 @@ def _reference(q, cache, rows, seen, scale, layer=0, split=None):
     table, lens, cells = cache.table.cpu(), cache.lens.tolist(), {}
     if split is None:
         split = 4 * U32 if q.dtype is torch.float32 else 2.0 ** -17  # three bf16 parts, or two
+    parts = 4 if q.dtype is torch.float32 else 0
     for i in range(n):
         r = int(rows[i])
         if not 0 <= r < cache.max_rows:
@@ -373,7 +375,7 @@ def _reference(q, cache, rows, seen, scale, layer=0, split=None):
         kt = k.transpose(1, 2).contiguous()
         w = torch.softmax(qq @ kt * scale, -1)
         S = (qq.abs() @ kt.abs() * abs(scale)).amax(-1, keepdim=True)
-        rel = 2 * (hd + 4) * U32 * S + 2 * S * U32 + split + (4 + 4 * (L / 16 + 2) + 2 * L) * U32
+        rel = 2 * (hd + 4 + parts) * U32 * S + 2 * S * U32 + split + (4 + 4 * (L / 16 + 2) + 2 * L) * U32
         out[i] = (w @ v).reshape(nh, hd)
         bound[i] = (2 * rel * (w @ v.abs())).reshape(nh, hd)
     return out, bound
