@@ -57,28 +57,34 @@ struct TileItem {
     int part, pieces;       // where its result goes, of how many pieces (1: out)
 };
 
-// The workspace: counts {items, tiles that are cut}; items; the tiles that are cut
-// {first item, pieces}; partials: per part and unit, {m, l} of each row, then the weighted sums.
+struct CutTile {
+    int token, count;  // as its items'
+    int part, pieces;  // its first partial, how many
+};
+
+// The workspace: counts {items, tiles that are cut, whether the items begin with the last}; items; the
+// tiles that are cut; partials: per part and unit, {m, l} of each row, then the weighted sums.
 struct PrefixPlan {
     int* counts;
     TileItem* item;
-    int2* cut;
+    CutTile* cut;
     float* partial;
     size_t bytes;
     SXQ_HD static size_t up(size_t v) { return (v + 255) / 256 * 256; }
     SXQ_HD PrefixPlan(void* ws, int n_q, int hd, const Geometry& g) {
         char* p = (char*)ws;
-        const int most = n_q + 2 * g.places;  // items: a tile each, and the pieces of cut ones
+        const int most = item_room(n_q, g);
         counts = (int*)p;
         p += 256;
         item = (TileItem*)p;
         p += up(sizeof(TileItem) * (size_t)most);
-        cut = (int2*)p;
-        p += up(sizeof(int2) * (size_t)g.places);
+        cut = (CutTile*)p;
+        p += up(sizeof(CutTile) * (size_t)g.places);
         partial = (float*)p;
         p += 2 * (size_t)g.places * g.units * part_floats(g.rows, hd) * sizeof(float);
         bytes = (size_t)(p - (char*)ws);
     }
+    SXQ_HD static int item_room(int n_q, const Geometry& g) { return n_q + 2 * g.places; }  // a tile each, and the pieces of cut ones
     SXQ_HD static size_t part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 };
 
@@ -89,107 +95,138 @@ SXQ_DEV int seen(const KvAttend& A, const int32_t* pos, const KvPool& P, int t, 
 }
 
 // A thousand queries at a time, a thread each (the next chunk's under way): where its run began and
-// which of the chunk's tiles it is in by ballots, the tiles' counts and limits in LDS.
+// which tile it is in by ballots, the last two thousand tiles in LDS.  While there are no more than a
+// thousand tiles they stay there until all queries are seen, so that a short call's tiles are cut where
+// they are, and are written once, the last tile first.
+constexpr int kTilesKept = 1024, kTileRing = 2 * kTilesKept;
 __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, const int32_t* pos, const KvPool P, const Geometry g,
                                                           bool may_cut) {
-    __shared__ int s_wave[2][16], s_limit[1025], s_count[1025], s_token[1025], s_row[1025], s_cut;
+    __shared__ __attribute__((aligned(16))) int s_wave[2][16];
+    __shared__ int s_limit[kTileRing], s_end[kTileRing], s_token[kTileRing], s_row[kTileRing], s_cut;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const PrefixPlan plan(A.ws, A.n_q, P.hd, g);
     const uint64_t upto = ~(uint64_t)0 >> (63 - lane);
+    auto tile = [&](int i) {
+        const int k = i & (kTileRing - 1), limit = s_limit[k];
+        return TileItem{s_token[k], s_end[k] - s_token[k], s_row[k], limit, 0, (limit + g.keys - 1) / g.keys, 0, 1};
+    };
     if (tid == 0) s_cut = 0;
+    bool kept = true;        // no tile is written yet
     int tiles = 0, run = 0;  // so far; where the run that reaches into the chunk began
     int row_next = tid < A.n_q ? A.rows[tid] : -1, before_next = tid > 0 && tid < A.n_q ? A.rows[tid - 1] : -1;
-    int pos_next = tid < A.n_q ? pos[tid] : -1;
+    int after_next = tid + 1 < A.n_q ? A.rows[tid + 1] : -1, pos_next = tid < A.n_q ? pos[tid] : -1;
     for (int c0 = 0; c0 < A.n_q; c0 += 1024) {
-        const int t = c0 + tid, row = row_next, before = before_next, at_pos = pos_next;
+        const int t = c0 + tid, row = row_next, before = before_next, after = after_next, at_pos = pos_next;
         const bool live = (uint32_t)row < (uint32_t)A.n_rows;
         const int len = live ? A.lens[row] : 0;
         const int t2 = t + 1024;
         row_next = t2 < A.n_q ? A.rows[t2] : -1;
         before_next = t2 < A.n_q ? A.rows[t2 - 1] : -1;
+        after_next = t2 + 1 < A.n_q ? A.rows[t2 + 1] : -1;
         pos_next = t2 < A.n_q ? pos[t2] : -1;
-        for (int i = tid; i < 1025; i += 1024) s_limit[i] = s_count[i] = 0;
+        s_limit[(tiles + tid) & (kTileRing - 1)] = 0;
         const uint64_t begins = __ballot(t < A.n_q && (t == 0 || before != row));
         if (lane == 0) s_wave[0][wave] = begins ? c0 + 64 * wave + 63 - __builtin_clzll(begins) : -1;
         __syncthreads();
         int start = run;
-        for (int w = 0; w < wave; ++w) start = max(start, s_wave[0][w]);
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            const int begin = s_wave[0][w];
+            start = max(start, w < wave ? begin : -1);
+            run = max(run, begin);
+        }
         if (begins & upto) start = c0 + 64 * wave + 63 - __builtin_clzll(begins & upto);
-        const bool first = live && (t - start) % g.tokens == 0;
+        const int in_tile = (t - start) % g.tokens;
+        const bool first = live && in_tile == 0;
         const uint64_t firsts = __ballot(first);
         if (lane == 0) s_wave[1][wave] = __builtin_popcountll(firsts);
-        for (int w = 0; w < 16; ++w) run = max(run, s_wave[0][w]);
         __syncthreads();
-        int at = __builtin_popcountll(firsts & upto), count = 0;  // tiles of the chunk up to this query (0: the last chunk's last)
+        int at = tiles - 1 + __builtin_popcountll(firsts & upto), count = 0;  // this query's tile (tiles - 1: the last chunk's last)
+#pragma unroll
         for (int w = 0; w < 16; ++w) {
-            if (w < wave) at += s_wave[1][w];
-            count += s_wave[1][w];
+            const int here = s_wave[1][w];
+            at += w < wave ? here : 0;
+            count += here;
         }
-        if (live) {
-            atomicMax(&s_limit[at], seen_of(len, at_pos, A.max_blocks, P.shift));
-            atomicAdd(&s_count[at], 1);
-        }
+        at = live ? at & (kTileRing - 1) : -1;
+        // the tile's most: a query less than the next one, as most are, need not say its own
+        const int sees = live ? seen_of(len, at_pos, A.max_blocks, P.shift) : 0;
+        const int next_at = __shfl_down(at, 1, 64), next_sees = __shfl_down(sees, 1, 64);
+        if (live && (lane == 63 || next_at != at || sees > next_sees)) atomicMax(&s_limit[at], sees);
+        if (live && (t + 1 == A.n_q || after != row || in_tile == g.tokens - 1)) s_end[at] = t + 1;
         if (first) {
             s_token[at] = t;
             s_row[at] = row;
         }
         __syncthreads();
-        for (int i = tid; i <= count; i += 1024) {
-            if (i > 0) {
-                plan.item[tiles + i - 1] = TileItem{s_token[i], s_count[i], s_row[i], s_limit[i], 0, (s_limit[i] + g.keys - 1) / g.keys, 0, 1};
-            } else if (s_count[0] > 0) {
-                TileItem& last = plan.item[tiles - 1];
-                last.count += s_count[0];
-                last.limit = max(last.limit, s_limit[0]);
-                last.end = (last.limit + g.keys - 1) / g.keys;
-            }
+        const int new_tiles = tiles + count;
+        if (new_tiles > kTilesKept) {
+            for (int i = (kept ? 0 : tiles - 1) + tid; i < new_tiles; i += 1024) plan.item[i] = tile(i);
+            kept = false;
+            __syncthreads();
         }
-        tiles += count;
-        __syncthreads();
+        tiles = new_tiles;
     }
     // Pieces: where there are not many more tiles than places, those longer than a place's share are cut
     // into such shares (a tile a thread).  No more than 2 * places pieces are of cut tiles.
     int items = tiles;
-    if (may_cut && tiles <= 1024 && tiles < kRounds * g.places) {
-        TileItem mine{};
-        if (tid < tiles) {
-            if (A.n_q <= 1024) mine = TileItem{s_token[tid + 1], s_count[tid + 1], s_row[tid + 1], s_limit[tid + 1], 0, (s_limit[tid + 1] + g.keys - 1) / g.keys, 0, 1};
-            else mine = plan.item[tid];
-        }
-        auto scan = [&](int v, int turn, int& all) {  // the sum over the threads up to this one
-            v = wave_scan(v);
-            if (lane == 63) s_wave[turn][wave] = v;
-            __syncthreads();
-            int lower = 0;
-            all = 0;
-            for (int w = 0; w < 16; ++w) {
-                if (w == wave) lower = all;
-                all += s_wave[turn][w];
+    if (kept) {
+        const TileItem none{};
+        TileItem mine = tid < tiles ? tile(tid) : none;
+        if (!may_cut || tiles >= kRounds * g.places) {
+            if (tid < tiles) plan.item[tiles - 1 - tid] = mine;
+        } else {
+            auto scan = [&](int v, int turn, int& all) {  // the sum over the threads up to this one
+                v = wave_scan(v);
+                if (lane == 63) s_wave[turn][wave] = v;
+                __syncthreads();
+                int lower = 0;
+                all = 0;
+#pragma unroll
+                for (int w = 0; w < 16; ++w) {
+                    const int here = s_wave[turn][w];
+                    lower += w < wave ? here : 0;
+                    all += here;
+                }
+                return v + lower;
+            };
+            int work, both;
+            scan(mine.end, 0, work);  // (2^30 positions a tile at most, 2^35 of all: 2^29 tiles of keys)
+            const int piece = max(g.min_piece, (work + g.places - 1) / g.places);
+            // A quarter more stays whole.  Kernel and join, us, by half more / a quarter more / none: three f32
+            // prompts of 1412 tokens 55.4 / 53.0 / 63.2, 16 drafts of 5 20.8 / 19.9 / 20.0, a chunk of 2048 after
+            // 30720 1370 / 1365 / 1495 (none: more pieces than places).
+            const int keys = mine.end, n = tid >= tiles ? 0 : 4 * keys > 5 * piece ? (keys + piece - 1) / piece : 1;
+            const int upto_me = scan(n + (n > 1 ? n << 16 : 0), 1, both);  // items, and those of cut tiles
+            items = both & 0xFFFF;
+            const int at = items - (upto_me & 0xFFFF), part = (upto_me >> 16) - n;
+            if (n > 1) plan.cut[atomicAdd(&s_cut, 1)] = CutTile{mine.token, mine.count, part, n};
+            for (int k = 0; k < n; ++k) {
+                mine.first = (int)((int64_t)keys * k / n);
+                mine.end = (int)((int64_t)keys * (k + 1) / n);
+                mine.part = n > 1 ? part + k : 0;
+                mine.pieces = n;
+                plan.item[at + n - 1 - k] = mine;
             }
-            return v + lower;
-        };
-        int work, both;
-        scan(mine.end, 0, work);  // (2^30 positions a tile at most, 2^35 of all: 2^29 tiles of keys)
-        const int piece = max(g.min_piece, (work + g.places - 1) / g.places);
-        // (half as much again stays whole)
-        const int keys = mine.end, n = tid >= tiles ? 0 : 2 * keys > 3 * piece ? (keys + piece - 1) / piece : 1;
-        const int upto_me = scan(n + (n > 1 ? n << 16 : 0), 1, both);  // items, and those of cut tiles
-        items = both & 0xFFFF;
-        const int at = (upto_me & 0xFFFF) - n, part = (upto_me >> 16) - n;
-        if (n > 1) plan.cut[atomicAdd(&s_cut, 1)] = make_int2(at, n);
-        for (int k = 0; k < n; ++k) {
-            mine.first = (int)((int64_t)keys * k / n);
-            mine.end = (int)((int64_t)keys * (k + 1) / n);
-            mine.part = n > 1 ? part + k : 0;
-            mine.pieces = n;
-            plan.item[at + k] = mine;
+            __syncthreads();
         }
-        __syncthreads();
     }
     if (tid == 0) {
         plan.counts[0] = items;
         plan.counts[1] = s_cut;
+        plan.counts[2] = kept;
     }
+}
+
+// Item w of units * items, those of the last tile first (of one request the last queries see the most).
+// The count and the item it most often is are loaded together.
+SXQ_DEV bool item_of(const PrefixPlan& plan, int n_q, const Geometry& g, int64_t w, TileItem& it) {
+    const int k = (int)(w / g.units);
+    it = plan.item[min(k, PrefixPlan::item_room(n_q, g) - 1)];
+    const int items = plan.counts[0];
+    if (k >= items) return false;
+    if (!plan.counts[2]) it = plan.item[items - 1 - k];
+    return true;
 }
 
 // ---- the attention -----------------------------------------------------------------------
@@ -265,7 +302,6 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
     const int col32 = lane & 31, hf = lane >> 5;
     const int hd = FULL ? HDP : P.hd;
     const PrefixPlan plan(A.ws, A.n_q, hd, geo);
-    const int items = __builtin_amdgcn_readfirstlane(plan.counts[0]);
     // (a negative scale is the positive one over negated queries: the running maximum wants factors
     // of 0 or more)
     const float scale2 = fabsf(A.scale) * 1.44269504088896340736f;
@@ -285,8 +321,8 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
     const uint32_t koff = (uint32_t)(kkey & 15) * ps + (kin ? kc : 0), voff = (uint32_t)(4 * vf + 8 * vhalf) * ps + (vin ? vc : 0);
 
     int turn = 0;
-    // long items first: of one request the last queries see the most
-    for (int64_t w = blockIdx.x; w < (int64_t)items * geo.units; w += gridDim.x) {
+    TileItem it;
+    for (int64_t w = blockIdx.x; item_of(plan, A.n_q, geo, w, it); w += gridDim.x) {
         Nans<HDP>* const nans = &s_nans[turn++ & 1];
         if constexpr (C::kNan) {  // (its readers were done before the last item's first barrier)
             if (tid < HDP) nans->first[tid] = INT32_MAX;
@@ -294,7 +330,6 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
         }
         const int unit = (int)(w % geo.units), kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
         const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0);
-        TileItem it = plan.item[items - 1 - (int)(w / geo.units)];
         it.row = __builtin_amdgcn_readfirstlane(it.row);
         it.limit = __builtin_amdgcn_readfirstlane(it.limit);
         it.first = __builtin_amdgcn_readfirstlane(it.first);
@@ -645,9 +680,9 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(cons
     const int r = lane & 15, g = lane >> 4;
     const int hd = FULL ? HDP : P.hd;
     const PrefixPlan plan(A.ws, A.n_q, hd, geo);
-    const int w = blockIdx.x / geo.units, unit = blockIdx.x - w * geo.units;
-    if (w >= plan.counts[0]) return;
-    const TileItem it = plan.item[w];
+    const int unit = blockIdx.x % geo.units;
+    TileItem it;
+    if (!item_of(plan, A.n_q, geo, blockIdx.x, it)) return;
     const int kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
     const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0), n_rows = it.count * heads;
     const float scale2 = A.scale * 1.44269504088896340736f;
@@ -954,32 +989,32 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(cons
 template <typename TQ>
 __global__ __launch_bounds__(256) void k_kv8_prefix_join(const KvAttend A, const KvPool P, const Geometry geo) {
     const PrefixPlan plan(A.ws, A.n_q, P.hd, geo);
-    const int cuts = plan.counts[1], hd = P.hd, per = hd / 4, at_once = 256 / per;  // rows a workgroup takes at once
+    const int hd = P.hd, per = hd / 4, at_once = 256 / per;  // rows a workgroup takes at once
     const int steps = (geo.rows + at_once - 1) / at_once;
     const int sub = threadIdx.x / per, col = 4 * (threadIdx.x - sub * per);
-    for (int w = blockIdx.x; w < cuts * geo.units * steps; w += gridDim.x) {
-        const int step = w % steps, unit = w / steps % geo.units, row = step * at_once + sub;
-        const int2 cut = plan.cut[w / steps / geo.units];
-        const TileItem it = plan.item[cut.x];
+    for (int w = blockIdx.x;; w += gridDim.x) {
+        const int step = w % steps, unit = w / steps % geo.units, k = w / steps / geo.units, row = step * at_once + sub;
+        const CutTile cut = plan.cut[min(k, geo.places - 1)];  // (with the count, not after it)
+        if (k >= plan.counts[1]) break;
         const int kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
         const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0);
-        if (sub >= at_once || row >= it.count * heads) continue;
-        const float* part = plan.partial + ((size_t)it.part * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
+        if (sub >= at_once || row >= cut.count * heads) continue;
+        const float* part = plan.partial + ((size_t)cut.part * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
         const size_t stride = (size_t)geo.units * PrefixPlan::part_floats(geo.rows, hd);
         float m = -INFINITY, l = 0.0f;
         v4f v = {0.f, 0.f, 0.f, 0.f};
-        for (int k0 = 0; k0 < cut.y; k0 += 4) {
+        for (int k0 = 0; k0 < cut.pieces; k0 += 4) {
             float2 ml[4];
             v4f x[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const float* p = part + min(k0 + u, cut.y - 1) * stride;
+                const float* p = part + min(k0 + u, cut.pieces - 1) * stride;
                 ml[u] = *(const float2*)(p + 2 * row);
                 x[u] = *(const v4f*)(p + 2 * geo.rows + (size_t)row * hd + col);
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                if (k0 + u >= cut.y) break;
+                if (k0 + u >= cut.pieces) break;
                 const float mn = fmaxf(m, ml[u].x);
                 const float up = m > -INFINITY ? exp2_fast(m - mn) : 1.0f;  // (no weights, or NaN: as they are)
                 const float f = ml[u].x > -INFINITY ? exp2_fast(ml[u].x - mn) : 1.0f;
@@ -990,7 +1025,7 @@ __global__ __launch_bounds__(256) void k_kv8_prefix_join(const KvAttend A, const
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const float f[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
-        store4((TQ*)A.out + (int64_t)(it.token + row / heads) * A.out_stride + (int64_t)(h0 + row % heads) * hd + col, f);
+        store4((TQ*)A.out + (int64_t)(cut.token + row / heads) * A.out_stride + (int64_t)(h0 + row % heads) * hd + col, f);
     }
 }
 
