@@ -62,8 +62,8 @@ struct CutTile {
     int part, pieces;  // its first partial, how many
 };
 
-// The workspace: counts {items, tiles that are cut, whether the items begin with the last}; items; the
-// tiles that are cut; partials: per part and unit, {m, l} of each row, then the weighted sums.
+// The workspace: counts {items, tiles that are cut, their pieces, whether the items begin with the last};
+// items; the tiles that are cut; partials: per part and unit, {m, l} of each row, then the weighted sums.
 struct PrefixPlan {
     int* counts;
     TileItem* item;
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, cons
     }
     // Pieces: where there are not many more tiles than places, those longer than a place's share are cut
     // into such shares (a tile a thread).  No more than 2 * places pieces are of cut tiles.
-    int items = tiles;
+    int items = tiles, pieces = 0;
     if (kept) {
         const TileItem none{};
         TileItem mine = tid < tiles ? tile(tid) : none;
@@ -199,22 +199,29 @@ __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, cons
             const int keys = mine.end, n = tid >= tiles ? 0 : 4 * keys > 5 * piece ? (keys + piece - 1) / piece : 1;
             const int upto_me = scan(n + (n > 1 ? n << 16 : 0), 1, both);  // items, and those of cut tiles
             items = both & 0xFFFF;
-            const int at = items - (upto_me & 0xFFFF), part = (upto_me >> 16) - n;
+            pieces = both >> 16;
+            const int before = (upto_me & 0xFFFF) - n, part = (upto_me >> 16) - n;
             if (n > 1) plan.cut[atomicAdd(&s_cut, 1)] = CutTile{mine.token, mine.count, part, n};
-            for (int k = 0; k < n; ++k) {
-                mine.first = (int)((int64_t)keys * k / n);
-                mine.end = (int)((int64_t)keys * (k + 1) / n);
-                mine.part = n > 1 ? part + k : 0;
-                mine.pieces = n;
-                plan.item[at + n - 1 - k] = mine;
-            }
+            // (in the ring's second half: the items before the tile's, its first part, its pieces)
+            int *const s_before = s_limit + kTilesKept, *const s_part = s_token + kTilesKept, *const s_pieces = s_end + kTilesKept;
+            s_before[tid] = before;
+            s_part[tid] = part;
+            s_pieces[tid] = n;
             __syncthreads();
+            for (int i = tid; i < items; i += 1024) {  // an item a thread
+                const int o = owner(s_before, tiles, i), k = i - s_before[o];
+                TileItem it = tile(o);
+                const int64_t all = it.end;
+                it.pieces = s_pieces[o];
+                it.part = it.pieces > 1 ? s_part[o] + k : 0;
+                it.first = (int)(all * k / it.pieces);
+                it.end = (int)(all * (k + 1) / it.pieces);
+                plan.item[items - 1 - i] = it;
+            }
         }
     }
     if (tid == 0) {
-        plan.counts[0] = items;
-        plan.counts[1] = s_cut;
-        plan.counts[2] = kept;
+        *(int4*)plan.counts = make_int4(items, s_cut, pieces, kept);
     }
 }
 
@@ -223,9 +230,9 @@ __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, cons
 SXQ_DEV bool item_of(const PrefixPlan& plan, int n_q, const Geometry& g, int64_t w, TileItem& it) {
     const int k = (int)(w / g.units);
     it = plan.item[min(k, PrefixPlan::item_room(n_q, g) - 1)];
-    const int items = plan.counts[0];
-    if (k >= items) return false;
-    if (!plan.counts[2]) it = plan.item[items - 1 - k];
+    const int4 counts = *(const int4*)plan.counts;
+    if (k >= counts.x) return false;
+    if (!counts.w) it = plan.item[counts.x - 1 - k];
     return true;
 }
 
@@ -676,355 +683,378 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(cons
     __shared__ __attribute__((aligned(16))) float s_acc[4][16][HDP + 4];
     __shared__ Nans<HDP> nans;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r = lane & 15, g = lane >> 4;
     const int hd = FULL ? HDP : P.hd;
     const PrefixPlan plan(A.ws, A.n_q, hd, geo);
-    const int unit = blockIdx.x % geo.units;
     TileItem it;
-    if (!item_of(plan, A.n_q, geo, blockIdx.x, it)) return;
-    const int kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
-    const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0), n_rows = it.count * heads;
-    const float scale2 = A.scale * 1.44269504088896340736f;
-    if constexpr (C::kNan) {
-        if (tid < HDP) nans.first[tid] = INT32_MAX;
-        if (tid == 0) nans.any = 0;
-        __syncthreads();
-    }
-
-    const uint32_t ps = (uint32_t)P.pos_stride;
-    const uint32_t kcol = 16 * g, koff = r * ps, vcol = D * r;
-    const bool vin = FULL || (int)vcol < hd;
-    uint32_t voff[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) voff[i] = (4 * g + i) * ps + (vin ? vcol : 0);
-    const char* kpool = (const char*)P.k + (int64_t)kh * P.head_stride;
-    const char* vpool = (const char*)P.v + (int64_t)kh * P.head_stride;
-    const float* kscale = P.k_scale + (int64_t)kh * P.scale_head_stride;
-    const float* vscale = P.v_scale + (int64_t)kh * P.scale_head_stride;
-
-    const int32_t* table = A.table + (int64_t)it.row * A.table_stride;
-    const int t_last = (it.limit + 15) / 16 - 1;  // the last half tile (16 positions) with a position
-    const int t_end = min(it.end * (kFewKeys / 16), t_last + 1);
-    // lane j: the page (-1: absent) and scales of the wave's half tile j of a batch of 64
-    const int t0 = it.first * (kFewKeys / 16) + wave * H, log_p = P.shift - kScaleShift, block_mask = (P.page >> kScaleShift) - 1;
-    auto tile_of = [&](int batch) { return t0 + (batch * 64 + lane) / H * (4 * H) + (lane & (H - 1)); };
-    auto page_batch = [&](int batch) {
-        const int t = tile_of(batch);
-        int id = -1;
-        if (t < t_end) id = table[t >> log_p];
-        return kv_page_ok(id, P.n_pages) ? id : -1;
-    };
-    auto scale_batch = [&](const float* scales, int batch, int id) {
-        float s = 0.0f;
-        if (id >= 0) s = scales[(int64_t)id * P.scale_page_stride + (tile_of(batch) & block_mask)];
-        return s;
-    };
-    int pages = page_batch(0), pages_next = -1;
-    float ks_lane = scale_batch(kscale, 0, pages), vs_lane = scale_batch(vscale, 0, pages), ks_next = 0.0f, vs_next = 0.0f;
-
-    v4f acc[NR][D];
-    float m[NR], l[NR];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        m[n] = -INFINITY;
-        l[n] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < D; ++d) acc[n][d] = (v4f){0.f, 0.f, 0.f, 0.f};
-    }
-    uint32_t kreg[H][KS][4], vreg[H][4][VD];
-    int id[H];
-    int64_t at[H];
-    auto place = [&](int t, int k) {
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            id[h] = __builtin_amdgcn_readlane(pages, k * H + h);
-            at[h] = max(id[h], 0) * P.page_stride + (int64_t)((uint32_t)(((t + h) * 16) & (P.page - 1)) * (uint64_t)ps);
+    for (int64_t w = blockIdx.x; item_of(plan, A.n_q, geo, w, it); w += gridDim.x) {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));  // (the lane's offsets anew for each item: kept over the loop they spill)
+        const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
+        const int unit = (int)(w % geo.units);
+        const int kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
+        const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0), n_rows = it.count * heads;
+        const float scale2 = A.scale * 1.44269504088896340736f;
+        if constexpr (C::kNan) {
+            if (tid < HDP) nans.first[tid] = INT32_MAX;
+            if (tid == 0) nans.any = 0;
+            __syncthreads();
         }
-    };
-    auto load_k = [&]() {
-#pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                v4u v;
-                if constexpr (FULL) v = *(const v4u*)(kpool + at[h] + 64 * s + (koff + kcol));
-                else v = *(const v4u*)(kpool + at[h] + (koff + ((int)(64 * s + kcol) < hd ? 64 * s + kcol : 0)));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) kreg[h][s][e] = v[e];
-            }
-    };
-    auto load_v = [&]() {
-#pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                typedef uint32_t vec __attribute__((ext_vector_type(VD == 1 ? 2 : VD)));
-                const char* src = vpool + at[h] + voff[i];
-                if constexpr (VD == 1) vreg[h][i][0] = *(const uint32_t*)src;
-                else {
-                    const vec v = *(const vec*)src;
-#pragma unroll
-                    for (int e = 0; e < VD; ++e) vreg[h][i][e] = v[e];
-                }
-            }
-    };
-    int t = t0, k = 0;  // the tile's first half, its number in the batch
-    if (t < t_end) {
-        place(t, 0);
-        load_k();
-        load_v();
-        if (t + 64 / H * (4 * H) < t_end) pages_next = page_batch(1);
-    }
-    // this lane's rows (those past the last repeat it)
-    int limit[NR], least = INT32_MAX, qcol[2 * KS];
-    bool qin[2 * KS];
-#pragma unroll
-    for (int s = 0; s < 2 * KS; ++s) {
-        qcol[s] = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-        qin[s] = FULL || qcol[s] < hd;
-    }
-    V8 qreg[NR][QP][2 * KS];
-    float row_scale[NR];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        const int rho = min(16 * n + r, n_rows - 1), tok = it.token + rho / heads, head = h0 + rho % heads;
-        limit[n] = seen(A, pos, P, tok, it.row);
-        least = min(least, limit[n]);
-        row_scale[n] = scale2 * load_query<TQ>((const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd, qcol, qin, qreg[n],
-                                               [](float v) { return head_max(v); });
-    }
-#pragma unroll
-    for (int o = 8; o >= 1; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
-    least = __builtin_amdgcn_readfirstlane(least);
 
-    int batch = 1;
-    while (t < t_end) {
-        const int next = t + 4 * H;
-        const bool more = next < t_end;
-        float ks[H], vs[H];
-        bool okh[H], absent = false;
+        const uint32_t ps = (uint32_t)P.pos_stride;
+        const uint32_t kcol = 16 * g, koff = r * ps, vcol = D * r;
+        const bool vin = FULL || (int)vcol < hd;
+        uint32_t voff[4];
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-            ks[h] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks_lane), k * H + h));
-            vs[h] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs_lane), k * H + h));
-            okh[h] = id[h] >= 0;
-            absent |= !okh[h];
-        }
-        const bool partial = (t + H) * 16 > least || absent;  // some row does not see some position
-        float x[NR][H][4];
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            v4f c[NR];
-#pragma unroll
-            for (int n = 0; n < NR; ++n) c[n] = (v4f){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                if constexpr (!FULL) {
-                    const bool in = (int)(64 * s + kcol) < hd;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) kreg[h][s][e] = in ? kreg[h][s][e] : 0;
-                }
-#pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    const V8 key = __builtin_bit_cast(V8, Operand<C, M>::eight(kreg[h][s][2 * f], kreg[h][s][2 * f + 1]));
-#pragma unroll
-                    for (int p = QP - 1; p >= 0; --p)  // the small parts first
-#pragma unroll
-                        for (int n = 0; n < NR; ++n) c[n] = mfma16(key, qreg[n][p][2 * s + f], c[n]);
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < NR; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[n][h][i] = c[n][i] * (row_scale[n] * ks[h]);
-                    if (partial && (!okh[h] || (t + h) * 16 + 4 * g + i >= limit[n])) x[n][h][i] = -INFINITY;
-                }
-        }
-        const int t_now = t;
-        if (more) {
-            if (++k == 64 / H) {
-                k = 0;
-                pages = pages_next;
-                ks_lane = ks_next;
-                vs_lane = vs_next;
-                pages_next = page_batch(++batch);
-            } else if (k == 2) {
-                ks_next = scale_batch(kscale, batch, pages_next);
-                vs_next = scale_batch(vscale, batch, pages_next);
-            }
-            place(next, k);
-            load_k();
-        }
-        // values that no row of the item sees may hold anything, and a NaN belongs to the rows that see
-        // its position (a weight of zero would not keep it from the others): zeros in their place, and
-        // a column's first NaN noted
-        if (partial)
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int p = (t_now + h) * 16 + 4 * g + i;
-                    const bool in = okh[h] && p < it.limit && vin;
-#pragma unroll
-                    for (int e = 0; e < VD; ++e) {
-                        uint32_t& v = vreg[h][i][e];
-                        v = in ? v : 0;
-                        if constexpr (C::kNan)
-                            if (((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u)
-                                for (int b = 0; b < 32; b += 8)
-                                    if ((v >> b & 0x7F) == 0x7F) {
-                                        v &= ~(0xFFu << b);
-                                        atomicMin(&nans.first[vcol + 4 * e + b / 8], p);
-                                        nans.any = 1;
-                                    }
-                    }
-                }
-        v8bf part[NR][WP];
+        for (int i = 0; i < 4; ++i) voff[i] = (4 * g + i) * ps + (vin ? vcol : 0);
+        const char* kpool = (const char*)P.k + (int64_t)kh * P.head_stride;
+        const char* vpool = (const char*)P.v + (int64_t)kh * P.head_stride;
+        const float* kscale = P.k_scale + (int64_t)kh * P.scale_head_stride;
+        const float* vscale = P.v_scale + (int64_t)kh * P.scale_head_stride;
+
+        const int32_t* table = A.table + (int64_t)it.row * A.table_stride;
+        const int t_last = (it.limit + 15) / 16 - 1;  // the last half tile (16 positions) with a position
+        const int t_end = min(it.end * (kFewKeys / 16), t_last + 1);
+        // lane j: the page (-1: absent) and scales of the wave's half tile j of a batch of 64
+        const int t0 = it.first * (kFewKeys / 16) + wave * H, log_p = P.shift - kScaleShift, block_mask = (P.page >> kScaleShift) - 1;
+        auto tile_of = [&](int batch) { return t0 + (batch * 64 + lane) / H * (4 * H) + (lane & (H - 1)); };
+        auto page_batch = [&](int batch) {
+            const int t = tile_of(batch);
+            int id = -1;
+            if (t < t_end) id = table[t >> log_p];
+            return kv_page_ok(id, P.n_pages) ? id : -1;
+        };
+        auto scale_batch = [&](const float* scales, int batch, int id) {
+            float s = 0.0f;
+            if (id >= 0) s = scales[(int64_t)id * P.scale_page_stride + (tile_of(batch) & block_mask)];
+            return s;
+        };
+        int pages = page_batch(0), pages_next = -1;
+        float ks_lane = scale_batch(kscale, 0, pages), vs_lane = scale_batch(vscale, 0, pages), ks_next = 0.0f, vs_next = 0.0f;
+
+        v4f acc[NR][D];
+        float m[NR], l[NR];
 #pragma unroll
         for (int n = 0; n < NR; ++n) {
-            float mx = x[n][0][0];
+            m[n] = -INFINITY;
+            l[n] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < D; ++d) acc[n][d] = (v4f){0.f, 0.f, 0.f, 0.f};
+        }
+        uint32_t kreg[H][KS][4], vreg[H][4][VD];
+        int id[H];
+        int64_t at[H];
+        auto place = [&](int t, int k) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                id[h] = __builtin_amdgcn_readlane(pages, k * H + h);
+                at[h] = max(id[h], 0) * P.page_stride + (int64_t)((uint32_t)(((t + h) * 16) & (P.page - 1)) * (uint64_t)ps);
+            }
+        };
+        auto load_k = [&]() {
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[n][h][i]);
-            if (__any(mx > m[n])) {
-                const float mn = fmaxf(m[n], head_max(mx));
-                const float al = m[n] > -INFINITY ? exp2_fast(m[n] - mn) : 1.0f;  // nothing but zeros before
-                l[n] *= al;
+                for (int s = 0; s < KS; ++s) {
+                    v4u v;
+                    if constexpr (FULL) v = *(const v4u*)(kpool + at[h] + 64 * s + (koff + kcol));
+                    else v = *(const v4u*)(kpool + at[h] + (koff + ((int)(64 * s + kcol) < hd ? 64 * s + kcol : 0)));
 #pragma unroll
-                for (int d = 0; d < D; ++d) acc[n][d] *= al;
-                m[n] = mn;
-            }
-            const float base = m[n] > -INFINITY ? m[n] : 0.0f;
+                    for (int e = 0; e < 4; ++e) kreg[h][s][e] = v[e];
+                }
+        };
+        auto load_v = [&]() {
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float v = exp2_fast(x[n][h][i] - base);
-                    l[n] += v;
-                    v *= vs[h];
+                    typedef uint32_t vec __attribute__((ext_vector_type(VD == 1 ? 2 : VD)));
+                    const char* src = vpool + at[h] + voff[i];
+                    if constexpr (VD == 1) vreg[h][i][0] = *(const uint32_t*)src;
+                    else {
+                        const vec v = *(const vec*)src;
 #pragma unroll
-                    for (int p = 0; p < WP; ++p) {
-                        part[n][p][4 * h + i] = (__bf16)v;
-                        v -= (float)part[n][p][4 * h + i];
+                        for (int e = 0; e < VD; ++e) vreg[h][i][e] = v[e];
                     }
                 }
+        };
+        int t = t0, k = 0;  // the tile's first half, its number in the batch
+        if (t < t_end) {
+            place(t, 0);
+            load_k();
+            load_v();
+            if (t + 64 / H * (4 * H) < t_end) pages_next = page_batch(1);
+        }
+        // this lane's rows (those past the last repeat it)
+        int limit[NR], least = INT32_MAX, qcol[2 * KS];
+        bool qin[2 * KS];
+#pragma unroll
+        for (int s = 0; s < 2 * KS; ++s) {
+            qcol[s] = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+            qin[s] = FULL || qcol[s] < hd;
+        }
+        V8 qreg[NR][QP][2 * KS];
+        float row_scale[NR];
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const int rho = min(16 * n + r, n_rows - 1), tok = it.token + rho / heads, head = h0 + rho % heads;
+            limit[n] = seen(A, pos, P, tok, it.row);
+            least = min(least, limit[n]);
+            row_scale[n] = scale2 * load_query<TQ>((const TQ*)A.q + (int64_t)tok * A.q_stride + (int64_t)head * hd, qcol, qin, qreg[n],
+                                                   [](float v) { return head_max(v); });
         }
 #pragma unroll
-        for (int q = 0; q < VD; ++q) {
-            uint32_t col[4][4];  // [pair of positions][column]
-#pragma unroll
-            for (int j = 0; j < 4; ++j)  // positions 2 j and 2 j + 1 of the lane's eight
-                Operand<C, __bf16>::columns(vreg[j >> 1][2 * (j & 1)][q], vreg[j >> 1][2 * (j & 1) + 1][q], col[j]);
-#pragma unroll
-            for (int p = WP - 1; p >= 0; --p)
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-#pragma unroll
-                    for (int n = 0; n < NR; ++n)
-                        acc[n][4 * q + c] = mfma16(__builtin_bit_cast(v8bf, (v4u){col[0][c], col[1][c], col[2][c], col[3][c]}), part[n][p], acc[n][4 * q + c]);
-        }
-        if (more) load_v();
-        t = next;
-    }
+        for (int o = 8; o >= 1; o >>= 1) least = min(least, __shfl_xor(least, o, 64));
+        least = __builtin_amdgcn_readfirstlane(least);
 
-    // the four waves' sums, 16 rows at a time
-    const bool alone = it.pieces == 1;
-    float* to = plan.partial + ((size_t)it.part * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
+        int batch = 1;
+        while (t < t_end) {
+            const int next = t + 4 * H;
+            const bool more = next < t_end;
+            float ks[H], vs[H];
+            bool okh[H], absent = false;
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-        if (16 * n >= n_rows) break;
-        if (n) __syncthreads();
-        l[n] = head_sum(l[n]);
-        if (g == 0) {
-            s_m[wave][r] = m[n];
-            s_l[wave][r] = l[n];
-        }
-        __syncthreads();
-        float M = s_m[0][r];
-#pragma unroll
-        for (int w2 = 1; w2 < 4; ++w2) M = fmaxf(M, s_m[w2][r]);
-        const float f = m[n] > -INFINITY ? exp2_fast(m[n] - M) : 1.0f;  // (no weights, or NaN: as they are)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < D; ++e) s_acc[wave][r][(4 * g + i) * D + e] = acc[n][e][i] * f;
-        __syncthreads();
-        const int per = hd / 4;
-        for (int o = tid; o < min(16, n_rows - 16 * n) * per; o += 256) {
-            const int row = o / per, c = 4 * (o - row * per), rho = 16 * n + row, tok = it.token + rho / heads;
-            float top = s_m[0][row], sum = 0.0f;
-#pragma unroll
-            for (int w2 = 1; w2 < 4; ++w2) top = fmaxf(top, s_m[w2][row]);
-            v4f v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int w2 = 0; w2 < 4; ++w2) {
-                sum += s_l[w2][row] * (s_m[w2][row] > -INFINITY ? exp2_fast(s_m[w2][row] - top) : 1.0f);
-                v += *(const v4f*)&s_acc[w2][row][c];
+            for (int h = 0; h < H; ++h) {
+                ks[h] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks_lane), k * H + h));
+                vs[h] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vs_lane), k * H + h));
+                okh[h] = id[h] >= 0;
+                absent |= !okh[h];
             }
-            if constexpr (C::kNan)
-                if (nans.any) {
-                    const int lim = seen(A, pos, P, tok, it.row);
+            const bool partial = (t + H) * 16 > least || absent;  // some row does not see some position
+            float x[NR][H][4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (nans.first[c + e] < lim) v[e] = NAN;
+            for (int h = 0; h < H; ++h) {
+                v4f c[NR];
+#pragma unroll
+                for (int n = 0; n < NR; ++n) c[n] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    if constexpr (!FULL) {
+                        const bool in = (int)(64 * s + kcol) < hd;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) kreg[h][s][e] = in ? kreg[h][s][e] : 0;
+                    }
+#pragma unroll
+                    for (int f = 0; f < 2; ++f) {
+                        const V8 key = __builtin_bit_cast(V8, Operand<C, M>::eight(kreg[h][s][2 * f], kreg[h][s][2 * f + 1]));
+#pragma unroll
+                        for (int p = QP - 1; p >= 0; --p)  // the small parts first
+#pragma unroll
+                            for (int n = 0; n < NR; ++n) c[n] = mfma16(key, qreg[n][p][2 * s + f], c[n]);
+                    }
                 }
-            if (alone) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const float out[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
-                store4((TQ*)A.out + (int64_t)tok * A.out_stride + (int64_t)(h0 + rho % heads) * hd + c, out);
-            } else {
-                *(v4f*)(to + 2 * geo.rows + (size_t)rho * hd + c) = v;
-                if (c == 0) *(float2*)(to + 2 * rho) = make_float2(top, sum);
+#pragma unroll
+                for (int n = 0; n < NR; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[n][h][i] = c[n][i] * (row_scale[n] * ks[h]);
+                        if (partial && (!okh[h] || (t + h) * 16 + 4 * g + i >= limit[n])) x[n][h][i] = -INFINITY;
+                    }
+            }
+            const int t_now = t;
+            if (more) {
+                if (++k == 64 / H) {
+                    k = 0;
+                    pages = pages_next;
+                    ks_lane = ks_next;
+                    vs_lane = vs_next;
+                    pages_next = page_batch(++batch);
+                } else if (k == 2) {
+                    ks_next = scale_batch(kscale, batch, pages_next);
+                    vs_next = scale_batch(vscale, batch, pages_next);
+                }
+                place(next, k);
+                load_k();
+            }
+            // values that no row of the item sees may hold anything, and a NaN belongs to the rows that see
+            // its position (a weight of zero would not keep it from the others): zeros in their place, and
+            // a column's first NaN noted
+            if (partial)
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int p = (t_now + h) * 16 + 4 * g + i;
+                        const bool in = okh[h] && p < it.limit && vin;
+#pragma unroll
+                        for (int e = 0; e < VD; ++e) {
+                            uint32_t& v = vreg[h][i][e];
+                            v = in ? v : 0;
+                            if constexpr (C::kNan)
+                                if (((v & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u)
+                                    for (int b = 0; b < 32; b += 8)
+                                        if ((v >> b & 0x7F) == 0x7F) {
+                                            v &= ~(0xFFu << b);
+                                            atomicMin(&nans.first[vcol + 4 * e + b / 8], p);
+                                            nans.any = 1;
+                                        }
+                        }
+                    }
+            v8bf part[NR][WP];
+#pragma unroll
+            for (int n = 0; n < NR; ++n) {
+                float mx = x[n][0][0];
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[n][h][i]);
+                if (__any(mx > m[n])) {
+                    const float mn = fmaxf(m[n], head_max(mx));
+                    const float al = m[n] > -INFINITY ? exp2_fast(m[n] - mn) : 1.0f;  // nothing but zeros before
+                    l[n] *= al;
+#pragma unroll
+                    for (int d = 0; d < D; ++d) acc[n][d] *= al;
+                    m[n] = mn;
+                }
+                const float base = m[n] > -INFINITY ? m[n] : 0.0f;
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v = exp2_fast(x[n][h][i] - base);
+                        l[n] += v;
+                        v *= vs[h];
+#pragma unroll
+                        for (int p = 0; p < WP; ++p) {
+                            part[n][p][4 * h + i] = (__bf16)v;
+                            v -= (float)part[n][p][4 * h + i];
+                        }
+                    }
+            }
+#pragma unroll
+            for (int q = 0; q < VD; ++q) {
+                uint32_t col[4][4];  // [pair of positions][column]
+#pragma unroll
+                for (int j = 0; j < 4; ++j)  // positions 2 j and 2 j + 1 of the lane's eight
+                    Operand<C, __bf16>::columns(vreg[j >> 1][2 * (j & 1)][q], vreg[j >> 1][2 * (j & 1) + 1][q], col[j]);
+#pragma unroll
+                for (int p = WP - 1; p >= 0; --p)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int n = 0; n < NR; ++n)
+                            acc[n][4 * q + c] = mfma16(__builtin_bit_cast(v8bf, (v4u){col[0][c], col[1][c], col[2][c], col[3][c]}), part[n][p], acc[n][4 * q + c]);
+            }
+            if (more) load_v();
+            t = next;
+        }
+
+        // the four waves' sums, 16 rows at a time
+        const bool alone = it.pieces == 1;
+        float* to = plan.partial + ((size_t)it.part * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            if (16 * n >= n_rows) break;
+            if (n) __syncthreads();
+            l[n] = head_sum(l[n]);
+            if (g == 0) {
+                s_m[wave][r] = m[n];
+                s_l[wave][r] = l[n];
+            }
+            __syncthreads();
+            float M = s_m[0][r];
+#pragma unroll
+            for (int w2 = 1; w2 < 4; ++w2) M = fmaxf(M, s_m[w2][r]);
+            const float f = m[n] > -INFINITY ? exp2_fast(m[n] - M) : 1.0f;  // (no weights, or NaN: as they are)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < D; ++e) s_acc[wave][r][(4 * g + i) * D + e] = acc[n][e][i] * f;
+            __syncthreads();
+            const int per = hd / 4;
+            for (int o = tid; o < min(16, n_rows - 16 * n) * per; o += 256) {
+                const int row = o / per, c = 4 * (o - row * per), rho = 16 * n + row, tok = it.token + rho / heads;
+                float top = s_m[0][row], sum = 0.0f;
+#pragma unroll
+                for (int w2 = 1; w2 < 4; ++w2) top = fmaxf(top, s_m[w2][row]);
+                v4f v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w2 = 0; w2 < 4; ++w2) {
+                    sum += s_l[w2][row] * (s_m[w2][row] > -INFINITY ? exp2_fast(s_m[w2][row] - top) : 1.0f);
+                    v += *(const v4f*)&s_acc[w2][row][c];
+                }
+                if constexpr (C::kNan)
+                    if (nans.any) {
+                        const int lim = seen(A, pos, P, tok, it.row);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (nans.first[c + e] < lim) v[e] = NAN;
+                    }
+                if (alone) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    const float out[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+                    store4((TQ*)A.out + (int64_t)tok * A.out_stride + (int64_t)(h0 + rho % heads) * hd + c, out);
+                } else {
+                    *(v4f*)(to + 2 * geo.rows + (size_t)rho * hd + c) = v;
+                    if (c == 0) *(float2*)(to + 2 * rho) = make_float2(top, sum);
+                }
             }
         }
+        __syncthreads();  // (the sums' readers are done)
     }
 }
 
 // ---- the join ------------------------------------------------------------------------------
-// The pieces of each cut tile, in their order, four columns of a row a thread, four pieces' loads at
-// a time.
+// Running maximum, sum and weighted values of four columns, and those of further keys added to them.
+struct Joined {
+    float m, l;
+    v4f v;
+    SXQ_DEV void add(float m2, float l2, v4f v2) {
+        const float mn = fmaxf(m, m2);
+        const float up = m > -INFINITY ? exp2_fast(m - mn) : 1.0f;  // (no weights, or NaN: as they are)
+        const float f = m2 > -INFINITY ? exp2_fast(m2 - mn) : 1.0f;
+        l = l * up + l2 * f;
+        v = v * up + v2 * f;
+        m = mn;
+    }
+};
+
+// The pieces of each cut tile, four columns of a row a thread, four pieces' loads at a time.  Where there
+// are many pieces a tile, `share` threads take a row's in turn and the first joins what they have, in order:
+// one request's 8 tokens after 30000 are 2 tiles of 128 pieces (heads of 64), 5 us so and 50 in one chain.
 template <typename TQ>
 __global__ __launch_bounds__(256) void k_kv8_prefix_join(const KvAttend A, const KvPool P, const Geometry geo) {
+    __shared__ Joined s_part[256];
     const PrefixPlan plan(A.ws, A.n_q, P.hd, geo);
-    const int hd = P.hd, per = hd / 4, at_once = 256 / per;  // rows a workgroup takes at once
+    const int4 counts = *(const int4*)plan.counts;
+    const int tid = threadIdx.x, hd = P.hd, per = hd / 4, most = 256 / per;
+    const int share = max(1, min(most, counts.z / max(4 * counts.y, 1))), at_once = most / share;  // rows a workgroup takes at once
     const int steps = (geo.rows + at_once - 1) / at_once;
-    const int sub = threadIdx.x / per, col = 4 * (threadIdx.x - sub * per);
-    for (int w = blockIdx.x;; w += gridDim.x) {
-        const int step = w % steps, unit = w / steps % geo.units, k = w / steps / geo.units, row = step * at_once + sub;
-        const CutTile cut = plan.cut[min(k, geo.places - 1)];  // (with the count, not after it)
-        if (k >= plan.counts[1]) break;
+    const int sub = tid / per, col = 4 * (tid - sub * per), k_first = sub / at_once;
+    for (int w = blockIdx.x; w < counts.y * geo.units * steps; w += gridDim.x) {
+        const int step = w % steps, unit = w / steps % geo.units, row = step * at_once + sub % at_once;
+        const CutTile cut = plan.cut[w / steps / geo.units];
         const int kh = unit / geo.parts, h0 = kh * geo.group + (unit - kh * geo.parts) * geo.rows;
         const int heads = min(min(geo.rows, geo.group), (kh + 1) * geo.group - h0);
-        if (sub >= at_once || row >= cut.count * heads) continue;
+        const bool live = k_first < share && row < cut.count * heads;
         const float* part = plan.partial + ((size_t)cut.part * geo.units + unit) * PrefixPlan::part_floats(geo.rows, hd);
         const size_t stride = (size_t)geo.units * PrefixPlan::part_floats(geo.rows, hd);
-        float m = -INFINITY, l = 0.0f;
-        v4f v = {0.f, 0.f, 0.f, 0.f};
-        for (int k0 = 0; k0 < cut.pieces; k0 += 4) {
+        Joined sum{-INFINITY, 0.0f, {0.f, 0.f, 0.f, 0.f}};
+        for (int k0 = k_first; live && k0 < cut.pieces; k0 += 4 * share) {
             float2 ml[4];
             v4f x[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const float* p = part + min(k0 + u, cut.pieces - 1) * stride;
+                const float* p = part + min(k0 + u * share, cut.pieces - 1) * stride;
                 ml[u] = *(const float2*)(p + 2 * row);
                 x[u] = *(const v4f*)(p + 2 * geo.rows + (size_t)row * hd + col);
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (k0 + u >= cut.pieces) break;
-                const float mn = fmaxf(m, ml[u].x);
-                const float up = m > -INFINITY ? exp2_fast(m - mn) : 1.0f;  // (no weights, or NaN: as they are)
-                const float f = ml[u].x > -INFINITY ? exp2_fast(ml[u].x - mn) : 1.0f;
-                l = l * up + ml[u].y * f;
-                v = v * up + x[u] * f;
-                m = mn;
-            }
+            for (int u = 0; u < 4; ++u)
+                if (k0 + u * share < cut.pieces) sum.add(ml[u].x, ml[u].y, x[u]);
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const float f[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+        if (share > 1) {
+            if (live && k_first) s_part[tid] = sum;
+            __syncthreads();
+            if (live && !k_first)
+                for (int i = 1; i < share; ++i) {
+                    const Joined o = s_part[tid + i * at_once * per];
+                    sum.add(o.m, o.l, o.v);
+                }
+            __syncthreads();
+        }
+        if (!live || k_first) continue;
+        const float inv = sum.l == 0.0f ? 0.0f : 1.0f / sum.l;
+        const float f[4] = {sum.v[0] * inv, sum.v[1] * inv, sum.v[2] * inv, sum.v[3] * inv};
         store4((TQ*)A.out + (int64_t)(cut.token + row / heads) * A.out_stride + (int64_t)(h0 + row % heads) * hd + col, f);
     }
 }
@@ -1033,7 +1063,11 @@ template <typename TQ, typename C, int HDP, bool FULL>
 hipError_t prefix_launch(const KvAttend& a, const int32_t* pos, const KvPool& p, const Geometry& g, hipStream_t s) {
     const int64_t most = ((int64_t)a.n_q + 2 * g.places) * g.units;
     if (g.rows == kFewRows) {
-        hipLaunchKernelGGL((k_kv8_prefix_few<TQ, C, HDP, FULL>), dim3((unsigned)most), dim3(256), 0, s, a, pos, p, g);
+        // (as many as a map's tiles and pieces, were each row of the table in it, but not tens of
+        // thousands that find nothing)
+        const int64_t tiles = (a.n_q + g.tokens - 1) / g.tokens + std::min(a.n_rows, a.n_q) + 2 * (int64_t)g.places;
+        const int grid = (int)std::min<int64_t>(most, std::min<int64_t>(tiles * g.units, 8192));
+        hipLaunchKernelGGL((k_kv8_prefix_few<TQ, C, HDP, FULL>), dim3(grid), dim3(256), 0, s, a, pos, p, g);
     } else {
         const int grid = (int)std::min<int64_t>(most, HDP <= 128 ? 512 : 256);
         hipLaunchKernelGGL((k_kv8_prefix<TQ, C, HDP, FULL>), dim3(grid), dim3(256), 0, s, a, pos, p, g);
@@ -1053,9 +1087,8 @@ template <typename TQ>
 hipError_t prefix_by_code(const KvAttend& a, const int32_t* pos, const KvPool& p, const Geometry& g, bool may_cut, hipStream_t s) {
     const hipError_t e = p.dtype == kI8 ? prefix_by_width<TQ, I8>(a, pos, p, g, s) : prefix_by_width<TQ, E4M3>(a, pos, p, g, s);
     if (e != hipSuccess || !may_cut) return e;
-    const int at_once = 256 / (p.hd / 4), steps = (g.rows + at_once - 1) / at_once;
-    const int64_t all = (int64_t)g.places * g.units * steps;  // (a cut tile has two pieces at least)
-    hipLaunchKernelGGL((k_kv8_prefix_join<TQ>), dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(1024, all))), dim3(256), 0, s, a, p, g);
+    const int64_t all = (int64_t)g.places * g.units * g.rows;
+    hipLaunchKernelGGL((k_kv8_prefix_join<TQ>), dim3((unsigned)std::min<int64_t>(1024, all)), dim3(256), 0, s, a, p, g);
     return hipGetLastError();
 }
 
@@ -1070,9 +1103,12 @@ size_t kv8_prefix_workspace(const KvPool& p, int n_q, int nh) {
 }
 
 hipError_t launch_kv8_prefix(const KvAttend& a, const int32_t* pos, const KvPool& p, hipStream_t s) {
-    const int group = a.nh / p.nkv;
-    // Drafted tokens and the like, 32 rows a request or fewer on average: the few-row kernel.
-    const bool few = (int64_t)a.n_q * group <= (int64_t)kFewRows * std::min(a.n_rows, 64) || (int64_t)a.n_q * group <= kFewRows;
+    // Few rows (drafted tokens, short prompts): the kernel of 32-row tiles.  Few / wide, us: 16 requests of
+    // 1000 positions and 5 new tokens, 32 / 8 heads of 128, bf16 24 / 31, f32 29 / 42; 64 of 16 bf16 61 / 62,
+    // f32 82 / 101; 512 after 4000 88 / 95 and 124 / 154, 1024 162 / 158 and 232 / 262, 2048 318 / 257 and 455 /
+    // 429; three prompts of 1412 tokens 47 / 39 and 65 / 56; 16 / 4 heads of 256, 512 after 4000 102 / 174, 64 of
+    // 32 142 / 107; 14 / 2 heads of 64, 256 after 4000 29 / 37, 512 51 / 38.
+    const bool few = (int64_t)a.n_q * a.nh <= (p.hd <= 64 ? 4096 : a.q_dtype == kF32 && p.hd <= 128 ? 32768 : 16384);
     const Geometry g(a.nh, p.nkv, p.hd, a.q_dtype == kF32, few);
     // (many more tiles than places, whatever the map: nothing is cut)
     const bool may_cut = (a.n_q + g.tokens - 1) / g.tokens < kRounds * g.places;
