@@ -94,6 +94,12 @@ SXQ_DEV float wave_max(float v) {
 // that.  A workgroup, of 4 waves / waves a unit heads, looks for the runs that begin among its `chunk`
 // tokens.  The queries' heads are other workgroups of the launch (from kv_groups on), QT tokens and
 // 256 / lh heads each.
+// A code needs its block's largest element, so that a block's rows have to meet before any is stored: in
+// registers, and each element is read and written once.  What bounds it: 8192 bf16 tokens of 32 + 16
+// heads of 128 take 49 us, 185 MB at 3.8 TB/s (a large copy: 5.1), 1412 f32 ones 15.4, 61 MB at 3.9: memory,
+// and the start of workgroups; a step's few tokens 4.7, where an empty launch takes 2: the loads of slots,
+// rows and angles, which wait for each other.  (The queries by a launch of their own: 70 against 66 us
+// for the 8192, before the keys' and values' part was as it is.)
 template <typename TI, typename C, int NP, int QT>
 __global__ __launch_bounds__(256) void k_kv8_append(const KvAppend A, const KvPool P, int lh, int chunk, int kv_groups, int q_groups) {
     __shared__ float2 s_amax[2][4];
@@ -297,7 +303,9 @@ struct Eight<E4M3> : EightCodes<E4M3> {};
 
 // A workgroup's `tokens` entries (up to kReadTokens): their slots once (range by search, page by table) through
 // LDS, then eight elements of K and V a thread at a time.  Up to kReadRanges ranges are read whole by
-// every workgroup, so that a small call is four loads in turn, not a search's too.
+// every workgroup, so that a small call is four loads in turn, not a search's too.  What bounds it:
+// 64 requests of 1000 to 16384 positions, 8 heads of 128, from int8 into bf16 in 416 us, the codes in and
+// the values out at a copy's rate; 500 positions in 4.2.
 constexpr int kReadTokens = 16, kReadRanges = 255, kReadAhead = 4;
 template <typename T, typename TO>
 __global__ __launch_bounds__(256) void k_kv_read(const KvRead A, const KvPool P, int tokens) {

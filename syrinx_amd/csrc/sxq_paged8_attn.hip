@@ -31,6 +31,10 @@ inline int attend_places(int hd) { return hd <= 64 ? 1024 : hd <= 128 ? 512 : 25
 // weights before these are cut into bf16 parts (three under f32 queries, else two).  Lane (r, g) of the result holds head r at
 // positions 4 g + i; the weights are used in those registers, so the lane loads HDP / 16 columns of
 // the values 4 g + i, two of a column meeting in a register by byte permutes before they are widened.
+// What bounds it: the keys' and values' bytes, 64 requests of 1000 to 16384 positions, 32 / 8 heads of 128
+// in 153 us, 4.7 TB/s (two workgroups a CU for the registers; three are 151 there and 17.8 against 16 us for
+// 16 requests of 256 to 2045; tiles of 64 positions a wave instead of 32: 153 and 18.5); 16 requests in
+// 16 us, of which 6 are the bytes and the rest the launch, the first loads one after another and the join.
 template <typename TQ, typename C, int HDP, bool FULL>
 __global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv8_attend(const KvAttend A, const KvPool P,
                                                                                          int target) {

@@ -97,7 +97,8 @@ SXQ_DEV int seen(const KvAttend& A, const int32_t* pos, const KvPool& P, int t, 
 // A thousand queries at a time, a thread each (the next chunk's under way): where its run began and
 // which tile it is in by ballots, the last two thousand tiles in LDS.  While there are no more than a
 // thousand tiles they stay there until all queries are seen, so that a short call's tiles are cut where
-// they are, and are written once, the last tile first.
+// they are, and are written once, the last tile first.  80 queries 5 us, 1412 6.3: an empty launch and the loads
+// of rows, lengths and positions, which wait for each other.
 constexpr int kTilesKept = 1024, kTileRing = 2 * kTilesKept;
 __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, const int32_t* pos, const KvPool P, const Geometry g,
                                                           bool may_cut) {
@@ -291,7 +292,11 @@ struct Nans {
 // 4 (lane / 32) + i % 4) and the softmax of a row is two lanes'; weighted values: A = 32 columns x 16 keys,
 // B = the weights in the registers that the scores came in, the values' keys laid out in LDS to match.
 // What bounds it: the matrix cores' products and the lanes' work on the weights (an exponential, the
-// maximum, the sum, the rounding) take turns on a SIMD's two waves.
+// maximum, the sum, the rounding) take turns on a SIMD's two waves.  A chunk of 2048 bf16 queries after 30720
+// positions, 32 / 8 heads of 128, takes 1320 us, 800 TFLOP/s (a large matrix product: 1217); f32 queries,
+// in two parts, and weights in three, 1.7 to 1.85 times a bf16 call.  Of a short prompt much is the beginning
+// (tile, pages, scales, codes and queries, loads that wait for each other): a call of one tile of keys
+// takes 9.5 us (f32 14.7), each further one of that item 2.1 (3.5).
 template <typename TQ, typename C, int HDP, bool FULL>
 __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const KvAttend A, const int32_t* pos,
                                                                                                  const KvPool P, const Geometry geo) {
@@ -671,7 +676,8 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
 // ---- few rows ------------------------------------------------------------------------------
 // One item of up to 32 rows: the waves go through the keys as those of k_kv8_attend do, 32 each of every
 // 128, keys and values straight into registers, two tiles of 16 rows on each operand; then the four
-// waves' sums are added up through LDS.  What bounds it is the keys' bytes, or latency.
+// waves' sums are added up through LDS.  What bounds it is the keys' bytes, or latency: 16 requests' 5 drafted
+// tokens over 256 to 2040 positions in 14 us, of which 4.3 are the bytes.
 template <typename TQ, typename C, int HDP, bool FULL>
 __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(const KvAttend A, const int32_t* pos, const KvPool P,
                                                                           const Geometry geo) {

@@ -466,6 +466,19 @@ def test_attend_many_requests(cuda, ct, n, long):
 PREFIX_SPLIT = {"f32": 4 * U32, "f16": 2.0 ** -17, "bf16": 2.0 ** -8}
 
 
+def _attend(cache, q, rows, pos, form):
+    """attend, as one token's (form False), or over prefixes by tiles of few rows (True) or of many, as
+    calls of more than 32768 rows of heads take them: entries of no request fill it up."""
+    if form != "wide":
+        return cache.attend(0, q, rows=rows, pos=pos)
+    n, more = q.shape[0], 32768 // q.shape[1] + 1
+    none = torch.full((more,), -1, dtype=torch.int32, device=q.device)
+    out = torch.full((n + more, *q.shape[1:]), 7.0, dtype=q.dtype, device=q.device)
+    cache.attend(0, torch.cat([q, torch.zeros_like(out[n:])]), rows=torch.cat([rows, none]), pos=torch.cat([pos, none]), out=out)
+    assert bool((out[n:] == 7).all())
+    return out[:n]
+
+
 def _check_prefix(cache, g, cuda, rows, pos, nh, qt, scale=None, some=None):
     hd, n = cache.head_dim, len(rows)
     i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
@@ -479,6 +492,9 @@ def _check_prefix(cache, g, cuda, rows, pos, nh, qt, scale=None, some=None):
     _close(got[some][live], want[live], bound[live], DT[qt], f"{nh}/{cache.n_kv_heads}x{hd}")
     assert bool((got[some][~live] == 7).all())
     assert torch.equal(cache.attend(0, q, rows=i32(rows), pos=i32(pos), scale=scale, out=torch.full_like(q, 7.0)), got)
+    if scale is None:
+        wide = _attend(cache, q, i32(rows), i32(pos), "wide")
+        _close(wide[some][live], want[live], bound[live], DT[qt], f"{nh}/{cache.n_kv_heads}x{hd}, many rows a tile")
     return q, got
 
 
@@ -532,6 +548,29 @@ def test_prefix_of_the_last_token_is_attend(cuda, ct):
     assert float(((one - got).abs().to(F64) - 2 * (bound + U32 * want.abs())).max()) <= 0
 
 
+@pytest.mark.parametrize("n,nh,nkv,hd", [(2500, 1, 1, 16), (1500, 64, 64, 16), (1100, 16, 16, 128), (2048, 2, 1, 128)])
+def test_prefix_of_many_tiles(cuda, n, nh, nkv, hd):
+    """Requests that take turns, so that each query is a tile: more of them than stay in LDS, or than are
+    cut; one run over a thousand queries among them."""
+    lens = [40, 25, 2000]
+    cache, g = _filled(cuda, nkv, hd, 16, lens, "e4m3", n)
+    rng = np.random.default_rng(n)
+    rows, pos = [i % 2 for i in range(n)], rng.integers(0, 40, n).tolist()
+    at = n // 2 - 20
+    rows[at:at + 40], pos[at:at + 40] = [2] * 40, list(range(1900, 1940))
+    some = rng.permutation(n)[:60].tolist() + [0, n - 1, at, at + 39]
+    _check_prefix(cache, g, cuda, rows, pos, nh, "bf16", some=some)
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("nh,nkv,hd", [(14, 2, 64), (6, 2, 48), (4, 1, 256)])
+def test_prefix_of_few_tiles_in_many_pieces(cuda, qt, ct, nh, nkv, hd):
+    """A few queries after a long prefix: a row's pieces are joined by several threads."""
+    cache, g = _filled(cuda, nkv, hd, 64, [20000, 50], ct, hd)
+    _check_prefix(cache, g, cuda, [0] * 5, list(range(19995, 20000)), nh, qt)
+    _check_prefix(cache, g, cuda, [0, 1], [12345, 49], nh, qt)
+
+
 @pytest.mark.parametrize("n", [3000])
 def test_prefix_many_requests(cuda, n):
     rng = np.random.default_rng(n)
@@ -544,7 +583,7 @@ def test_prefix_many_requests(cuda, n):
 
 
 @pytest.mark.parametrize("qt,ct", TYPES)
-@pytest.mark.parametrize("prefix", [False, True])
+@pytest.mark.parametrize("prefix", [False, True, "wide"])
 def test_attention_of_unlike_scales(cuda, qt, ct, prefix):
     """Blocks whose scales lie many powers of two apart, keys and values both; peaked, flat and equal
     scores; a scale near the smallest."""
@@ -558,13 +597,13 @@ def test_attention_of_unlike_scales(cuda, qt, ct, prefix):
     q = _queries(g, cuda, 2, 4, hd, qt)
     rows = torch.tensor([0, 1], dtype=torch.int32, device=cuda)
     pos = torch.full((2,), L - 1, dtype=torch.int32, device=cuda) if prefix else None
-    got = cache.attend(0, q, rows=rows, pos=pos)
+    got = _attend(cache, q, rows, pos, prefix)
     want, bound = _reference(q, cache, [0, 1], [L, L], hd ** -0.5, split=PREFIX_SPLIT[qt] if prefix else None)
     # (weights below 2^-126 of their largest times a value's scale may be flushed: 2^-120 of that scale's values)
     _close(got, want, bound + 2.0 ** -100, DT[qt])
 
 
-@pytest.mark.parametrize("prefix", [False, True])
+@pytest.mark.parametrize("prefix", [False, True, "wide"])
 def test_attention_of_codes_that_are_nan(cuda, prefix):
     """An e4m3 NaN makes the heads that read it NaN, and no others; past a query's positions, in absent
     pages and behind the length none is reached."""
@@ -575,13 +614,13 @@ def test_attention_of_codes_that_are_nan(cuda, prefix):
     pos = torch.tensor([n - 1 for n in lens], dtype=torch.int32, device=cuda) if prefix else None
     for qt in ("f32", "bf16", "f16"):
         q = _queries(g, cuda, 3, 4, 64, qt)
-        clean = cache.attend(0, q, rows=rows, pos=pos).clone()
+        clean = _attend(cache, q, rows, pos, prefix).clone()
         assert bool(clean.isfinite().all())
         t = cache.table.tolist()
         was = cache.k[0, t[1][1], 0, 3, 5].clone(), cache.v[0, t[0][1], 1, 7, 9].clone()
         cache.k[0, t[1][1], 0, 3, 5] = nan
         cache.v[0, t[0][1], 1, 7, 9] = nan  # request 0's last position, column 9
-        got = cache.attend(0, q, rows=rows, pos=pos)
+        got = _attend(cache, q, rows, pos, prefix)
         assert bool(got[1, :2].isnan().all()) and torch.equal(got[1, 2:], clean[1, 2:])
         assert torch.equal(got[0, :2], clean[0, :2]) and torch.equal(got[2], clean[2])
         assert bool(got[0, 2:, 9].isnan().all())
@@ -590,14 +629,14 @@ def test_attention_of_codes_that_are_nan(cuda, prefix):
         if prefix:  # queries that do not see them, beside others that do
             both = torch.cat([q, q]).view(2, 3, 4, 64).transpose(0, 1).reshape(6, 4, 64).contiguous()
             two = torch.tensor([0, 0, 1, 1, 2, 2], dtype=torch.int32, device=cuda)
-            got = cache.attend(0, both, rows=two, pos=torch.tensor([38, 39, 34, 99, 16, 16], dtype=torch.int32, device=cuda))
+            got = _attend(cache, both, two, torch.tensor([38, 39, 34, 99, 16, 16], dtype=torch.int32, device=cuda), prefix)
             assert bool(got[0::2].isfinite().all()) and torch.equal(got[5], clean[2])
-            got = cache.attend(0, q, rows=rows, pos=torch.tensor([38, 34, 16], dtype=torch.int32, device=cuda))
+            got = _attend(cache, q, rows, torch.tensor([38, 34, 16], dtype=torch.int32, device=cuda), prefix)
             assert bool(got.isfinite().all())
         cache.k[0, t[1][1], 0, 3, 5], cache.v[0, t[0][1], 1, 7, 9] = was
 
 
-@pytest.mark.parametrize("prefix", [False, True])
+@pytest.mark.parametrize("prefix", [False, True, "wide"])
 @pytest.mark.parametrize("ct", ["i8", "e4m3"])
 def test_attention_over_absent_pages(cuda, ct, prefix):
     cache, g = _filled(cuda, 2, 64, 16, [200, 33, 64], ct, 11)
@@ -608,19 +647,20 @@ def test_attention_over_absent_pages(cuda, ct, prefix):
     rows = torch.arange(3, dtype=torch.int32, device=cuda)
     pos = torch.tensor([199, 32, 63], dtype=torch.int32, device=cuda) if prefix else None
     want, bound = _reference(q, cache, range(3), [200, 33, 64], 0.125, split=PREFIX_SPLIT["bf16"])
-    got = cache.attend(0, q, rows=rows, pos=pos)
+    got = _attend(cache, q, rows, pos, prefix)
     _close(got, want, bound, torch.bfloat16)
     assert not bool(got[2].any())
     # lengths outside the table's width: negative is empty, too long its whole width
     cache.lens.copy_(torch.tensor([-3, 2**31 - 1, 64], dtype=torch.int32))
     if prefix:
-        got = cache.attend(0, q, rows=rows, pos=torch.full_like(pos, 2**31 - 1))
+        got = _attend(cache, q, rows, torch.full_like(pos, 2**31 - 1), prefix)
     else:
         got = cache.attend(0, q, rows=rows)
     assert not bool(got[0].any()) and not bool(got[2].any())
 
 
-def test_prefix_queries_before_a_nan(cuda):
+@pytest.mark.parametrize("prefix", [True, "wide"])
+def test_prefix_queries_before_a_nan(cuda, prefix):
     """Queries of one tile before and after a NaN key and a NaN value: those that do not see it are as
     without it, the others NaN (of the value: in its column)."""
     cache, g = _filled(cuda, 2, 64, 16, [300], "e4m3", 3)
@@ -629,12 +669,12 @@ def test_prefix_queries_before_a_nan(cuda):
     pos = torch.arange(300, dtype=torch.int32, device=cuda)
     for qt in ("f32", "bf16", "f16"):
         q = _queries(g, cuda, 300, 4, 64, qt)
-        clean = cache.attend(0, q, rows=rows, pos=pos).clone()
+        clean = _attend(cache, q, rows, pos, prefix).clone()
         at_v, at_k = int(cache.table[0, 70 // 16]), int(cache.table[0, 200 // 16])
         was = cache.v[0, at_v, 1, 70 % 16, 9].clone(), cache.k[0, at_k, 0, 200 % 16, 0].clone()
         cache.v[0, at_v, 1, 70 % 16, 9] = nan
         cache.k[0, at_k, 0, 200 % 16, 0] = nan
-        got = cache.attend(0, q, rows=rows, pos=pos)
+        got = _attend(cache, q, rows, pos, prefix)
         cols = [c for c in range(64) if c != 9]
         assert torch.equal(got[:70], clean[:70]) and torch.equal(got[:200, :2], clean[:200, :2])
         assert bool(got[70:, 2:, 9].isnan().all()) and bool(got[200:, :2].isnan().all())
