@@ -89,7 +89,7 @@ struct PrefixPlan {
 };
 
 // The positions that a query sees, of its request's length and its position.
-SXQ_DEV int seen_of(int len, int pos, int max_blocks, int shift) { return min(kv_clamp_len(len, max_blocks, shift), max(pos, -1) + 1); }
+SXQ_DEV int seen_of(int len, int pos, int max_blocks, int shift) { return min(kv_clamp_len(len, max_blocks, shift) - 1, max(pos, -1)) + 1; }
 SXQ_DEV int seen(const KvAttend& A, const int32_t* pos, const KvPool& P, int t, int row) {
     return seen_of(A.lens[row], pos[t], A.max_blocks, P.shift);
 }

@@ -659,6 +659,18 @@ def test_attention_over_absent_pages(cuda, ct, prefix):
     assert not bool(got[0].any()) and not bool(got[2].any())
 
 
+@pytest.mark.parametrize("form", [True, "wide"])
+def test_prefix_positions_past_the_end(cuda, form):
+    """A position past the request's length, up to the largest there is, sees what the request has."""
+    cache, g = _filled(cuda, 2, 64, 32, [77, 300], "i8", 5)
+    q = _queries(g, cuda, 4, 4, 64, "f32")
+    rows = torch.tensor([0, 0, 1, 1], dtype=torch.int32, device=cuda)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    want = _attend(cache, q, rows, i32(76, 76, 299, 299), form)
+    assert torch.equal(_attend(cache, q, rows, i32(77, 2**31 - 1, 2**31 - 1, 2**31 - 2), form), want)
+    assert not bool(_attend(cache, q, rows, i32(-1, -2**31, -2**31, -1), form).any())
+
+
 @pytest.mark.parametrize("prefix", [True, "wide"])
 def test_prefix_queries_before_a_nan(cuda, prefix):
     """Queries of one tile before and after a NaN key and a NaN value: those that do not see it are as
