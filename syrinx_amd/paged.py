@@ -44,6 +44,7 @@ _COUNTER_BYTES = 262144  # SXQ_KV_COUNTER_BYTES: the part of a workspace that st
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _DTYPES_8 = {torch.int8: 24, torch.float8_e4m3fn: 0x101}  # SXQ_I8, SXQ_E4M3: of pages only
+_F32, _I32 = torch.float32, torch.int32
 _P = ctypes.c_void_p
 
 
@@ -200,35 +201,37 @@ class PagedKvCache:
         map's tokens must be in the order in which `reserve` lays them (a block's next to one
         another): each block of SCALE_BLOCK positions gets the smallest power of two that holds what
         it is given, or keeps a larger one, and its earlier codes follow."""
-        hd, dev, dtype, shape = self.head_dim, self.device, qkv.dtype, qkv.shape
+        hd, dev, dtype, shape, steps = self.head_dim, self.device, qkv.dtype, qkv.shape, qkv.stride()
         width = (n_heads + 2 * self.n_kv_heads) * hd
         code = _DTYPES.get(dtype)
-        if code is None or qkv.get_device() != self._index or len(shape) != 2 or shape[1] != width or qkv.stride(1) != 1:
+        if code is None or qkv.get_device() != self._index or len(shape) != 2 or shape[1] != width or steps[1] != 1:
             raise ValueError(f"PagedKvCache.append: qkv must be [T, {width}] f32, f16 or bf16 rows on {dev}, got "
                              f"{dtype} {tuple(shape)} on {qkv.device}")
         tokens = shape[0]
-        stride = qkv.stride(0) if tokens > 1 else width
+        stride = steps[0] if tokens > 1 else width
         if stride < width:
             raise ValueError(f"PagedKvCache.append: qkv's rows overlap (stride {stride}, width {width})")
         slots, pos = slot_map.slots, slot_map.pos
-        self._want("slots", slots, torch.int32)
-        self._want("pos", pos, torch.int32)
+        self._want("slots", slots, _I32)
+        self._want("pos", pos, _I32)
         if slots.numel() < tokens or pos.numel() < tokens:
             raise ValueError(f"PagedKvCache.append: {tokens} tokens, a map of {min(slots.numel(), pos.numel())}")
         qn = kn = cos = sin = None
         positions = 0
         if q_norm is not None:
-            self._want("q_norm", q_norm, torch.float32, hd)
+            self._want("q_norm", q_norm, _F32, hd)
             qn = q_norm.data_ptr()
         if k_norm is not None:
-            self._want("k_norm", k_norm, torch.float32, hd)
+            if k_norm is not q_norm:
+                self._want("k_norm", k_norm, _F32, hd)
             kn = k_norm.data_ptr()
         if rope is not None:
             c, s = rope
             positions = c.shape[0]
+            table = (positions, hd // 2)
             for name, t in (("cos", c), ("sin", s)):
-                self._want(name, t, torch.float32)
-                if t.shape != (positions, hd // 2) or positions < 1:
+                self._want(name, t, _F32)
+                if t.shape != table or positions < 1:
                     raise ValueError(f"PagedKvCache.append: {name} must be [positions, {hd // 2}], got {tuple(t.shape)}")
             cos, sin = c.data_ptr(), s.data_ptr()
         if out is None:
