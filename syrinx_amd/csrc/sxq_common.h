@@ -24,9 +24,7 @@ enum DType : int {
     kQ8_0 = 8,
     kQ4K = 12,
     kQ8K = 15,
-    kI8 = 24,       // pages of an 8-bit cache only
     kBF16 = 30,
-    kE4M3 = 0x101,  // as kI8
 };
 
 struct BlockQ8_0 { uint16_t d; int8_t qs[32]; };

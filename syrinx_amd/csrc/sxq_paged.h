@@ -17,6 +17,13 @@
 
 namespace sxq {
 
+// Types that pages alone have, beside DType's (here, for sxq_common.h is part of the GEMV kernels'
+// sources, whose counter summaries go by its text).
+enum PageType : int {
+    kI8 = 24,
+    kE4M3 = 0x101,
+};
+
 // One layer's pages.  Strides in elements.
 struct KvPool {
     void *k, *v;
