@@ -26,11 +26,13 @@ may be captured into a graph.  The reference keeps one growing tensor per stream
 (nn.rs:325-339, crates/syrinx-lm/src/cv2/attention.rs:50-66) and attend its attention of one new
 token (nn.rs:340-352).
 
-The calls of one cache share its tables, and are ordered as the caller orders its streams.
+The calls of one cache share its tables, and are ordered as the caller orders its streams.  Threads
+may attend at once, on one stream or on several, but for calls that are given one workspace.
 """
 from __future__ import annotations
 
 import ctypes
+import threading
 from dataclasses import dataclass
 from typing import Optional
 
@@ -123,7 +125,7 @@ class PagedKvCache:
         # page 0 on top of the stack
         self.free = torch.arange(self.n_pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.free_count = torch.full((1,), self.n_pages, dtype=torch.int32, device=device)
-        self._need, self._ws = {}, {}
+        self._need, self._ws, self._lock = {}, {}, threading.Lock()
 
     def _pages(self, k, v, k_scale, v_scale):
         unit, blocks = self.head_dim * self.page_size, self.page_size // SCALE_BLOCK
@@ -354,19 +356,19 @@ class PagedKvCache:
             scale = hd ** -0.5
         if n == 0:
             return out
-        if workspace is None:
-            workspace = self._kept_workspace(n, n_heads, pos is not None)
-        else:
-            self._want("workspace", workspace, torch.uint8)
         if pos is not None:
-            check(lib().sxq_kv_prefix_attention(self._index, self._layer(layer), code, q.data_ptr(), strides[0], n, n_heads,
-                                                rows, pos.data_ptr(), self.lens.data_ptr(), self.max_rows,
-                                                self.table.data_ptr(), self.max_blocks, self.max_blocks, scale,
-                                                out.data_ptr(), strides[1], workspace.data_ptr(), workspace.numel(),
-                                                self._stream()))
+            call = lib().sxq_kv_prefix_attention
+            seen = (pos.data_ptr(), self.lens.data_ptr())
+        else:
+            call, seen = lib().sxq_kv_attention, (self.lens.data_ptr(),)
+        head = (self._index, self._layer(layer), code, q.data_ptr(), strides[0], n, n_heads, rows, *seen, self.max_rows,
+                self.table.data_ptr(), self.max_blocks, self.max_blocks, scale, out.data_ptr(), strides[1])
+        if workspace is not None:
+            self._want("workspace", workspace, torch.uint8)
+            check(call(*head, workspace.data_ptr(), workspace.numel(), self._stream()))
             return out
-        check(lib().sxq_kv_attention(self._index, self._layer(layer), code, q.data_ptr(), strides[0], n, n_heads, rows,
-                                     self.lens.data_ptr(), self.max_rows, self.table.data_ptr(), self.max_blocks,
-                                     self.max_blocks, scale, out.data_ptr(), strides[1], workspace.data_ptr(),
-                                     workspace.numel(), self._stream()))
+        # a call's launches hand over through the stream's workspace: another thread's may not come between
+        with self._lock:
+            workspace = self._kept_workspace(n, n_heads, pos is not None)
+            check(call(*head, workspace.data_ptr(), workspace.numel(), self._stream()))
         return out
