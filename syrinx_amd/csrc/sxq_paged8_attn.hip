@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256, HDP <= 64 ? 4 : HDP <= 128 ? 2 : 1) void k_kv8
                     for (int q = QP - 1; q >= 0; --q) c = mfma(key, qreg[q][2 * s + f], c);  // the small parts first
                 }
             }
-            const float factor = row_scale * ks[h];
+            const float factor = score_factor<TQ>(row_scale, ks[h]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[h][i] = c[i] * factor;
         }

@@ -81,6 +81,15 @@ struct Query<float> {
     typedef _Float16 M;
     static constexpr int kQP = 2;
 };
+// What a row's products with a block's codes are to be multiplied by: the row's factor times the keys'
+// scale; of an f32 row never too large or too small for an f32 (its power of two and a scale may be 2^200
+// together, or 2^-200): infinity times a product of zero, or zero times an infinite one, would be NaN.
+template <typename TQ>
+SXQ_DEV float score_factor(float row, float scale) {
+    const float f = row * scale;
+    if constexpr (Query<TQ>::kQP == 1) return f;
+    else return __builtin_copysignf(__builtin_amdgcn_fmed3f(fabsf(f), 0x1p-126f, 0x1.fffffep127f), f);
+}
 template <typename M>
 struct Vec8;
 template <>

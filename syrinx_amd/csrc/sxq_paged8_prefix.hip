@@ -559,7 +559,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
             }
             float factor[NB];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) factor[b] = row_scale * ks[b];
+            for (int b = 0; b < NB; ++b) factor[b] = score_factor<TQ>(row_scale, ks[b]);
             float mx = -INFINITY;
             if (key0 + kKeys > least || absent) {
 #pragma unroll
@@ -851,12 +851,14 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(cons
                     }
                 }
 #pragma unroll
-                for (int n = 0; n < NR; ++n)
+                for (int n = 0; n < NR; ++n) {
+                    const float factor = score_factor<TQ>(row_scale[n], ks[h]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        x[n][h][i] = c[n][i] * (row_scale[n] * ks[h]);
+                        x[n][h][i] = c[n][i] * factor;
                         if (partial && (!okh[h] || (t + h) * 16 + 4 * g + i >= limit[n])) x[n][h][i] = -INFINITY;
                     }
+                }
             }
             const int t_now = t;
             if (more) {

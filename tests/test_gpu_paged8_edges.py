@@ -44,3 +44,32 @@ def test_threads_attend_on_one_stream_at_once(cuda):
     for i in range(2):
         assert len(got[i]) == 50
         assert all(torch.equal(x, calls[i][3]) and torch.equal(y, calls[i][4]) for x, y in got[i])
+
+
+@pytest.mark.parametrize("form", [False, True, "wide"])
+@pytest.mark.parametrize("ct", ["i8", "e4m3"])
+def test_scores_of_rows_and_scales_far_apart(cuda, ct, form):
+    """f32 queries whose power of two and the keys' scale pass f32's range together.  A huge element
+    that meets zeros in every key has scores of zero: even weights.  An infinite one that meets
+    negative codes alone has scores of -inf: no weights, zeros."""
+    L, hd = 300, 64
+    cache, g = _filled(cuda, 1, hd, 16, [L], ct, 4)
+    held = cache.table[0, :-(-L // 16)].long()
+    values = (cache.v[0, held, 0].float() * cache.v_scale[0, held, 0, 0][:, None, None]).to(F64).view(-1, hd)[:L]
+    rows, pos = _i32(cuda, [0]), _i32(cuda, [L - 1]) if form else None
+    codes = cache.k[0].float().nan_to_num(3.0)
+    q = torch.zeros((1, 2, hd), device=cuda)
+    for first, scale, by in ((0.0, 2.0 ** 60, 2.0 ** 100), (0.0, 2.0 ** 100, -2.0 ** 127), (-1.0, 2.0 ** -30, math.inf),
+                             (-2.0, 2.0 ** -100, math.inf)):
+        codes[..., 0] = first
+        cache.k[0] = codes.to(cache.k.dtype)
+        cache.k_scale[0, held] = scale
+        q[:] = 0
+        q[..., 0] = by
+        got = _attend(cache, q, rows, pos, form)
+        if first:
+            assert not bool(got.any()), (first, scale, by)
+        else:
+            # even weights, each 1 / L within 2^-16 (parts, exponential, a sum of L terms), a value off by nothing
+            off = (got[0, 0].to(F64) - values.mean(0)).abs()
+            assert bool((off <= 2.0 ** -16 * values.abs().mean(0)).all()), (first, scale, by)
