@@ -277,8 +277,13 @@ SXQ_DEV int v_swap(int col) {
     return keys_a_tile(HDP) == 64 ? (col >> 1 & 7) ^ (col >> 4 & 1) : col >> 2 & 3;
 }
 
-// Whether a scale may go into its weights' exponents: they then stay above what is flushed to zero down
-// to 2^-66 of the largest, and below infinity.
+// Whether a value scale goes into its weights' exponents, or multiplies the weights.  An exponent near the
+// scale's is rounded twice, by up to 2^-18 of the weight each time: below what one bf16 part is off by, not
+// below what two or three leave out.
+template <typename TQ>
+constexpr bool kScaleInExponent = kWeightParts<TQ> == 1;
+// Whether a scale may do so: the weights then stay above what is flushed to zero down to 2^-66 of the
+// largest, and below infinity.  Any other multiplies the values, where it takes nothing from the weights.
 SXQ_DEV bool plain_scale(float s) { return s >= 0x1p-60f && s < 0x1p100f; }
 
 // The first key of each column whose value is NaN.
@@ -305,6 +310,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
     typedef typename Query<TQ>::M M;
     typedef typename Vec8<M>::T V8;
     constexpr int QP = Query<TQ>::kQP, WP = kWeightParts<TQ>;
+    constexpr bool kLift = kScaleInExponent<TQ>;
     constexpr int KS = HDP / 16, CT = HDP / 32;  // steps over the head's elements, tiles of 32 columns
     constexpr int kKeys = Stage<HDP>::kKeys, NB = Stage<HDP>::kBlocks, KT = kKeys / 32;
     constexpr int kRowPieces = HDP / 16, KP = kKeys * kRowPieces / 256;  // pieces of 16 codes a key; a thread's
@@ -372,13 +378,18 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
         // (loads that wait for each other first, so that the others are under way with them)
         int pages = page_batch(0), pages_next = -1, batch = 0, at = 0;  // at: the next tile's first block in the batch
         float ks_lane = scale_batch(kscale, 0, pages), vs_lane = scale_batch(vscale, 0, pages), ks_next = 1.0f, vs_next = 1.0f;
-        // the exponent that a value scale puts on its weights, and what takes it out of their sum
-        float lift_lane = 0.0f, back_lane = 1.0f;
+        // what a value scale makes of its weights: the exponent that it puts on them, and what takes it out of
+        // their sum; or (kLift unset) what multiplies them
+        float lift_lane = kLift ? 0.0f : 1.0f, back_lane = 1.0f;
         bool odd_scales = false;
         auto scales_at_hand = [&]() {
             const bool plain = plain_scale(vs_lane);
-            lift_lane = plain ? __builtin_amdgcn_logf(vs_lane) : 0.0f;
-            back_lane = plain ? __builtin_amdgcn_rcpf(vs_lane) : 1.0f;
+            if constexpr (kLift) {
+                lift_lane = plain ? __builtin_amdgcn_logf(vs_lane) : 0.0f;
+                back_lane = plain ? __builtin_amdgcn_rcpf(vs_lane) : 1.0f;
+            } else {
+                lift_lane = plain ? vs_lane : 1.0f;
+            }
             odd_scales = __any(!plain);
         };
         if (blocks > b0 + 64) pages_next = page_batch(1);  // (later ones: -1 past the last block)
@@ -421,7 +432,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
             for (int b = 0; b < NB; ++b) {
                 ks_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ks_lane), at + b));
                 lift_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(lift_lane), at + b));
-                back_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(back_lane), at + b));
+                if constexpr (kLift) back_load[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(back_lane), at + b));
                 absent_load |= page(b) < 0 ? 1 << b : 0;
             }
             value_scale = 1.0f;
@@ -526,7 +537,10 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
         auto take = [&]() {  // the tile that was loaded is the one at hand
             absent = absent_load;
 #pragma unroll
-            for (int b = 0; b < NB; ++b) ks[b] = ks_load[b], lift[b] = lift_load[b], back[b] = back_load[b];
+            for (int b = 0; b < NB; ++b) {
+                ks[b] = ks_load[b], lift[b] = lift_load[b];
+                if constexpr (kLift) back[b] = back_load[b];
+            }
         };
         auto compute = [&](const Stage<HDP>& S, int key0) {
             v16f c[KT];
@@ -603,22 +617,23 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
 #pragma unroll
             for (int u = 0; u < NB; ++u) {
                 if (u + 1 < NB) fetch(u + 1);
-                // the weights of a block of 16 keys times its values' scale, which goes into the exponent;
-                // the row's sum takes it out again
-                const float down = base - lift[u];
+                // the weights of a block of 16 keys times its values' scale, and their sum without it
+                const float down = kLift ? base - lift[u] : base;
                 v8bf part[WP];
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     float x = exp2_fast(fmaf(c[u >> 1][8 * (u & 1) + j], factor[u], -down));
                     sum += x;
+                    if constexpr (!kLift) x *= lift[u];
 #pragma unroll
                     for (int p = 0; p < WP; ++p) {
                         part[p][j] = (__bf16)x;
                         x -= (float)part[p][j];
                     }
                 }
-                l = fmaf(sum, back[u], l);
+                if constexpr (kLift) l = fmaf(sum, back[u], l);
+                else l += sum;
 #pragma unroll
                 for (int p = WP - 1; p >= 0; --p)
 #pragma unroll

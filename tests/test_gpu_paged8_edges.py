@@ -73,3 +73,34 @@ def test_scores_of_rows_and_scales_far_apart(cuda, ct, form):
             # even weights, each 1 / L within 2^-16 (parts, exponential, a sum of L terms), a value off by nothing
             off = (got[0, 0].to(F64) - values.mean(0)).abs()
             assert bool((off <= 2.0 ** -16 * values.abs().mean(0)).all()), (first, scale, by)
+
+
+@pytest.mark.parametrize("qt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("form", [False, True, "wide"])
+@pytest.mark.parametrize("ct", ["i8", "e4m3"])
+def test_weights_beside_value_scales(cuda, ct, form, qt):
+    """Keys whose scores are all one power of two times the factor, so that each weight is exp(0) = 1 and
+    every sum exact: the half of the positions whose values are ones is a half, whatever the scales of
+    the other half's values (zeros), and whatever the scores."""
+    hd, L = 64, 32
+    cache, _ = _filled(cuda, 1, hd, 16, [L], ct, 5)
+    one, other = cache.table[0, :2].long().tolist()
+    cache.k[0] = torch.ones_like(cache.k[0].float()).to(cache.k.dtype)
+    cache.k_scale[0] = 0.5
+    cache.v[0] = torch.zeros_like(cache.v[0].float()).to(cache.v.dtype)
+    cache.v[0, one] = torch.ones_like(cache.v[0, one].float()).to(cache.v.dtype)
+    cache.v_scale[0, one] = 1.0
+    q = torch.zeros((1, 2, hd), dtype=DT[qt], device=cuda)
+    q[0, 0, 3], q[0, 1, 40] = 4.0, -8.0
+    rows, pos = _i32(cuda, [0]), _i32(cuda, [L - 1]) if form else None
+    for e in (0, -3, -9, -20, -33, -50, -60, -61, -100, 17, 99):
+        cache.v_scale[0, other] = 2.0 ** e
+        for scale in (0.125, 0.3, 0.7071, 1.1, 1.7):
+            n, more = 1, 32768 // 2 + 1
+            if form == "wide":
+                none = torch.full((more,), -1, dtype=torch.int32, device=cuda)
+                qq = torch.cat([q, torch.zeros((more, 2, hd), dtype=q.dtype, device=cuda)])
+                got = cache.attend(0, qq, rows=torch.cat([rows, none]), pos=torch.cat([pos, none]), scale=scale)[:n]
+            else:
+                got = cache.attend(0, q, rows=rows, pos=pos, scale=scale)
+            assert bool((got == 0.5).all()), (e, scale, float((got.float() - 0.5).abs().max()))
