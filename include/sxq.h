@@ -315,9 +315,9 @@ sxq_status sxq_kv_attention(int device, const sxq_kv_pages *pages, int q_dtype, 
  * over 8-bit pages: as sxq_kv_attention, but query i sees the positions 0 .. pos[i] of its request
  * (no more than it has; none if pos[i] < 0: zeros).  rows (not NULL) and pos are those of
  * sxq_kv_reserve's map: queries of one request that follow one another share its keys' loads,
- * whatever their positions; any other order is as right.  A weight is rounded to bf16 (2^-8 of
- * itself) for bf16 queries, is off by at most 2^-17 for f16 and 2^-22 for f32 ones.  A workspace holds nothing between
- * calls; calls that share one must not overlap. */
+ * whatever their positions; any other order is as right.  A weight is carried as there, but in a call
+ * of more than 4096 rows (n_q * n_heads) under bf16 queries it may be rounded to bf16 (2^-8 of itself).
+ * A workspace holds nothing between calls; calls that share one must not overlap. */
 sxq_status sxq_kv_prefix_attention_workspace(const sxq_kv_pages *pages, int n_q, int n_heads, size_t *bytes);
 sxq_status sxq_kv_prefix_attention(int device, const sxq_kv_pages *pages, int q_dtype, const void *q, int64_t q_stride,
                                    int n_q, int n_heads, const int32_t *rows, const int32_t *pos, const int32_t *lens,

@@ -253,13 +253,12 @@ SXQ_DEV float other_half(float v) {
     return (threadIdx.x & 32) ? a : b;
 }
 
-// Into how many bf16 parts a weight is cut.
-template <typename TQ>
-constexpr int kWeightParts = 1;
-template <>
-constexpr int kWeightParts<_Float16> = 2;
-template <>
-constexpr int kWeightParts<float> = 3;
+// Into how many bf16 parts a weight is cut.  Tiles of few rows as the attention of one token does it; those
+// of many rows into one under bf16 queries, off by 2^-8 of the weight, half a step of the output's own type:
+// a chunk of 2048 after 30720 takes 1310 us so and 1730 by two, its outputs 1.81e-3 and 1.65e-3 off (of
+// which the outputs' rounding is 1.65e-3).  (Few rows by one: 24.5 against 25.1 us for 16 drafts of 5.)
+template <typename TQ, bool MANY>
+constexpr int kWeightParts = sizeof(TQ) == 4 ? 3 : MANY && std::is_same_v<TQ, __bf16> ? 1 : 2;
 
 // A tile of keys and values in LDS, 16-bit: keys [key][element], values [column][key], the 16-byte pieces of
 // a row exchanged so that those of neighbouring rows lie on different banks.
@@ -281,7 +280,7 @@ SXQ_DEV int v_swap(int col) {
 // scale's is rounded twice, by up to 2^-18 of the weight each time: below what one bf16 part is off by, not
 // below what two or three leave out.
 template <typename TQ>
-constexpr bool kScaleInExponent = kWeightParts<TQ> == 1;
+constexpr bool kScaleInExponent = kWeightParts<TQ, true> == 1;
 // Whether a scale may do so: the weights then stay above what is flushed to zero down to 2^-66 of the
 // largest, and below infinity.  Any other multiplies the values, where it takes nothing from the weights.
 SXQ_DEV bool plain_scale(float s) { return s >= 0x1p-60f && s < 0x1p100f; }
@@ -309,7 +308,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
                                                                                                  const KvPool P, const Geometry geo) {
     typedef typename Query<TQ>::M M;
     typedef typename Vec8<M>::T V8;
-    constexpr int QP = Query<TQ>::kQP, WP = kWeightParts<TQ>;
+    constexpr int QP = Query<TQ>::kQP, WP = kWeightParts<TQ, true>;
     constexpr bool kLift = kScaleInExponent<TQ>;
     constexpr int KS = HDP / 16, CT = HDP / 32;  // steps over the head's elements, tiles of 32 columns
     constexpr int kKeys = Stage<HDP>::kKeys, NB = Stage<HDP>::kBlocks, KT = kKeys / 32;
@@ -701,7 +700,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(cons
     typedef typename Query<TQ>::M M;
     typedef typename Vec8<M>::T V8;
     constexpr int H = 2, NR = 2, KS = HDP / 64, D = HDP / 16, VD = D / 4;
-    constexpr int QP = Query<TQ>::kQP, WP = kWeightParts<TQ>;
+    constexpr int QP = Query<TQ>::kQP, WP = kWeightParts<TQ, false>;
     __shared__ float s_m[4][16], s_l[4][16];
     __shared__ __attribute__((aligned(16))) float s_acc[4][16][HDP + 4];
     __shared__ Nans<HDP> nans;

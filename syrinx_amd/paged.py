@@ -322,7 +322,8 @@ class PagedKvCache:
         its length, whatever the query's own position: of several new tokens of a request only
         the last is attended as a decoder does.  pos (int32 [n], over pages of 8 bits, with rows):
         query i sees positions 0 .. pos[i] only; queries of one request that follow one another are
-        computed together.  q: the pages' type, f32 over bf16 pages, or f32, f16 or bf16 over pages of
+        computed together, and in a call of more than 4096 rows of heads bf16 queries may have their
+        weights rounded to bf16.  q: the pages' type, f32 over bf16 pages, or f32, f16 or bf16 over pages of
         8 bits.  scale: 1 / sqrt(head_dim) by default.  A row of no request (rows[n] < 0) leaves out[n] as it was (without `out`:
         unset); an empty request gives zeros.  workspace: `workspace(n, n_heads)` (with positions:
         `workspace(n, n_heads, prefix=True)`), to keep its zeroing out of a captured graph."""

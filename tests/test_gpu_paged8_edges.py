@@ -104,3 +104,18 @@ def test_weights_beside_value_scales(cuda, ct, form, qt):
             else:
                 got = cache.attend(0, q, rows=rows, pos=pos, scale=scale)
             assert bool((got == 0.5).all()), (e, scale, float((got.float() - 0.5).abs().max()))
+
+
+@pytest.mark.parametrize("ct", ["i8", "e4m3"])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 64), (32, 8, 128), (4, 2, 256)])
+def test_drafts_keep_the_precision_of_one_token(cuda, ct, nh, nkv, hd):
+    """Positions in a call of few rows take nothing from its weights: bf16 queries too carry them in two
+    parts, as without positions (the bound that one part passes where values of both signs cancel)."""
+    lens = [40, 300, 1000, 7]
+    cache, g = _filled(cuda, nkv, hd, 32, lens, ct, hd)
+    rows = [r for r in range(4) for _ in range(5)]
+    pos = [lens[r] - 5 + j for r in range(4) for j in range(5)]
+    q = _queries(g, cuda, 20, nh, hd, "bf16")
+    got = cache.attend(0, q, rows=_i32(cuda, rows), pos=_i32(cuda, pos))
+    want, bound = _reference(q, cache, rows, [p + 1 for p in pos], hd ** -0.5, split=2.0 ** -17)
+    _close(got, want, bound, torch.bfloat16)
