@@ -59,4 +59,10 @@ SXQ_PG_HD int64_t kv_scale_at(const KvPool& p, int slot, int head) {
            ((slot & (p.page - 1)) >> kScaleShift);
 }
 
+// Into how many pieces a prefix attention cuts a tile of so many tiles of keys, a place's share of the
+// card being `piece` of them: a quarter more stays whole.  Kernel and join, us, by half more / a quarter
+// more / none: three f32 prompts of 1412 tokens 55.4 / 53.0 / 63.2, 16 drafts of 5 20.8 / 19.9 / 20.0, a
+// chunk of 2048 after 30720 1370 / 1365 / 1495 (none: more pieces than places).
+SXQ_PG_HD int kv_pieces(int keys, int piece) { return keys - piece > piece / 4 ? (keys - 1) / piece + 1 : 1; }
+
 }  // namespace sxq

@@ -21,19 +21,15 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 // ---- how the work is split ---------------------------------------------------------------
 // Consecutive queries of one request make tiles of whole tokens, `rows` rows (a token and a head of the
 // KV head's group) or fewer; a group of more heads than that is cut into parts of so many heads, a
-// token a tile.  A unit is a KV head and such a part.  A tile's keys are taken `keys` at a time; where
-// there are fewer tiles than the card has places, the longer ones are cut along their keys, into
+// token a tile.  A unit is a KV head and such a part.  A tile's keys are taken `keys` at a time; tiles
+// longer than one place's share of the card, of all tiles' keys, are cut along their keys, into
 // pieces whose results a launch of its own joins.  A launch of one workgroup writes the tiles and
-// pieces ("items") down, and the attention's workgroups go through them.
+// pieces ("items") down, from the map's live entries alone, and the attention's workgroups go through them.
 // Two kernels: `wide` tiles of 128 rows, whose waves share the keys through LDS, and `few` of 32, whose
 // waves share the rows and divide the keys.
 constexpr int kWideRows = 128, kFewRows = 32;
 constexpr int kFewKeys = 128;  // a tile of keys: 32 a wave
 SXQ_HD constexpr int keys_a_tile(int hd) { return hd <= 128 ? 64 : 32; }  // wide (registers)
-
-// With so many tiles a place, or more, none is cut: 600 tokens after 20000 beside 16 prompts of 400 364 us by 4 and
-// by 8, 625 by 2; a prompt of 10000 alone 1126, 1130 and 1123, as many short ones fill the places either way.
-constexpr int kRounds = 4;
 
 struct Geometry {
     int rows, keys;                   // of a tile
@@ -64,8 +60,7 @@ struct CutTile {
     int part, pieces;  // its first partial, how many
 };
 
-// The workspace: counts {items, tiles that are cut, their pieces, whether the items begin with the last};
-// items; the tiles that are cut; partials: per part and unit, {m, l} of each row, then the weighted sums.
+// The workspace: counts {items, tiles that are cut, their pieces, the first item's place}; items; the tiles that are cut; partials: per part and unit, {m, l} of each row, then the weighted sums.
 struct PrefixPlan {
     int* counts;
     TileItem* item;
@@ -86,7 +81,9 @@ struct PrefixPlan {
         p += 2 * (size_t)g.places * g.units * part_floats(g.rows, hd) * sizeof(float);
         bytes = (size_t)(p - (char*)ws);
     }
-    SXQ_HD static int item_room(int n_q, const Geometry& g) { return n_q + 2 * g.places; }  // a tile each, and the pieces of cut ones
+    // a tile each, and the pieces of cut ones (fewer than 2 * places, of fewer than `places` tiles: a tile of x
+    // > 5/4 shares makes ceil(x) <= 8/5 x pieces, and all tiles are `places` shares)
+    SXQ_HD static int item_room(int n_q, const Geometry& g) { return n_q + 2 * g.places; }
     SXQ_HD static size_t part_floats(int rows, int hd) { return (size_t)rows * (hd + 2); }
 };
 
@@ -99,15 +96,18 @@ SXQ_DEV int seen(const KvAttend& A, const int32_t* pos, const KvPool& P, int t, 
 // A thousand queries at a time, a thread each (the next chunk's under way): where its run began and
 // which tile it is in by ballots, the last two thousand tiles in LDS.  While there are no more than a
 // thousand tiles they stay there until all queries are seen, so that a short call's tiles are cut where
-// they are, and are written once, the last tile first.  80 queries 5 us, 1412 6.3: an empty launch and the loads
-// of rows, lengths and positions, which wait for each other.
+// they are, and are written once, the last tile first.  More go to the end of the items' room, the last
+// first too, and are cut from there a thousand at a time: the items of any number of them end before the
+// tiles behind them begin.  80 queries 5.3 us, 1412 7.1: an empty launch and the loads of rows, lengths and
+// positions, which wait for each other.  (Cut by what the map holds, not by its size: 4 tokens after 30000 in a
+// map of 8192 entries take 46 us in all, whole 790.)
 constexpr int kTilesKept = 1024, kTileRing = 2 * kTilesKept;
-__global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, const int32_t* pos, const KvPool P, const Geometry g,
-                                                          bool may_cut) {
+__global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, const int32_t* pos, const KvPool P, const Geometry g) {
     __shared__ __attribute__((aligned(16))) int s_wave[2][16];
     __shared__ int s_limit[kTileRing], s_end[kTileRing], s_token[kTileRing], s_row[kTileRing], s_cut;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const PrefixPlan plan(A.ws, A.n_q, P.hd, g);
+    const int room = PrefixPlan::item_room(A.n_q, g);
     const uint64_t upto = ~(uint64_t)0 >> (63 - lane);
     auto tile = [&](int i) {
         const int k = i & (kTileRing - 1), limit = s_limit[k];
@@ -164,68 +164,91 @@ __global__ __launch_bounds__(1024) void k_kv8_prefix_plan(const KvAttend A, cons
         __syncthreads();
         const int new_tiles = tiles + count;
         if (new_tiles > kTilesKept) {
-            for (int i = (kept ? 0 : tiles - 1) + tid; i < new_tiles; i += 1024) plan.item[i] = tile(i);
+            for (int i = (kept ? 0 : tiles - 1) + tid; i < new_tiles; i += 1024) plan.item[room - 1 - i] = tile(i);
             kept = false;
             __syncthreads();
         }
         tiles = new_tiles;
     }
-    // Pieces: where there are not many more tiles than places, those longer than a place's share are cut
-    // into such shares (a tile a thread).  No more than 2 * places pieces are of cut tiles.
-    int items = tiles, pieces = 0;
-    if (kept) {
-        const TileItem none{};
-        TileItem mine = tid < tiles ? tile(tid) : none;
-        if (!may_cut || tiles >= kRounds * g.places) {
-            if (tid < tiles) plan.item[tiles - 1 - tid] = mine;
-        } else {
-            auto scan = [&](int v, int turn, int& all) {  // the sum over the threads up to this one
-                v = wave_scan(v);
-                if (lane == 63) s_wave[turn][wave] = v;
-                __syncthreads();
-                int lower = 0;
-                all = 0;
+    // Pieces: tiles longer than a place's share of all keys are cut into such shares (a tile a thread).
+    auto scan = [&](int v, int turn, int& all) {  // the sum over the threads up to this one
+        v = wave_scan(v);
+        if (lane == 63) s_wave[turn][wave] = v;
+        __syncthreads();
+        int lower = 0;
+        all = 0;
 #pragma unroll
-                for (int w = 0; w < 16; ++w) {
-                    const int here = s_wave[turn][w];
-                    lower += w < wave ? here : 0;
-                    all += here;
+        for (int w = 0; w < 16; ++w) {
+            const int here = s_wave[turn][w];
+            lower += w < wave ? here : 0;
+            all += here;
+        }
+        return v + lower;
+    };
+    int items = 0, pieces = 0, base = 0;
+    // The items of `here` tiles, which lie in LDS from the ring's begin on; mine: tile here - 1 - tid.
+    auto cut = [&](int here, const TileItem& mine, int piece) {
+        const int n = tid < here ? kv_pieces(mine.end, piece) : 0;
+        int both;
+        const int upto_me = scan(n + (n > 1 ? n << 16 : 0), 1, both);  // items, and those of cut tiles
+        const int part = pieces + (upto_me >> 16) - n, count = both & 0xFFFF;
+        if (n > 1) plan.cut[atomicAdd(&s_cut, 1)] = CutTile{mine.token, mine.count, part, n};
+        // (in the ring's second half: the items before the tile's, its first part, its pieces)
+        int *const s_before = s_limit + kTilesKept, *const s_part = s_token + kTilesKept, *const s_pieces = s_end + kTilesKept;
+        s_before[tid] = (upto_me & 0xFFFF) - n;
+        s_part[tid] = part;
+        s_pieces[tid] = n;
+        __syncthreads();
+        for (int i = tid; i < count; i += 1024) {  // an item a thread
+            const int o = owner(s_before, here, i), j = i - s_before[o];
+            TileItem it = tile(here - 1 - o);
+            const int64_t all = it.end;
+            it.pieces = s_pieces[o];
+            it.part = it.pieces > 1 ? s_part[o] + j : 0;
+            it.first = (int)(all * j / it.pieces);
+            it.end = (int)(all * (j + 1) / it.pieces);
+            plan.item[items + i] = it;
+        }
+        items += count;
+        pieces += both >> 16;
+    };
+    // (2^30 positions a tile at most, 2^35 of all: 2^30 tiles of 32 keys, and one a tile for its last)
+    int work;
+    if (kept) {
+        const TileItem none{}, mine = tid < tiles ? tile(tiles - 1 - tid) : none;
+        scan(mine.end, 0, work);
+        cut(tiles, mine, max(g.min_piece, (work + g.places - 1) / g.places));
+    } else {
+        int keys = 0, longest = 0;
+        for (int i = tid; i < tiles; i += 1024) {
+            const int k = plan.item[room - tiles + i].end;
+            keys += k;
+            longest = max(longest, k);
+        }
+        scan(keys, 0, work);
+        const int piece = max(g.min_piece, (work + g.places - 1) / g.places);
+        if (!__syncthreads_or(kv_pieces(longest, piece) > 1)) {
+            items = tiles;
+            base = room - tiles;
+        } else {
+            for (int r0 = 0; r0 < tiles; r0 += 1024) {  // from the last tile back
+                const int here = min(1024, tiles - r0);
+                TileItem mine{};
+                __syncthreads();  // (the readers of the tiles before these are done)
+                if (tid < here) {
+                    mine = plan.item[room - tiles + r0 + tid];
+                    const int k = here - 1 - tid;
+                    s_token[k] = mine.token;
+                    s_end[k] = mine.token + mine.count;
+                    s_row[k] = mine.row;
+                    s_limit[k] = mine.limit;
                 }
-                return v + lower;
-            };
-            int work, both;
-            scan(mine.end, 0, work);  // (2^30 positions a tile at most, 2^35 of all: 2^29 tiles of keys)
-            const int piece = max(g.min_piece, (work + g.places - 1) / g.places);
-            // A quarter more stays whole.  Kernel and join, us, by half more / a quarter more / none: three f32
-            // prompts of 1412 tokens 55.4 / 53.0 / 63.2, 16 drafts of 5 20.8 / 19.9 / 20.0, a chunk of 2048 after
-            // 30720 1370 / 1365 / 1495 (none: more pieces than places).
-            const int keys = mine.end, n = tid >= tiles ? 0 : 4 * keys > 5 * piece ? (keys + piece - 1) / piece : 1;
-            const int upto_me = scan(n + (n > 1 ? n << 16 : 0), 1, both);  // items, and those of cut tiles
-            items = both & 0xFFFF;
-            pieces = both >> 16;
-            const int before = (upto_me & 0xFFFF) - n, part = (upto_me >> 16) - n;
-            if (n > 1) plan.cut[atomicAdd(&s_cut, 1)] = CutTile{mine.token, mine.count, part, n};
-            // (in the ring's second half: the items before the tile's, its first part, its pieces)
-            int *const s_before = s_limit + kTilesKept, *const s_part = s_token + kTilesKept, *const s_pieces = s_end + kTilesKept;
-            s_before[tid] = before;
-            s_part[tid] = part;
-            s_pieces[tid] = n;
-            __syncthreads();
-            for (int i = tid; i < items; i += 1024) {  // an item a thread
-                const int o = owner(s_before, tiles, i), k = i - s_before[o];
-                TileItem it = tile(o);
-                const int64_t all = it.end;
-                it.pieces = s_pieces[o];
-                it.part = it.pieces > 1 ? s_part[o] + k : 0;
-                it.first = (int)(all * k / it.pieces);
-                it.end = (int)(all * (k + 1) / it.pieces);
-                plan.item[items - 1 - i] = it;
+                __syncthreads();
+                cut(here, mine, piece);
             }
         }
     }
-    if (tid == 0) {
-        *(int4*)plan.counts = make_int4(items, s_cut, pieces, kept);
-    }
+    if (tid == 0) *(int4*)plan.counts = make_int4(items, s_cut, pieces, base);
 }
 
 // Item w of units * items, those of the last tile first (of one request the last queries see the most).
@@ -235,7 +258,7 @@ SXQ_DEV bool item_of(const PrefixPlan& plan, int n_q, const Geometry& g, int64_t
     it = plan.item[min(k, PrefixPlan::item_room(n_q, g) - 1)];
     const int4 counts = *(const int4*)plan.counts;
     if (k >= counts.x) return false;
-    if (!counts.w) it = plan.item[counts.x - 1 - k];
+    if (counts.w) it = plan.item[counts.w + k];
     return true;
 }
 
@@ -1108,9 +1131,10 @@ hipError_t prefix_by_width(const KvAttend& a, const int32_t* pos, const KvPool& 
     return prefix_launch<TQ, C, 256, false>(a, pos, p, g, s);
 }
 template <typename TQ>
-hipError_t prefix_by_code(const KvAttend& a, const int32_t* pos, const KvPool& p, const Geometry& g, bool may_cut, hipStream_t s) {
+hipError_t prefix_by_code(const KvAttend& a, const int32_t* pos, const KvPool& p, const Geometry& g, hipStream_t s) {
     const hipError_t e = p.dtype == kI8 ? prefix_by_width<TQ, I8>(a, pos, p, g, s) : prefix_by_width<TQ, E4M3>(a, pos, p, g, s);
-    if (e != hipSuccess || !may_cut) return e;
+    if (e != hipSuccess) return e;
+    // (what is cut is known on the device alone: a map's entries may be anyone's or nobody's)
     const int64_t all = (int64_t)g.places * g.units * g.rows;
     hipLaunchKernelGGL((k_kv8_prefix_join<TQ>), dim3((unsigned)std::min<int64_t>(1024, all)), dim3(256), 0, s, a, p, g);
     return hipGetLastError();
@@ -1131,16 +1155,15 @@ hipError_t launch_kv8_prefix(const KvAttend& a, const int32_t* pos, const KvPool
     // 1000 positions and 5 new tokens, 32 / 8 heads of 128, bf16 24 / 31, f32 29 / 42; 64 of 16 bf16 61 / 62,
     // f32 82 / 101; 512 after 4000 88 / 95 and 124 / 154, 1024 162 / 158 and 232 / 262, 2048 318 / 257 and 455 /
     // 429; three prompts of 1412 tokens 47 / 39 and 65 / 56; 16 / 4 heads of 256, 512 after 4000 102 / 174, 64 of
-    // 32 142 / 107; 14 / 2 heads of 64, 256 after 4000 29 / 37, 512 51 / 38.
+    // 32 142 / 107; 14 / 2 heads of 64, 256 after 4000 29 / 37, 512 51 / 38.  (Entries of no request count as
+    // rows here: the host does not see them.)
     const bool few = (int64_t)a.n_q * a.nh <= (p.hd <= 64 ? 4096 : a.q_dtype == kF32 && p.hd <= 128 ? 32768 : 16384);
     const Geometry g(a.nh, p.nkv, p.hd, a.q_dtype == kF32, few);
-    // (many more tiles than places, whatever the map: nothing is cut)
-    const bool may_cut = (a.n_q + g.tokens - 1) / g.tokens < kRounds * g.places;
-    hipLaunchKernelGGL(k_kv8_prefix_plan, dim3(1), dim3(1024), 0, s, a, pos, p, g, may_cut);
+    hipLaunchKernelGGL(k_kv8_prefix_plan, dim3(1), dim3(1024), 0, s, a, pos, p, g);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    if (a.q_dtype == kF32) return prefix_by_code<float>(a, pos, p, g, may_cut, s);
-    if (a.q_dtype == kF16) return prefix_by_code<_Float16>(a, pos, p, g, may_cut, s);
-    return prefix_by_code<__bf16>(a, pos, p, g, may_cut, s);
+    if (a.q_dtype == kF32) return prefix_by_code<float>(a, pos, p, g, s);
+    if (a.q_dtype == kF16) return prefix_by_code<_Float16>(a, pos, p, g, s);
+    return prefix_by_code<__bf16>(a, pos, p, g, s);
 }
 
 }  // namespace sxq

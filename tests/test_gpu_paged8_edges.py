@@ -119,3 +119,69 @@ def test_drafts_keep_the_precision_of_one_token(cuda, ct, nh, nkv, hd):
     got = cache.attend(0, q, rows=_i32(cuda, rows), pos=_i32(cuda, pos))
     want, bound = _reference(q, cache, rows, [p + 1 for p in pos], hd ** -0.5, split=2.0 ** -17)
     _close(got, want, bound, torch.bfloat16)
+
+
+def _prefix_with_plan(cache, q, rows, pos, out=None):
+    """attend over prefixes, and what its plan says (the workspace begins with it): items, tiles that are
+    cut, their pieces."""
+    ws = cache.workspace(q.shape[0], q.shape[1], prefix=True)
+    got = cache.attend(0, q, rows=rows, pos=pos, out=out, workspace=ws)
+    return got, ws[:12].view(torch.int32).tolist()
+
+
+@pytest.mark.parametrize("qt", ["f32", "bf16"])
+@pytest.mark.parametrize("entries", [600, 8192])
+def test_padded_maps_are_cut_as_their_live_tokens_ask(cuda, entries, qt):
+    """A map of a captured step's fixed capacity, few of whose entries have tokens: what few tokens see of
+    a long request is divided over the card as in a call of these tokens alone."""
+    lens, nh, nkv, hd = [30000, 50], 32, 8, 128
+    cache, g = _filled(cuda, nkv, hd, 32, lens, "i8", 6)
+    at = [0, 1, 2, 3, 40, entries - 1]
+    rows, pos = [-1] * entries, [-1] * entries
+    for i, (r, p) in zip(at, [(0, 29996), (0, 29997), (0, 29998), (0, 29999), (1, 20), (0, 15000)]):
+        rows[i], pos[i] = r, p
+    q = _queries(g, cuda, entries, nh, hd, qt)
+    out = torch.full_like(q, 7.0)
+    got, (items, cut, pieces) = _prefix_with_plan(cache, q, _i32(cuda, rows), _i32(cuda, pos), out)
+    some, (items1, cut1, pieces1) = _prefix_with_plan(cache, q[at], _i32(cuda, [rows[i] for i in at]), _i32(cuda, [pos[i] for i in at]))
+    assert cut >= 2 and cut1 >= 2 and pieces > 20 and items == pieces + (3 - cut)
+    want, bound = _reference(q[at], cache, [rows[i] for i in at], [pos[i] + 1 for i in at], hd ** -0.5, split=PREFIX_SPLIT[qt])
+    _close(got[at], want, bound, DT[qt])
+    _close(some, want, bound, DT[qt])
+    rest = torch.ones(entries, dtype=torch.bool, device=cuda)
+    rest[at] = False
+    assert bool((got[rest] == 7).all())
+
+
+@pytest.mark.parametrize("short,nh,nkv,hd,qt", [(1100, 4, 1, 64, "bf16"), (300, 32, 8, 64, "f16"), (300, 32, 8, 128, "bf16"),
+                                                (3000, 8, 2, 32, "f32"), (2048, 2, 1, 256, "bf16"), (1023, 1, 1, 128, "f32")])
+def test_one_long_request_beside_many_short_ones_is_cut(cuda, short, nh, nkv, hd, qt):
+    """However many tiles there are, before and after it."""
+    rng = np.random.default_rng(short)
+    long = short // 3
+    lens = [int(v) for v in rng.integers(1, 40, short)]
+    lens.insert(long, 20000)
+    cache, g = _filled(cuda, nkv, hd, 16, lens, "e4m3", short)
+    rows, pos = [], []
+    for r, n in enumerate(lens):
+        for p in ([n - 1] if r != long else [17000, 19998, 19999]):
+            rows.append(r)
+            pos.append(p)
+    q = _queries(g, cuda, len(rows), nh, hd, qt)
+    got, (items, cut, pieces) = _prefix_with_plan(cache, q, _i32(cuda, rows), _i32(cuda, pos))
+    assert cut == 1 and pieces > 10 and items == short + pieces
+    some = [0, 1, long, long + 1, long + 2, long + 3, len(rows) - 1, len(rows) - 2] + rng.permutation(len(rows))[:80].tolist()
+    want, bound = _reference(q[some], cache, [rows[i] for i in some], [pos[i] + 1 for i in some], hd ** -0.5, split=PREFIX_SPLIT[qt])
+    _close(got[some], want, bound, DT[qt])
+
+
+def test_many_tiles_of_which_none_is_cut(cuda):
+    """More tiles than stay in LDS, alike in length: they go as they are, every query's result there."""
+    n, nh = 2600, 2
+    cache, g = _filled(cuda, 1, 32, 16, [int(v) for v in np.random.default_rng(1).integers(0, 60, n)], "i8", 9)
+    rows = list(range(n))
+    q = _queries(g, cuda, n, nh, 32, "f16")
+    got, (items, cut, pieces) = _prefix_with_plan(cache, q, _i32(cuda, rows), _i32(cuda, [1 << 30] * n))
+    assert (items, cut, pieces) == (n, 0, 0)
+    want, bound = _reference(q, cache, rows, [1 << 30] * n, 32 ** -0.5)
+    _close(got, want, bound, torch.float16)
