@@ -10,7 +10,7 @@ import torch
 
 from syrinx_amd.paged import PagedKvCache, SlotMap
 from test_gpu_paged import DT, F64, U32, _close
-from test_gpu_paged8 import CT, PREFIX_SPLIT, B, _attend, _cache, _filled, _queries, _reference, cuda  # noqa: F401
+from test_gpu_paged8 import CT, PREFIX_SPLIT, B, _attend, _cache, _code_values, _filled, _queries, _reference, cuda  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -185,3 +185,57 @@ def test_many_tiles_of_which_none_is_cut(cuda):
     assert (items, cut, pieces) == (n, 0, 0)
     want, bound = _reference(q, cache, rows, [1 << 30] * n, 32 ** -0.5)
     _close(got, want, bound, torch.float16)
+
+
+@pytest.mark.parametrize("it", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("ct", ["i8", "e4m3"])
+def test_append_of_rows_whose_norm_is_exact(cuda, ct, it):
+    """Rows of elements +-n: the root mean square is n, a row over it +-1 and times the weight the weight,
+    all exact, so that weights half way between two codes go to the even one, and queries are the
+    weights.  (n times the rounded inverse of these n is not 1.)"""
+    nh, nkv, hd = 2, 1, 64
+    ns = [41, 47, 55, 61, 82, 83, 94, 97, 107, 109]
+    cache = _cache(cuda, nkv, hd, ct, n_pages=10, page=16, rows=10, max_len=16)
+    sign = torch.where(torch.arange(hd, device=cuda) % 3 == 1, -1.0, 1.0)
+    qkv = (torch.tensor(ns, device=cuda, dtype=torch.float32)[:, None] * sign).repeat(1, nh + 2 * nkv).to(DT[it])
+    if ct == "i8":
+        w = (torch.arange(hd, device=cuda) + 63.5) * 2.0 ** -6  # codes of a scale of 2^-6
+    else:
+        w = (2 * torch.arange(hd, device=cuda) % 16 + 17) * 2.0 ** -4  # between two of eight codes
+    m = cache.reserve([1] * 10)
+    q = cache.append(0, qkv, m, n_heads=nh, q_norm=w, k_norm=w, eps=0.0).view(10, nh, hd)
+    assert torch.equal(q, (w * sign).to(DT[it]).expand(10, nh, hd))
+    s = cache.k_scale[0, m.slots.long() // 16, 0, 0].to(F64)
+    assert bool((s == (2.0 ** -6 if ct == "i8" else 2.0 ** -7)).all())
+    want = _code_values((w * sign).to(F64) / s[:, None], ct)
+    got = cache.k[0, m.slots.long() // 16, 0, m.slots.long() % 16]
+    assert torch.equal(got.float().to(F64), want)
+
+
+@pytest.mark.parametrize("ct", ["i8", "e4m3"])
+def test_append_of_rows_whose_norm_passes_the_range(cuda, ct):
+    """Rows whose mean square is infinite in f32 become zeros, but for what is infinite itself (NaN, not a
+    number's code); rows of zeros without an eps NaN; rows of the smallest and largest squares ordinary."""
+    hd = 32
+    cache = _cache(cuda, 1, hd, ct, n_pages=6, page=16, rows=6, max_len=16)
+    x = torch.ones((6, hd), device=cuda)
+    x[0] = 1e30
+    x[1, 3] = math.inf
+    x[2] = 0.0
+    x[3] = 2e-19
+    x[4] = 1e18
+    x[5] *= torch.where(torch.arange(hd, device=cuda) % 2 == 0, 1.0, -1.0)
+    w = torch.full((hd,), 2.0, device=cuda)
+    q = cache.append(0, x.repeat(1, 3), cache.reserve([1] * 6), n_heads=1, q_norm=w, k_norm=w, eps=0.0)
+    k, _ = cache.read(0, torch.arange(7, dtype=torch.int32, device=cuda), 6, dtype=torch.float32)
+    nan = torch.tensor(math.nan, device=cuda) if ct == "e4m3" else torch.tensor(0.0, device=cuda)
+    want = torch.full((6, hd), 2.0, device=cuda)
+    want[0] = 0.0
+    want[1] = 0.0
+    want[5] *= x[5]
+    got, one = q.clone(), torch.full((), math.nan, device=cuda)
+    want[1, 3], want[2] = one, one
+    assert torch.allclose(got, want, rtol=2.0 ** -20, atol=0, equal_nan=True)
+    want[1, 3], want[2] = nan, nan
+    # (codes: 2 is one of both kinds; within half a step where the norm rounds)
+    assert torch.allclose(k[:, 0], want, rtol=2.0 ** -4, atol=0, equal_nan=True)
