@@ -35,7 +35,7 @@ struct Geometry {
     int rows, keys;                   // of a tile
     int group, parts, units, tokens;  // heads a KV head; parts of a group; units; tokens a tile
     int places, min_piece;            // items of one unit that the card holds at once; tiles of keys
-    SXQ_HD Geometry(int nh, int nkv, int hd, bool f32, bool few) {
+    SXQ_HD Geometry(int nh, int nkv, int hd, bool few) {
         rows = few ? kFewRows : kWideRows;
         keys = few ? kFewKeys : keys_a_tile(hd);
         group = nh / nkv;
@@ -1140,25 +1140,28 @@ hipError_t prefix_by_code(const KvAttend& a, const int32_t* pos, const KvPool& p
     return hipGetLastError();
 }
 
+// Few rows (drafted tokens, short prompts): the kernel of 32-row tiles.  Few / wide, us: 16 requests of
+// 1000 positions and 5 new tokens, 32 / 8 heads of 128, bf16 24 / 31, f32 29 / 42; 64 of 16 bf16 61 / 62,
+// f32 82 / 101; 512 after 4000 88 / 95 and 124 / 154, 1024 162 / 158 and 232 / 262, 2048 318 / 257 and 455 /
+// 429; three prompts of 1412 tokens 47 / 39 and 65 / 56; 16 / 4 heads of 256, 512 after 4000 102 / 174, 64 of
+// 32 142 / 107; 14 / 2 heads of 64, 256 after 4000 29 / 37, 512 51 / 38.  (Entries of no request count as
+// rows here: the host does not see them.)
+inline bool few_rows(int n_q, int nh, int hd, int q_dtype) {
+    return (int64_t)n_q * nh <= (hd <= 64 ? 4096 : q_dtype == kF32 && hd <= 128 ? 32768 : 16384);
+}
+
 }  // namespace
 
 namespace sxq {
 
 size_t kv8_prefix_workspace(const KvPool& p, int n_q, int nh) {
-    size_t most = 0;
-    for (int form = 0; form < 4; ++form) most = std::max(most, PrefixPlan(nullptr, n_q, p.hd, Geometry(nh, p.nkv, p.hd, form & 1, form & 2)).bytes);
+    size_t most = 0;  // over the kernels that queries of one type or another take
+    for (int dtype : {kF32, kBF16}) most = std::max(most, PrefixPlan(nullptr, n_q, p.hd, Geometry(nh, p.nkv, p.hd, few_rows(n_q, nh, p.hd, dtype))).bytes);
     return most;
 }
 
 hipError_t launch_kv8_prefix(const KvAttend& a, const int32_t* pos, const KvPool& p, hipStream_t s) {
-    // Few rows (drafted tokens, short prompts): the kernel of 32-row tiles.  Few / wide, us: 16 requests of
-    // 1000 positions and 5 new tokens, 32 / 8 heads of 128, bf16 24 / 31, f32 29 / 42; 64 of 16 bf16 61 / 62,
-    // f32 82 / 101; 512 after 4000 88 / 95 and 124 / 154, 1024 162 / 158 and 232 / 262, 2048 318 / 257 and 455 /
-    // 429; three prompts of 1412 tokens 47 / 39 and 65 / 56; 16 / 4 heads of 256, 512 after 4000 102 / 174, 64 of
-    // 32 142 / 107; 14 / 2 heads of 64, 256 after 4000 29 / 37, 512 51 / 38.  (Entries of no request count as
-    // rows here: the host does not see them.)
-    const bool few = (int64_t)a.n_q * a.nh <= (p.hd <= 64 ? 4096 : a.q_dtype == kF32 && p.hd <= 128 ? 32768 : 16384);
-    const Geometry g(a.nh, p.nkv, p.hd, a.q_dtype == kF32, few);
+    const Geometry g(a.nh, p.nkv, p.hd, few_rows(a.n_q, a.nh, p.hd, a.q_dtype));
     hipLaunchKernelGGL(k_kv8_prefix_plan, dim3(1), dim3(1024), 0, s, a, pos, p, g);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     if (a.q_dtype == kF32) return prefix_by_code<float>(a, pos, p, g, s);

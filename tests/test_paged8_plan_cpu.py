@@ -1,10 +1,15 @@
 """How the prefix attention over 8-bit pages cuts its tiles (csrc/sxq_paged.h), enumerated on the CPU as
-the kernel uses it: pieces and cut tiles stay within the workspace's room, sizes within 32 bits."""
+the kernel uses it: pieces and cut tiles stay within the workspace's room, sizes within 32 bits; and the
+workspaces it asks for."""
+import ctypes
 import os
 import shutil
 import subprocess
 
 import pytest
+
+from syrinx_amd import _lib
+from syrinx_amd.paged import KvPages
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -63,3 +68,19 @@ def test_pieces(tmp_path):
                     os.path.join(ROOT, "syrinx_amd", "csrc"), str(src), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
+def _workspace(nh, nkv, hd, n_q):
+    p, size = KvPages(24, nkv, hd, 32, 4, None, None, nkv * 32 * hd, 32 * hd, hd, None, None, nkv * 2, 2), ctypes.c_size_t()
+    assert _lib.lib().sxq_kv_prefix_attention_workspace(ctypes.byref(p), n_q, nh, ctypes.byref(size)) == _lib.OK
+    return size.value
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(32, 8, 128), (14, 2, 64), (16, 1, 256), (64, 1, 128), (8, 8, 16), (300, 2, 64)])
+def test_a_workspace_is_of_the_tiles_that_its_calls_take(nh, nkv, hd):
+    """Calls of few rows are taken by tiles of 32 of them: their workspace has no room for the pieces of
+    tiles of 128.  More queries never need less: a workspace is good for any smaller call."""
+    few, many = 1, 1 + 32768 // nh
+    assert 3 * _workspace(nh, nkv, hd, few) < _workspace(nh, nkv, hd, many)
+    sizes = [_workspace(nh, nkv, hd, n) for n in range(1, 2 * many, max(1, many // 300))]
+    assert all(a <= b for a, b in zip(sizes, sizes[1:]))
