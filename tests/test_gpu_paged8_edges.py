@@ -239,3 +239,66 @@ def test_append_of_rows_whose_norm_passes_the_range(cuda, ct):
     want[1, 3], want[2] = nan, nan
     # (codes: 2 is one of both kinds; within half a step where the norm rounds)
     assert torch.allclose(k[:, 0], want, rtol=2.0 ** -4, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("ct,code", [("i8", 24), ("e4m3", 0x101)])
+@pytest.mark.parametrize("hd", [64, 80, 128, 256])
+def test_many_rows_over_pools_of_other_strides(cuda, ct, code, hd):
+    """Tiles of many rows over position-major pages, keys and values of one tensor, scales of one tensor,
+    queries and outputs as columns of wider rows: the bits of the same call over pages of their own."""
+    from syrinx_amd import lib
+    from syrinx_amd._lib import check
+    from syrinx_amd.paged import KvPages
+
+    nh, nkv, page, lens = 6, 2, 32, [5, 100, 33, 400]
+    plain, g = _filled(cuda, nkv, hd, page, lens, ct, hd)
+    n_pages = plain.n_pages
+    both = torch.full((n_pages, page, 2, nkv, hd + 16), 0x7F, dtype=torch.uint8, device=cuda)
+    sc = torch.full((n_pages, 2, nkv, page // B + 1), math.nan, device=cuda)
+    k, v = both[:, :, 0, :, :hd], both[:, :, 1, :, :hd]
+    for mine, scale, codes, scales in ((k, sc[:, 0], plain.k[0], plain.k_scale[0]), (v, sc[:, 1], plain.v[0], plain.v_scale[0])):
+        mine.copy_(codes.view(torch.uint8).transpose(1, 2))
+        scale[..., :page // B] = scales
+    pages = KvPages(code, nkv, hd, page, n_pages, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(2), k.stride(1),
+                    sc[:, 0].data_ptr(), sc[:, 1].data_ptr(), sc.stride(0), sc.stride(2))
+    live = [(r, p) for r, n in enumerate(lens) for p in range(max(0, n - 150), n)]
+    n = 32768 // nh + 1 + len(live)
+    rows = _i32(cuda, [r for r, _ in live] + [-1] * (n - len(live)))
+    pos = _i32(cuda, [p for _, p in live] + [-1] * (n - len(live)))
+    for qt in ("f32", "bf16", "f16"):
+        qw = (2 * torch.randn((n, (nh + 4) * hd), generator=g, device=cuda)).to(DT[qt])
+        q = qw.as_strided((n, nh, hd), (qw.stride(0), hd, 1))
+        buf = torch.full((n, (nh + 1) * hd), 3.0, device=cuda, dtype=DT[qt])
+        size = ctypes.c_size_t()
+        check(lib().sxq_kv_prefix_attention_workspace(ctypes.byref(pages), n, nh, ctypes.byref(size)))
+        ws = torch.full((size.value,), 0xA5, dtype=torch.uint8, device=cuda)
+        check(lib().sxq_kv_prefix_attention(0, ctypes.byref(pages), {"f32": 0, "f16": 1, "bf16": 30}[qt], q.data_ptr(), q.stride(0), n, nh,
+                                            rows.data_ptr(), pos.data_ptr(), plain.lens.data_ptr(), len(lens), plain.table.data_ptr(),
+                                            plain.max_blocks, plain.max_blocks, 0.1, buf.data_ptr(), buf.stride(0), ws.data_ptr(),
+                                            size.value, torch.cuda.current_stream().cuda_stream))
+        out = torch.full((n, nh, hd), 3.0, device=cuda, dtype=DT[qt])
+        want = plain.attend(0, q.contiguous(), rows=rows, pos=pos, scale=0.1, out=out)
+        assert bool(want[:len(live)].isfinite().all()) and bool((want[len(live):] == 3).all())
+        assert torch.equal(buf[:, :nh * hd].reshape(n, nh, hd), want) and bool((buf[:, nh * hd:] == 3).all())
+        some = [0, 4, 5, 104, 137, 138, len(live) - 1]
+        ref, bound = _reference(q[some].contiguous(), plain, [live[i][0] for i in some], [live[i][1] + 1 for i in some], 0.1,
+                                split=PREFIX_SPLIT[qt])
+        _close(want[some], ref, bound, DT[qt])
+
+
+@pytest.mark.parametrize("form", [True, "wide"])
+@pytest.mark.parametrize("hd,n_pages", [(64, 600000), (128, 300000), (256, 150000)])
+def test_prefixes_past_32_bits(cuda, hd, n_pages, form):
+    """Pages whose byte offsets pass 2^32: the bits of the same requests in a small cache's pages."""
+    nkv, nh, lens = 8, 32, [90, 20]
+    big = _cache(cuda, nkv, hd, "e4m3", n_pages=n_pages, page=16, rows=2, max_len=128)  # 4.9e9 bytes a pool
+    small = _cache(cuda, nkv, hd, "e4m3", n_pages=20, page=16, rows=2, max_len=128)
+    big.free.copy_(torch.arange(n_pages, dtype=torch.int32))  # the last page on top
+    x = torch.randn((110, 48 * hd), generator=torch.Generator(device=cuda).manual_seed(1), device=cuda).bfloat16()
+    outs = []
+    for cache in (big, small):
+        m = cache.reserve(lens)
+        q = cache.append(0, x, m, n_heads=nh).view(110, nh, hd)
+        outs.append((_attend(cache, q, m.rows, m.pos, form), m))
+    assert int(outs[0][1].slots.min()) > (n_pages - 10) * 16 and bool(outs[0][0].isfinite().all())
+    assert torch.equal(outs[0][0], outs[1][0])
