@@ -302,3 +302,38 @@ def test_prefixes_past_32_bits(cuda, hd, n_pages, form):
         outs.append((_attend(cache, q, m.rows, m.pos, form), m))
     assert int(outs[0][1].slots.min()) > (n_pages - 10) * 16 and bool(outs[0][0].isfinite().all())
     assert torch.equal(outs[0][0], outs[1][0])
+
+
+@pytest.mark.parametrize("form", [False, True, "wide"])
+@pytest.mark.parametrize("ct", ["i8", "e4m3"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_small_query_elements_beside_an_outlier(cuda, ct, form, hd):
+    """f32 queries, one element of which is 2^18 times the others and meets zeros in every key, so that
+    the scores are the small ones' alone: an element is off by 2^-22 of itself or 2^-39 of the largest,
+    a score by that times its keys, scaled (and (hd + 10) 2^-24 of the sum of its products' sizes)."""
+    L, nkv, nh = 200, 2, 8
+    cache, g = _filled(cuda, nkv, hd, 16, [L], ct, hd)
+    codes = cache.k[0].float()
+    codes[..., 5] = 0
+    cache.k[0] = codes.to(cache.k.dtype)
+    scale = 2.0 ** 18 * hd ** -0.5
+    q = 2.0 ** -18 * torch.randn((1, nh, hd), generator=g, device=cuda)
+    q[..., 5] = 1.7
+    if form:
+        more = 32768 // nh + 1 if form == "wide" else 0
+        rows, pos = _i32(cuda, [0] + [-1] * more), _i32(cuda, [L - 1] + [-1] * more)
+        got = cache.attend(0, torch.cat([q, torch.zeros((more, nh, hd), device=cuda)]), rows=rows, pos=pos, scale=scale)[:1]
+    else:
+        got = cache.attend(0, q, scale=scale)
+    p = torch.arange(L, device=cuda)
+    ids, at = cache.table[0].long()[p // 16], p % 16
+    k, v = ((c[0].float().to(F64) * s[0].to(F64).repeat_interleave(B, -1)[..., None])[ids, :, at].transpose(0, 1).contiguous()
+            for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    qq = q.to(F64).view(nkv, nh // nkv, hd)
+    kt = k.transpose(1, 2).contiguous()
+    w = torch.softmax(qq @ kt * scale, -1)
+    off = torch.maximum(2.0 ** -22 * qq.abs(), torch.full_like(qq, 2.0 ** -39 * 1.7))
+    delta = ((off + (hd + 10) * U32 * qq.abs()) @ kt.abs() * scale).amax(-1, keepdim=True)
+    bound = 2 * (2 * delta + (8 + 4 * (L / 16 + 2) + 2 * L) * U32) * (w @ v.abs())
+    assert float(delta.max()) < 2.0 ** -9  # (a part that is lost would be 2^-5 and more)
+    _close(got, (w @ v).reshape(1, nh, hd), bound.reshape(1, nh, hd), torch.float32)
