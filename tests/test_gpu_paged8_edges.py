@@ -337,3 +337,75 @@ def test_small_query_elements_beside_an_outlier(cuda, ct, form, hd):
     bound = 2 * (2 * delta + (8 + 4 * (L / 16 + 2) + 2 * L) * U32) * (w @ v.abs())
     assert float(delta.max()) < 2.0 ** -9  # (a part that is lost would be 2^-5 and more)
     _close(got, (w @ v).reshape(1, nh, hd), bound.reshape(1, nh, hd), torch.float32)
+
+
+def _forms(cache, q, rows, pos, form, scale):
+    """attend as one token's, or over prefixes in tiles of few or many rows."""
+    if not form:
+        return cache.attend(0, q, rows=rows, scale=scale)
+    more = 32768 // q.shape[1] + 1 if form == "wide" else 0
+    none = torch.full((more,), -1, dtype=torch.int32, device=q.device)
+    qq = torch.cat([q, torch.zeros((more, *q.shape[1:]), dtype=q.dtype, device=q.device)])
+    return cache.attend(0, qq, rows=torch.cat([rows, none]), pos=torch.cat([pos, none]), scale=scale)[:q.shape[0]]
+
+
+@pytest.mark.parametrize("qt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("form", [False, True, "wide"])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, -2.5, 1e-30, 4.0])
+def test_scales_of_either_sign(cuda, form, qt, scale):
+    lens = [300, 17, 1, 64]
+    cache, g = _filled(cuda, 2, 64, 16, lens, "e4m3", 12)
+    q = _queries(g, cuda, 4, 6, 64, qt)
+    got = _forms(cache, q, _i32(cuda, range(4)), _i32(cuda, [n - 1 for n in lens]), form, scale)
+    want, bound = _reference(q, cache, range(4), lens, scale, split=PREFIX_SPLIT[qt] if form else None)
+    _close(got, want, bound, DT[qt])
+
+
+@pytest.mark.parametrize("qt,ct", [("f32", "e4m3"), ("bf16", "i8"), ("f16", "e4m3")])
+@pytest.mark.parametrize("nh,nkv,hd", [(300, 2, 64), (130, 1, 128), (257, 1, 32), (129, 1, 256)])
+def test_prefix_of_groups_wider_than_a_tile(cuda, qt, ct, nh, nkv, hd):
+    """More query heads a KV head than a tile has rows, the last part of a group small."""
+    lens = [150, 9, 33]
+    cache, g = _filled(cuda, nkv, hd, 32, lens, ct, nh)
+    rows, pos = [0] * 40 + [1] * 3 + [2] * 33, list(range(110, 150)) + [6, 7, 8] + list(range(33))
+    for n in (76, 3):
+        q = _queries(g, cuda, n, nh, hd, qt)
+        got = _forms(cache, q, _i32(cuda, rows[:n]), _i32(cuda, pos[:n]), "wide" if n == 76 else True, hd ** -0.5)
+        want, bound = _reference(q, cache, rows[:n], [p + 1 for p in pos[:n]], hd ** -0.5, split=PREFIX_SPLIT[qt])
+        _close(got, want, bound, DT[qt])
+
+
+def test_prefix_of_two_hundred_thousand_tiles(cuda):
+    """Queries of alternating requests, one of a long one among them, which alone is cut."""
+    n, at, hd = 200000, 77777, 16
+    lens = [30, 60, 45, 40000]
+    cache, g = _filled(cuda, 1, hd, 16, lens, "i8", 3)
+    rows = np.arange(n) % 3
+    pos = np.random.default_rng(2).integers(0, 60, n)
+    rows[at], pos[at] = 3, 39999
+    q = _queries(g, cuda, n, 1, hd, "bf16")
+    got, (items, cut, pieces) = _prefix_with_plan(cache, q, _i32(cuda, rows.tolist()), _i32(cuda, pos.tolist()))
+    assert cut == 1 and pieces >= 2 and items == n - 1 + pieces
+    some = [0, 1, 1023, 1024, at - 1, at, at + 1, n - 1] + np.random.default_rng(1).integers(0, n, 300).tolist()
+    want, bound = _reference(q[some], cache, rows[some].tolist(), (pos[some] + 1).tolist(), hd ** -0.5, split=PREFIX_SPLIT["bf16"])
+    _close(got[some], want, bound, torch.bfloat16)
+    assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("it", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,inter", [(64, False), (80, True), (256, False)])
+def test_append_of_rows_at_odd_strides(cuda, it, hd, inter):
+    """Rows that begin at any element: the bits of the same rows packed."""
+    nh, nkv, T = 3, 2, 70
+    width = (nh + 2 * nkv) * hd
+    g = torch.Generator(device=cuda).manual_seed(hd)
+    wide = torch.randn((T, width + 7), generator=g, device=cuda).to(DT[it])
+    rope = tuple(torch.randn((90, hd // 2), generator=g, device=cuda) for _ in range(2))
+    w = torch.randn(hd, generator=g, device=cuda)
+    outs = []
+    for qkv in (wide[:, 3:3 + width], wide[:, 3:3 + width].contiguous()):
+        cache = _cache(cuda, nkv, hd, "e4m3", n_pages=8, page=16, rows=1, max_len=90)
+        m = cache.reserve([T])
+        q = cache.append(0, qkv, m, n_heads=nh, q_norm=w, k_norm=w, rope=rope, interleaved=inter)
+        outs.append((q, *cache.read(0, _i32(cuda, [0, T]), T, dtype=torch.float32)))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
