@@ -232,7 +232,8 @@ typedef struct {
  * the first that the call writes, are rescaled to it.  A code is x / s rounded to nearest, ties to
  * even; infinities become the largest code of their sign, a NaN becomes the e4m3 NaN, or int8's 0.
  * Rescaling by powers of two is exact for e4m3, but for values below 2^-6 of the scale, and rounds
- * int8 codes once more.  Dropping positions (sxq_kv_reserve) leaves scales as they are: a block that
+ * int8 codes once more (tokens written one at a time, as a decode step's, are rounded again at each
+ * growth of their block's scale: e4m3 is the type for those).  Dropping positions (sxq_kv_reserve) leaves scales as they are: a block that
  * is written on from its middle keeps the scale that the dropped ones asked for. */
 #define SXQ_KV_SCALE_BLOCK 16
 
@@ -290,7 +291,9 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
  * f32 queries), below the output's own rounding.  Over 8-bit pages q may be of any of the three
  * types: a code takes part exactly, an f32 query element in two f16 parts, off by at most 2^-22 of itself
  * or 2^-39 of its head's largest finite one, a weight (times its value's scale) in bf16 parts, off by
- * at most 2^-17 of itself (16-bit queries) or 2^-22.  rows int32 [n_q]: the table row of each query (NULL: b);
+ * at most 2^-17 of itself (16-bit queries) or 2^-22, where that product is 2^-100 or more (what lies
+ * below 2^-126 may count as zero); a 16-bit query's products with codes, before their scale, count as
+ * infinite where their sum passes f32's range.  rows int32 [n_q]: the table row of each query (NULL: b);
  * a query whose row lies outside 0 .. n_rows - 1 leaves its out row as it was.  A request
  * without positions (or whose pages are all absent) gives zeros.  max_blocks * page_size at
  * most 2^30, n_q times that at most 2^35, n_q at most 2^20.  What lies past a request's
@@ -303,7 +306,8 @@ sxq_status sxq_kv_append(int device, const sxq_kv_pages *pages, int in_dtype, co
  * workspace: sxq_kv_attention_workspace bytes, 256-byte aligned, of which the caller zeroes
  * the first SXQ_KV_COUNTER_BYTES before its first use; every call leaves them zero, and the
  * workspace good for any call that needs no more bytes.  Calls that share one must not
- * overlap: a captured graph keeps one of its own. */
+ * overlap, on the stream nor in their enqueueing (a call may be several launches: two threads' calls on
+ * one stream take turns): a captured graph keeps one of its own. */
 #define SXQ_KV_COUNTER_BYTES 262144
 sxq_status sxq_kv_attention_workspace(const sxq_kv_pages *pages, int n_q, int n_heads, size_t *bytes);
 sxq_status sxq_kv_attention(int device, const sxq_kv_pages *pages, int q_dtype, const void *q, int64_t q_stride,
@@ -317,7 +321,7 @@ sxq_status sxq_kv_attention(int device, const sxq_kv_pages *pages, int q_dtype, 
  * sxq_kv_reserve's map: queries of one request that follow one another share its keys' loads,
  * whatever their positions; any other order is as right.  A weight is carried as there, but in a call
  * of more than 4096 rows (n_q * n_heads) under bf16 queries it may be rounded to bf16 (2^-8 of itself).
- * A workspace holds nothing between calls; calls that share one must not overlap. */
+ * A workspace holds nothing between calls; calls that share one must not overlap, as there. */
 sxq_status sxq_kv_prefix_attention_workspace(const sxq_kv_pages *pages, int n_q, int n_heads, size_t *bytes);
 sxq_status sxq_kv_prefix_attention(int device, const sxq_kv_pages *pages, int q_dtype, const void *q, int64_t q_stride,
                                    int n_q, int n_heads, const int32_t *rows, const int32_t *pos, const int32_t *lens,

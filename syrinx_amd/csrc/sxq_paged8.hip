@@ -107,7 +107,7 @@ SXQ_DEV float wave_max(float v) {
 // 256 / lh heads each.
 // A code needs its block's largest element, so that a block's rows have to meet before any is stored: in
 // registers, and each element is read and written once.  What bounds it: 8192 bf16 tokens of 32 + 16
-// heads of 128 take 49 us, 185 MB at 3.8 TB/s (a large copy: 5.1), 1412 f32 ones 15.4, 61 MB at 3.9: memory,
+// heads of 128 take 50 us, 185 MB at 3.7 TB/s (a large copy: 5.2), 1412 f32 ones 15.8, 61 MB at 3.9: memory,
 // and the start of workgroups; a step's few tokens 4.7, where an empty launch takes 2: the loads of slots,
 // rows and angles, which wait for each other.  (The queries by a launch of their own: 70 against 66 us
 // for the 8192, before the keys' and values' part was as it is.)

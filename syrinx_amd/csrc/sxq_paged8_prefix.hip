@@ -321,9 +321,10 @@ struct Nans {
 // 4 (lane / 32) + i % 4) and the softmax of a row is two lanes'; weighted values: A = 32 columns x 16 keys,
 // B = the weights in the registers that the scores came in, the values' keys laid out in LDS to match.
 // What bounds it: the matrix cores' products and the lanes' work on the weights (an exponential, the
-// maximum, the sum, the rounding) take turns on a SIMD's two waves.  A chunk of 2048 bf16 queries after 30720
-// positions, 32 / 8 heads of 128, takes 1320 us, 800 TFLOP/s (a large matrix product: 1217); f32 queries,
-// in two parts, and weights in three, 1.7 to 1.85 times a bf16 call.  Of a short prompt much is the beginning
+// maximum, the sum, the rounding, the widening of the codes) take turns on a SIMD's two waves.  A chunk of 2048
+// bf16 queries after 30720 positions, 32 / 8 heads of 128, takes 1290 us, 825 TFLOP/s (a large matrix product: 1217;
+// 1415 on another card); f16 queries, weights in two parts, 1700; f32 ones, in two parts, weights in
+// three, 2460.  Of a short prompt much is the beginning
 // (tile, pages, scales, codes and queries, loads that wait for each other): a call of one tile of keys
 // takes 9.5 us (f32 14.7), each further one of that item 2.1 (3.5).
 template <typename TQ, typename C, int HDP, bool FULL>
@@ -716,7 +717,7 @@ __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix(const Kv
 // One item of up to 32 rows: the waves go through the keys as those of k_kv8_attend do, 32 each of every
 // 128, keys and values straight into registers, two tiles of 16 rows on each operand; then the four
 // waves' sums are added up through LDS.  What bounds it is the keys' bytes, or latency: 16 requests' 5 drafted
-// tokens over 256 to 2040 positions in 14 us, of which 4.3 are the bytes.
+// tokens over 256 to 2040 positions in 15 us, of which 4.3 are the bytes.
 template <typename TQ, typename C, int HDP, bool FULL>
 __global__ __launch_bounds__(256, HDP <= 128 ? 2 : 1) void k_kv8_prefix_few(const KvAttend A, const int32_t* pos, const KvPool P,
                                                                           const Geometry geo) {
@@ -1141,11 +1142,11 @@ hipError_t prefix_by_code(const KvAttend& a, const int32_t* pos, const KvPool& p
 }
 
 // Few rows (drafted tokens, short prompts): the kernel of 32-row tiles.  Few / wide, us: 16 requests of
-// 1000 positions and 5 new tokens, 32 / 8 heads of 128, bf16 24 / 31, f32 29 / 42; 64 of 16 bf16 61 / 62,
-// f32 82 / 101; 512 after 4000 88 / 95 and 124 / 154, 1024 162 / 158 and 232 / 262, 2048 318 / 257 and 455 /
-// 429; three prompts of 1412 tokens 47 / 39 and 65 / 56; 16 / 4 heads of 256, 512 after 4000 102 / 174, 64 of
-// 32 142 / 107; 14 / 2 heads of 64, 256 after 4000 29 / 37, 512 51 / 38.  (Entries of no request count as
-// rows here: the host does not see them.)
+// 1000 positions and 5 new tokens, 32 / 8 heads of 128, bf16 26 / 30, f32 30 / 41; 64 of 16 bf16 67 / 58,
+// f32 82 / 101; 512 after 4000 92 / 87 and 118 / 149, 1024 172 / 143 and 219 / 254, 2048 353 / 232 and 451 /
+// 438; three prompts of 1412 tokens 47 / 38 and 62 / 57; 500 requests of 200 positions and 2 tokens 91 / 110 and
+// 117 / 203; 16 / 4 heads of 256, 512 after 4000 bf16 109 / 174, 64 of 32 152 / 102; 14 / 2 heads of 64, 256
+// after 4000 32 / 29, 512 53 / 36.  (Entries of no request count as rows here: the host does not see them.)
 inline bool few_rows(int n_q, int nh, int hd, int q_dtype) {
     return (int64_t)n_q * nh <= (hd <= 64 ? 4096 : q_dtype == kF32 && hd <= 128 ? 32768 : 16384);
 }

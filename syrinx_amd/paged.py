@@ -81,7 +81,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 class PagedKvCache:
     """Keys and values of up to max_rows requests of up to max_len positions (rounded up to whole
     pages) in n_pages pages of page_size positions (a power of two, 16..1024).  dtype: float32,
-    float16, bfloat16, or int8 / float8_e4m3fn with scales (head_dim then a multiple of 16).
+    float16, bfloat16, or int8 / float8_e4m3fn with scales (head_dim then a multiple of 16).  Tokens
+    that are appended one at a time belong in float8_e4m3fn: int8 codes are rounded again whenever their
+    block's scale grows, up to half a step each time.
 
     k, v: [n_layers, n_pages, n_kv_heads, page_size, head_dim]; of 8 bits also k_scale, v_scale: f32
     [n_layers, n_pages, n_kv_heads, page_size / SCALE_BLOCK]; table: int32 [max_rows, blocks];
