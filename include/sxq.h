@@ -233,8 +233,9 @@ typedef struct {
  * even; infinities become the largest code of their sign, a NaN becomes the e4m3 NaN, or int8's 0.
  * Rescaling by powers of two is exact for e4m3, but for values below 2^-6 of the scale, and rounds
  * int8 codes once more (tokens written one at a time, as a decode step's, are rounded again at each
- * growth of their block's scale: e4m3 is the type for those).  Dropping positions (sxq_kv_reserve) leaves scales as they are: a block that
- * is written on from its middle keeps the scale that the dropped ones asked for. */
+ * growth of their block's scale: e4m3 is the type for those).  Dropping positions (sxq_kv_reserve)
+ * leaves scales as they are: a block that is written on from its middle keeps the scale that the
+ * dropped ones asked for. */
 #define SXQ_KV_SCALE_BLOCK 16
 
 /* Block tables and slot maps from the requests' lengths.  Request r of n_rows holds lens[r]

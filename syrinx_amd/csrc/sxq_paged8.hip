@@ -61,9 +61,10 @@ SXQ_DEV void norm_rope(const KvAppend& A, int hd, int lh, bool live, bool norm, 
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
         for (int o = lh >> 1; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
-        // x / rms: a product with the rounded inverse rounds twice, and codes at a border move; the first
-        // quotient's remainder, exact, corrects it (two steps of Newton's for a quotient; a division itself costs 54
-        // us for 49 at 8192 bf16 tokens of 32 + 16 heads of 128)
+        // x / rms: a product with the rounded inverse rounds twice, and codes at a border move; its remainder,
+        // which a fused product gives exactly, corrects it (Markstein's last step of a division; 8192 bf16
+        // tokens of 32 + 16 heads of 128 take 49 us without it, 50 so and 54 by divisions).  Means outside
+        // that step's range, zeros and infinities among them, are divided by.
         const float rms = sqrtf(ss / (float)hd + A.eps), inv = 1.0f / rms;
         if (__all(rms > 0x1p-100f && rms < 0x1p100f)) {
 #pragma unroll

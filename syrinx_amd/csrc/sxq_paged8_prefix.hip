@@ -60,7 +60,8 @@ struct CutTile {
     int part, pieces;  // its first partial, how many
 };
 
-// The workspace: counts {items, tiles that are cut, their pieces, the first item's place}; items; the tiles that are cut; partials: per part and unit, {m, l} of each row, then the weighted sums.
+// The workspace: counts {items, tiles that are cut, their pieces, the first item's place}; items; the
+// tiles that are cut; partials: per part and unit, {m, l} of each row, then the weighted sums.
 struct PrefixPlan {
     int* counts;
     TileItem* item;

@@ -8,7 +8,6 @@ import numpy as np
 import pytest
 import torch
 
-from syrinx_amd.paged import PagedKvCache, SlotMap
 from test_gpu_paged import DT, F64, U32, _close
 from test_gpu_paged8 import CT, PREFIX_SPLIT, B, _attend, _cache, _code_values, _filled, _queries, _reference, cuda  # noqa: F401
 
@@ -409,3 +408,36 @@ def test_append_of_rows_at_odd_strides(cuda, it, hd, inter):
         q = cache.append(0, qkv, m, n_heads=nh, q_norm=w, k_norm=w, rope=rope, interleaved=inter)
         outs.append((q, *cache.read(0, _i32(cuda, [0, T]), T, dtype=torch.float32)))
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("entries,nh", [(3000, 8), (40, 8)])
+def test_a_captured_map_whose_tokens_change(cuda, entries, nh):
+    """One graph, its map's entries nobody's, one long request's, everybody's in turn: what is cut is
+    decided at each replay, and each is the eager call."""
+    lens = [9000, 40, 300, 1]
+    cache, g = _filled(cuda, 2, 64, 16, lens, "i8", 8)
+    rows, pos = _i32(cuda, [-1] * entries), _i32(cuda, [-1] * entries)
+    q = _queries(g, cuda, entries, nh, 64, "bf16")
+    out = torch.zeros_like(q)
+    ws = cache.workspace(entries, nh, prefix=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        cache.attend(0, q, rows=rows, pos=pos, out=out, workspace=ws)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attend(0, q, rows=rows, pos=pos, out=out, workspace=ws)
+    rng = np.random.default_rng(entries)
+    maps = [([-1] * entries, [-1] * entries), ([0] * 3 + [-1] * (entries - 3), [8997, 8998, 8999] + [-1] * (entries - 3)),
+            (rng.integers(-1, 5, entries).tolist(), rng.integers(-1, 9000, entries).tolist()),
+            ([2] * entries, (np.arange(entries) % 300).tolist()), ([-1] * (entries - 1) + [0], [0] * (entries - 1) + [8999])]
+    for turn, (r, p) in enumerate(maps + maps):
+        rows.copy_(_i32(cuda, r))
+        pos.copy_(_i32(cuda, p))
+        out.fill_(7.0)
+        graph.replay()
+        if turn % 2:
+            torch.cuda.synchronize()
+        want = cache.attend(0, q, rows=rows, pos=pos, out=torch.full_like(q, 7.0))
+        assert torch.equal(out, want), turn
